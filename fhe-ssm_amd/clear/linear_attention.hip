@@ -2,6 +2,7 @@
 //
 //   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t          (S: dk x dv, float32)
 #include <algorithm>
+#include <type_traits>
 
 #include "clear.hpp"
 
@@ -137,6 +138,443 @@ void launch_recurrent(const Args& a, uint32_t grid, hipStream_t st) {
     else go(k_recurrent<T, V, 128 / step>);
 }
 
+// ------------------------------------------------------------------------------------------------ by chunks
+// Chunks of 64 tokens, on the matrix cores.  With G_i the sum of the chunk's log decays up to token i:
+//     o_i = exp(G_i) q_i S + sum_{j <= i} exp(G_i - G_j) (q_i . k_j) v_j,   S' = exp(G_63) S + sum_j exp(G_63 - G_j) k_j v_j^T
+// The sums of decays and their differences are taken in 64 bits (in units of log 2): in 32 bits a chunk of strong decays would
+// lose what its neighbouring tokens have in common.  Matrix operands are bf16 pieces of a value, each the upper 8 bits of what
+// the ones before it left: one piece is a bf16 input, two a float16 one, three a float32 one, so products of inputs are exact.
+// Decayed keys go into the state as three pieces (24 bits, as the state is held).  The scores and the state that the outputs
+// read go in as three pieces for float32 outputs and as two (17 bits, the last rounded) for the 16-bit ones, whose own
+// rounding is 2^5 to 2^8 times that.
+constexpr int kChunk = 64, kPad = 8;  // a row of LDS is padded by 16 bytes: 16 rows' reads of 16 bytes meet no bank twice
+
+template <class X>
+struct Pieces;
+template <>
+struct Pieces<bf16> {
+    static constexpr int in = 1, mid = 2;
+};
+template <>
+struct Pieces<f16> {
+    static constexpr int in = 2, mid = 2;
+};
+template <>
+struct Pieces<float> {
+    static constexpr int in = 3, mid = 3;
+};
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// four floats as N pieces of four bf16 each; the last piece is rounded
+template <int N>
+__device__ inline void split4(const float (&x)[4], u32x2 (&to)[N]) {
+    float f[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+    for (int p = 0; p < N; p++) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (p + 1 < N) {
+                const uint32_t a = __float_as_uint(f[2 * i]) & 0xffff0000u, b = __float_as_uint(f[2 * i + 1]) & 0xffff0000u;
+                to[p][i] = a >> 16 | b;
+                f[2 * i] -= __uint_as_float(a);
+                f[2 * i + 1] -= __uint_as_float(b);
+            } else {
+                typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+                to[p][i] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)f[2 * i], (bf16)f[2 * i + 1]});
+            }
+        }
+    }
+}
+
+// four channels of a row, zeros past its end; wide: the row lies on four elements
+template <class X>
+__device__ inline void load4(const X* p, int left, bool wide, X (&to)[4]) {
+    typedef X x4 __attribute__((ext_vector_type(4)));
+    if (wide && left >= 4) {
+        const x4 v = *(const x4*)p;
+#pragma unroll
+        for (int i = 0; i < 4; i++) to[i] = v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) to[i] = i < left ? p[i] : (X)0.f;
+    }
+}
+
+// c += a b over the pieces of both, the smallest first; what is left out is below 2^-24 of the product
+template <int A, int B>
+__device__ inline f32x4 mma(const bf16x8 (&a)[A], const bf16x8 (&b)[B], f32x4 c) {
+#pragma unroll
+    for (int s = A + B - 2 < 2 ? A + B - 2 : 2; s >= 0; s--)
+#pragma unroll
+        for (int i = 0; i < A; i++)
+            if (s - i >= 0 && s - i < B) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
+    return c;
+}
+
+__device__ inline bf16x8 read8(const uint16_t* p) { return *(const bf16x8*)p; }
+__device__ inline bf16x8 read44(const uint16_t* p, const uint16_t* q) {
+    const u32x2 a = *(const u32x2*)p, b = *(const u32x2*)q;
+    return __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+}
+
+struct ChunkArgs {
+    Args a;
+    uint32_t segments, segment;  // a segment's tokens, a multiple of a chunk
+    float* joint;                // [segment][lane, head][dk][dv]: what a segment adds to the state, then the state before it
+    double* sums;                // [segment][lane, head]: the log decay of a segment
+    bool wide_q, wide_k, wide_v, wide_out;
+};
+
+template <class X, int DK, int TV>
+struct ChunkShared {
+    uint16_t k[Pieces<X>::in][kChunk][DK + kPad];       // keys, a token a row
+    uint16_t kt[3][DK][kChunk + kPad];                  // decayed keys, a channel a row
+    uint16_t vt[Pieces<X>::in][TV][kChunk + kPad];      // values, a channel a row
+    uint16_t st[Pieces<X>::mid][TV][DK + kPad];         // the state before the chunk, a column a row
+    double sum[kChunk];
+    int poisoned;                                       // the last chunk (its first token + 1) with a value not finite
+};
+
+// A workgroup takes TV columns of one head's state over one segment of one lane's tokens.  Wave w has the outputs of tokens
+// 16 w .. 16 w + 15 of a chunk (transposed: a lane has one token and four neighbouring channels) and a quarter of the state's
+// 16 x 16 tiles.  The scores of a token, as they come out of one product (a lane: one query, four neighbouring keys), go into
+// the next one without leaving their registers: the values are read in the order of keys that this makes.
+// out: outputs from the state before the segment; otherwise what the segment adds to the state, and its log decay.
+template <class X, int DK, int TV, bool kOut>
+__global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
+    constexpr int P = Pieces<X>::in, M = Pieces<X>::mid, KK = DK / 32, CT = TV / 16, ST = DK / 16 * CT / 4;
+    constexpr int kKeyBlocks = DK * kChunk / 16 / 256 ? DK * kChunk / 16 / 256 : 1;  // 4 x 4 blocks of a thread
+    constexpr int kValueBlocks = TV * kChunk / 16 / 256 ? TV * kChunk / 16 / 256 : 1;
+    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
+    auto& s = *(ChunkShared<X, DK, TV>*)shared_bytes;
+    const Args& a = c.a;
+    const uint32_t items = gridDim.x / c.segments / a.tiles;
+    const uint32_t tile = blockIdx.x % a.tiles, item = blockIdx.x / a.tiles % items, seg = blockIdx.x / a.tiles / items;
+    const uint32_t h = item % a.heads, lane = item / a.heads, col0 = tile * TV;
+    const int wave = threadIdx.x / 64, l = threadIdx.x % 64, lr = l % 16, lg = l / 16;
+    const X* q = (const X*)a.q + lane * a.qs[0] + (h / a.q_each) * a.qs[2];
+    const X* k = (const X*)a.k + lane * a.ks[0] + (h / a.k_each) * a.ks[2];
+    const X* v = (const X*)a.v + lane * a.vs[0] + h * a.vs[2] + col0;
+    const float* g = a.g + lane * a.gs[0] + h * a.gs[2];
+    X* out = (X*)a.out + lane * a.os[0] + h * a.os[2] + col0;
+    const int len = a.lengths ? min(max(a.lengths[lane], 0), (int)a.tokens) : (int)a.tokens;
+    const int first = (int)(seg * c.segment), last = min((int)min((uint64_t)(seg + 1) * c.segment, (uint64_t)a.tokens), len);
+    const int dk = a.dk, cols = min((int)(a.dv - col0), TV);
+    const size_t part = ((size_t)(kOut && c.segments == 1 ? 0 : seg) * items + item) * a.dk * a.dv;
+
+    // a thread's 4 x 4 blocks (tokens by channels) of keys and values
+    X kx[kKeyBlocks][4][4], vx[kValueBlocks][4][4], qx[KK][2][4];
+    float gx = 0.f;
+    const auto block = [&](int b, int width, int& token, int& channel) {
+        const int at = threadIdx.x + 256 * b;
+        channel = at % (width / 4) * 4;
+        token = at / (width / 4) * 4;
+    };
+    const auto fetch = [&](int t0) {
+        const int n = min(kChunk, last - t0);
+        gx = l < n ? floored(g[(int64_t)(t0 + l) * a.gs[1]]) : 0.f;
+#pragma unroll
+        for (int b = 0; b < kKeyBlocks; b++) {
+            int t, d;
+            block(b, DK, t, d);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                load4(k + (int64_t)(t0 + t + i) * a.ks[1] + d, t + i < n ? dk - d : 0, c.wide_k, kx[b][i]);
+        }
+#pragma unroll
+        for (int b = 0; b < kValueBlocks; b++) {
+            int t, d;
+            block(b, TV, t, d);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                load4(v + (int64_t)(t0 + t + i) * a.vs[1] + d, t + i < n ? cols - d : 0, c.wide_v, vx[b][i]);
+        }
+        if constexpr (kOut) {
+            const int t = wave * 16 + lr;
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int d = kk * 32 + lg * 8 + i * 4;
+                    load4(q + (int64_t)(t0 + t) * a.qs[1] + d, t < n ? dk - d : 0, c.wide_q, qx[kk][i]);
+                }
+        }
+    };
+
+    // the state: tile i of this wave covers rows d0(i) .. + 15 and columns c0(i) .. + 15, a lane has column lr, rows 4 lg ..
+    f32x4 S[ST];
+    const auto d0 = [&](int i) { return (wave * ST + i) / CT * 16; };
+    const auto c0 = [&](int i) { return (wave * ST + i) % CT * 16; };
+    const float* from = kOut ? (c.segments == 1 ? a.state_in : c.joint) : nullptr;
+#pragma unroll
+    for (int i = 0; i < ST; i++) {
+        S[i] = f32x4{0, 0, 0, 0};
+        if (from && c0(i) + lr < cols) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int d = d0(i) + lg * 4 + r;
+                if (d < dk) S[i][r] = from[part + (size_t)d * a.dv + col0 + c0(i) + lr];
+            }
+        }
+    }
+    if (threadIdx.x == 0) s.poisoned = 0;
+    double total = 0.;
+    if (first < last) fetch(first);
+    for (int t0 = first; t0 < last; t0 += kChunk) {
+        // sums of the decays: lane l of every wave has token l
+        double sum = (double)gx * 1.4426950408889634;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const double o = __shfl_up(sum, d);
+            if (l >= d) sum += o;
+        }
+        const double whole = __shfl(sum, 63);
+        total += whole;
+        const float weight = exp2f((float)(whole - sum)), all = exp2f((float)whole);
+        __syncthreads();  // the chunk before has been read
+        if (threadIdx.x < kChunk) s.sum[l] = sum;
+#pragma unroll
+        for (int b = 0; b < kKeyBlocks; b++) {
+            int t, d;
+            block(b, DK, t, d);
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = __shfl(weight, (t + i) % 64);
+            if (t < kChunk) {
+                if constexpr (kOut) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float f[4] = {to_f32(kx[b][i][0]), to_f32(kx[b][i][1]), to_f32(kx[b][i][2]), to_f32(kx[b][i][3])};
+                        u32x2 piece[P];
+                        split4(f, piece);
+#pragma unroll
+                        for (int p = 0; p < P; p++) *(u32x2*)&s.k[p][t + i][d] = piece[p];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float f[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) f[i] = to_f32(kx[b][i][e]) * w[i];
+                    u32x2 piece[3];
+                    split4(f, piece);
+#pragma unroll
+                    for (int p = 0; p < 3; p++) *(u32x2*)&s.kt[p][d + e][t] = piece[p];
+                }
+            }
+        }
+        bool odd = false;
+#pragma unroll
+        for (int b = 0; b < kValueBlocks; b++) {
+            int t, d;
+            block(b, TV, t, d);
+            if (t < kChunk) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float f[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        f[i] = to_f32(vx[b][i][e]);
+                        odd |= !(fabsf(f[i]) < INFINITY);
+                    }
+                    u32x2 piece[P];
+                    split4(f, piece);
+#pragma unroll
+                    for (int p = 0; p < P; p++) *(u32x2*)&s.vt[p][d + e][t] = piece[p];
+                }
+            }
+        }
+        if (kOut && odd) s.poisoned = t0 + 1;
+        bf16x8 Q[KK][P];
+        if constexpr (kOut) {
+#pragma unroll
+            for (int i = 0; i < ST; i++) {
+                const float f[4] = {S[i][0], S[i][1], S[i][2], S[i][3]};
+                u32x2 piece[M];
+                split4(f, piece);
+#pragma unroll
+                for (int p = 0; p < M; p++) *(u32x2*)&s.st[p][c0(i) + lr][d0(i) + lg * 4] = piece[p];
+            }
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                u32x2 piece[2][P];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float f[4] = {to_f32(qx[kk][i][0]), to_f32(qx[kk][i][1]), to_f32(qx[kk][i][2]), to_f32(qx[kk][i][3])};
+                    split4(f, piece[i]);
+                }
+#pragma unroll
+                for (int p = 0; p < P; p++)
+                    Q[kk][p] = __builtin_bit_cast(bf16x8, u32x4{piece[0][p].x, piece[0][p].y, piece[1][p].x, piece[1][p].y});
+            }
+        }
+        __syncthreads();
+        if (t0 + kChunk < last) fetch(t0 + kChunk);
+
+        if constexpr (kOut) {
+            const double mine = s.sum[wave * 16 + lr];
+            f32x4 O[CT];
+            const float before = exp2f((float)mine);
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                O[ct] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++) {
+                    bf16x8 st[M];
+#pragma unroll
+                    for (int p = 0; p < M; p++) st[p] = read8(&s.st[p][ct * 16 + lr][kk * 32 + lg * 8]);
+                    O[ct] = mma(st, Q[kk], O[ct]);
+                }
+                O[ct] *= before;
+            }
+            const bool poisoned = s.poisoned == t0 + 1;
+#pragma unroll
+            for (int pair = 0; pair < 2; pair++) {
+                if (pair * 2 > wave) break;
+                u32x2 piece[2][M];
+                float p4[2][4];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int jt = pair * 2 + u;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) p4[u][r] = 0.f;
+                    if (jt <= wave) {
+                        f32x4 score = {0, 0, 0, 0};
+#pragma unroll
+                        for (int kk = 0; kk < KK; kk++) {
+                            bf16x8 kr[P];
+#pragma unroll
+                            for (int p = 0; p < P; p++) kr[p] = read8(&s.k[p][jt * 16 + lr][kk * 32 + lg * 8]);
+                            score = mma(kr, Q[kk], score);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int j = jt * 16 + lg * 4 + r;
+                            const float p = score[r] * exp2f((float)(mine - s.sum[j]));
+                            p4[u][r] = j <= wave * 16 + lr ? p : 0.f;
+                        }
+                    }
+                    split4(p4[u], piece[u]);
+                }
+                if (!poisoned) {
+                    bf16x8 pr[M];
+#pragma unroll
+                    for (int p = 0; p < M; p++)
+                        pr[p] = __builtin_bit_cast(bf16x8, u32x4{piece[0][p].x, piece[0][p].y, piece[1][p].x, piece[1][p].y});
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        bf16x8 vr[P];
+#pragma unroll
+                        for (int p = 0; p < P; p++) {
+                            const uint16_t* row = &s.vt[p][ct * 16 + lr][pair * 32 + lg * 4];
+                            vr[p] = read44(row, row + 16);
+                        }
+                        O[ct] = mma(vr, pr, O[ct]);
+                    }
+                } else {
+                    // a value here is infinite or NaN: a product with a score of 0 would carry it to tokens before its own,
+                    // so the sums are taken over each token's own past, one by one
+                    for (int ct = 0; ct < CT; ct++)
+                        for (int e = 0; e < 16; e++) {
+                            float o = 0.f;
+                            for (int u = 0; u < 2; u++)
+                                for (int r = 0; r < 4; r++) {
+                                    const int j = (pair * 2 + u) * 16 + lg * 4 + r;
+                                    if (j > wave * 16 + lr) continue;
+                                    float x = 0.f;
+                                    for (int p = P - 1; p >= 0; p--)
+                                        x += __uint_as_float((uint32_t)s.vt[p][ct * 16 + e][j] << 16);
+                                    o = fmaf(p4[u][r], x, o);
+                                }
+                            o += __shfl_xor(o, 16);
+                            o += __shfl_xor(o, 32);
+                            if (e / 4 == lg)
+#pragma unroll
+                                for (int i = 0; i < CT; i++)
+#pragma unroll
+                                    for (int r = 0; r < 4; r++)
+                                        if (i == ct && r == e % 4) O[i][r] += o;
+                        }
+                }
+            }
+            const int t = t0 + wave * 16 + lr;
+            if (t < last) {
+                X* row = out + (int64_t)t * a.os[1];
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    const int e = ct * 16 + lg * 4;
+                    typedef X x4 __attribute__((ext_vector_type(4)));
+                    x4 o;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) o[r] = from_f32<X>(O[ct][r] * a.scale);
+                    if (c.wide_out && e + 4 <= cols) *(x4*)(row + e) = o;
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (e + r < cols) row[e + r] = o[r];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < ST; i++) {
+            S[i] *= all;
+#pragma unroll
+            for (int kk = 0; kk < kChunk / 32; kk++) {
+                bf16x8 kt[3], vt[P];
+#pragma unroll
+                for (int p = 0; p < 3; p++) kt[p] = read8(&s.kt[p][d0(i) + lr][kk * 32 + lg * 8]);
+#pragma unroll
+                for (int p = 0; p < P; p++) vt[p] = read8(&s.vt[p][c0(i) + lr][kk * 32 + lg * 8]);
+                S[i] = mma(kt, vt, S[i]);
+            }
+        }
+    }
+    if constexpr (kOut) {  // the rows past a lane's length, each with the segment it lies in
+        const int end = (int)min((uint64_t)(seg + 1) * c.segment, (uint64_t)a.tokens), zero = max(last, first);
+        for (int e = threadIdx.x; e < (end - zero) * TV; e += 256)
+            if (e % TV < cols) out[(int64_t)(zero + e / TV) * a.os[1] + e % TV] = (X)0.f;
+    }
+    float* into = kOut ? (c.segments == 1 ? a.state_out : nullptr) : c.joint;
+    if (into) {
+#pragma unroll
+        for (int i = 0; i < ST; i++)
+            if (c0(i) + lr < cols) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int d = d0(i) + lg * 4 + r;
+                    if (d < dk) into[part + (size_t)d * a.dv + col0 + c0(i) + lr] = S[i][r];
+                }
+            }
+    }
+    if (!kOut && tile == 0 && threadIdx.x == 0) c.sums[(size_t)seg * items + item] = total;
+}
+
+// what each segment adds becomes the state before it, along the segments; the state after the last one is the result
+__global__ __launch_bounds__(256) void k_join(ChunkArgs c, uint32_t items) {
+    const size_t square = (size_t)c.a.dk * c.a.dv, at = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= items * square) return;
+    const size_t item = at / square;
+    float S = c.a.state_in ? c.a.state_in[at] : 0.f;
+    constexpr uint32_t kBatch = 8;  // loads in flight
+    for (uint32_t s0 = 0; s0 < c.segments; s0 += kBatch) {
+        float add[kBatch], decay[kBatch];
+#pragma unroll
+        for (uint32_t i = 0; i < kBatch; i++)
+            if (s0 + i < c.segments) {
+                add[i] = c.joint[(s0 + i) * items * square + at];
+                decay[i] = exp2f((float)c.sums[(s0 + i) * items + item]);
+            }
+#pragma unroll
+        for (uint32_t i = 0; i < kBatch; i++)
+            if (s0 + i < c.segments) {
+                c.joint[(s0 + i) * items * square + at] = S;
+                S = fmaf(decay[i], S, add[i]);
+            }
+    }
+    if (c.a.state_out) c.a.state_out[at] = S;
+}
+
 // ------------------------------------------------------------------------------------------------ host
 int check(const fhe_ssm_linear_attention* a) {
     if (!a) return fail(CKKS_EINVAL, "linear attention: null description");
@@ -146,7 +584,7 @@ int check(const fhe_ssm_linear_attention* a) {
     if (a->q_heads < 1 || a->k_heads < 1 || a->heads % a->q_heads || a->heads % a->k_heads)
         return fail(CKKS_EINVAL, "linear attention: %u heads cannot share %u query and %u key heads", a->heads, a->q_heads,
                     a->k_heads);
-    const uint64_t tiles = (a->dv + kCols - 1) / kCols;
+    const uint64_t tiles = (a->dv + 31) / 32;  // the narrowest that a kernel takes
     if ((uint64_t)a->lanes * a->heads > 0x7fffffffull / tiles || a->tokens > 0x1000000u)
         return fail(CKKS_EINVAL, "linear attention: too many lanes, heads or tokens");
     return CKKS_OK;
@@ -167,25 +605,88 @@ Args arguments(const fhe_ssm_linear_attention* a, const void* q, const void* k, 
 }
 
 template <class F>
-int by_type(uint32_t type, F&& f) {
-    if (type == FHE_SSM_F32) f(0.f);
-    else if (type == FHE_SSM_BF16) f(bf16{});
-    else f(f16{});
-    return CKKS_OK;
+auto by_type(uint32_t type, F&& f) {
+    if (type == FHE_SSM_F32) return f(0.f);
+    if (type == FHE_SSM_BF16) return f(bf16{});
+    return f(f16{});
+}
+
+// how a prompt is cut: by token (segments 0), or by chunks in so many segments
+struct Plan {
+    uint32_t tile, segments, segment;
+    size_t sums_at, bytes;
+};
+
+Plan plan(const fhe_ssm_linear_attention* a) {
+    Plan p{};
+    p.tile = a->type == FHE_SSM_F32 && a->dk > 64 ? 32 : 64;  // three pieces of 128 channels fill the LDS at 32 columns
+    if (a->tokens < 32 || !a->lanes) return p;
+    const uint32_t items = a->lanes * a->heads, groups = items * ((a->dv + p.tile - 1) / p.tile);
+    const uint32_t chunks = (a->tokens + kChunk - 1) / kChunk;
+    p.segments = 1;
+    if (groups < 256 && chunks >= 8) p.segments = std::min(chunks, 512 / groups);
+    const uint32_t each = (chunks + p.segments - 1) / p.segments;
+    p.segment = each * kChunk;
+    p.segments = (chunks + each - 1) / each;
+    if (p.segments > 1) {
+        p.sums_at = ((size_t)p.segments * items * a->dk * a->dv * 4 + 255) / 256 * 256;
+        p.bytes = p.sums_at + (size_t)p.segments * items * 8;
+    }
+    return p;
+}
+
+template <class X, int DK, int TV>
+int launch_chunks(const ChunkArgs& c, uint32_t items, hipStream_t st) {
+    const uint32_t grid = items * c.a.tiles * c.segments, bytes = sizeof(ChunkShared<X, DK, TV>);
+    // LDS past 64 KB is asked for by name
+    const auto go = [&](auto kernel) -> int {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return fail(CKKS_EHIP, "linear attention: %s", hipGetErrorString(e));
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), bytes, st, c);
+        return CKKS_OK;
+    };
+    if (c.segments > 1) {
+        if (int rc = go(k_chunks<X, DK, TV, false>)) return rc;
+        const size_t n = (size_t)items * c.a.dk * c.a.dv;
+        hipLaunchKernelGGL(k_join, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, c, items);
+    }
+    return go(k_chunks<X, DK, TV, true>);
 }
 
 int run(const fhe_ssm_linear_attention* a, const void* q, const void* k, const void* v, const float* g,
-        const int32_t* lengths, const float* state_in, float* state_out, void* out, void* stream) {
+        const int32_t* lengths, const float* state_in, float* state_out, void* out, void* workspace,
+        size_t workspace_bytes, void* stream) {
     if (a->lanes == 0) return CKKS_OK;
     if (a->tokens && (!q || !k || !v || !g || !out)) return fail(CKKS_EINVAL, "linear attention: null argument");
-    const Args r = arguments(a, q, k, v, g, lengths, state_in, state_out, out);
-    const uint32_t grid = a->lanes * a->heads * r.tiles;
-    const bool wide = a->dv % 4 == 0 && aligned(state_in, 16) && aligned(state_out, 16);
-    by_type(a->type, [&](auto t) {
-        if (wide) launch_recurrent<decltype(t), 4>(r, grid, (hipStream_t)stream);
-        else launch_recurrent<decltype(t), 1>(r, grid, (hipStream_t)stream);
+    Args r = arguments(a, q, k, v, g, lengths, state_in, state_out, out);
+    const hipStream_t st = (hipStream_t)stream;
+    const Plan p = plan(a);
+    if (!p.segments) {
+        const bool wide = a->dv % 4 == 0 && aligned(state_in, 16) && aligned(state_out, 16);
+        by_type(a->type, [&](auto t) {
+            const uint32_t grid = a->lanes * a->heads * r.tiles;
+            if (wide) launch_recurrent<decltype(t), 4>(r, grid, st);
+            else launch_recurrent<decltype(t), 1>(r, grid, st);
+        });
+        return launched("linear attention");
+    }
+    if (p.bytes && (!workspace || workspace_bytes < p.bytes || !aligned(workspace, 8)))
+        return fail(CKKS_EINVAL, "linear attention: a workspace of %zu bytes on 8 is needed", p.bytes);
+    r.tiles = (a->dv + p.tile - 1) / p.tile;
+    const size_t four = 4 * type_bytes(a->type);
+    const auto wide = [&](const void* at, const int64_t* stride) {
+        return aligned(at, four) && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
+    };
+    const ChunkArgs c{r, p.segments, p.segment, (float*)workspace, (double*)((char*)workspace + p.sums_at),
+                      wide(q, r.qs), wide(k, r.ks), wide(v, r.vs), wide(out, r.os)};
+    const uint32_t items = a->lanes * a->heads;
+    const int rc = by_type(a->type, [&](auto t) {
+        typedef decltype(t) X;
+        if (a->dk <= 32) return launch_chunks<X, 32, 64>(c, items, st);
+        if (a->dk <= 64) return launch_chunks<X, 64, 64>(c, items, st);
+        return launch_chunks<X, 128, std::is_same<X, float>::value ? 32 : 64>(c, items, st);
     });
-    return launched("linear attention");
+    return rc ? rc : launched("linear attention");
 }
 
 }  // namespace
@@ -196,7 +697,7 @@ extern "C" {
 int fhe_ssm_linear_attention_workspace(const fhe_ssm_linear_attention* a, size_t* bytes) {
     if (int rc = clear::check(a)) return rc;
     if (!bytes) return clear::fail(CKKS_EINVAL, "linear attention: null argument");
-    *bytes = 0;
+    *bytes = clear::plan(a).bytes;
     return CKKS_OK;
 }
 
@@ -205,7 +706,7 @@ int fhe_ssm_linear_attention_prompt(const fhe_ssm_linear_attention* a, const voi
                                     float* state_out, void* out, void* workspace, size_t workspace_bytes,
                                     void* stream) {
     if (int rc = clear::check(a)) return rc;
-    return clear::run(a, q, k, v, log_decay, lengths, state_in, state_out, out, stream);
+    return clear::run(a, q, k, v, log_decay, lengths, state_in, state_out, out, workspace, workspace_bytes, stream);
 }
 
 int fhe_ssm_linear_attention_step(const fhe_ssm_linear_attention* a, const void* q, const void* k, const void* v,
@@ -213,7 +714,7 @@ int fhe_ssm_linear_attention_step(const fhe_ssm_linear_attention* a, const void*
                                   void* stream) {
     if (int rc = clear::check(a)) return rc;
     if (a->tokens != 1) return clear::fail(CKKS_EINVAL, "linear attention: a step has one token, not %u", a->tokens);
-    return clear::run(a, q, k, v, log_decay, nullptr, state_in, state_out, out, stream);
+    return clear::run(a, q, k, v, log_decay, nullptr, state_in, state_out, out, nullptr, 0, stream);
 }
 
 }  // extern "C"

@@ -165,6 +165,27 @@ def test_prompt_decays_at_their_ends(T, kind):
     check_prompt(q, k, v, g, state)
 
 
+@pytest.mark.parametrize("T", [20, 64, 200, 1500])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_prompt_values_that_are_not_finite_stay_in_their_future(T, kind):
+    """an infinite value or a NaN reaches no token before its own, no other channel and no other lane or head"""
+    q, k, v, g, state = attention_case(2, T, 2, 2, 2, 64, 64, TYPES[kind], T)
+    want, left = run_prompt(q, k, v, g, state)
+    at = [(0, T // 2, 1, 7, math.inf), (0, T - 1, 0, 3, math.nan), (1, T // 3, 0, 63, -math.inf)]
+    for b, t, h, c, x in at:
+        v[b, t, h, c] = x
+    out, into = run_prompt(q, k, v, g, state)
+    hit, hit_state = torch.zeros_like(out, dtype=torch.bool), torch.zeros_like(into, dtype=torch.bool)
+    for b, t, h, c, _ in at:
+        hit[b, t:, h, c], hit_state[b, h, :, c] = True, True
+    assert not torch.isfinite(out[hit]).any() and not torch.isfinite(into[hit_state]).any()
+    # elsewhere the same sums in another order
+    size, size_left = recurrence(q.abs(), k.abs(), v.nan_to_num(0, 0, 0).abs(), g, state.abs(), torch.full((2,), T, device="cuda"), 1.0)
+    allowed = (2 * (4 * T + 128) * 2.0**-24) * size + 2 * ROUNDING[out.dtype] * want.double().abs()
+    assert ((out.double() - want.double()).abs() <= allowed)[~hit].all()
+    assert ((into.double() - left.double()).abs() <= 2 * (4 * T + 128) * 2.0**-24 * size_left)[~hit_state].all()
+
+
 @pytest.mark.parametrize("T", [4, 150])
 def test_prompt_one_decay_per_head(T):
     q, k, v, _, state = attention_case(2, T, 4, 4, 2, 64, 64, torch.bfloat16, 3)
