@@ -1,10 +1,17 @@
 // sample.hip -- the draw of a token under temperature, top-k, top-p and min-p.
 //
-// With the largest logit m, an entry weighs e = exp((l - m) / temperature) <= 1, held as a whole number of 2^-44: sums of
-// up to 2^18 entries are exact in 64 bits, so they do not depend on their order.  Entries are ordered by a key: the
-// logit's bits, turned so that unsigned comparison orders them; equal keys by index.  top-k and top-p each keep a prefix
-// of that order, named by the key t of its last entry and the number n of entries of that key in it; the shorter prefix is
-// what both keep.
+// With the largest logit m, an entry lies d = log2(e) (m - l) / temperature below it and weighs e = 2^-d.  Entries with
+// d >= 46.5 weigh nothing: all 2^18 of them together would be below 2^-28 of the largest, and no draw of 24 bits tells them.
+// Weights that are summed in no fixed order (by LDS atomics, over lists) are whole numbers of 2^-44, sums over all entries
+// 64-bit floats in a fixed order: a row gives the same token every time.  Entries are ordered by a key, the logit's bits
+// turned so that unsigned comparison orders them, and equal keys by index.
+//
+// One workgroup takes a row and passes over it a few times, from the caches after the first: short loops over vectors in
+// flight.  (A row held in registers, 64 logits a thread, was slower: every pass, unrolled over them, is code that runs once
+// and has to be fetched.)  The first pass takes the largest logit, and the whole weight where it will be needed.  Filters that
+// keep few entries go by a list: the largest logits of the 1,024 threads already hold k entries (or a nucleus' mass), so the
+// smallest of those that do bounds the list from below, and what lies above it, a few more than are kept, is ranked entry
+// against entry.  Filters that keep many go by a histogram of d, and by the entries of the bin where they end.
 #include <algorithm>
 
 #include "clear.hpp"
@@ -13,8 +20,11 @@ namespace clear {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kUnit = 44;              // e is held in units of 2^-44
-constexpr uint32_t kMostVocab = 1u << 18;
+constexpr int kList = 1024, kBins = 1024;
+constexpr float kSpan = 46.5f, kBinsEach = 22.f;  // d below kSpan; bins of d, the last below kBins
+constexpr int kUnit = 44;                         // whole weights are in units of 2^-44
+constexpr uint32_t kMostVocab = 1u << 18;         // their sums fit 64 bits
+constexpr uint32_t kNever = 0xffffffffu;
 
 // 0: never drawn (NaN, -inf); otherwise rising with the logit; 0 and -0 are one
 __device__ inline uint32_t key_of(float x) {
@@ -24,131 +34,404 @@ __device__ inline uint32_t key_of(float x) {
 }
 __device__ inline float of_key(uint32_t k) { return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k); }
 
-// floor(e 2^44) of a float in [0, 1]
+// floor(e 2^44) of a float in [2^-63, 1]
 __device__ inline uint64_t fixed(float e) {
     const uint32_t b = __float_as_uint(e);
     const uint64_t m = (uint64_t)((b & 0x7fffffu) | 0x800000u) << (kUnit - 23);
     return m >> min(127u - (b >> 23), 63u);
 }
 
-struct Row {
-    float top, rate;  // the largest logit; log2(e) / temperature
-    __device__ float e(float x) const {
-        return x >= top ? 1.f : exp2f((x - top) * rate);  // the largest also where it is +inf or the rate is
-    }
-};
-
-__device__ inline uint64_t wave_sum(uint64_t x) {
-#pragma unroll
-    for (int m = 32; m; m /= 2) x += __shfl_xor(x, m);
-    return x;
+// ---------------------------------------------------------------- sums over lanes, by row shifts and row broadcasts
+template <int kControl, int kRows>
+__device__ inline uint64_t moved(uint64_t x) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, kControl, kRows, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), kControl, kRows, 0xf, false);
+    return (uint64_t)hi << 32 | lo;
+}
+template <int kControl, int kRows, class T>
+__device__ inline T plus_moved(T x) {
+    return x + __builtin_bit_cast(T, moved<kControl, kRows>(__builtin_bit_cast(uint64_t, x)));
+}
+// lane l: the sum of lanes 0 .. l
+template <class T>
+__device__ inline T wave_scan(T x) {
+    x = plus_moved<0x111, 0xf>(x);
+    x = plus_moved<0x112, 0xf>(x);
+    x = plus_moved<0x114, 0xf>(x);
+    x = plus_moved<0x118, 0xf>(x);
+    x = plus_moved<0x142, 0xa>(x);
+    return plus_moved<0x143, 0xc>(x);
+}
+template <class T>
+__device__ inline T from_lane(T x, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+    return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+}
+template <class T>
+__device__ inline T wave_sum(T x) {
+    return from_lane(wave_scan(x), 63);
+}
+__device__ inline uint32_t wave_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane((int)x, 63);
 }
 
 struct Shared {
-    uint64_t part[kWaves], mass[256];
-    uint32_t count[256];
-    uint64_t found[3];
+    uint64_t bins[kBins];                   // a histogram; with a list: what is kept of each of its entries
+    uint64_t order[kList], weight[kList];   // a list: key and flipped index, as one number that falls along the order; weight
+    uint64_t order2[kList], weight2[kList]; // of a list's entries those of one bin
+    uint64_t part[2][kWaves];               // the waves' sums, of two blocks of sums in turn
+    uint64_t above;
+    uint32_t listed, listed2, low, bin, found;
 };
 
-__device__ inline uint64_t block_sum(uint64_t x, Shared& s) {
+// The sum over the workgroup, in a fixed order.  turn: 0 and 1 in turn, so that one barrier is enough.
+template <class T>
+__device__ inline T block_sum(T x, Shared& s, int turn) {
     x = wave_sum(x);
+    T* part = (T*)s.part[turn];
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
     __syncthreads();
-    if (threadIdx.x % 64 == 0) s.part[threadIdx.x / 64] = x;
-    __syncthreads();
-    uint64_t t = 0;
-    for (int w = 0; w < kWaves; w++) t += s.part[w];
+    T t = part[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) t += part[w];
     return t;
 }
 
-// The prefix of the order that reaches `want` (1 <= want <= the sum over all) when entries count weigh(key): the key of
-// its last entry, what lies above that key, by digits of 8 bits from the top.
-template <class T, class W>
-__device__ inline uint32_t threshold(const T* x, uint32_t vocab, uint64_t want, Shared& s, uint64_t& above, W&& weigh) {
-    uint32_t key = 0;
-    above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += kThreads) s.mass[i] = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
-            const float v = to_f32(x[i]);
-            const uint32_t k = key_of(v);
-            if (k && (shift == 24 || k >> (shift + 8) == key >> (shift + 8)))
-                atomicAdd((unsigned long long*)&s.mass[k >> shift & 255], (unsigned long long)weigh(k, v));
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            uint64_t sum = above;
-            int d = 255;
-            for (; d > 0 && sum + s.mass[d] < want; d--) sum += s.mass[d];
-            s.found[0] = d;
-            s.found[1] = sum;
-        }
-        __syncthreads();
-        key |= (uint32_t)s.found[0] << shift;
-        above = s.found[1];
-        __syncthreads();
-    }
-    return key;
-}
-
-// the first index up to which weigh(key, logit, index) sums to at least `want`, or vocab
-template <class T, class W>
-__device__ inline uint32_t first_reaching(const T* x, uint32_t vocab, uint64_t want, Shared& s, W&& weigh) {
+// The first bin up to which the bins' sum is at least `want` (in s.bin, kNever if there is none) and the sum before it (in
+// s.above).  s.bin must be kNever before, with a barrier between; ends with a barrier.
+__device__ inline void find_bin(uint64_t want, Shared& s, int turn) {
+    const uint64_t mine = s.bins[threadIdx.x], upto = wave_scan(mine);
+    if (threadIdx.x % 64 == 63) s.part[turn][threadIdx.x / 64] = upto;
+    __syncthreads();
     uint64_t before = 0;
-    for (uint32_t i0 = 0; i0 < vocab; i0 += kThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        uint64_t w = 0;
-        if (i < vocab) {
-            const float v = to_f32(x[i]);
-            const uint32_t k = key_of(v);
-            if (k) w = weigh(k, v, i);
-        }
-        const uint64_t sum = block_sum(w, s);
-        if (before + sum >= want) {
-            uint64_t upto = w;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const uint64_t o = __shfl_up(upto, d);
-                if ((int)(threadIdx.x % 64) >= d) upto += o;
-            }
-            for (int v = 0; v < (int)threadIdx.x / 64; v++) upto += s.part[v];
-            upto += before;
-            if (upto >= want && upto - w < want) s.found[0] = i;
-            __syncthreads();
-            return (uint32_t)s.found[0];
-        }
-        before += sum;
+    for (int w = 0; w < (int)threadIdx.x / 64; w++) before += s.part[turn][w];
+    if (before + upto - mine < want && before + upto >= want) {
+        s.bin = threadIdx.x;
+        s.above = before + upto - mine;
     }
-    return vocab;
+    __syncthreads();
 }
 
-template <class T>
-__global__ __launch_bounds__(kThreads) void k_sample(const T* __restrict__ logits, uint32_t vocab, int64_t stride,
-                                                     const float* __restrict__ draws, fhe_ssm_sample_params p,
-                                                     int64_t* __restrict__ tokens, float* __restrict__ logprobs) {
+// ---------------------------------------------------------------- a row's logits
+// A wave has a contiguous part of the row, taken 64 vectors of 16 bytes at a time; NaN and what lies outside are -inf.
+template <class X>
+struct Row {
+    static constexpr int kVec = 16 / sizeof(X), kStep = 64 * kVec, kFlight = 4;  // vectors of a thread in flight
+    typedef X vec __attribute__((ext_vector_type(kVec)));
+    const X* x;        // moved back to a multiple of 16 bytes
+    int skip, end;     // the row lies at skip .. end - 1 from there
+    int vectors, at0;  // of a thread; its wave's first element
+    __device__ Row(const X* row, int vocab) {
+        skip = (int)((uintptr_t)row % 16 / sizeof(X));
+        x = row - skip;
+        end = skip + vocab;
+        vectors = (end + kThreads * kVec - 1) / (kThreads * kVec);
+        at0 = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * vectors * kStep;
+    }
+    // f(vector of floats, index of its first) for every vector of the thread
+    template <class F>
+    __device__ __forceinline__ void vectors_of(F&& f) const {
+        const int mine = threadIdx.x % 64 * kVec;
+#pragma unroll 1
+        for (int j = 0; j < vectors; j += kFlight) {
+            const int at = at0 + j * kStep;
+            vec v[kFlight];
+            if (at >= skip && at + kFlight * kStep <= end) {
+#pragma unroll
+                for (int u = 0; u < kFlight; u++) v[u] = *(const vec*)(x + at + u * kStep + mine);
+            } else {
+#pragma unroll
+                for (int u = 0; u < kFlight; u++)
+#pragma unroll
+                    for (int c = 0; c < kVec; c++) {
+                        const int i = at + u * kStep + mine + c;
+                        v[u][c] = j + u < vectors && i >= skip && i < end ? x[i] : (X)-INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < kFlight; u++)
+                if (j + u < vectors) {
+                    float one[kVec];
+#pragma unroll
+                    for (int c = 0; c < kVec; c++) one[c] = fmaxf(to_f32((X)v[u][c]), -INFINITY);
+                    f(one, at + u * kStep + mine - skip);
+                }
+        }
+    }
+    // f(logit, index) for every element of the thread
+    template <class F>
+    __device__ __forceinline__ void each(F&& f) const {
+        vectors_of([&](const float (&one)[kVec], int i) {
+#pragma unroll
+            for (int c = 0; c < kVec; c++) f(one[c], (uint32_t)(i + c));
+        });
+    }
+};
+
+struct Scale {
+    float top, rate;  // log2(e) / temperature, held to where products with it are not NaN
+    // how far below the largest, in powers of two
+    __device__ float d(float x) const { return x >= top ? 0.f : (top - x) * rate; }
+    __device__ static float e(float d) { return __builtin_amdgcn_exp2f(-d); }
+};
+
+// what the filters by rank keep: logits above x, and those that equal it up to index `last`
+struct Prefix {
+    float x;
+    uint32_t last;
+    __device__ bool has(float v, uint32_t index) const { return v > x || (v == x && index <= last); }
+};
+
+// The first index up to which the weights w(logit, index) >= 0 sum to more than target(their whole sum); mine: the sum over
+// the thread's own entries.  Where rounding leaves none, the last one that weighs.  At least one weight is above 0.
+// First the wave whose part it lies in, then all threads on that part, a vector each.
+template <class R, class W, class T>
+__device__ __forceinline__ uint32_t locate(const R& row, Shared& s, double mine, double& whole, W&& w, T&& target_of) {
+    const int wave = threadIdx.x / 64, l = threadIdx.x % 64;
+    double* part = (double*)s.part[0];
+    mine = wave_sum(mine);
+    __syncthreads();
+    if (l == 0) part[wave] = mine;
+    __syncthreads();
+    double run = 0., before = 0.;
+    for (int v = 0; v < kWaves; v++) run += part[v];
+    whole = run;
+    const double target = target_of(run);
+    int from = 0;
+    bool reached = false;
+    run = 0.;
+    for (int v = 0; v < kWaves; v++) {
+        if (!reached && part[v] > 0.) {
+            from = v;
+            before = run;
+            reached = run + part[v] > target;
+        }
+        run += part[v];
+    }
+    reached = false;
+    double* split = (double*)s.part[1];
+    for (int v0 = 0; v0 < row.vectors * 64 && !reached; v0 += kThreads) {
+        const int i = from * row.vectors * R::kStep + (v0 + (int)threadIdx.x) * R::kVec;
+        float one[R::kVec];
+        double vector = 0.;
+#pragma unroll
+        for (int c = 0; c < R::kVec; c++) {
+            const bool in = v0 + (int)threadIdx.x < row.vectors * 64 && i + c >= row.skip && i + c < row.end;
+            one[c] = in ? w(fmaxf(to_f32(row.x[i + c]), -INFINITY), (uint32_t)(i + c - row.skip)) : 0.f;
+            vector += (double)one[c];
+        }
+        const double upto = wave_scan(vector);
+        if (l == 63) split[wave] = upto;
+        __syncthreads();
+        double mine0 = 0.;
+        int last = -1;  // the wave that holds it
+        run = before;
+        for (int v = 0; v < kWaves; v++) {
+            if (!reached && split[v] > 0.) {
+                last = v;
+                mine0 = run;
+                reached = run + split[v] > target;
+            }
+            run += split[v];
+        }
+        before = run;
+        if (wave == last) {
+            const uint64_t over = __ballot(mine0 + upto > target && vector > 0.), some = __ballot(vector > 0.);
+            const int lane = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+            if (l == lane) {
+                double sum = mine0 + upto - vector;
+                bool hit = false;
+#pragma unroll
+                for (int c = 0; c < R::kVec; c++)
+                    if (!hit && one[c] > 0.f) {
+                        sum += (double)one[c];
+                        hit = sum > target;
+                        s.found = (uint32_t)(i + c - row.skip);
+                    }
+            }
+        }
+        __syncthreads();
+    }
+    return s.found;
+}
+
+// An entry of a short list against all others: how many come before it and what they weigh.  Some threads share an entry;
+// `first` is one of them.
+constexpr int kShort = 128;
+struct Ranked {
+    bool first;
+    int rank;
+    uint64_t order, weight, before;
+};
+__device__ inline int sharing(int n) { return n > 64 ? 8 : 16; }
+__device__ inline Ranked rank_short(const Shared& s, int n) {
+    const int each = sharing(n), i = threadIdx.x / each, sub = threadIdx.x % each;
+    Ranked r{i < n && sub == 0, 0, i < n ? s.order[i] : 0, i < n ? s.weight[i] : 0, 0};
+    for (int j = sub; j < n; j += each) {
+        const uint64_t o = s.order[j], w = s.weight[j];
+        if (o > r.order) {
+            r.before += w;
+            r.rank++;
+        }
+    }
+    for (int m = 1; m < each; m *= 2) {
+        r.before += __shfl_xor(r.before, m);
+        r.rank += __shfl_xor(r.rank, m);
+    }
+    return r;
+}
+
+// A long list, an entry a thread: the entry up to which the weights sum to at least `want`, 1 <= want <= their sum, in falling
+// order (its order is returned).  bin: rises along the order.  A histogram by bin, then the entries of the bin that has it
+// against each other.
+__device__ inline uint64_t cross(Shared& s, bool in, uint32_t bin, uint64_t order, uint64_t weight, uint64_t want) {
+    __syncthreads();
+    s.bins[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s.bin = kNever, s.listed2 = 0;
+    __syncthreads();
+    if (in) atomicAdd((unsigned long long*)&s.bins[bin], (unsigned long long)weight);
+    __syncthreads();
+    find_bin(want, s, 0);
+    want -= s.above;
+    in = in && bin == s.bin;
+    if (in) {
+        const uint32_t at = atomicAdd(&s.listed2, 1u);
+        s.order2[at] = order;
+        s.weight2[at] = weight;
+    }
+    __syncthreads();
+    if (in) {
+        uint64_t before = 0;
+        for (uint32_t j = 0; j < s.listed2; j++) before += s.order2[j] > order ? s.weight2[j] : 0;
+        if (before < want && before + weight >= want) s.above = order;
+    }
+    __syncthreads();
+    return s.above;
+}
+__device__ inline void add_to_list(Shared& s, float x, uint32_t index, uint64_t weight) {
+    const uint32_t at = atomicAdd(&s.listed, 1u);
+    if (at < kList) {
+        s.order[at] = (uint64_t)key_of(x) << 32 | ~index;
+        s.weight[at] = weight;
+    }
+}
+
+// The shortest prefix of the order, inside `in`, that has `want` entries (by_rank) or whose whole weights sum to at least
+// `want`; all of `in` if none does.  Entries with d >= limit must not be needed for it.  A histogram of d gives the bin that
+// it ends in; that bin's entries go into a list and are ranked, or, where they are too many, by the digits of their keys.
+template <class R>
+__device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Shared& s, Prefix in, bool by_rank, uint64_t want,
+                                           float limit) {
+    const auto clear = [&] {
+        __syncthreads();
+        s.bins[threadIdx.x] = 0;
+        if (threadIdx.x == 0) s.bin = kNever, s.listed = 0;
+        __syncthreads();
+    };
+    clear();
+    row.each([&](float x, uint32_t i) {
+        const float d = scale.d(x);
+        if (d < limit && in.has(x, i))
+            atomicAdd((unsigned long long*)&s.bins[(int)(d * kBinsEach)], by_rank ? 1ull : (unsigned long long)fixed(Scale::e(d)));
+    });
+    __syncthreads();
+    find_bin(want, s, 0);
+    const uint32_t bin = s.bin;
+    if (bin == kNever) return in;
+    want -= s.above;
+    row.each([&](float x, uint32_t i) {
+        const float d = scale.d(x);
+        if (d < limit && (uint32_t)(d * kBinsEach) == bin && in.has(x, i))
+            add_to_list(s, x, i, by_rank ? 1ull : fixed(Scale::e(d)));
+    });
+    __syncthreads();
+    if (s.listed <= kList) {
+        const bool there = threadIdx.x < s.listed;
+        const uint64_t order = there ? s.order[threadIdx.x] : 0;
+        const float d = there ? scale.d(of_key((uint32_t)(order >> 32))) : 0.f;
+        const uint64_t last = cross(s, there, there ? min((uint32_t)((d * kBinsEach - (float)bin) * kBins), kBins - 1u) : 0, order,
+                                    there ? s.weight[threadIdx.x] : 0, want);
+        return Prefix{of_key((uint32_t)(last >> 32)), ~(uint32_t)last};
+    }
+    uint32_t key = 0;
+    uint64_t same = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        clear();
+        row.each([&](float x, uint32_t i) {
+            const float d = scale.d(x);
+            const uint32_t k = key_of(x);
+            if (d < limit && (uint32_t)(d * kBinsEach) == bin && (shift == 24 || k >> (shift + 8) == key >> (shift + 8)) &&
+                in.has(x, i))
+                atomicAdd((unsigned long long*)&s.bins[255 - (k >> shift & 255)], by_rank ? 1ull : (unsigned long long)fixed(Scale::e(d)));
+        });
+        __syncthreads();
+        find_bin(want, s, shift / 8 % 2);
+        if (s.bin == kNever) return in;
+        key |= (255 - s.bin) << shift;
+        same = s.bins[s.bin];
+        want -= s.above;
+    }
+    const float x = of_key(key);  // the last key; of the entries that have it the first n
+    const uint64_t one = by_rank ? 1 : fixed(Scale::e(scale.d(x))), n = (want + one - 1) / one;
+    if (n * one >= same) return Prefix{x, x == in.x ? in.last : kNever};
+    double whole, mine = 0.;
+    row.each([&](float v, uint32_t) { mine += v == x ? 1. : 0.; });
+    const uint32_t last = locate(
+        row, s, mine, whole, [&](float v, uint32_t) { return v == x ? 1.f : 0.f; }, [&](double) { return (double)n - 0.5; });
+    return Prefix{x, last};
+}
+
+template <class X>
+__global__ __launch_bounds__(kThreads, 8) void k_sample(const X* __restrict__ logits, uint32_t vocab, int64_t stride,
+                                                        const float* __restrict__ draws, fhe_ssm_sample_params p,
+                                                        int64_t* __restrict__ tokens, float* __restrict__ logprobs) {
     __shared__ Shared s;
     const uint32_t r = blockIdx.x;
-    const T* x = logits + (int64_t)r * stride;
+    const Row<X> row(logits + (int64_t)r * stride, (int)vocab);
     float temperature = p.temperature ? p.temperature[r] : 1.f;
     int k = p.top_k ? p.top_k[r] : 0;
     const float top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p && p.min_p[r] > 0.f ? fminf(p.min_p[r], 1.f) : 0.f;
     float u = draws[r];
     u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
     if (!(temperature > 0.f)) temperature = 1.f, k = 1;  // the first of the largest
+    const bool by_rank = k > 0 && (uint32_t)k < vocab, by_mass = top_p < 1.f;
+    const float rate = fminf(fmaxf(1.44269504088896341f / temperature, 1e-30f), 1e30f);
 
-    uint32_t most = 0;
-    uint64_t there = 0;
-    for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
-        const uint32_t key = key_of(to_f32(x[i]));
-        most = max(most, key);
-        there += key != 0;
-    }
+    s.bins[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s.listed = 0, s.low = kNever, s.bin = kNever;
+
+    // the thread's largest logit, and the weight of its entries against it
+    float mine = -INFINITY;
+    double weight = 0.;
+    const bool weigh = !by_rank && (by_mass || min_p == 0.f);
+    if (weigh)
+        row.vectors_of([&](const float(&x)[Row<X>::kVec], int) {
+            float most = x[0];
 #pragma unroll
-    for (int m = 32; m; m /= 2) most = max(most, (uint32_t)__shfl_xor(most, m));
-    if (threadIdx.x % 64 == 0) s.part[threadIdx.x / 64] = most;
+            for (int c = 1; c < Row<X>::kVec; c++) most = fmaxf(most, x[c]);
+            if (most > mine) {
+                weight *= (double)__builtin_amdgcn_exp2f((mine - most) * rate);
+                mine = most;
+            }
+            if (mine > -INFINITY) {
+#pragma unroll
+                for (int c = 0; c < Row<X>::kVec; c++) weight += (double)__builtin_amdgcn_exp2f((x[c] - mine) * rate);
+            }
+        });
+    else row.each([&](float x, uint32_t) { mine = fmaxf(mine, x); });
+    const uint32_t key = wave_max(key_of(mine));
+    if (threadIdx.x % 64 == 0) s.part[0][threadIdx.x / 64] = key;
     __syncthreads();
-    for (int w = 0; w < kWaves; w++) most = max(most, (uint32_t)s.part[w]);
-    there = block_sum(there, s);
+    uint32_t most = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) most = max(most, (uint32_t)s.part[0][w]);
     if (!most) {
         if (threadIdx.x == 0) {
             tokens[r] = -1;
@@ -156,70 +439,132 @@ __global__ __launch_bounds__(kThreads) void k_sample(const T* __restrict__ logit
         }
         return;
     }
-    const Row row{of_key(most), 1.44269504088896341f / temperature};
-
-    // top-k: the key of the k-th entry and how many of that key are kept
-    uint32_t t = 1;
-    uint64_t n = ~0ull, above;
-    if (k > 0 && (uint64_t)k < there) {
-        t = threshold(x, vocab, k, s, above, [](uint32_t, float) { return 1ull; });
-        n = k - above;
-    }
-    // mass of what top-k keeps
-    const bool some = n != ~0ull;
-    uint64_t mass = 0;
-    for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
-        const float v = to_f32(x[i]);
-        const uint32_t key = key_of(v);
-        if (key && (some ? key > t : true)) mass += fixed(row.e(v));
-    }
-    mass = block_sum(mass, s);
-    uint64_t one = some ? fixed(row.e(of_key(t))) : 0;  // each of the entries of key t
-    uint64_t total = mass + (some ? n * one : 0);
-    if (top_p < 1.f) {
-        const uint64_t want = max((uint64_t)ceil((double)max(top_p, 0.f) * (double)total), (uint64_t)1);
-        // ties of key t weigh what top-k keeps of them, on the first to come: only their sum matters here
-        uint64_t more;
-        if (some && want > mass) {  // ends among top-k's last ties
-            n = min(n, one ? (want - mass + one - 1) / one : n);
-        } else {
-            const uint32_t bound = t;
-            t = threshold(x, vocab, want, s, more, [&](uint32_t key, float v) -> uint64_t {
-                return some && key <= bound ? 0 : fixed(row.e(v));
-            });
-            one = fixed(row.e(of_key(t)));
-            n = one ? (want - more + one - 1) / one : ~0ull;
-        }
-    }
-    const bool cut = t > 1 || n != ~0ull;
-    // the last kept index among the entries of key t
-    uint32_t last = vocab;
-    if (cut && n != ~0ull)
-        last = first_reaching(x, vocab, n, s, [&](uint32_t key, float, uint32_t) -> uint64_t { return key == t; });
-    const auto weight = [&](uint32_t key, float v, uint32_t i) -> uint64_t {
-        if (!(key > t || (key == t && i <= last))) return 0;
-        const float e = row.e(v);
-        return min_p > 0.f && e < min_p ? 0 : fixed(e);
+    const Scale scale{of_key(most), rate};
+    const float part = fmaxf(top_p, 0.f);
+    const auto enough = [&](double whole) { return max((uint64_t)ceil((double)part * whole), (uint64_t)1); };
+    const auto weight_of = [&](const Prefix& kept) {  // of the thread's entries in the prefix
+        double sum = 0.;
+        row.each([&](float x, uint32_t i) {
+            const float d = scale.d(x);
+            if (d < kSpan && kept.has(x, i)) sum += (double)Scale::e(d);
+        });
+        return sum;
     };
-    uint64_t kept = 0;
-    for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
-        const float v = to_f32(x[i]);
-        const uint32_t key = key_of(v);
-        if (key) kept += weight(key, v, i);
+
+    // a list of the entries that can be kept, which lie above a bound
+    bool listed = false;
+    uint64_t want = 0;  // by mass alone: the nucleus' weight
+    float low = -INFINITY;
+    const float d_mine = scale.d(mine);
+    if (weigh) {
+        if (scale.top == INFINITY) weight = weight_of(Prefix{-INFINITY, kNever});
+        else weight = mine > -INFINITY ? weight * (double)Scale::e(d_mine) : 0.;
     }
-    kept = block_sum(kept, s);
-    uint64_t want = (uint64_t)((double)u * (double)kept);
-    want = min(want, kept - 1) + 1;
-    const uint32_t token = min(first_reaching(x, vocab, want, s, weight), vocab - 1);
-    if (threadIdx.x == 0) {
-        tokens[r] = token;
-        if (logprobs) {
-            // in 64 bits: a float32 exponent of 10 and more would lose what a close bound on the result can tell
-            const float v = to_f32(x[token]);
-            const double off = v == row.top ? 0. : ((double)v - (double)row.top) / (double)temperature;
-            logprobs[r] = (float)(off - log1p((double)(kept - (1ull << kUnit)) * 0x1p-44));
+    if (by_rank || by_mass) {
+        // from the threads' largest: enough of them, or enough weight
+        const bool counts = d_mine < kSpan;
+        if (!by_rank) want = enough(block_sum(weight, s, 1) * 0x1p44);
+        if (counts)
+            atomicAdd((unsigned long long*)&s.bins[(int)(d_mine * kBinsEach)], by_rank ? 1ull : (unsigned long long)fixed(Scale::e(d_mine)));
+        __syncthreads();
+        find_bin(by_rank ? (uint64_t)k : want, s, 0);
+        listed = s.bin != kNever;
+        if (listed) {
+            if (counts && (uint32_t)(d_mine * kBinsEach) <= s.bin) atomicMin(&s.low, key_of(mine));
+            __syncthreads();
+            low = of_key(s.low);
         }
+    } else if (min_p > 0.f) {  // a little below the least weight that min-p keeps
+        listed = true;
+        low = scale.top - (1.f - __builtin_amdgcn_logf(min_p)) / rate;
     }
+    if (listed) {
+        row.each([&](float x, uint32_t i) {
+            if (x >= low) {
+                const float d = scale.d(x);
+                if (d < kSpan) add_to_list(s, x, i, fixed(Scale::e(d)));
+            }
+        });
+        __syncthreads();
+        listed = s.listed <= kList;
+    }
+    // in 64 bits: a float32 exponent of 10 and more would lose what a close bound on the result can tell
+    const auto write = [&](uint32_t token, float x, double rest) {  // rest: what is kept, less the largest
+        tokens[r] = token;
+        const double off = x >= scale.top ? 0. : ((double)x - (double)scale.top) / (double)temperature;
+        if (logprobs) logprobs[r] = (float)(off - log1p(rest));
+    };
+    if (listed && s.listed <= kShort) {
+        const int n = s.listed, each = sharing(n), i = threadIdx.x / each;
+        const auto [first, rank, order, weight, before] = rank_short(s, n);
+        bool kept = !by_rank || rank < k;
+        if (by_mass) {
+            if (by_rank) want = enough((double)block_sum(first && kept ? weight : 0, s, 1));
+            kept = kept && before < want;
+        }
+        const float x = of_key((uint32_t)(order >> 32)), e = Scale::e(scale.d(x));
+        kept = kept && !(e < min_p);
+        if (first) s.bins[i] = kept ? weight : 0;
+        const uint64_t whole = block_sum(first && kept ? weight : 0, s, 0);
+        const uint64_t target = min((uint64_t)((double)u * (double)whole), whole - 1);
+        uint64_t upto = 0;
+        const uint32_t flipped = (uint32_t)order;
+        for (int j = threadIdx.x % each; j < n; j += each)
+            if ((uint32_t)s.order[j] >= flipped) upto += s.bins[j];
+        for (int m = 1; m < each; m *= 2) upto += __shfl_xor(upto, m);
+        if (first && kept && upto > target && upto - weight <= target) write(~flipped, x, (double)(whole - (1ull << kUnit)) * 0x1p-44);
+        return;
+    }
+    if (listed) {
+        const bool there = threadIdx.x < s.listed;
+        const uint64_t order = there ? s.order[threadIdx.x] : 0, weight = there ? s.weight[threadIdx.x] : 0;
+        const float x = there ? of_key((uint32_t)(order >> 32)) : low, d = scale.d(x), deep = scale.d(low);
+        const uint32_t bin = deep > 0.f ? min((uint32_t)(d * ((kBins - 1) / deep)), kBins - 1u) : 0;
+        bool kept = there;
+        if (by_rank) {  // all threads take part in each of these
+            const uint64_t last = cross(s, there, bin, order, 1, (uint64_t)k);
+            kept = kept && order >= last;
+        }
+        if (by_mass) {
+            if (by_rank) want = enough((double)block_sum(kept ? weight : 0, s, 1));
+            const uint64_t last = cross(s, kept, bin, order, weight, want);
+            kept = kept && order >= last;
+        }
+        kept = kept && !(Scale::e(d) < min_p);
+        const uint64_t whole = block_sum(kept ? weight : 0, s, 1);
+        const uint64_t target = min((uint64_t)((double)u * (double)whole), whole - 1);
+        const uint32_t flipped = (uint32_t)order, index = ~flipped;
+        const uint64_t token = cross(s, kept, there ? (uint32_t)((uint64_t)index * kBins / vocab) : 0, flipped, weight, target + 1);
+        if (kept && flipped == (uint32_t)token) write(index, x, (double)(whole - (1ull << kUnit)) * 0x1p-44);
+        return;
+    }
+
+    Prefix keep{-INFINITY, kNever};
+#pragma unroll 1
+    for (int mass = 0; mass < 2; mass++) {
+        if (!(mass ? by_mass : by_rank)) continue;
+        if (mass && by_rank) {
+            __syncthreads();
+            want = enough(block_sum(weight_of(keep), s, 1) * 0x1p44);
+        }
+        keep = shortest(row, scale, s, keep, !mass, mass ? want : (uint64_t)k, kSpan);
+    }
+    if (!weigh || by_mass) {
+        weight = 0.;
+        row.each([&](float x, uint32_t i) {
+            const float d = scale.d(x), e = Scale::e(d);
+            if (d < kSpan && !(e < min_p) && keep.has(x, i)) weight += (double)e;
+        });
+    }
+    double whole;
+    const uint32_t token = locate(
+        row, s, weight, whole,
+        [&](float x, uint32_t i) {
+            const float d = scale.d(x), e = Scale::e(d);
+            return d < kSpan && !(e < min_p) && keep.has(x, i) ? e : 0.f;
+        },
+        [&](double sum) { return (double)u * sum; });
+    if (threadIdx.x == 0) write(token, to_f32(logits[(int64_t)r * stride + min(token, vocab - 1)]), whole - 1.);
 }
 
 }  // namespace
@@ -236,8 +581,9 @@ extern "C" int fhe_ssm_sample(uint32_t type, const void* logits, uint32_t rows, 
     if (!logits || !draws || !params || !tokens) return fail(CKKS_EINVAL, "sample: null argument");
     if (row_stride < 0) return fail(CKKS_EINVAL, "sample: negative stride");
     const auto go = [&](auto t) {
-        hipLaunchKernelGGL(k_sample<decltype(t)>, dim3(rows), dim3(kThreads), 0, (hipStream_t)stream,
-                           (const decltype(t)*)logits, vocab, row_stride, draws, *params, tokens, logprobs);
+        typedef decltype(t) X;
+        hipLaunchKernelGGL(k_sample<X>, dim3(rows), dim3(kThreads), 0, (hipStream_t)stream, (const X*)logits, vocab, row_stride,
+                           draws, *params, tokens, logprobs);
     };
     if (type == FHE_SSM_F32) go(0.f);
     else if (type == FHE_SSM_BF16) go(bf16{});
