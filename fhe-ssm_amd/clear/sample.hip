@@ -87,9 +87,19 @@ struct Shared {
     uint64_t order[kList], weight[kList];   // a list: key and flipped index, as one number that falls along the order; weight
     uint64_t order2[kList], weight2[kList]; // of a list's entries those of one bin
     uint64_t part[2][kWaves];               // the waves' sums, of two blocks of sums in turn
+    uint64_t extra[kWaves];                 // what the entries of a list add to the waves' parts of the row
     uint64_t above;
     uint32_t listed, listed2, low, bin, found;
 };
+
+// Of sixteen values, one a wave: their sums up to each (lane w: up to value w, the same in every row of 16 lanes).
+template <class T>
+__device__ inline T scan16(T x) {
+    x = plus_moved<0x111, 0xf>(x);
+    x = plus_moved<0x112, 0xf>(x);
+    x = plus_moved<0x114, 0xf>(x);
+    return plus_moved<0x118, 0xf>(x);
+}
 
 // The sum over the workgroup, in a fixed order.  turn: 0 and 1 in turn, so that one barrier is enough.
 template <class T>
@@ -98,10 +108,7 @@ __device__ inline T block_sum(T x, Shared& s, int turn) {
     T* part = (T*)s.part[turn];
     if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
     __syncthreads();
-    T t = part[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; w++) t += part[w];
-    return t;
+    return from_lane(scan16(part[threadIdx.x % 16]), 15);
 }
 
 // The first bin up to which the bins' sum is at least `want` (in s.bin, kNever if there is none) and the sum before it (in
@@ -110,8 +117,8 @@ __device__ inline void find_bin(uint64_t want, Shared& s, int turn) {
     const uint64_t mine = s.bins[threadIdx.x], upto = wave_scan(mine);
     if (threadIdx.x % 64 == 63) s.part[turn][threadIdx.x / 64] = upto;
     __syncthreads();
-    uint64_t before = 0;
-    for (int w = 0; w < (int)threadIdx.x / 64; w++) before += s.part[turn][w];
+    const uint64_t part = s.part[turn][threadIdx.x % 16];
+    const uint64_t before = from_lane(scan16(part) - part, __builtin_amdgcn_readfirstlane(threadIdx.x / 64));
     if (before + upto - mine < want && before + upto >= want) {
         s.bin = threadIdx.x;
         s.above = before + upto - mine;
@@ -135,6 +142,7 @@ struct Row {
         vectors = (end + kThreads * kVec - 1) / (kThreads * kVec);
         at0 = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * vectors * kStep;
     }
+    __device__ int wave_of(uint32_t index) const { return ((int)index + skip) / (vectors * kStep); }
     // f(vector of floats, index of its first) for every vector of the thread
     template <class F>
     __device__ __forceinline__ void vectors_of(F&& f) const {
@@ -178,8 +186,28 @@ struct Row {
 struct Scale {
     float top, rate;  // log2(e) / temperature, held to where products with it are not NaN
     // how far below the largest, in powers of two
-    __device__ float d(float x) const { return x >= top ? 0.f : (top - x) * rate; }
+    __device__ float d(float x) const { return fmaxf((top - x) * rate, 0.f); }  // the NaN of inf - inf becomes 0
     __device__ static float e(float d) { return __builtin_amdgcn_exp2f(-d); }
+};
+
+// Weights summed.  Those of the largest logit, 1, are counted apart: what the others add to them, which a close
+// log-probability hangs on, keeps its float32 bits.
+struct Sum {
+    double rest = 0.;
+    int ones = 0;
+    // f(c): the weight of entry c; one(c): whether it is counted
+    template <int N, class F, class O>
+    __device__ __forceinline__ void add(F&& f, O&& one) {
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < N; c++) {
+            const bool is = one(c);
+            sum += is ? 0.f : f(c);
+            ones += is;
+        }
+        rest += (double)sum;
+    }
+    __device__ double whole() const { return rest + (double)ones; }
 };
 
 // what the filters by rank keep: logits above x, and those that equal it up to index `last`
@@ -190,63 +218,60 @@ struct Prefix {
 };
 
 // The first index up to which the weights w(logit, index) >= 0 sum to more than target(their whole sum); mine: the sum over
-// the thread's own entries.  Where rounding leaves none, the last one that weighs.  At least one weight is above 0.
-// First the wave whose part it lies in, then all threads on that part, a vector each.
+// the thread's own entries, which s.extra adds to by waves.  Where rounding leaves none, the last one that weighs.  At least
+// one weight is above 0.  First the wave whose part it lies in, then all threads on that part, a vector each.
 template <class R, class W, class T>
 __device__ __forceinline__ uint32_t locate(const R& row, Shared& s, double mine, double& whole, W&& w, T&& target_of) {
-    const int wave = threadIdx.x / 64, l = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64;
+    // of the waves' sums the first that reaches the target, or the last that weighs; `before`: in, the sum before all of them,
+    // out, the sum before that one
+    const auto reaching = [&](const double* parts, double target, double& before, bool& reached, double& all) {
+        const double part = parts[l % 16], upto = scan16(part);
+        const uint32_t over = (uint32_t)__ballot(before + upto > target && part > 0.) & 0xffffu;
+        const uint32_t some = (uint32_t)__ballot(part > 0.) & 0xffffu;
+        reached = over != 0;
+        const int at = over ? __builtin_ctz(over) : some ? 31 - __builtin_clz(some) : 0;
+        all = before + from_lane(upto, 15);
+        before = at ? before + from_lane(upto, at - 1) : before;
+        return some ? at : -1;
+    };
     double* part = (double*)s.part[0];
-    mine = wave_sum(mine);
+    mine = wave_sum(mine) + (double)s.extra[wave] * 0x1p-44;
     __syncthreads();
     if (l == 0) part[wave] = mine;
     __syncthreads();
-    double run = 0., before = 0.;
-    for (int v = 0; v < kWaves; v++) run += part[v];
-    whole = run;
-    const double target = target_of(run);
-    int from = 0;
-    bool reached = false;
-    run = 0.;
-    for (int v = 0; v < kWaves; v++) {
-        if (!reached && part[v] > 0.) {
-            from = v;
-            before = run;
-            reached = run + part[v] > target;
-        }
-        run += part[v];
-    }
+    whole = from_lane(scan16(part[l % 16]), 15);
+    const double target = target_of(whole);
+    double before = 0., all;
+    bool reached;
+    const int from = max(reaching(part, target, before, reached, all), 0);
     reached = false;
     double* split = (double*)s.part[1];
     for (int v0 = 0; v0 < row.vectors * 64 && !reached; v0 += kThreads) {
+        const bool in = v0 + (int)threadIdx.x < row.vectors * 64;
         const int i = from * row.vectors * R::kStep + (v0 + (int)threadIdx.x) * R::kVec;
+        typename R::vec v;
+        if (in && i >= row.skip && i + R::kVec <= row.end) v = *(const typename R::vec*)(row.x + i);
+        else
+#pragma unroll
+            for (int c = 0; c < R::kVec; c++) v[c] = in && i + c >= row.skip && i + c < row.end ? row.x[i + c] : -INFINITY;
         float one[R::kVec];
         double vector = 0.;
 #pragma unroll
         for (int c = 0; c < R::kVec; c++) {
-            const bool in = v0 + (int)threadIdx.x < row.vectors * 64 && i + c >= row.skip && i + c < row.end;
-            one[c] = in ? w(fmaxf(to_f32(row.x[i + c]), -INFINITY), (uint32_t)(i + c - row.skip)) : 0.f;
+            one[c] = w(fmaxf(to_f32(v[c]), -INFINITY), (uint32_t)(i + c - row.skip));
             vector += (double)one[c];
         }
         const double upto = wave_scan(vector);
         if (l == 63) split[wave] = upto;
         __syncthreads();
-        double mine0 = 0.;
-        int last = -1;  // the wave that holds it
-        run = before;
-        for (int v = 0; v < kWaves; v++) {
-            if (!reached && split[v] > 0.) {
-                last = v;
-                mine0 = run;
-                reached = run + split[v] > target;
-            }
-            run += split[v];
-        }
-        before = run;
+        double run = before;
+        const int last = reaching(split, target, run, reached, before);
         if (wave == last) {
-            const uint64_t over = __ballot(mine0 + upto > target && vector > 0.), some = __ballot(vector > 0.);
+            const uint64_t over = __ballot(run + upto > target && vector > 0.), some = __ballot(vector > 0.);
             const int lane = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
             if (l == lane) {
-                double sum = mine0 + upto - vector;
+                double sum = run + upto - vector;
                 bool hit = false;
 #pragma unroll
                 for (int c = 0; c < R::kVec; c++)
@@ -325,15 +350,29 @@ __device__ inline void add_to_list(Shared& s, float x, uint32_t index, uint64_t 
 
 // The shortest prefix of the order, inside `in`, that has `want` entries (by_rank) or whose whole weights sum to at least
 // `want`; all of `in` if none does.  Entries with d >= limit must not be needed for it.  A histogram of d gives the bin that
-// it ends in; that bin's entries go into a list and are ranked, or, where they are too many, by the digits of their keys.
+// it ends in; that bin's entries go into a list, or, where they are too many, by the digits of their keys.
+// kept: the weight of the thread's entries in the prefix that weigh at least `least`, where s.extra has not got it.
 template <class R>
 __device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Shared& s, Prefix in, bool by_rank, uint64_t want,
-                                           float limit) {
+                                           float limit, float least, double& kept) {
     const auto clear = [&] {
         __syncthreads();
         s.bins[threadIdx.x] = 0;
+        if (threadIdx.x < kWaves) s.extra[threadIdx.x] = 0;
         if (threadIdx.x == 0) s.bin = kNever, s.listed = 0;
         __syncthreads();
+    };
+    const auto weigh = [&](const Prefix& p) {
+        Sum sum;
+        row.vectors_of([&](const float(&x)[R::kVec], uint32_t i) {
+            sum.add<R::kVec>(
+                [&](int c) {
+                    const float d = scale.d(x[c]), e = Scale::e(d);
+                    return d < kSpan && e >= least && p.has(x[c], i + c) ? e : 0.f;
+                },
+                [&](int c) { return x[c] == scale.top && p.has(x[c], i + c); });
+        });
+        kept = sum.whole();
     };
     clear();
     row.each([&](float x, uint32_t i) {
@@ -344,20 +383,40 @@ __device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Sha
     __syncthreads();
     find_bin(want, s, 0);
     const uint32_t bin = s.bin;
-    if (bin == kNever) return in;
+    if (bin == kNever) {
+        weigh(in);
+        return in;
+    }
     want -= s.above;
-    row.each([&](float x, uint32_t i) {
-        const float d = scale.d(x);
-        if (d < limit && (uint32_t)(d * kBinsEach) == bin && in.has(x, i))
-            add_to_list(s, x, i, by_rank ? 1ull : fixed(Scale::e(d)));
-    });
+    {
+        const float from = (float)bin;
+        Sum sum;
+        row.vectors_of([&](const float(&x)[R::kVec], uint32_t i) {
+            uint32_t hits = 0;
+            sum.add<R::kVec>(
+                [&](int c) {
+                    const float d = scale.d(x[c]), at = d * kBinsEach, e = Scale::e(d);
+                    const bool has = in.has(x[c], i + c);
+                    hits |= (at >= from && at < from + 1.f && d < limit && has ? 1u : 0u) << c;
+                    return at < from && e >= least && has ? e : 0.f;
+                },
+                [&](int c) { return bin > 0 && x[c] == scale.top && in.has(x[c], i + c); });
+#pragma unroll
+            for (int c = 0; c < R::kVec; c++)
+                if (hits >> c & 1) add_to_list(s, x[c], i + c, by_rank ? 1ull : fixed(Scale::e(scale.d(x[c]))));
+        });
+        kept = sum.whole();
+    }
     __syncthreads();
     if (s.listed <= kList) {
         const bool there = threadIdx.x < s.listed;
         const uint64_t order = there ? s.order[threadIdx.x] : 0;
-        const float d = there ? scale.d(of_key((uint32_t)(order >> 32))) : 0.f;
+        const float d = there ? scale.d(of_key((uint32_t)(order >> 32))) : 0.f, e = Scale::e(d);
         const uint64_t last = cross(s, there, there ? min((uint32_t)((d * kBinsEach - (float)bin) * kBins), kBins - 1u) : 0, order,
                                     there ? s.weight[threadIdx.x] : 0, want);
+        if (there && order >= last && e >= least)
+            atomicAdd((unsigned long long*)&s.extra[row.wave_of(~(uint32_t)order)], (unsigned long long)fixed(e));
+        __syncthreads();
         return Prefix{of_key((uint32_t)(last >> 32)), ~(uint32_t)last};
     }
     uint32_t key = 0;
@@ -373,19 +432,25 @@ __device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Sha
         });
         __syncthreads();
         find_bin(want, s, shift / 8 % 2);
-        if (s.bin == kNever) return in;
+        if (s.bin == kNever) {
+            weigh(in);
+            return in;
+        }
         key |= (255 - s.bin) << shift;
         same = s.bins[s.bin];
         want -= s.above;
     }
     const float x = of_key(key);  // the last key; of the entries that have it the first n
     const uint64_t one = by_rank ? 1 : fixed(Scale::e(scale.d(x))), n = (want + one - 1) / one;
-    if (n * one >= same) return Prefix{x, x == in.x ? in.last : kNever};
-    double whole, mine = 0.;
-    row.each([&](float v, uint32_t) { mine += v == x ? 1. : 0.; });
-    const uint32_t last = locate(
-        row, s, mine, whole, [&](float v, uint32_t) { return v == x ? 1.f : 0.f; }, [&](double) { return (double)n - 0.5; });
-    return Prefix{x, last};
+    Prefix p{x, x == in.x ? in.last : kNever};
+    if (n * one < same) {
+        double whole, mine = 0.;
+        row.each([&](float v, uint32_t) { mine += v == x ? 1. : 0.; });
+        p.last = locate(
+            row, s, mine, whole, [&](float v, uint32_t) { return v == x ? 1.f : 0.f; }, [&](double) { return (double)n - 0.5; });
+    }
+    weigh(p);
+    return p;
 }
 
 template <class X>
@@ -405,11 +470,12 @@ __global__ __launch_bounds__(kThreads, 8) void k_sample(const X* __restrict__ lo
     const float rate = fminf(fmaxf(1.44269504088896341f / temperature, 1e-30f), 1e30f);
 
     s.bins[threadIdx.x] = 0;
+    if (threadIdx.x < kWaves) s.extra[threadIdx.x] = 0;
     if (threadIdx.x == 0) s.listed = 0, s.low = kNever, s.bin = kNever;
 
     // the thread's largest logit, and the weight of its entries against it
     float mine = -INFINITY;
-    double weight = 0.;
+    Sum sum;
     const bool weigh = !by_rank && (by_mass || min_p == 0.f);
     if (weigh)
         row.vectors_of([&](const float(&x)[Row<X>::kVec], int) {
@@ -417,13 +483,13 @@ __global__ __launch_bounds__(kThreads, 8) void k_sample(const X* __restrict__ lo
 #pragma unroll
             for (int c = 1; c < Row<X>::kVec; c++) most = fmaxf(most, x[c]);
             if (most > mine) {
-                weight *= (double)__builtin_amdgcn_exp2f((mine - most) * rate);
+                sum.rest = sum.whole() * (double)__builtin_amdgcn_exp2f((mine - most) * rate);
+                sum.ones = 0;
                 mine = most;
             }
-            if (mine > -INFINITY) {
-#pragma unroll
-                for (int c = 0; c < Row<X>::kVec; c++) weight += (double)__builtin_amdgcn_exp2f((x[c] - mine) * rate);
-            }
+            if (mine > -INFINITY)
+                sum.add<Row<X>::kVec>([&](int c) { return __builtin_amdgcn_exp2f((x[c] - mine) * rate); },
+                                      [&](int c) { return x[c] == mine; });
         });
     else row.each([&](float x, uint32_t) { mine = fmaxf(mine, x); });
     const uint32_t key = wave_max(key_of(mine));
@@ -442,23 +508,15 @@ __global__ __launch_bounds__(kThreads, 8) void k_sample(const X* __restrict__ lo
     const Scale scale{of_key(most), rate};
     const float part = fmaxf(top_p, 0.f);
     const auto enough = [&](double whole) { return max((uint64_t)ceil((double)part * whole), (uint64_t)1); };
-    const auto weight_of = [&](const Prefix& kept) {  // of the thread's entries in the prefix
-        double sum = 0.;
-        row.each([&](float x, uint32_t i) {
-            const float d = scale.d(x);
-            if (d < kSpan && kept.has(x, i)) sum += (double)Scale::e(d);
-        });
-        return sum;
-    };
-
     // a list of the entries that can be kept, which lie above a bound
     bool listed = false;
     uint64_t want = 0;  // by mass alone: the nucleus' weight
     float low = -INFINITY;
     const float d_mine = scale.d(mine);
-    if (weigh) {
-        if (scale.top == INFINITY) weight = weight_of(Prefix{-INFINITY, kNever});
-        else weight = mine > -INFINITY ? weight * (double)Scale::e(d_mine) : 0.;
+    double weight = mine > -INFINITY ? sum.whole() * (double)Scale::e(d_mine) : 0.;
+    if (weigh && scale.top == INFINITY) {  // the differences to it were not numbers
+        weight = 0.;
+        row.each([&](float x, uint32_t) { weight += x == INFINITY ? 1. : 0.; });
     }
     if (by_rank || by_mass) {
         // from the threads' largest: enough of them, or enough weight
@@ -479,10 +537,16 @@ __global__ __launch_bounds__(kThreads, 8) void k_sample(const X* __restrict__ lo
         low = scale.top - (1.f - __builtin_amdgcn_logf(min_p)) / rate;
     }
     if (listed) {
-        row.each([&](float x, uint32_t i) {
-            if (x >= low) {
-                const float d = scale.d(x);
-                if (d < kSpan) add_to_list(s, x, i, fixed(Scale::e(d)));
+        row.vectors_of([&](const float(&x)[Row<X>::kVec], uint32_t i) {
+            float most = x[0];
+#pragma unroll
+            for (int c = 1; c < Row<X>::kVec; c++) most = fmaxf(most, x[c]);
+            if (most >= low) {
+#pragma unroll
+                for (int c = 0; c < Row<X>::kVec; c++) {
+                    const float d = scale.d(x[c]);
+                    if (x[c] >= low && d < kSpan) add_to_list(s, x[c], i + c, fixed(Scale::e(d)));
+                }
             }
         });
         __syncthreads();
@@ -543,19 +607,20 @@ __global__ __launch_bounds__(kThreads, 8) void k_sample(const X* __restrict__ lo
 #pragma unroll 1
     for (int mass = 0; mass < 2; mass++) {
         if (!(mass ? by_mass : by_rank)) continue;
-        if (mass && by_rank) {
-            __syncthreads();
-            want = enough(block_sum(weight_of(keep), s, 1) * 0x1p44);
+        float limit = kSpan;
+        if (mass) {
+            if (by_rank) want = enough((block_sum(weight, s, 1) + from_lane(scan16((double)s.extra[threadIdx.x % 16]), 15) * 0x1p-44) * 0x1p44);
+            // n entries below 1 / n of what may be missing cannot matter: what is above them is enough
+            const double missing = ((double)want / part - (double)want) * 0x1p-44;
+            if (part > 0.f && missing > 0.) limit = fminf(kSpan, 1.f + __builtin_amdgcn_logf((float)((double)vocab / missing)));
         }
-        keep = shortest(row, scale, s, keep, !mass, mass ? want : (uint64_t)k, kSpan);
+        keep = shortest(row, scale, s, keep, !mass, mass ? want : (uint64_t)k, limit, mass || !by_mass ? min_p : 0.f, weight);
     }
-    if (!weigh || by_mass) {
-        weight = 0.;
-        row.each([&](float x, uint32_t i) {
+    if (!weigh && !by_rank && !by_mass)  // min-p alone, with a list that was too long
+        row.each([&](float x, uint32_t) {
             const float d = scale.d(x), e = Scale::e(d);
-            if (d < kSpan && !(e < min_p) && keep.has(x, i)) weight += (double)e;
+            weight += d < kSpan && e >= min_p ? (double)e : 0.;
         });
-    }
     double whole;
     const uint32_t token = locate(
         row, s, weight, whole,
