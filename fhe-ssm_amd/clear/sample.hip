@@ -130,7 +130,7 @@ __device__ inline void find_bin(uint64_t want, Shared& s, int turn) {
 // A wave has a contiguous part of the row, taken 64 vectors of 16 bytes at a time; NaN and what lies outside are -inf.
 template <class X>
 struct Row {
-    static constexpr int kVec = 16 / sizeof(X), kStep = 64 * kVec, kFlight = 4;  // vectors of a thread in flight
+    static constexpr int kVec = 16 / sizeof(X), kStep = 64 * kVec, kFlight = sizeof(X);  // vectors of a thread in flight: 16 logits
     typedef X vec __attribute__((ext_vector_type(kVec)));
     const X* x;        // moved back to a multiple of 16 bytes
     int skip, end;     // the row lies at skip .. end - 1 from there
@@ -143,15 +143,17 @@ struct Row {
         at0 = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * vectors * kStep;
     }
     __device__ int wave_of(uint32_t index) const { return ((int)index + skip) / (vectors * kStep); }
-    // f(vector of floats, index of its first) for every vector of the thread
+    // f(logits, index): the thread's logits, kFlight vectors at a time; logit e has index + place(e)
+    static constexpr int kGroup = kFlight * kVec;
+    __device__ static int place(int e) { return e / kVec * kStep + e % kVec; }  // of logit e of a group, from its first
     template <class F>
-    __device__ __forceinline__ void vectors_of(F&& f) const {
+    __device__ __forceinline__ void groups(F&& f) const {
         const int mine = threadIdx.x % 64 * kVec;
 #pragma unroll 1
         for (int j = 0; j < vectors; j += kFlight) {
             const int at = at0 + j * kStep;
             vec v[kFlight];
-            if (at >= skip && at + kFlight * kStep <= end) {
+            if (at >= skip && at + kFlight * kStep <= end && j + kFlight <= vectors) {
 #pragma unroll
                 for (int u = 0; u < kFlight; u++) v[u] = *(const vec*)(x + at + u * kStep + mine);
             } else {
@@ -163,22 +165,19 @@ struct Row {
                         v[u][c] = j + u < vectors && i >= skip && i < end ? x[i] : (X)-INFINITY;
                     }
             }
+            float one[kGroup];
 #pragma unroll
-            for (int u = 0; u < kFlight; u++)
-                if (j + u < vectors) {
-                    float one[kVec];
-#pragma unroll
-                    for (int c = 0; c < kVec; c++) one[c] = fmaxf(to_f32((X)v[u][c]), -INFINITY);
-                    f(one, at + u * kStep + mine - skip);
-                }
+            for (int e = 0; e < kGroup; e++) one[e] = numbered(to_f32((X)v[e / kVec][e % kVec]));
+            f(one, at + mine - skip);
         }
     }
+    __device__ static float numbered(float x) { return fmaxf(x, -INFINITY); }  // NaN: -inf
     // f(logit, index) for every element of the thread
     template <class F>
     __device__ __forceinline__ void each(F&& f) const {
-        vectors_of([&](const float (&one)[kVec], int i) {
+        groups([&](const float(&one)[kGroup], int i) {
 #pragma unroll
-            for (int c = 0; c < kVec; c++) f(one[c], (uint32_t)(i + c));
+            for (int e = 0; e < kGroup; e++) f(one[e], (uint32_t)(i + place(e)));
         });
     }
 };
@@ -202,8 +201,9 @@ struct Sum {
 #pragma unroll
         for (int c = 0; c < N; c++) {
             const bool is = one(c);
-            sum += is ? 0.f : f(c);
-            ones += is;
+            const float e = f(c);  // computed for all: a select costs less than a branch
+            sum += is ? 0.f : e;
+            ones += is ? 1 : 0;
         }
         rest += (double)sum;
     }
@@ -214,7 +214,7 @@ struct Sum {
 struct Prefix {
     float x;
     uint32_t last;
-    __device__ bool has(float v, uint32_t index) const { return v > x || (v == x && index <= last); }
+    __device__ bool has(float v, uint32_t index) const { return (v > x) | ((v == x) & (index <= last)); }
 };
 
 // The first index up to which the weights w(logit, index) >= 0 sum to more than target(their whole sum); mine: the sum over
@@ -259,7 +259,7 @@ __device__ __forceinline__ uint32_t locate(const R& row, Shared& s, double mine,
         double vector = 0.;
 #pragma unroll
         for (int c = 0; c < R::kVec; c++) {
-            one[c] = w(fmaxf(to_f32(v[c]), -INFINITY), (uint32_t)(i + c - row.skip));
+            one[c] = w(R::numbered(to_f32(v[c])), (uint32_t)(i + c - row.skip));
             vector += (double)one[c];
         }
         const double upto = wave_scan(vector);
@@ -352,9 +352,11 @@ __device__ inline void add_to_list(Shared& s, float x, uint32_t index, uint64_t 
 // `want`; all of `in` if none does.  Entries with d >= limit must not be needed for it.  A histogram of d gives the bin that
 // it ends in; that bin's entries go into a list, or, where they are too many, by the digits of their keys.
 // kept: the weight of the thread's entries in the prefix that weigh at least `least`, where s.extra has not got it.
-template <class R>
-__device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Shared& s, Prefix in, bool by_rank, uint64_t want,
-                                           float limit, float least, double& kept) {
+// kInside: whether `in` leaves anything out.
+template <bool by_rank, bool kInside, class R>
+__device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Shared& s, Prefix in, uint64_t want, float limit,
+                                           float least, double& kept) {
+    const auto inside = [&](float x, uint32_t index) { return !kInside || in.has(x, index); };
     const auto clear = [&] {
         __syncthreads();
         s.bins[threadIdx.x] = 0;
@@ -364,20 +366,20 @@ __device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Sha
     };
     const auto weigh = [&](const Prefix& p) {
         Sum sum;
-        row.vectors_of([&](const float(&x)[R::kVec], uint32_t i) {
-            sum.add<R::kVec>(
+        row.groups([&](const float(&x)[R::kGroup], uint32_t i) {
+            sum.add<R::kGroup>(
                 [&](int c) {
                     const float d = scale.d(x[c]), e = Scale::e(d);
-                    return d < kSpan && e >= least && p.has(x[c], i + c) ? e : 0.f;
+                    return ((d < kSpan) & (e >= least) & p.has(x[c], i + R::place(c))) ? e : 0.f;
                 },
-                [&](int c) { return x[c] == scale.top && p.has(x[c], i + c); });
+                [&](int c) { return (x[c] == scale.top) & p.has(x[c], i + R::place(c)); });
         });
         kept = sum.whole();
     };
     clear();
     row.each([&](float x, uint32_t i) {
         const float d = scale.d(x);
-        if (d < limit && in.has(x, i))
+        if ((d < limit) & inside(x, i))
             atomicAdd((unsigned long long*)&s.bins[(int)(d * kBinsEach)], by_rank ? 1ull : (unsigned long long)fixed(Scale::e(d)));
     });
     __syncthreads();
@@ -389,21 +391,26 @@ __device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Sha
     }
     want -= s.above;
     {
-        const float from = (float)bin;
+        const float from = (float)bin, upto = fminf(from + 1.f, limit * kBinsEach);
         Sum sum;
-        row.vectors_of([&](const float(&x)[R::kVec], uint32_t i) {
+        row.groups([&](const float(&x)[R::kGroup], uint32_t i) {
             uint32_t hits = 0;
-            sum.add<R::kVec>(
+            sum.add<R::kGroup>(
                 [&](int c) {
                     const float d = scale.d(x[c]), at = d * kBinsEach, e = Scale::e(d);
-                    const bool has = in.has(x[c], i + c);
-                    hits |= (at >= from && at < from + 1.f && d < limit && has ? 1u : 0u) << c;
-                    return at < from && e >= least && has ? e : 0.f;
+                    const bool has = inside(x[c], i + R::place(c));
+                    hits |= ((at >= from) & (at < upto) & has) ? 1u << c : 0u;
+                    return ((at < from) & (e >= least) & has) ? e : 0.f;
                 },
-                [&](int c) { return bin > 0 && x[c] == scale.top && in.has(x[c], i + c); });
+                [&](int c) { return (bin > 0) & (x[c] == scale.top) & inside(x[c], i + R::place(c)); });
+            while (hits) {  // few
+                const int c = __builtin_ctz(hits);
+                hits &= hits - 1;
+                float v = x[0];
 #pragma unroll
-            for (int c = 0; c < R::kVec; c++)
-                if (hits >> c & 1) add_to_list(s, x[c], i + c, by_rank ? 1ull : fixed(Scale::e(scale.d(x[c]))));
+                for (int b = 1; b < R::kGroup; b++) v = b == c ? x[b] : v;
+                add_to_list(s, v, i + R::place(c), by_rank ? 1ull : fixed(Scale::e(scale.d(v))));
+            }
         });
         kept = sum.whole();
     }
@@ -427,7 +434,7 @@ __device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Sha
             const float d = scale.d(x);
             const uint32_t k = key_of(x);
             if (d < limit && (uint32_t)(d * kBinsEach) == bin && (shift == 24 || k >> (shift + 8) == key >> (shift + 8)) &&
-                in.has(x, i))
+                inside(x, i))
                 atomicAdd((unsigned long long*)&s.bins[255 - (k >> shift & 255)], by_rank ? 1ull : (unsigned long long)fixed(Scale::e(d)));
         });
         __syncthreads();
@@ -478,18 +485,18 @@ __global__ __launch_bounds__(kThreads, 8) void k_sample(const X* __restrict__ lo
     Sum sum;
     const bool weigh = !by_rank && (by_mass || min_p == 0.f);
     if (weigh)
-        row.vectors_of([&](const float(&x)[Row<X>::kVec], int) {
+        row.groups([&](const float(&x)[Row<X>::kGroup], int) {
             float most = x[0];
 #pragma unroll
-            for (int c = 1; c < Row<X>::kVec; c++) most = fmaxf(most, x[c]);
+            for (int c = 1; c < Row<X>::kGroup; c++) most = fmaxf(most, x[c]);
             if (most > mine) {
                 sum.rest = sum.whole() * (double)__builtin_amdgcn_exp2f((mine - most) * rate);
                 sum.ones = 0;
                 mine = most;
             }
             if (mine > -INFINITY)
-                sum.add<Row<X>::kVec>([&](int c) { return __builtin_amdgcn_exp2f((x[c] - mine) * rate); },
-                                      [&](int c) { return x[c] == mine; });
+                sum.add<Row<X>::kGroup>([&](int c) { return __builtin_amdgcn_exp2f((x[c] - mine) * rate); },
+                                        [&](int c) { return x[c] == mine; });
         });
     else row.each([&](float x, uint32_t) { mine = fmaxf(mine, x); });
     const uint32_t key = wave_max(key_of(mine));
@@ -537,16 +544,17 @@ __global__ __launch_bounds__(kThreads, 8) void k_sample(const X* __restrict__ lo
         low = scale.top - (1.f - __builtin_amdgcn_logf(min_p)) / rate;
     }
     if (listed) {
-        row.vectors_of([&](const float(&x)[Row<X>::kVec], uint32_t i) {
+        row.groups([&](const float(&x)[Row<X>::kGroup], uint32_t i) {
             float most = x[0];
 #pragma unroll
-            for (int c = 1; c < Row<X>::kVec; c++) most = fmaxf(most, x[c]);
+            for (int c = 1; c < Row<X>::kGroup; c++) most = fmaxf(most, x[c]);
             if (most >= low) {
 #pragma unroll
-                for (int c = 0; c < Row<X>::kVec; c++) {
-                    const float d = scale.d(x[c]);
-                    if (x[c] >= low && d < kSpan) add_to_list(s, x[c], i + c, fixed(Scale::e(d)));
-                }
+                for (int c = 0; c < Row<X>::kGroup; c++)
+                    if (x[c] >= low) {
+                        const float d = scale.d(x[c]);
+                        if (d < kSpan) add_to_list(s, x[c], i + Row<X>::place(c), fixed(Scale::e(d)));
+                    }
             }
         });
         __syncthreads();
@@ -604,17 +612,17 @@ __global__ __launch_bounds__(kThreads, 8) void k_sample(const X* __restrict__ lo
     }
 
     Prefix keep{-INFINITY, kNever};
-#pragma unroll 1
-    for (int mass = 0; mass < 2; mass++) {
-        if (!(mass ? by_mass : by_rank)) continue;
+    if (by_rank) {
+        keep = shortest<true, false>(row, scale, s, keep, (uint64_t)k, kSpan, by_mass ? 0.f : min_p, weight);
+        if (by_mass) want = enough((block_sum(weight, s, 1) + from_lane(scan16((double)s.extra[threadIdx.x % 16]), 15) * 0x1p-44) * 0x1p44);
+    }
+    if (by_mass) {
+        // n entries below 1 / n of the weight that may be missing cannot matter: what is above them is enough
+        const double missing = ((double)want / part - (double)want) * 0x1p-44;
         float limit = kSpan;
-        if (mass) {
-            if (by_rank) want = enough((block_sum(weight, s, 1) + from_lane(scan16((double)s.extra[threadIdx.x % 16]), 15) * 0x1p-44) * 0x1p44);
-            // n entries below 1 / n of what may be missing cannot matter: what is above them is enough
-            const double missing = ((double)want / part - (double)want) * 0x1p-44;
-            if (part > 0.f && missing > 0.) limit = fminf(kSpan, 1.f + __builtin_amdgcn_logf((float)((double)vocab / missing)));
-        }
-        keep = shortest(row, scale, s, keep, !mass, mass ? want : (uint64_t)k, limit, mass || !by_mass ? min_p : 0.f, weight);
+        if (part > 0.f && missing > 0.) limit = fminf(kSpan, 1.f + __builtin_amdgcn_logf((float)((double)vocab / missing)));
+        keep = by_rank ? shortest<false, true>(row, scale, s, keep, want, limit, min_p, weight)
+                       : shortest<false, false>(row, scale, s, keep, want, limit, min_p, weight);
     }
     if (!weigh && !by_rank && !by_mass)  // min-p alone, with a list that was too long
         row.each([&](float x, uint32_t) {
