@@ -28,7 +28,7 @@ struct Q4Args {
     void* y;
     int64_t xs, ys;
     uint32_t out, in, rows, blocks, groups, per_group;  // per_group: blocks of a group, for groups of a block or more
-    uint32_t tiles, splits, per_wave;                   // splits of the columns, blocks of one
+    uint32_t tiles, splits, per_wave, chunk;            // splits of the columns, blocks of one, those at once in LDS
     bool wide_x, wide_y;
 };
 
@@ -119,140 +119,133 @@ struct Groups {
 };
 
 // A workgroup's eight waves take 8 / splits tiles of 16 outputs, for 16 C rows of x, and share the columns by `splits`.  x goes
-// through LDS, as the operands that the matrix instructions take, with each group's sum of x, in chunks: eight units of 128
-// columns of 16 rows, U a wave, which wait in the wave's registers while the chunk before them is used.  Weights come from
-// memory two blocks ahead of their use.
+// through LDS in chunks of blocks, as the operands that the matrix instructions take, with each group's sum of x.  Weights
+// come from memory A blocks ahead of their use, in a loop without branches: past one the compiler no longer knows how many
+// loads are under way, and waits for nearly all of them (the head for 32 rows took 11.3 us so).
 // F: groups of a block of 128 columns.  kPacked: up to five float32 rows, whose three parts are the columns of one tile and are
 // summed at the end, instead of three products each.
-constexpr int kWaves = 8, kAhead = 2;
-constexpr uint32_t kMostLds = 150 << 10, kPackedRows = 5;
-template <class X, Kind K, int F, int C, int U, bool kPacked>
+constexpr int kWaves = 8;
+constexpr uint32_t kPackedRows = 5, kCus = 256;
+constexpr uint32_t kLds = 64 << 10, kMostLds = 150 << 10;  // of a workgroup: two a CU, or one where it has to be
+template <class X, bool kPacked>
+constexpr int kProducts = std::is_same<X, float>::value && !kPacked ? 3 : 1;  // of an operand pair
+template <class X, bool kPacked>
+constexpr int kAheadOf = kProducts<X, kPacked> == 1 ? 4 : 2;  // A
+
+template <class X, Kind K, int F, int C, bool kPacked>
 __global__ __launch_bounds__(64 * kWaves) void k_product(Q4Args a) {
     typedef typename std::conditional<std::is_same<X, f16>::value, f16, bf16>::type E;
-    constexpr int P = std::is_same<X, float>::value && !kPacked ? 3 : 1, kFrag = 4 * C * P;  // operands of a block
+    constexpr int P = kProducts<X, kPacked>, A = kAheadOf<X, kPacked>, kFrag = 4 * C * P;  // operands of a block
     constexpr int kParts = std::is_same<X, float>::value ? 3 : 1;
     typedef typename Codes<E>::vec vec;
     extern __shared__ __attribute__((aligned(16))) char s_bytes[];
     const int l = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t split = wave % a.splits, tiles_at = kWaves / a.splits, chunk = kWaves * U / (a.splits * C);
+    const uint32_t split = wave % a.splits, tiles_at = kWaves / a.splits, chunk = a.chunk;
     const uint32_t tile = blockIdx.x * tiles_at + wave / a.splits, row0 = blockIdx.y * (16 * C);
     const uint32_t from = min(split * a.per_wave, a.blocks), to = min(from + a.per_wave, a.blocks);
-    vec* s_x = (vec*)s_bytes;                                // [split][block of the chunk][j][c][p][lane]
-    float* s_one = (float*)(s_x + kWaves * U * 4 * P * 64);  // [split][block of the chunk][f][c][row]
+    vec* s_x = (vec*)s_bytes;                                        // [split][block of the chunk][j][c][p][lane]
+    float* s_one = (float*)(s_x + a.splits * chunk * kFrag * 64);    // [split][block of the chunk][f][c][row]
 
     uint32_t mask = Codes<E>::mask, sixteen = Codes<E>::sixteen;
     asm("" : "+s"(mask));
     asm("" : "+v"(sixteen));
-    u32x4 w[kAhead];
-    Groups<K, F> g[kAhead];
+    vec ones;
+#pragma unroll
+    for (int i = 0; i < 8; i++) ones[i] = (E)1.f;
+    u32x4 w[A];
+    Groups<K, F> g[A];
     const size_t held = min(tile, a.tiles - 1);
-    // past the end the last block again: a load without a branch needs no wait before it
     const auto load = [&](int slot, uint32_t at) __attribute__((always_inline)) {
-        const uint32_t b = min(at, a.blocks - 1);
+        const uint32_t b = min(at, a.blocks - 1);  // past the end the last block again
         const size_t tb = held * a.blocks + b;
         w[slot] = (a.codes + tb * 64)[l];
         const size_t group = F > 1 || a.per_group == 1 ? tb * F : held * a.groups + b / a.per_group;
         g[slot].load(a.scales + (group << (K + 1)) * kRowTile + (l / 16 * 4 * F << (K + 1)));
     };
-    // a wave's units of the chunk at b0: unit u is 16 rows c of a split's block
-    Eight<X> raw[U][4];
-    const auto unit = [&](int u, uint32_t b0, uint32_t& c, uint32_t& sb, uint32_t& b) __attribute__((always_inline)) {
-        const uint32_t e = wave + kWaves * u;
-        c = e % C;
-        sb = e / C;
-        const uint32_t in_split = b0 + sb % chunk;
-        b = sb / chunk * a.per_wave + in_split;
-        return sb < a.splits * chunk && in_split < a.per_wave && b < a.blocks;
-    };
-    const uint32_t part = kPacked ? min((uint32_t)(l % 16) / a.rows, 2u) : 0;  // of the lane's row
-    const auto fetch = [&](uint32_t b0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            uint32_t c, sb, b;
-            if (!unit(u, b0, c, sb, b)) continue;
-            // lanes past the last row read it again; what they get is not stored
-            const uint32_t row = kPacked ? min(l % 16 - part * a.rows, a.rows - 1) : min(row0 + c * 16 + l % 16, a.rows - 1);
-            const X* x = (const X*)a.x + (int64_t)row * a.xs;
-#pragma unroll
-            for (int j = 0; j < 4; j++) raw[u][j].load(x, b * kBlock + j * 32 + l / 16 * 8, a.in, a.wide_x);
-        }
-    };
-    fetch(0);
-#pragma unroll
-    for (int u = 0; u < kAhead; u++) load(u, from + u);
+    for (int u = 0; u < A; u++) load(u, from + u);
 
     f32x4 total[C];
 #pragma unroll
     for (int c = 0; c < C; c++) total[c] = f32x4{0, 0, 0, 0};
+    const auto use = [&](int slot, uint32_t sb) __attribute__((always_inline)) {  // sb: the block's place in LDS
+#pragma unroll
+        for (int f = 0; f < F; f++) {
+            f32x4 sum[C];
+#pragma unroll
+            for (int c = 0; c < C; c++) sum[c] = f32x4{0, 0, 0, 0};
+            // all operands of the group are asked for before the first is waited for
+            vec x[4 / F][C][P];
+#pragma unroll
+            for (int j = 0; j < 4 / F; j++)
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int p = 0; p < P; p++) x[j][c][p] = s_x[((size_t)sb * kFrag + ((f * (4 / F) + j) * C + c) * P + p) * 64 + l];
+            if constexpr (C * P <= 4) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 4 / F; j++) {
+                const vec code = decode<E>(w[slot][f * (4 / F) + j], mask, sixteen);
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int p = P - 1; p >= 0; p--) sum[c] = Codes<E>::mma(code, x[j][c][p], sum[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const float one = s_one[((size_t)sb * F + f) * (16 * C) + c * 16 + l % 16];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    total[c][i] = fmaf(g[slot].scale(i, f), K == kHalf ? sum[c][i] + one : fmaf(-g[slot].zero(i, f), one, sum[c][i]),
+                                       total[c][i]);
+            }
+        }
+    };
+    const uint32_t part = kPacked ? min((uint32_t)(l % 16) / a.rows, 2u) : 0;  // of the lane's row
     for (uint32_t b0 = 0; b0 < a.per_wave; b0 += chunk) {
         if (b0) __syncthreads();  // the chunk before has been used
+        for (uint32_t e = wave; e < a.splits * chunk * C; e += kWaves) {
+            const uint32_t c = e % C, sb = e / C, in_split = b0 + sb % chunk, b = sb / chunk * a.per_wave + in_split;
+            if (in_split >= a.per_wave || b >= a.blocks) continue;
+            // lanes past the last row read it again; what they get is not stored
+            const uint32_t row = kPacked ? min(l % 16 - part * a.rows, a.rows - 1) : min(row0 + c * 16 + l % 16, a.rows - 1);
+            const X* x = (const X*)a.x + (int64_t)row * a.xs;
+            Eight<X> raw[4];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            uint32_t c, sb, b;
-            if (!unit(u, b0, c, sb, b)) continue;
-            float one[F];
+            for (int j = 0; j < 4; j++) raw[j].load(x, b * kBlock + j * 32 + l / 16 * 8, a.in, a.wide_x);
+            f32x4 one[F];  // a product with ones sums a row over all lanes that have a part of it
+#pragma unroll
+            for (int f = 0; f < F; f++) one[f] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 vec parts[kParts], mine[P];
-                operands(raw[u][j], parts);
+                operands(raw[j], parts);
                 if constexpr (kPacked) mine[0] = part == 0 ? parts[0] : part == 1 ? parts[1] : parts[2];
                 else
 #pragma unroll
                     for (int p = 0; p < P; p++) mine[p] = parts[p];
-                float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float v = 0.f;
-#pragma unroll
-                    for (int p = P - 1; p >= 0; p--) v += to_f32((E)mine[p][i]);
-                    sum += v;
-                }
-                one[j * F / 4] = j % (4 / F) ? one[j * F / 4] + sum : sum;
+                for (int p = P - 1; p >= 0; p--) one[j * F / 4] = Codes<E>::mma(ones, mine[p], one[j * F / 4]);
 #pragma unroll
                 for (int p = 0; p < P; p++) s_x[((size_t)sb * kFrag + (j * C + c) * P + p) * 64 + l] = mine[p];
             }
 #pragma unroll
-            for (int f = 0; f < F; f++) {
-                one[f] += __shfl_xor(one[f], 16);
-                one[f] += __shfl_xor(one[f], 32);
-                if (l < 16) s_one[((size_t)sb * F + f) * (16 * C) + c * 16 + l] = K == kHalf ? -24.f * one[f] : one[f];
-            }
+            for (int f = 0; f < F; f++)
+                if (l < 16) s_one[((size_t)sb * F + f) * (16 * C) + c * 16 + l] = K == kHalf ? -24.f * one[f][0] : one[f][0];
         }
         __syncthreads();
-        if (b0 + chunk < a.per_wave) fetch(b0 + chunk);
-        const uint32_t end = min(to, from + b0 + chunk);
-        for (uint32_t b1 = from + b0; b1 < end; b1 += kAhead) {
+        const uint32_t begin = min(from + b0, to), end = min(to, from + b0 + chunk), at = split * chunk;
+        uint32_t b = begin;
+        for (; b + A <= end; b += A) {
 #pragma unroll
-            for (int u = 0; u < kAhead; u++) {
-                const uint32_t b = b1 + u;
-                if (b >= end) break;
-                const uint32_t sb = split * chunk + (b - from - b0);
-#pragma unroll
-                for (int f = 0; f < F; f++) {
-                    f32x4 sum[C];
-#pragma unroll
-                    for (int c = 0; c < C; c++) sum[c] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int j = f * (4 / F); j < (f + 1) * (4 / F); j++) {
-                        const vec code = decode<E>(w[u][j], mask, sixteen);
-#pragma unroll
-                        for (int c = 0; c < C; c++)
-#pragma unroll
-                            for (int p = P - 1; p >= 0; p--)
-                                sum[c] = Codes<E>::mma(code, s_x[((size_t)sb * kFrag + (j * C + c) * P + p) * 64 + l], sum[c]);
-                    }
-#pragma unroll
-                    for (int c = 0; c < C; c++) {
-                        const float one = s_one[((size_t)sb * F + f) * (16 * C) + c * 16 + l % 16];
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            total[c][i] = fmaf(g[u].scale(i, f), K == kHalf ? sum[c][i] + one : fmaf(-g[u].zero(i, f), one, sum[c][i]),
-                                               total[c][i]);
-                    }
-                }
-                load(u, b + kAhead);
+            for (int u = 0; u < A; u++) {
+                use(u, at + b - begin + u);
+                load(u, b + u + A);
             }
         }
+#pragma unroll
+        for (int u = 0; u < A - 1; u++)  // only behind the last chunk, and the loads with it
+            if (b + u < end) use(u, at + b - begin + u);
     }
     const auto store = [&](f32x4 t, uint32_t at, int c) __attribute__((always_inline)) {
         if constexpr (kPacked) {
@@ -298,47 +291,39 @@ __global__ __launch_bounds__(64 * kWaves) void k_product(Q4Args a) {
 
 template <class X, Kind K, int F>
 int launch_rows(const Q4Args& a, hipStream_t st) {
-    constexpr bool kSplit = std::is_same<X, float>::value;  // rows in three parts
+    constexpr bool kFloats = std::is_same<X, float>::value;
     const uint32_t row_tiles = (a.rows + 15) / 16;
-    // The columns are split until there are 2,048 waves.  A chunk of one unit a wave has at least two blocks of each split up to
-    // splits C = 4; at 8 it takes two units a wave, which three parts have no LDS for.
-    const auto splits = [&](uint32_t C, uint32_t most) {
+    const bool packed = kFloats && a.rows <= kPackedRows;
+    const uint32_t P = kFloats && !packed ? 3 : 1, A = P == 1 ? 4 : 2;
+    const auto frag = [&](uint32_t C) { return C * (4096 * P + 64 * F); };  // of a block in LDS
+    // the columns are split until there are 2,048 waves, as far as A blocks of each split fit the LDS
+    const auto splits = [&](uint32_t C) {
         const uint32_t groups = (row_tiles + C - 1) / C;
         uint32_t n = 1;
-        while (a.tiles * groups * n < 2048 && 2 * n <= a.blocks && 2 * n * C <= most) n *= 2;
+        while (n < kWaves && a.tiles * groups * n < 2048 && 2 * n <= a.blocks && 2 * n * A * frag(C) <= kMostLds) n *= 2;
         return n;
     };
-    const bool packed = kSplit && a.rows <= kPackedRows;
-    const uint32_t most = kSplit && !packed ? 4 : 8;
     // 16 C rows share a read of the weights; fewer where that alone leaves the GPU empty
     uint32_t C = row_tiles > 2 ? 4 : row_tiles;
-    while (C > 1 && a.tiles * ((row_tiles + C - 1) / C) * splits(C, most) < 1024) C /= 2;
-    const auto go = [&](auto kernel, uint32_t U, uint32_t P) -> int {
+    while (C > 1 && a.tiles * ((row_tiles + C - 1) / C) * splits(C) < 1024) C /= 2;
+    const auto go = [&](auto kernel) -> int {
         Q4Args b = a;
-        b.splits = splits(C, most);
+        b.splits = splits(C);
         b.per_wave = (a.blocks + b.splits - 1) / b.splits;
-        const uint32_t tiles = kWaves / b.splits, units = kWaves * U;
-        const uint32_t bytes = std::max(units * (4096 * P + 64 * F), b.splits > 1 ? kWaves * C * 1024 : 0u);
+        const uint32_t each = kWaves / b.splits;
+        const dim3 grid((a.tiles + each - 1) / each, (row_tiles + C - 1) / C);
+        const uint32_t room = grid.x * grid.y <= kCus ? kMostLds : kLds;  // one workgroup a CU, or two
+        b.chunk = std::min(b.per_wave, std::max(A, room / (b.splits * frag(C)) / A * A));
+        const uint32_t bytes = std::max(b.splits * b.chunk * frag(C), b.splits > 1 ? kWaves * C * 1024 : 0u);
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != hipSuccess) return fail(CKKS_EHIP, "4-bit product: %s", hipGetErrorString(e));
-        hipLaunchKernelGGL(kernel, dim3((a.tiles + tiles - 1) / tiles, (row_tiles + C - 1) / C), dim3(64 * kWaves), bytes, st, b);
+        hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), bytes, st, b);
         return launched("4-bit product");
     };
-    const bool two = splits(C, most) * C > 4;
-    if constexpr (kSplit) {
-        if (packed) return two ? go(k_product<X, K, F, 1, 2, true>, 2, 1) : go(k_product<X, K, F, 1, 1, true>, 1, 1);
-        return C == 1 ? go(k_product<X, K, F, 1, 1, false>, 1, 3)
-             : C == 2 ? go(k_product<X, K, F, 2, 1, false>, 1, 3)
-                      : go(k_product<X, K, F, 4, 1, false>, 1, 3);
-    } else {
-        if (two)
-            return C == 1 ? go(k_product<X, K, F, 1, 2, false>, 2, 1)
-                 : C == 2 ? go(k_product<X, K, F, 2, 2, false>, 2, 1)
-                          : go(k_product<X, K, F, 4, 2, false>, 2, 1);
-        return C == 1 ? go(k_product<X, K, F, 1, 1, false>, 1, 1)
-             : C == 2 ? go(k_product<X, K, F, 2, 1, false>, 1, 1)
-                      : go(k_product<X, K, F, 4, 1, false>, 1, 1);
+    if constexpr (kFloats) {
+        if (packed) return go(k_product<X, K, F, 1, true>);
     }
+    return C == 1 ? go(k_product<X, K, F, 1, false>) : C == 2 ? go(k_product<X, K, F, 2, false>) : go(k_product<X, K, F, 4, false>);
 }
 
 template <class X, Kind K>

@@ -145,7 +145,7 @@ int fhe_ssm_q4_product(const fhe_ssm_q4_matrix* m, const void* weights, uint32_t
     const uint8_t* at = (const uint8_t*)weights;
     const size_t size = type_bytes(type);
     const Q4Args a{(const u32x4*)at, (const char*)at + lay.scales_at, x, y, x_stride, y_stride, m->out, m->in, rows, lay.blocks,
-                 lay.groups, std::max(1u, m->group / kBlock), lay.tiles, 1, 0,
+                 lay.groups, std::max(1u, m->group / kBlock), lay.tiles, 1, 0, 0,
                  aligned(x, 16) && x_stride * size % 16 == 0, aligned(y, 4 * size) && y_stride % 4 == 0};
     const hipStream_t st = (hipStream_t)stream;
     return type == FHE_SSM_F32 ? launch_q4<float>(a, lay.kind, m->group, st)
