@@ -27,6 +27,7 @@ struct Args {
     int64_t qs[3], ks[3], vs[3], gs[3], os[3];
 };
 
+__device__ inline float power(float x) { return __builtin_amdgcn_exp2f(x); }  // 2^x, 0 below 2^-126
 __device__ inline float floored(float g) { return g < kFloor ? kFloor : g; }  // a NaN stays one
 
 // Token by token, the state in registers.  A workgroup holds 64 columns of one head's state (columns never meet); its four
@@ -147,7 +148,10 @@ void launch_recurrent(const Args& a, uint32_t grid, hipStream_t st) {
 // Decayed keys go into the state as three pieces (24 bits, as the state is held).  The scores and the state that the outputs
 // read go in as three pieces for float32 outputs and as two (17 bits, the last rounded) for the 16-bit ones, whose own
 // rounding is 2^5 to 2^8 times that.
-constexpr int kChunk = 64, kPad = 8;  // a row of LDS is padded by 16 bytes: 16 rows' reads of 16 bytes meet no bank twice
+constexpr int kChunk = 64;
+// Padding of rows in LDS, in 16-bit words.  kPad: 16 rows' reads of 16 bytes meet no bank more often than they must; kPadT: so
+// do 16 channels' writes of four tokens, four rows apart, and reads of 8 bytes.
+constexpr int kPad = 8, kPadT = 4;
 
 template <class X>
 struct Pieces;
@@ -187,17 +191,44 @@ __device__ inline void split4(const float (&x)[4], u32x2 (&to)[N]) {
     }
 }
 
-// four channels of a row, zeros past its end; wide: the row lies on four elements
+// Channels d .. d + 3 of a row of `count`.  What lies outside is read from somewhere inside, so that no load waits for a
+// branch, and made zero when it is used (keep): the loads of a chunk are under way while the one before is worked on, and a
+// use of any would wait for them.  wide: rows lie on four elements and count is a multiple of 4.
 template <class X>
-__device__ inline void load4(const X* p, int left, bool wide, X (&to)[4]) {
+struct Four {
     typedef X x4 __attribute__((ext_vector_type(4)));
-    if (wide && left >= 4) {
-        const x4 v = *(const x4*)p;
+    typedef typename std::conditional<sizeof(X) == 4, u32x4, uint32_t __attribute__((ext_vector_type(2)))>::type words;
+    words raw;
+    template <bool wide>
+    __device__ __forceinline__ void load(const X* row, int d, int count) {
+        if constexpr (wide) raw = *(const words*)(row + (d < count ? d : 0));
+        else {
+            x4 v;
 #pragma unroll
-        for (int i = 0; i < 4; i++) to[i] = v[i];
-    } else {
+            for (int i = 0; i < 4; i++) v[i] = row[d + i < count ? d + i : 0];
+            raw = __builtin_bit_cast(words, v);
+        }
+    }
+    __device__ __forceinline__ void keep(bool row, int d, int count) {  // zeros outside
+        constexpr int each = sizeof(words) / sizeof(uint32_t) == 4 ? 1 : 2;
 #pragma unroll
-        for (int i = 0; i < 4; i++) to[i] = i < left ? p[i] : (X)0.f;
+        for (int i = 0; i < 4 / each; i++) {
+            uint32_t mask = 0;
+#pragma unroll
+            for (int e = 0; e < each; e++) mask |= (row & (d + i * each + e < count)) ? (each == 1 ? ~0u : 0xffffu << (16 * e)) : 0u;
+            raw[i] &= mask;
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const { return to_f32((X)__builtin_bit_cast(x4, raw)[i]); }
+};
+
+// a row's four channels as they are in memory, in pieces
+template <class X, int N>
+__device__ __forceinline__ void pieces(const Four<X>& x, u32x2 (&to)[N]) {
+    if constexpr (N == 1) to[0] = x.raw;
+    else {
+        const float f[4] = {x[0], x[1], x[2], x[3]};
+        split4(f, to);
     }
 }
 
@@ -223,14 +254,14 @@ struct ChunkArgs {
     uint32_t segments, segment;  // a segment's tokens, a multiple of a chunk
     float* joint;                // [segment][lane, head][dk][dv]: what a segment adds to the state, then the state before it
     double* sums;                // [segment][lane, head]: the log decay of a segment
-    bool wide_q, wide_k, wide_v, wide_out;
+    bool wide_in, wide_out;
 };
 
 template <class X, int DK, int TV>
 struct ChunkShared {
     uint16_t k[Pieces<X>::in][kChunk][DK + kPad];       // keys, a token a row
-    uint16_t kt[3][DK][kChunk + kPad];                  // decayed keys, a channel a row
-    uint16_t vt[Pieces<X>::in][TV][kChunk + kPad];      // values, a channel a row
+    uint16_t kt[3][DK][kChunk + kPadT];                  // decayed keys, a channel a row
+    uint16_t vt[Pieces<X>::in][TV][kChunk + kPadT];      // values, a channel a row
     uint16_t st[Pieces<X>::mid][TV][DK + kPad];         // the state before the chunk, a column a row
     double sum[kChunk];
     int poisoned;                                       // the last chunk (its first token + 1) with a value not finite
@@ -264,42 +295,67 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
     const size_t part = ((size_t)(kOut && c.segments == 1 ? 0 : seg) * items + item) * a.dk * a.dv;
 
     // a thread's 4 x 4 blocks (tokens by channels) of keys and values
-    X kx[kKeyBlocks][4][4], vx[kValueBlocks][4][4], qx[KK][2][4];
+    Four<X> kx[kKeyBlocks][4], vx[kValueBlocks][4], qx[KK][2];
     float gx = 0.f;
+    // neighbouring lanes have neighbouring channels, whose loads come together
     const auto block = [&](int b, int width, int& token, int& channel) {
         const int at = threadIdx.x + 256 * b;
         channel = at % (width / 4) * 4;
         token = at / (width / 4) * 4;
     };
-    const auto fetch = [&](int t0) {
+    const auto fetch_as = [&](int t0, auto how) __attribute__((always_inline)) {
+        constexpr bool wide = decltype(how)::value;
         const int n = min(kChunk, last - t0);
-        gx = l < n ? floored(g[(int64_t)(t0 + l) * a.gs[1]]) : 0.f;
+        gx = g[(int64_t)(t0 + min(l, n - 1)) * a.gs[1]];
 #pragma unroll
         for (int b = 0; b < kKeyBlocks; b++) {
             int t, d;
             block(b, DK, t, d);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                load4(k + (int64_t)(t0 + t + i) * a.ks[1] + d, t + i < n ? dk - d : 0, c.wide_k, kx[b][i]);
+            for (int i = 0; i < 4; i++) kx[b][i].template load<wide>(k + (int64_t)(t0 + min(t + i, n - 1)) * a.ks[1], d, dk);
         }
 #pragma unroll
         for (int b = 0; b < kValueBlocks; b++) {
             int t, d;
             block(b, TV, t, d);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                load4(v + (int64_t)(t0 + t + i) * a.vs[1] + d, t + i < n ? cols - d : 0, c.wide_v, vx[b][i]);
+            for (int i = 0; i < 4; i++) vx[b][i].template load<wide>(v + (int64_t)(t0 + min(t + i, n - 1)) * a.vs[1], d, cols);
         }
         if constexpr (kOut) {
             const int t = wave * 16 + lr;
 #pragma unroll
             for (int kk = 0; kk < KK; kk++)
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int d = kk * 32 + lg * 8 + i * 4;
-                    load4(q + (int64_t)(t0 + t) * a.qs[1] + d, t < n ? dk - d : 0, c.wide_q, qx[kk][i]);
-                }
+                for (int i = 0; i < 2; i++)
+                    qx[kk][i].template load<wide>(q + (int64_t)(t0 + min(t, n - 1)) * a.qs[1], kk * 32 + lg * 8 + i * 4, dk);
         }
+    };
+    const auto cut = [&](int n) __attribute__((always_inline)) {  // of a chunk of n tokens: zeros past them and past the channels
+        gx = l < n ? gx : 0.f;
+#pragma unroll
+        for (int b = 0; b < kKeyBlocks; b++) {
+            int t, d;
+            block(b, DK, t, d);
+#pragma unroll
+            for (int i = 0; i < 4; i++) kx[b][i].keep(t + i < n, d, dk);
+        }
+#pragma unroll
+        for (int b = 0; b < kValueBlocks; b++) {
+            int t, d;
+            block(b, TV, t, d);
+#pragma unroll
+            for (int i = 0; i < 4; i++) vx[b][i].keep(t + i < n, d, cols);
+        }
+        if constexpr (kOut) {
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) qx[kk][i].keep(wave * 16 + lr < n, kk * 32 + lg * 8 + i * 4, dk);
+        }
+    };
+    const auto fetch = [&](int t0) __attribute__((always_inline)) {  // one branch for all loads: each of its own waited for them
+        if (c.wide_in) fetch_as(t0, std::true_type{});
+        else fetch_as(t0, std::false_type{});
     };
 
     // the state: tile i of this wave covers rows d0(i) .. + 15 and columns c0(i) .. + 15, a lane has column lr, rows 4 lg ..
@@ -323,15 +379,10 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
     if (first < last) fetch(first);
     for (int t0 = first; t0 < last; t0 += kChunk) {
         // sums of the decays: lane l of every wave has token l
-        double sum = (double)gx * 1.4426950408889634;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const double o = __shfl_up(sum, d);
-            if (l >= d) sum += o;
-        }
-        const double whole = __shfl(sum, 63);
+        if (last - t0 < kChunk || dk < DK || cols < TV) cut(last - t0);
+        const double sum = wave_scan((double)floored(gx) * 1.4426950408889634), whole = from_lane(sum, 63);
         total += whole;
-        const float weight = exp2f((float)(whole - sum)), all = exp2f((float)whole);
+        const float weight = power((float)(whole - sum)), all = power((float)whole);
         __syncthreads();  // the chunk before has been read
         if (threadIdx.x < kChunk) s.sum[l] = sum;
 #pragma unroll
@@ -340,23 +391,20 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
             block(b, DK, t, d);
             float w[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = __shfl(weight, (t + i) % 64);
+            for (int i = 0; i < 4; i++) w[i] = __shfl(weight, (t + i) % kChunk);
             if (t < kChunk) {
                 if constexpr (kOut) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float f[4] = {to_f32(kx[b][i][0]), to_f32(kx[b][i][1]), to_f32(kx[b][i][2]), to_f32(kx[b][i][3])};
                         u32x2 piece[P];
-                        split4(f, piece);
+                        pieces(kx[b][i], piece);
 #pragma unroll
                         for (int p = 0; p < P; p++) *(u32x2*)&s.k[p][t + i][d] = piece[p];
                     }
                 }
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float f[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) f[i] = to_f32(kx[b][i][e]) * w[i];
+                    const float f[4] = {kx[b][0][e] * w[0], kx[b][1][e] * w[1], kx[b][2][e] * w[2], kx[b][3][e] * w[3]};
                     u32x2 piece[3];
                     split4(f, piece);
 #pragma unroll
@@ -372,12 +420,9 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
             if (t < kChunk) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float f[4];
+                    const float f[4] = {vx[b][0][e], vx[b][1][e], vx[b][2][e], vx[b][3][e]};
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        f[i] = to_f32(vx[b][i][e]);
-                        odd |= !(fabsf(f[i]) < INFINITY);
-                    }
+                    for (int i = 0; i < 4; i++) odd |= !(fabsf(f[i]) < INFINITY);
                     u32x2 piece[P];
                     split4(f, piece);
 #pragma unroll
@@ -400,10 +445,7 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
             for (int kk = 0; kk < KK; kk++) {
                 u32x2 piece[2][P];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float f[4] = {to_f32(qx[kk][i][0]), to_f32(qx[kk][i][1]), to_f32(qx[kk][i][2]), to_f32(qx[kk][i][3])};
-                    split4(f, piece[i]);
-                }
+                for (int i = 0; i < 2; i++) pieces(qx[kk][i], piece[i]);
 #pragma unroll
                 for (int p = 0; p < P; p++)
                     Q[kk][p] = __builtin_bit_cast(bf16x8, u32x4{piece[0][p].x, piece[0][p].y, piece[1][p].x, piece[1][p].y});
@@ -415,7 +457,7 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
         if constexpr (kOut) {
             const double mine = s.sum[wave * 16 + lr];
             f32x4 O[CT];
-            const float before = exp2f((float)mine);
+            const float before = power((float)mine);
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 O[ct] = f32x4{0, 0, 0, 0};
@@ -451,7 +493,7 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const int j = jt * 16 + lg * 4 + r;
-                            const float p = score[r] * exp2f((float)(mine - s.sum[j]));
+                            const float p = score[r] * power((float)(mine - s.sum[j]));
                             p4[u][r] = j <= wave * 16 + lr ? p : 0.f;
                         }
                     }
@@ -523,9 +565,9 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
             for (int kk = 0; kk < kChunk / 32; kk++) {
                 bf16x8 kt[3], vt[P];
 #pragma unroll
-                for (int p = 0; p < 3; p++) kt[p] = read8(&s.kt[p][d0(i) + lr][kk * 32 + lg * 8]);
+                for (int p = 0; p < 3; p++) kt[p] = read44(&s.kt[p][d0(i) + lr][kk * 32 + lg * 8], &s.kt[p][d0(i) + lr][kk * 32 + lg * 8 + 4]);
 #pragma unroll
-                for (int p = 0; p < P; p++) vt[p] = read8(&s.vt[p][c0(i) + lr][kk * 32 + lg * 8]);
+                for (int p = 0; p < P; p++) vt[p] = read44(&s.vt[p][c0(i) + lr][kk * 32 + lg * 8], &s.vt[p][c0(i) + lr][kk * 32 + lg * 8 + 4]);
                 S[i] = mma(kt, vt, S[i]);
             }
         }
@@ -563,7 +605,7 @@ __global__ __launch_bounds__(256) void k_join(ChunkArgs c, uint32_t items) {
         for (uint32_t i = 0; i < kBatch; i++)
             if (s0 + i < c.segments) {
                 add[i] = c.joint[(s0 + i) * items * square + at];
-                decay[i] = exp2f((float)c.sums[(s0 + i) * items + item]);
+                decay[i] = power((float)c.sums[(s0 + i) * items + item]);
             }
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; i++)
@@ -674,11 +716,11 @@ int run(const fhe_ssm_linear_attention* a, const void* q, const void* k, const v
         return fail(CKKS_EINVAL, "linear attention: a workspace of %zu bytes on 8 is needed", p.bytes);
     r.tiles = (a->dv + p.tile - 1) / p.tile;
     const size_t four = 4 * type_bytes(a->type);
-    const auto wide = [&](const void* at, const int64_t* stride) {
-        return aligned(at, four) && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
+    const auto wide = [&](const void* at, const int64_t* stride, uint32_t channels) {
+        return aligned(at, four) && channels % 4 == 0 && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
     };
     const ChunkArgs c{r, p.segments, p.segment, (float*)workspace, (double*)((char*)workspace + p.sums_at),
-                      wide(q, r.qs), wide(k, r.ks), wide(v, r.vs), wide(out, r.os)};
+                      wide(q, r.qs, a->dk) && wide(k, r.ks, a->dk) && wide(v, r.vs, a->dv), wide(out, r.os, a->dv)};
     const uint32_t items = a->lanes * a->heads;
     const int rc = by_type(a->type, [&](auto t) {
         typedef decltype(t) X;

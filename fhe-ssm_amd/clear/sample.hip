@@ -42,37 +42,6 @@ __device__ inline uint64_t fixed(float e) {
     return m >> min(127u - (b >> 23), 63u);
 }
 
-// ---------------------------------------------------------------- sums over lanes, by row shifts and row broadcasts
-template <int kControl, int kRows>
-__device__ inline uint64_t moved(uint64_t x) {
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, kControl, kRows, 0xf, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), kControl, kRows, 0xf, false);
-    return (uint64_t)hi << 32 | lo;
-}
-template <int kControl, int kRows, class T>
-__device__ inline T plus_moved(T x) {
-    return x + __builtin_bit_cast(T, moved<kControl, kRows>(__builtin_bit_cast(uint64_t, x)));
-}
-// lane l: the sum of lanes 0 .. l
-template <class T>
-__device__ inline T wave_scan(T x) {
-    x = plus_moved<0x111, 0xf>(x);
-    x = plus_moved<0x112, 0xf>(x);
-    x = plus_moved<0x114, 0xf>(x);
-    x = plus_moved<0x118, 0xf>(x);
-    x = plus_moved<0x142, 0xa>(x);
-    return plus_moved<0x143, 0xc>(x);
-}
-template <class T>
-__device__ inline T from_lane(T x, int lane) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
-    return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
-}
-template <class T>
-__device__ inline T wave_sum(T x) {
-    return from_lane(wave_scan(x), 63);
-}
 __device__ inline uint32_t wave_max(uint32_t x) {
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
