@@ -254,7 +254,7 @@ struct ChunkArgs {
     uint32_t segments, segment;  // a segment's tokens, a multiple of a chunk
     float* joint;                // [segment][lane, head][dk][dv]: what a segment adds to the state, then the state before it
     double* sums;                // [segment][lane, head]: the log decay of a segment
-    bool wide_in, wide_out;
+    bool wide_in, wide_out, near;  // near: a chunk's rows lie within 32-bit offsets
 };
 
 template <class X, int DK, int TV>
@@ -353,8 +353,47 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
                 for (int i = 0; i < 2; i++) qx[kk][i].keep(wave * 16 + lr < n, kk * 32 + lg * 8 + i * 4, dk);
         }
     };
+    // a whole chunk of whole rows: a uniform address for each load, and 32-bit offsets of the threads that stay
+    uint32_t k_off[kKeyBlocks], v_off[kValueBlocks];
+#pragma unroll
+    for (int b = 0; b < kKeyBlocks; b++) {
+        int t, d;
+        block(b, DK, t, d);
+        k_off[b] = (uint32_t)(t * (int)a.ks[1] + d) * sizeof(X);
+    }
+#pragma unroll
+    for (int b = 0; b < kValueBlocks; b++) {
+        int t, d;
+        block(b, TV, t, d);
+        v_off[b] = (uint32_t)(t * (int)a.vs[1] + d) * sizeof(X);
+    }
+    const uint32_t q_off = (uint32_t)((wave * 16 + lr) * (int)a.qs[1] + lg * 8) * sizeof(X), g_off = (uint32_t)(l * (int)a.gs[1]) * 4;
+    const auto fetch_whole = [&](int t0) __attribute__((always_inline)) {
+        typedef typename Four<X>::words words;
+        gx = *(const float*)((const char*)(g + (int64_t)t0 * a.gs[1]) + g_off);
+#pragma unroll
+        for (int b = 0; b < kKeyBlocks; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (kKeyBlocks > 1 || DK == 64 || threadIdx.x < DK * kChunk / 16)
+                    kx[b][i].raw = *(const words*)((const char*)(k + (int64_t)(t0 + i) * a.ks[1]) + k_off[b]);
+#pragma unroll
+        for (int b = 0; b < kValueBlocks; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (kValueBlocks > 1 || TV == 64 || threadIdx.x < TV * kChunk / 16)
+                    vx[b][i].raw = *(const words*)((const char*)(v + (int64_t)(t0 + i) * a.vs[1]) + v_off[b]);
+        if constexpr (kOut) {
+            const char* row = (const char*)(q + (int64_t)t0 * a.qs[1]);
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) qx[kk][i].raw = *(const words*)(row + q_off + (kk * 32 + i * 4) * (int)sizeof(X));
+        }
+    };
     const auto fetch = [&](int t0) __attribute__((always_inline)) {  // one branch for all loads: each of its own waited for them
-        if (c.wide_in) fetch_as(t0, std::true_type{});
+        if (c.near && dk == DK && cols == TV && last - t0 >= kChunk) fetch_whole(t0);
+        else if (c.wide_in) fetch_as(t0, std::true_type{});
         else fetch_as(t0, std::false_type{});
     };
 
@@ -418,6 +457,19 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
             int t, d;
             block(b, TV, t, d);
             if (t < kChunk) {
+                if constexpr (P == 1) {  // the 16-bit values themselves, four tokens of a channel together
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t take = e % 2 ? 0x07060302u : 0x05040100u;
+                        u32x2 turned;
+                        turned.x = __builtin_amdgcn_perm(vx[b][1].raw[e / 2], vx[b][0].raw[e / 2], take);
+                        turned.y = __builtin_amdgcn_perm(vx[b][3].raw[e / 2], vx[b][2].raw[e / 2], take);
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+                            odd |= (turned[i] & 0x7f80u) == 0x7f80u || (turned[i] & 0x7f800000u) == 0x7f800000u;
+                        *(u32x2*)&s.vt[0][d + e][t] = turned;
+                    }
+                } else
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float f[4] = {vx[b][0][e], vx[b][1][e], vx[b][2][e], vx[b][3][e]};
@@ -598,7 +650,7 @@ __global__ __launch_bounds__(256) void k_join(ChunkArgs c, uint32_t items) {
     if (at >= items * square) return;
     const size_t item = at / square;
     float S = c.a.state_in ? c.a.state_in[at] : 0.f;
-    constexpr uint32_t kBatch = 8;  // loads in flight
+    constexpr uint32_t kBatch = 16;  // loads in flight
     for (uint32_t s0 = 0; s0 < c.segments; s0 += kBatch) {
         float add[kBatch], decay[kBatch];
 #pragma unroll
@@ -719,8 +771,10 @@ int run(const fhe_ssm_linear_attention* a, const void* q, const void* k, const v
     const auto wide = [&](const void* at, const int64_t* stride, uint32_t channels) {
         return aligned(at, four) && channels % 4 == 0 && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
     };
-    const ChunkArgs c{r, p.segments, p.segment, (float*)workspace, (double*)((char*)workspace + p.sums_at),
-                      wide(q, r.qs, a->dk) && wide(k, r.ks, a->dk) && wide(v, r.vs, a->dv), wide(out, r.os, a->dv)};
+    ChunkArgs c{r, p.segments, p.segment, (float*)workspace, (double*)((char*)workspace + p.sums_at),
+                      wide(q, r.qs, a->dk) && wide(k, r.ks, a->dk) && wide(v, r.vs, a->dv), wide(out, r.os, a->dv), false};
+    const auto small = [&](const int64_t* stride) { return stride[1] >= 0 && stride[1] < (1 << 22); };
+    c.near = c.wide_in && small(r.qs) && small(r.ks) && small(r.vs) && small(r.gs);
     const uint32_t items = a->lanes * a->heads;
     const int rc = by_type(a->type, [&](auto t) {
         typedef decltype(t) X;
