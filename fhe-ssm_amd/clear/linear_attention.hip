@@ -368,22 +368,23 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
         v_off[b] = (uint32_t)(t * (int)a.vs[1] + d) * sizeof(X);
     }
     const uint32_t q_off = (uint32_t)((wave * 16 + lr) * (int)a.qs[1] + lg * 8) * sizeof(X), g_off = (uint32_t)(l * (int)a.gs[1]) * 4;
-    const auto fetch_whole = [&](int t0) __attribute__((always_inline)) {
+    // in parts, between the steps of the chunk before: in one go they fill the queue of the memory unit, and the wave stands
+    const auto fetch_whole = [&](int t0, int what) __attribute__((always_inline)) {
         typedef typename Four<X>::words words;
-        gx = *(const float*)((const char*)(g + (int64_t)t0 * a.gs[1]) + g_off);
+        if (what == 0) gx = *(const float*)((const char*)(g + (int64_t)t0 * a.gs[1]) + g_off);
 #pragma unroll
         for (int b = 0; b < kKeyBlocks; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if (kKeyBlocks > 1 || DK == 64 || threadIdx.x < DK * kChunk / 16)
+                if (what == 0) if (kKeyBlocks > 1 || DK == 64 || threadIdx.x < DK * kChunk / 16)
                     kx[b][i].raw = *(const words*)((const char*)(k + (int64_t)(t0 + i) * a.ks[1]) + k_off[b]);
 #pragma unroll
         for (int b = 0; b < kValueBlocks; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if (kValueBlocks > 1 || TV == 64 || threadIdx.x < TV * kChunk / 16)
+                if (what == 1) if (kValueBlocks > 1 || TV == 64 || threadIdx.x < TV * kChunk / 16)
                     vx[b][i].raw = *(const words*)((const char*)(v + (int64_t)(t0 + i) * a.vs[1]) + v_off[b]);
-        if constexpr (kOut) {
+        if (kOut && what == 2) {
             const char* row = (const char*)(q + (int64_t)t0 * a.qs[1]);
 #pragma unroll
             for (int kk = 0; kk < KK; kk++)
@@ -391,9 +392,9 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
                 for (int i = 0; i < 2; i++) qx[kk][i].raw = *(const words*)(row + q_off + (kk * 32 + i * 4) * (int)sizeof(X));
         }
     };
-    const auto fetch = [&](int t0) __attribute__((always_inline)) {  // one branch for all loads: each of its own waited for them
-        if (c.near && dk == DK && cols == TV && last - t0 >= kChunk) fetch_whole(t0);
-        else if (c.wide_in) fetch_as(t0, std::true_type{});
+    const auto whole_rows = [&](int t0) { return c.near && dk == DK && cols == TV && last - t0 >= kChunk; };
+    const auto fetch_cut = [&](int t0) __attribute__((always_inline)) {  // one branch for all loads: each of its own waited
+        if (c.wide_in) fetch_as(t0, std::true_type{});
         else fetch_as(t0, std::false_type{});
     };
 
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
     }
     if (threadIdx.x == 0) s.poisoned = 0;
     double total = 0.;
-    if (first < last) fetch(first);
+    if (first < last) fetch_cut(first);
     for (int t0 = first; t0 < last; t0 += kChunk) {
         // sums of the decays: lane l of every wave has token l
         if (last - t0 < kChunk || dk < DK || cols < TV) cut(last - t0);
@@ -504,7 +505,10 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
             }
         }
         __syncthreads();
-        if (t0 + kChunk < last) fetch(t0 + kChunk);
+        const int t1 = t0 + kChunk;
+        const bool more = t1 < last && whole_rows(t1);
+        if (more) fetch_whole(t1, 0);
+        else if (t1 < last) fetch_cut(t1);
 
         if constexpr (kOut) {
             const double mine = s.sum[wave * 16 + lr];
@@ -522,6 +526,7 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
                 }
                 O[ct] *= before;
             }
+            if (more) fetch_whole(t1, 1);
             const bool poisoned = s.poisoned == t0 + 1;
 #pragma unroll
             for (int pair = 0; pair < 2; pair++) {
@@ -609,6 +614,10 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
                             if (e + r < cols) row[e + r] = o[r];
                 }
             }
+        }
+        if (more) {
+            if (!kOut) fetch_whole(t1, 1);
+            fetch_whole(t1, 2);
         }
 #pragma unroll
         for (int i = 0; i < ST; i++) {
@@ -706,6 +715,8 @@ auto by_type(uint32_t type, F&& f) {
 }
 
 // how a prompt is cut: by token (segments 0), or by chunks in so many segments
+// By token 12 heads of 64 take 4.2 us for one token, 9.8 for 8 and 0.9 for each more, by chunks 7.0 us for up to 64.
+constexpr uint32_t kByToken = 4;
 struct Plan {
     uint32_t tile, segments, segment;
     size_t sums_at, bytes;
@@ -713,10 +724,14 @@ struct Plan {
 
 Plan plan(const fhe_ssm_linear_attention* a) {
     Plan p{};
-    p.tile = a->type == FHE_SSM_F32 && a->dk > 64 ? 32 : 64;  // three pieces of 128 channels fill the LDS at 32 columns
-    if (a->tokens < 32 || !a->lanes) return p;
-    const uint32_t items = a->lanes * a->heads, groups = items * ((a->dv + p.tile - 1) / p.tile);
-    const uint32_t chunks = (a->tokens + kChunk - 1) / kChunk;
+    if (a->tokens <= kByToken || !a->lanes) return p;
+    const uint32_t items = a->lanes * a->heads, chunks = (a->tokens + kChunk - 1) / kChunk;
+    // 64 columns of the state to a workgroup, or 32 where that leaves the GPU empty, though their keys and scores are worked
+    // out twice (12 heads of one prompt: 64 tokens 8.3 against 7.0 us, 2,048 29.1 against 27.1; 8,192 50 against 58).  The three
+    // pieces of float32 leave LDS for two workgroups of 32 columns on a CU (4 prompts of 2,048: 79.7 against 70.4 us).
+    const uint64_t wide = (uint64_t)items * ((a->dv + 63) / 64);
+    p.tile = a->type == FHE_SSM_F32 || (wide <= 192 && wide * chunks <= 384) ? 32 : 64;
+    const uint32_t groups = items * ((a->dv + p.tile - 1) / p.tile);
     p.segments = 1;
     if (groups < 256 && chunks >= 8) p.segments = std::min(chunks, 512 / groups);
     const uint32_t each = (chunks + p.segments - 1) / p.segments;
@@ -778,9 +793,14 @@ int run(const fhe_ssm_linear_attention* a, const void* q, const void* k, const v
     const uint32_t items = a->lanes * a->heads;
     const int rc = by_type(a->type, [&](auto t) {
         typedef decltype(t) X;
-        if (a->dk <= 32) return launch_chunks<X, 32, 64>(c, items, st);
-        if (a->dk <= 64) return launch_chunks<X, 64, 64>(c, items, st);
-        return launch_chunks<X, 128, std::is_same<X, float>::value ? 32 : 64>(c, items, st);
+        if constexpr (!std::is_same<X, float>::value)
+            if (p.tile == 64)
+                return a->dk <= 32 ? launch_chunks<X, 32, 64>(c, items, st)
+                     : a->dk <= 64 ? launch_chunks<X, 64, 64>(c, items, st)
+                                   : launch_chunks<X, 128, 64>(c, items, st);
+        return a->dk <= 32 ? launch_chunks<X, 32, 32>(c, items, st)
+             : a->dk <= 64 ? launch_chunks<X, 64, 32>(c, items, st)
+                           : launch_chunks<X, 128, 32>(c, items, st);
     });
     return rc ? rc : launched("linear attention");
 }
