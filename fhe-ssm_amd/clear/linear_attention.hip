@@ -257,14 +257,32 @@ struct ChunkArgs {
     bool wide_in, wide_out, near;  // near: a chunk's rows lie within 32-bit offsets
 };
 
+// What the outputs read, keys (a token a row) and the state before the chunk (a column a row), and what the state's update
+// reads, decayed keys (a channel a row).  Of more than 64 channels the second takes the place of the first, at two barriers
+// more, so that two workgroups fit a CU (4 prompts of 2,048, heads of 128: 140 against 98 us; of 64 it costs: 32 prompts of 512
+// to 1024 78 against 89 us).
 template <class X, int DK, int TV>
-struct ChunkShared {
-    uint16_t k[Pieces<X>::in][kChunk][DK + kPad];       // keys, a token a row
-    uint16_t kt[3][DK][kChunk + kPadT];                  // decayed keys, a channel a row
-    uint16_t vt[Pieces<X>::in][TV][kChunk + kPadT];      // values, a channel a row
-    uint16_t st[Pieces<X>::mid][TV][DK + kPad];         // the state before the chunk, a column a row
+struct KeysApart {
+    uint16_t k[Pieces<X>::in][kChunk][DK + kPad];
+    uint16_t st[Pieces<X>::mid][TV][DK + kPad];
+    uint16_t kt[3][DK][kChunk + kPadT];
+};
+template <class X, int DK, int TV>
+struct KeysInTurn {
+    union {
+        struct {
+            uint16_t k[Pieces<X>::in][kChunk][DK + kPad];
+            uint16_t st[Pieces<X>::mid][TV][DK + kPad];
+        };
+        uint16_t kt[3][DK][kChunk + kPadT];
+    };
+};
+constexpr bool in_turn(int DK) { return DK > 64; }
+template <class X, int DK, int TV>
+struct ChunkShared : std::conditional<in_turn(DK), KeysInTurn<X, DK, TV>, KeysApart<X, DK, TV>>::type {
+    uint16_t vt[Pieces<X>::in][TV][kChunk + kPadT];  // values, a channel a row
     double sum[kChunk];
-    int poisoned;                                       // the last chunk (its first token + 1) with a value not finite
+    int poisoned;                                    // the last chunk (its first token + 1) with a value not finite
 };
 
 // A workgroup takes TV columns of one head's state over one segment of one lane's tokens.  Wave w has the outputs of tokens
@@ -273,7 +291,7 @@ struct ChunkShared {
 // the next one without leaving their registers: the values are read in the order of keys that this makes.
 // out: outputs from the state before the segment; otherwise what the segment adds to the state, and its log decay.
 template <class X, int DK, int TV, bool kOut>
-__global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
+__global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>) * 2 <= 160 << 10 ? 2 : 1)) void k_chunks(ChunkArgs c) {
     constexpr int P = Pieces<X>::in, M = Pieces<X>::mid, KK = DK / 32, CT = TV / 16, ST = DK / 16 * CT / 4;
     constexpr int kKeyBlocks = DK * kChunk / 16 / 256 ? DK * kChunk / 16 / 256 : 1;  // 4 x 4 blocks of a thread
     constexpr int kValueBlocks = TV * kChunk / 16 / 256 ? TV * kChunk / 16 / 256 : 1;
@@ -425,15 +443,12 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
         const float weight = power((float)(whole - sum)), all = power((float)whole);
         __syncthreads();  // the chunk before has been read
         if (threadIdx.x < kChunk) s.sum[l] = sum;
+        if constexpr (kOut) {
 #pragma unroll
-        for (int b = 0; b < kKeyBlocks; b++) {
-            int t, d;
-            block(b, DK, t, d);
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = __shfl(weight, (t + i) % kChunk);
-            if (t < kChunk) {
-                if constexpr (kOut) {
+            for (int b = 0; b < kKeyBlocks; b++) {
+                int t, d;
+                block(b, DK, t, d);
+                if (t < kChunk) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         u32x2 piece[P];
@@ -442,16 +457,30 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
                         for (int p = 0; p < P; p++) *(u32x2*)&s.k[p][t + i][d] = piece[p];
                     }
                 }
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float f[4] = {kx[b][0][e] * w[0], kx[b][1][e] * w[1], kx[b][2][e] * w[2], kx[b][3][e] * w[3]};
-                    u32x2 piece[3];
-                    split4(f, piece);
-#pragma unroll
-                    for (int p = 0; p < 3; p++) *(u32x2*)&s.kt[p][d + e][t] = piece[p];
-                }
             }
         }
+        const auto decayed_keys = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int b = 0; b < kKeyBlocks; b++) {
+                int t, d;
+                block(b, DK, t, d);
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = __shfl(weight, (t + i) % kChunk);
+                if (t < kChunk) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float f[4] = {kx[b][0][e] * w[0], kx[b][1][e] * w[1], kx[b][2][e] * w[2], kx[b][3][e] * w[3]};
+                        u32x2 piece[3];
+                        split4(f, piece);
+#pragma unroll
+                        for (int p = 0; p < 3; p++) *(u32x2*)&s.kt[p][d + e][t] = piece[p];
+                    }
+                }
+            }
+        };
+        constexpr bool kLater = kOut && in_turn(DK);
+        if constexpr (!kLater) decayed_keys();
         bool odd = false;
 #pragma unroll
         for (int b = 0; b < kValueBlocks; b++) {
@@ -507,8 +536,10 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
         __syncthreads();
         const int t1 = t0 + kChunk;
         const bool more = t1 < last && whole_rows(t1);
-        if (more) fetch_whole(t1, 0);
-        else if (t1 < last) fetch_cut(t1);
+        if (!kLater) {
+            if (more) fetch_whole(t1, 0);
+            else if (t1 < last) fetch_cut(t1);
+        }
 
         if constexpr (kOut) {
             const double mine = s.sum[wave * 16 + lr];
@@ -615,10 +646,17 @@ __global__ __launch_bounds__(256) void k_chunks(ChunkArgs c) {
                 }
             }
         }
+        if constexpr (kLater) {
+            __syncthreads();  // keys and state have been read
+            decayed_keys();
+        }
         if (more) {
             if (!kOut) fetch_whole(t1, 1);
             fetch_whole(t1, 2);
-        }
+            if (kLater) fetch_whole(t1, 0);
+        } else if (kLater && t1 < last)
+            fetch_cut(t1);
+        if (kLater) __syncthreads();
 #pragma unroll
         for (int i = 0; i < ST; i++) {
             S[i] *= all;
