@@ -101,13 +101,20 @@ def _type(t) -> int:
     return code
 
 
+_names: dict = {}
+
+
 def _is(t, dtype: str) -> bool:
-    return str(t.dtype) == dtype
+    name = _names.get(t.dtype)
+    if name is None:
+        name = _names[t.dtype] = str(t.dtype)
+    return name == dtype
 
 
 def _on_device(*tensors) -> None:
     for t in tensors:
-        _need(t is None or t.is_cuda, "tensors must be on the GPU")
+        if t is not None and not t.is_cuda:
+            raise ClearError("tensors must be on the GPU")
 
 
 def _ptr(t):
@@ -284,8 +291,8 @@ def sample(logits, draws, tokens, logprobs=None, temperature=None, top_k=None, t
                            ("logprobs", logprobs, "torch.float32"), ("temperature", temperature, "torch.float32"),
                            ("top_k", top_k, "torch.int32"), ("top_p", top_p, "torch.float32"),
                            ("min_p", min_p, "torch.float32")):
-        _need(t is None or (_is(t, dtype) and t.shape == (rows,) and t.is_contiguous()),
-              f"{name} must be contiguous {dtype[6:]} [{rows}]")
+        if t is not None and not (_is(t, dtype) and t.shape == (rows,) and t.is_contiguous()):
+            raise ClearError(f"{name} must be contiguous {dtype[6:]} [{rows}]")
     p = SampleParams(_ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p))
     check(load().fhe_ssm_sample(_type(logits), logits.data_ptr(), rows, vocab, stride[0], draws.data_ptr(),
                                 ctypes.addressof(p), tokens.data_ptr(), _ptr(logprobs), stream))
