@@ -131,11 +131,16 @@ template <class X, bool kPacked>
 constexpr int kProducts = std::is_same<X, float>::value && !kPacked ? 3 : 1;  // of an operand pair
 template <class X, bool kPacked>
 constexpr int kAheadOf = kProducts<X, kPacked> == 1 ? 4 : 2;  // A
+// Sums of a group: of three products the first has one of its own, as its terms are short and their sum, and what the zero
+// point takes out of it, hardly round (46 rows of 1,231 columns in groups of 128 are off by 1.8e-7, with one sum by 1.3e-6;
+// 64 rows times 4,096 x 4,096 take 37.8 against 34.9 us).
+template <class X, bool kPacked>
+constexpr int kSums = kProducts<X, kPacked> == 3 ? 2 : 1;
 
 template <class X, Kind K, int F, int C, bool kPacked>
 __global__ __launch_bounds__(64 * kWaves) void k_product(Q4Args a) {
     typedef typename std::conditional<std::is_same<X, f16>::value, f16, bf16>::type E;
-    constexpr int P = kProducts<X, kPacked>, A = kAheadOf<X, kPacked>, kFrag = 4 * C * P;  // operands of a block
+    constexpr int P = kProducts<X, kPacked>, A = kAheadOf<X, kPacked>, Q = kSums<X, kPacked>, kFrag = 4 * C * P;  // operands of a block
     constexpr int kParts = std::is_same<X, float>::value ? 3 : 1;
     typedef typename Codes<E>::vec vec;
     extern __shared__ __attribute__((aligned(16))) char s_bytes[];
@@ -144,7 +149,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_product(Q4Args a) {
     const uint32_t tile = blockIdx.x * tiles_at + wave / a.splits, row0 = blockIdx.y * (16 * C);
     const uint32_t from = min(split * a.per_wave, a.blocks), to = min(from + a.per_wave, a.blocks);
     vec* s_x = (vec*)s_bytes;                                        // [split][block of the chunk][j][c][p][lane]
-    float* s_one = (float*)(s_x + a.splits * chunk * kFrag * 64);    // [split][block of the chunk][f][c][row]
+    float* s_one = (float*)(s_x + a.splits * chunk * kFrag * 64);    // [split][block of the chunk][f][sum][c][row]
 
     uint32_t mask = Codes<E>::mask, sixteen = Codes<E>::sixteen;
     asm("" : "+s"(mask));
@@ -171,9 +176,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_product(Q4Args a) {
     const auto use = [&](int slot, uint32_t sb) __attribute__((always_inline)) {  // sb: the block's place in LDS
 #pragma unroll
         for (int f = 0; f < F; f++) {
-            f32x4 sum[C];
+            f32x4 sum[Q][C];
 #pragma unroll
-            for (int c = 0; c < C; c++) sum[c] = f32x4{0, 0, 0, 0};
+            for (int c = 0; c < Q * C; c++) sum[c / C][c % C] = f32x4{0, 0, 0, 0};
             // all operands of the group are asked for before the first is waited for
             vec x[4 / F][C][P];
 #pragma unroll
@@ -189,15 +194,23 @@ __global__ __launch_bounds__(64 * kWaves) void k_product(Q4Args a) {
 #pragma unroll
                 for (int c = 0; c < C; c++)
 #pragma unroll
-                    for (int p = P - 1; p >= 0; p--) sum[c] = Codes<E>::mma(code, x[j][c][p], sum[c]);
+                    for (int p = P - 1; p >= 0; p--) sum[min(p, Q - 1)][c] = Codes<E>::mma(code, x[j][c][p], sum[min(p, Q - 1)][c]);
             }
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                const float one = s_one[((size_t)sb * F + f) * (16 * C) + c * 16 + l % 16];
+                float one[Q];
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    total[c][i] = fmaf(g[slot].scale(i, f), K == kHalf ? sum[c][i] + one : fmaf(-g[slot].zero(i, f), one, sum[c][i]),
-                                       total[c][i]);
+                for (int n = 0; n < Q; n++) one[n] = s_one[((size_t)sb * F + f) * (16 * C * Q) + (n * C + c) * 16 + l % 16];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float centred = 0.f;
+#pragma unroll
+                    for (int n = Q - 1; n >= 0; n--) {
+                        const float x = K == kHalf ? sum[n][c][i] + one[n] : fmaf(-g[slot].zero(i, f), one[n], sum[n][c][i]);
+                        centred = n == Q - 1 ? x : x + centred;
+                    }
+                    total[c][i] = fmaf(g[slot].scale(i, f), centred, total[c][i]);
+                }
             }
         }
     };
@@ -213,9 +226,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_product(Q4Args a) {
             Eight<X> raw[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) raw[j].load(x, b * kBlock + j * 32 + l / 16 * 8, a.in, a.wide_x);
-            f32x4 one[F];  // a product with ones sums a row over all lanes that have a part of it
+            f32x4 one[Q][F];  // a product with ones sums a row over all lanes that have a part of it
 #pragma unroll
-            for (int f = 0; f < F; f++) one[f] = f32x4{0, 0, 0, 0};
+            for (int f = 0; f < Q * F; f++) one[f / F][f % F] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 vec parts[kParts], mine[P];
@@ -225,13 +238,16 @@ __global__ __launch_bounds__(64 * kWaves) void k_product(Q4Args a) {
 #pragma unroll
                     for (int p = 0; p < P; p++) mine[p] = parts[p];
 #pragma unroll
-                for (int p = P - 1; p >= 0; p--) one[j * F / 4] = Codes<E>::mma(ones, mine[p], one[j * F / 4]);
+                for (int p = P - 1; p >= 0; p--) one[min(p, Q - 1)][j * F / 4] = Codes<E>::mma(ones, mine[p], one[min(p, Q - 1)][j * F / 4]);
 #pragma unroll
                 for (int p = 0; p < P; p++) s_x[((size_t)sb * kFrag + (j * C + c) * P + p) * 64 + l] = mine[p];
             }
 #pragma unroll
             for (int f = 0; f < F; f++)
-                if (l < 16) s_one[((size_t)sb * F + f) * (16 * C) + c * 16 + l] = K == kHalf ? -24.f * one[f][0] : one[f][0];
+#pragma unroll
+                for (int n = 0; n < Q; n++)
+                    if (l < 16)
+                        s_one[((size_t)sb * F + f) * (16 * C * Q) + (n * C + c) * 16 + l] = K == kHalf ? -24.f * one[n][f][0] : one[n][f][0];
         }
         __syncthreads();
         const uint32_t begin = min(from + b0, to), end = min(to, from + b0 + chunk), at = split * chunk;
@@ -295,24 +311,24 @@ int launch_rows(const Q4Args& a, hipStream_t st) {
     const uint32_t row_tiles = (a.rows + 15) / 16;
     const bool packed = kFloats && a.rows <= kPackedRows;
     const uint32_t P = kFloats && !packed ? 3 : 1, A = P == 1 ? 4 : 2;
-    const auto frag = [&](uint32_t C) { return C * (4096 * P + 64 * F); };  // of a block in LDS
+    const auto frag = [&](uint32_t C) { return C * (4096 * P + 64 * F * (P == 3 ? 2 : 1)); };  // of a block in LDS
     // the columns are split until there are 2,048 waves, as far as A blocks of each split fit the LDS
     const auto splits = [&](uint32_t C) {
         const uint32_t groups = (row_tiles + C - 1) / C;
         uint32_t n = 1;
-        while (n < kWaves && a.tiles * groups * n < 2048 && 2 * n <= a.blocks && 2 * n * A * frag(C) <= kMostLds) n *= 2;
+        while (n < kWaves && (uint64_t)a.tiles * groups * n < 2048 && 2 * n <= a.blocks && 2 * n * A * frag(C) <= kMostLds) n *= 2;
         return n;
     };
     // 16 C rows share a read of the weights; fewer where that alone leaves the GPU empty
     uint32_t C = row_tiles > 2 ? 4 : row_tiles;
-    while (C > 1 && a.tiles * ((row_tiles + C - 1) / C) * splits(C) < 1024) C /= 2;
+    while (C > 1 && (uint64_t)a.tiles * ((row_tiles + C - 1) / C) * splits(C) < 1024) C /= 2;
     const auto go = [&](auto kernel) -> int {
         Q4Args b = a;
         b.splits = splits(C);
         b.per_wave = (a.blocks + b.splits - 1) / b.splits;
         const uint32_t each = kWaves / b.splits;
         const dim3 grid((a.tiles + each - 1) / each, (row_tiles + C - 1) / C);
-        const uint32_t room = grid.x * grid.y <= kCus ? kMostLds : kLds;  // one workgroup a CU, or two
+        const uint32_t room = (uint64_t)grid.x * grid.y <= kCus ? kMostLds : kLds;  // one workgroup a CU, or two
         b.chunk = std::min(b.per_wave, std::max(A, room / (b.splits * frag(C)) / A * A));
         const uint32_t bytes = std::max(b.splits * b.chunk * frag(C), b.splits > 1 ? kWaves * C * 1024 : 0u);
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
