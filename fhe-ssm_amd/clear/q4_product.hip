@@ -26,7 +26,7 @@ Layout layout(const fhe_ssm_q4_matrix& m) {
     Layout y;
     y.tiles = (m.out + kRowTile - 1) / kRowTile;
     y.blocks = (m.in + kBlock - 1) / kBlock;
-    y.groups_given = (m.in + m.group - 1) / m.group;
+    y.groups_given = (m.in - 1) / m.group + 1;
     y.each = m.group < kBlock ? kBlock / m.group : 1;
     y.groups = m.group < kBlock ? y.blocks * y.each : y.groups_given;  // whole blocks of small groups
     y.kind = m.scale_type != FHE_SSM_F16 ? kFloat : m.has_zeros ? kHalfZero : kHalf;
@@ -47,7 +47,16 @@ __global__ __launch_bounds__(256) void k_arrange_codes(const uint8_t* __restrict
     const size_t tb = at / 256;
     const uint32_t row = (uint32_t)(tb / blocks) * kRowTile + l % 16, col = (uint32_t)(tb % blocks) * kBlock + j * 32 + l / 16 * 8;
     uint32_t w = 0;
-    if (row < out) {
+    if (row < out && col + 8 <= in) {
+        uint32_t given;
+        __builtin_memcpy(&given, codes + (int64_t)row * stride + col / 2, 4);
+        const auto every_other = [](uint32_t c) {
+            c &= 0x0f0f0f0fu;
+            c = (c | c >> 4) & 0x00ff00ffu;
+            return (c | c >> 8) & 0xffffu;
+        };
+        w = every_other(given) | every_other(given >> 4) << 16;
+    } else if (row < out) {
         for (uint32_t i = 0; i < 8; i++) {
             if (col + i >= in) break;
             const uint32_t c = codes[(int64_t)row * stride + (col + i) / 2] >> (i % 2 * 4) & 15;
@@ -87,7 +96,7 @@ int check(const fhe_ssm_q4_matrix* m) {
         return fail(CKKS_EINVAL, "4-bit product: group %u is none of 32, 64 and the multiples of 128", m->group);
     if (m->scale_type > FHE_SSM_F16) return fail(CKKS_EINVAL, "4-bit product: unknown type of scales %u", m->scale_type);
     const Layout y = layout(*m);
-    if ((uint64_t)y.tiles * y.blocks > 0x7fffffffull || (uint64_t)y.tiles * y.groups > 0x7fffffffull)
+    if ((uint64_t)y.tiles * y.blocks > 0xffffffull)  // a launch has less than 2^32 threads
         return fail(CKKS_EINVAL, "4-bit product: the matrix is too large");
     return CKKS_OK;
 }

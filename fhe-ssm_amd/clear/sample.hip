@@ -621,7 +621,7 @@ extern "C" int fhe_ssm_sample(uint32_t type, const void* logits, uint32_t rows, 
     using namespace clear;
     if (type > FHE_SSM_F16) return fail(CKKS_EINVAL, "sample: unknown type %u", type);
     if (vocab < 1 || vocab > kMostVocab) return fail(CKKS_EINVAL, "sample: a vocabulary of %u is not in [1, %u]", vocab, kMostVocab);
-    if (rows > 0x7fffffffu) return fail(CKKS_EINVAL, "sample: too many rows");
+    if (rows > 0x3fffffu) return fail(CKKS_EINVAL, "sample: too many rows");  // a launch has less than 2^32 threads
     if (rows == 0) return CKKS_OK;
     if (!logits || !draws || !params || !tokens) return fail(CKKS_EINVAL, "sample: null argument");
     if (row_stride < 0) return fail(CKKS_EINVAL, "sample: negative stride");

@@ -149,3 +149,17 @@ def test_quantize_q4_of_a_zero_matrix():
     ops, _ = clear()
     codes, scales, _ = ops.quantize_q4(np.zeros((2, 40), np.float32), 32)
     assert (codes == 0x88).all() and np.isfinite(scales.astype(np.float32)).all() and (scales > 0).all()
+
+
+def test_sizes_that_pass_32_bits_are_refused():
+    """counts of workgroups and groups near 2^32, which must not wrap around"""
+    ops, lib = clear()
+    n = ctypes.c_size_t()
+    for change in (dict(dv=0xffffffff), dict(dv=0xffffffe1), dict(lanes=1 << 22, heads=8, q_heads=2, k_heads=2)):
+        refused(lib, lib.fhe_ssm_linear_attention_workspace(attention_sizes(ops, **change), ctypes.byref(n)), "too many")
+    refused(lib, lib.fhe_ssm_q4_bytes(ctypes.byref(ops.Q4Sizes(1 << 20, 1 << 19, 128, 0, 0)), ctypes.byref(n)), "too large")
+    # a group far longer than a row: one group a row
+    one, far = ctypes.c_size_t(), ctypes.c_size_t()
+    assert lib.fhe_ssm_q4_bytes(ctypes.byref(ops.Q4Sizes(16, 256, 256, 0, 0)), ctypes.byref(one)) == 0
+    assert lib.fhe_ssm_q4_bytes(ctypes.byref(ops.Q4Sizes(16, 256, 0xffffff80, 0, 0)), ctypes.byref(far)) == 0
+    assert far.value == one.value
