@@ -674,7 +674,8 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
         for (int e = threadIdx.x; e < (end - zero) * TV; e += 256)
             if (e % TV < cols) out[(int64_t)(zero + e / TV) * a.os[1] + e % TV] = (X)0.f;
     }
-    float* into = kOut ? (c.segments == 1 ? a.state_out : nullptr) : c.joint;
+    float* into = kOut ? (seg + 1 == c.segments ? a.state_out : nullptr) : c.joint;
+    const size_t into_at = kOut ? (size_t)item * a.dk * a.dv : part;
     if (into) {
 #pragma unroll
         for (int i = 0; i < ST; i++)
@@ -682,36 +683,38 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int d = d0(i) + lg * 4 + r;
-                    if (d < dk) into[part + (size_t)d * a.dv + col0 + c0(i) + lr] = S[i][r];
+                    if (d < dk) into[into_at + (size_t)d * a.dv + col0 + c0(i) + lr] = S[i][r];
                 }
             }
     }
     if (!kOut && tile == 0 && threadIdx.x == 0) c.sums[(size_t)seg * items + item] = total;
 }
 
-// what each segment adds becomes the state before it, along the segments; the state after the last one is the result
-__global__ __launch_bounds__(256) void k_join(ChunkArgs c, uint32_t items) {
-    const size_t square = (size_t)c.a.dk * c.a.dv, at = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= items * square) return;
-    const size_t item = at / square;
+// What each segment but the last adds becomes the state before it, along the segments; the last one's is stored behind them.
+// 64 threads and one head a workgroup, so that the segments' decays are read once by each wave (2 lanes of 12 heads, 32
+// segments, 12.6 MB read and written).  kBatch: loads in flight, past the last segment the last again.
+constexpr int kJoinThreads = 64;
+template <uint32_t kBatch>
+__global__ __launch_bounds__(kJoinThreads) void k_join(ChunkArgs c) {
+    const uint32_t square = c.a.dk * c.a.dv, e = blockIdx.x * kJoinThreads + threadIdx.x, item = blockIdx.y, items = gridDim.y;
+    if (e >= square) return;
+    const size_t at = (size_t)item * square + e, each = (size_t)items * square;
     float S = c.a.state_in ? c.a.state_in[at] : 0.f;
-    constexpr uint32_t kBatch = 16;  // loads in flight
     for (uint32_t s0 = 0; s0 < c.segments; s0 += kBatch) {
         float add[kBatch], decay[kBatch];
 #pragma unroll
-        for (uint32_t i = 0; i < kBatch; i++)
-            if (s0 + i < c.segments) {
-                add[i] = c.joint[(s0 + i) * items * square + at];
-                decay[i] = power((float)c.sums[(s0 + i) * items + item]);
-            }
+        for (uint32_t i = 0; i < kBatch; i++) {
+            const uint32_t s = min(s0 + i, c.segments - 2);
+            add[i] = c.joint[s * each + at];
+            decay[i] = power((float)c.sums[(size_t)s * items + item]);
+        }
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; i++)
             if (s0 + i < c.segments) {
-                c.joint[(s0 + i) * items * square + at] = S;
+                c.joint[(s0 + i) * each + at] = S;
                 S = fmaf(decay[i], S, add[i]);
             }
     }
-    if (c.a.state_out) c.a.state_out[at] = S;
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -782,20 +785,23 @@ Plan plan(const fhe_ssm_linear_attention* a) {
 
 template <class X, int DK, int TV>
 int launch_chunks(const ChunkArgs& c, uint32_t items, hipStream_t st) {
-    const uint32_t grid = items * c.a.tiles * c.segments, bytes = sizeof(ChunkShared<X, DK, TV>);
+    const uint32_t bytes = sizeof(ChunkShared<X, DK, TV>);
     // LDS past 64 KB is asked for by name
-    const auto go = [&](auto kernel) -> int {
+    const auto go = [&](auto kernel, const ChunkArgs& c) -> int {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != hipSuccess) return fail(CKKS_EHIP, "linear attention: %s", hipGetErrorString(e));
-        hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), bytes, st, c);
+        hipLaunchKernelGGL(kernel, dim3(items * c.a.tiles * c.segments), dim3(256), bytes, st, c);
         return CKKS_OK;
     };
     if (c.segments > 1) {
-        if (int rc = go(k_chunks<X, DK, TV, false>)) return rc;
-        const size_t n = (size_t)items * c.a.dk * c.a.dv;
-        hipLaunchKernelGGL(k_join, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, c, items);
+        ChunkArgs before = c;  // what the last segment adds, nothing reads
+        before.segments--;
+        if (int rc = go(k_chunks<X, DK, TV, false>, before)) return rc;
+        const uint32_t square = c.a.dk * c.a.dv;
+        hipLaunchKernelGGL(c.segments > 9 ? k_join<32> : k_join<8>, dim3((square + kJoinThreads - 1) / kJoinThreads, items),
+                           dim3(kJoinThreads), 0, st, c);
     }
-    return go(k_chunks<X, DK, TV, true>);
+    return go(k_chunks<X, DK, TV, true>, c);
 }
 
 int run(const fhe_ssm_linear_attention* a, const void* q, const void* k, const void* v, const float* g,
