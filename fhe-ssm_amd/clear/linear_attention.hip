@@ -33,7 +33,7 @@ __device__ inline float floored(float g) { return g < kFloor ? kFloor : g; }  //
 // Token by token, the state in registers.  A workgroup holds 64 columns of one head's state (columns never meet); its four
 // waves and their lanes share the rows: a lane holds V columns of R rows.  o_t is the sum over rows: lanes of a wave by
 // shuffles, waves through LDS.  For up to four tokens; it is bound by its launch and by reading and writing the state once:
-// 32 lanes of 12 heads of 64, 12.6 MB, take 5.3 us in the kernel, one lane 4.2.
+// 32 lanes of 12 heads of 64, 6.3 MB read and written, take 5.1 us in the kernel, one lane 4.2.
 template <class T, int V, int R>
 __global__ __launch_bounds__(kWaves * 64) void k_recurrent(Args a) {
     constexpr int kColLanes = kCols / V, kRowLanes = 64 / kColLanes, kStep = kWaves * kRowLanes, kRows = kStep * R;
@@ -257,7 +257,7 @@ struct ChunkArgs {
 
 // What the outputs read, keys (a token a row) and the state before the chunk (a column a row), and what the state's update
 // reads, decayed keys (a channel a row).  Of more than 64 channels the second takes the place of the first, at two barriers
-// more, so that two workgroups fit a CU (4 prompts of 2,048, heads of 128: 140 against 98 us; of 64 it costs: 32 prompts of 512
+// more, so that two workgroups fit a CU (4 prompts of 2,048, heads of 128: 140 against 97 us; of 64 it costs: 32 prompts of 512
 // to 1024 78 against 89 us).
 template <class X, int DK, int TV>
 struct KeysApart {
@@ -287,7 +287,10 @@ struct ChunkShared : std::conditional<in_turn(DK), KeysInTurn<X, DK, TV>, KeysAp
 // 16 w .. 16 w + 15 of a chunk (transposed: a lane has one token and four neighbouring channels) and a quarter of the state's
 // 16 x 16 tiles.  The scores of a token, as they come out of one product (a lane: one query, four neighbouring keys), go into
 // the next one without leaving their registers: the values are read in the order of keys that this makes.
-// out: outputs from the state before the segment; otherwise what the segment adds to the state, and its log decay.
+// kOut: outputs from the state before the segment; otherwise what the segment adds to the state, and its log decay.
+// It is bound by the latency of a chunk's chain (decays, LDS, scores, outputs, state; about 9,400 cycles, in which the vector
+// units are busy for a third and the matrix units for a tenth): 32 prompts of 512 to 1,024 tokens, 12 heads of 64, 120 MB,
+// take 80 us; one of 8,192 tokens 47 us, 14 of them for what segments add, 6.5 to join them and 27 for the outputs.
 template <class X, int DK, int TV, bool kOut>
 __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>) * 2 <= 160 << 10 ? 2 : 1)) void k_chunks(ChunkArgs c) {
     constexpr int P = Pieces<X>::in, M = Pieces<X>::mid, KK = DK / 32, CT = TV / 16, ST = DK / 16 * CT / 4;
@@ -691,8 +694,8 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
 }
 
 // What each segment but the last adds becomes the state before it, along the segments; the last one's is stored behind them.
-// 64 threads and one head a workgroup, so that the segments' decays are read once by each wave (2 lanes of 12 heads, 32
-// segments, 12.6 MB read and written).  kBatch: loads in flight, past the last segment the last again.
+// 64 threads and one head a workgroup, so that the segments' decays are read once by each wave (12 heads, 32 segments,
+// 6.3 MB read and written: 6.5 us, of it about 2.5 the launch).  kBatch: loads in flight, past the last segment the last again.
 constexpr int kJoinThreads = 64;
 template <uint32_t kBatch>
 __global__ __launch_bounds__(kJoinThreads) void k_join(ChunkArgs c) {
@@ -766,13 +769,16 @@ Plan plan(const fhe_ssm_linear_attention* a) {
     if (a->tokens <= (uint32_t)kByToken || !a->lanes) return p;
     const uint32_t items = a->lanes * a->heads, chunks = (a->tokens + kChunk - 1) / kChunk;
     // 64 columns of the state to a workgroup, or 32 where that leaves the GPU empty, though their keys and scores are worked
-    // out twice (12 heads of one prompt: 64 tokens 8.3 against 7.0 us, 2,048 29.1 against 27.1; 8,192 50 against 58).  The three
-    // pieces of float32 leave LDS for two workgroups of 32 columns on a CU (4 prompts of 2,048: 79.7 against 70.4 us).
+    // out twice (12 heads of one prompt: 64 tokens 8.3 against 7.0 us, 2,048 29.1 against 27.1; 8,192 50 against 58).  The
+    // three pieces of float32 leave LDS for two workgroups of 32 columns on a CU (4 prompts of 2,048: 79.7 against 70.4 us).
     const uint64_t wide = (uint64_t)items * ((a->dv + 63) / 64);
     p.tile = a->type == FHE_SSM_F32 || (wide <= 192 && wide * chunks <= 384) ? 32 : 64;
     const uint32_t groups = items * ((a->dv + p.tile - 1) / p.tile);
     p.segments = 1;
-    if (groups < 256 && chunks >= 8) p.segments = std::min(chunks, 512 / groups);
+    // the chunks of a prompt one after the other, or in segments on 512 workgroups, with two launches more (12 heads of one
+    // prompt: 256 tokens 15.8 against 13.8 us, 8,192 450 against 47, on 1,024 workgroups 51.6; 32 ragged prompts, which are
+    // 384 workgroups in themselves, 80 against 126)
+    if (groups < 256 && chunks >= 4) p.segments = std::min(chunks, 512 / groups);
     const uint32_t each = (chunks + p.segments - 1) / p.segments;
     p.segment = each * kChunk;
     p.segments = (chunks + each - 1) / each;

@@ -121,9 +121,14 @@ struct Groups {
 // A workgroup's eight waves take 8 / splits tiles of 16 outputs, for 16 C rows of x, and share the columns by `splits`.  x goes
 // through LDS in chunks of blocks, as the operands that the matrix instructions take, with each group's sum of x.  Weights
 // come from memory A blocks ahead of their use, in a loop without branches: past one the compiler no longer knows how many
-// loads are under way, and waits for nearly all of them (the head for 32 rows took 11.3 us so).
+// loads are under way, and waits for nearly all of them.  (Six or eight blocks ahead leave room for fewer waves: 16 rows times
+// 16,384 x 8,192 21.6 us, 64 rows 67.7 against 52.5; two blocks of x under way while they are laid out, 32 rows of a head
+// 14.5 against 11.4: more registers and more code that runs once.)
+// It is bound by the weights' way from memory, and for a head by the first and last microseconds of a launch: 65,536 x 768 (27
+// MB with scales) 7.6 us for one row, 11.4 for 32; 16,384 x 8,192 (69 MB) 18.7 us for one row, 3.6 TB/s, 22.6 for 16, 52.5 for
+// 64, a third of the rate of a large matrix product.
 // F: groups of a block of 128 columns.  kPacked: up to five float32 rows, whose three parts are the columns of one tile and are
-// summed at the end, instead of three products each.
+// summed at the end, instead of three products each (one row of a head 8.9 against 11.3 us).
 constexpr int kWaves = 8;
 constexpr uint32_t kPackedRows = 5, kCus = 256;
 constexpr uint32_t kLds = 64 << 10, kMostLds = 150 << 10;  // of a workgroup: two a CU, or one where it has to be
@@ -312,14 +317,16 @@ int launch_rows(const Q4Args& a, hipStream_t st) {
     const bool packed = kFloats && a.rows <= kPackedRows;
     const uint32_t P = kFloats && !packed ? 3 : 1, A = P == 1 ? 4 : 2;
     const auto frag = [&](uint32_t C) { return C * (4096 * P + 64 * F * (P == 3 ? 2 : 1)); };  // of a block in LDS
-    // the columns are split until there are 2,048 waves, as far as A blocks of each split fit the LDS
+    // the columns are split until there are 2,048 waves (16 rows times 16,384 x 8,192: 22.6 us; 1,024 or 4,096 waves: 26.0), as
+    // far as A blocks of each split fit the LDS
     const auto splits = [&](uint32_t C) {
         const uint32_t groups = (row_tiles + C - 1) / C;
         uint32_t n = 1;
         while (n < kWaves && (uint64_t)a.tiles * groups * n < 2048 && 2 * n <= a.blocks && 2 * n * A * frag(C) <= kMostLds) n *= 2;
         return n;
     };
-    // 16 C rows share a read of the weights; fewer where that alone leaves the GPU empty
+    // 16 C rows share a read of the weights; fewer where that alone leaves the GPU empty (64 float32 rows times 4,096 x 4,096:
+    // 37.8 against 91.4 us)
     uint32_t C = row_tiles > 2 ? 4 : row_tiles;
     while (C > 1 && (uint64_t)a.tiles * ((row_tiles + C - 1) / C) * splits(C) < 1024) C /= 2;
     const auto go = [&](auto kernel) -> int {
@@ -328,7 +335,7 @@ int launch_rows(const Q4Args& a, hipStream_t st) {
         b.per_wave = (a.blocks + b.splits - 1) / b.splits;
         const uint32_t each = kWaves / b.splits;
         const dim3 grid((a.tiles + each - 1) / each, (row_tiles + C - 1) / C);
-        const uint32_t room = (uint64_t)grid.x * grid.y <= kCus ? kMostLds : kLds;  // one workgroup a CU, or two
+        const uint32_t room = (uint64_t)grid.x * grid.y <= kCus ? kMostLds : kLds;  // one workgroup a CU, or two (16 rows, 16,384 x 8,192: 22.6, 26.8 us)
         b.chunk = std::min(b.per_wave, std::max(A, room / (b.splits * frag(C)) / A * A));
         const uint32_t bytes = std::max(b.splits * b.chunk * frag(C), b.splits > 1 ? kWaves * C * 1024 : 0u);
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);

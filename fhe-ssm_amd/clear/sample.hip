@@ -12,6 +12,10 @@
 // keep few entries go by a list: the largest logits of the 1,024 threads already hold k entries (or a nucleus' mass), so the
 // smallest of those that do bounds the list from below, and what lies above it, a few more than are kept, is ranked entry
 // against entry.  Filters that keep many go by a histogram of d, and by the entries of the bin where they end.
+//
+// It is bound by the vector instructions of a row's passes on its one CU: of 65,536 float32 logits 5 us for the largest and the
+// whole weight, 3 for a list; 9 for the histogram, 11 for its bin and the weight before it, 2 to find the draw.  A row without
+// filters takes 9.7 us, 40 entries 11.5, a nucleus from a list 13.5, from the histogram 33; 32 rows take as long as one.
 #include <algorithm>
 
 #include "clear.hpp"
