@@ -176,14 +176,14 @@ def _described(q, k, v, g, state_in, state_out, out, scale, tokens_axis):
         if len(_attention) >= 256:
             _attention.clear()
         a = _attention[key] = _describe(q, k, v, g, state_in, state_out, out, scale, tokens_axis)
-    return a[1]
+    return a  # the description, which its caller holds while it is used, and its address
 
 
 def linear_attention_workspace(q, k, v) -> int:
     """device bytes that linear_attention_prompt needs for tensors of these shapes (0 for many)"""
     n = _size()
-    check(load().fhe_ssm_linear_attention_workspace(_described(q, k, v, None, None, None, None, 1.0, True),
-                                                    ctypes.byref(n)))
+    a = _described(q, k, v, None, None, None, None, 1.0, True)
+    check(load().fhe_ssm_linear_attention_workspace(a[1], ctypes.byref(n)))
     return n.value
 
 
@@ -201,7 +201,7 @@ def linear_attention_prompt(q, k, v, log_decay, state_in, state_out, out, scale:
               "lengths must be contiguous int32 [lanes]")
     a = _described(q, k, v, log_decay, state_in, state_out, out, scale, True)
     check(load().fhe_ssm_linear_attention_prompt(
-        a, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(lengths), _ptr(state_in), _ptr(state_out),
+        a[1], q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(lengths), _ptr(state_in), _ptr(state_out),
         out.data_ptr(), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), stream))
 
 
@@ -209,7 +209,7 @@ def linear_attention_step(q, k, v, log_decay, state_in, state_out, out, scale: f
     """linear_attention_prompt for one token of every lane: the same tensors without the token axis"""
     _on_device(q, k, v, log_decay, state_in, state_out, out)
     a = _described(q, k, v, log_decay, state_in, state_out, out, scale, False)
-    check(load().fhe_ssm_linear_attention_step(a, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+    check(load().fhe_ssm_linear_attention_step(a[1], q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
                                                _ptr(state_in), _ptr(state_out), out.data_ptr(), stream))
 
 
