@@ -43,7 +43,8 @@ const char* fhe_ssm_clear_last_error(void);
  * Strides are in elements, in the order lane, token, head, and may be any (0 shares one row among many), except that
  * different output rows must not overlap; channels are contiguous.  State: [lanes][heads][dk][dv], contiguous;
  * state_in null means zero, state_out null drops the new state, and the two may be the same buffer.  out must overlap
- * no input.  A decay of -inf clears a finite state; one below -1000 is taken as that. */
+ * no input.  A decay of -inf clears a finite state; one below -1000 is taken as that.  What is not finite in an input
+ * reaches its own lane's heads from its token on, and nothing before; there an infinity may come out as NaN. */
 typedef struct {
     uint32_t type; /* of q, k, v and out */
     uint32_t lanes, tokens, heads, q_heads, k_heads, dk, dv;
