@@ -143,28 +143,19 @@ void launch_recurrent(const Args& a, uint32_t grid, hipStream_t st) {
 // The sums of decays and their differences are taken in 64 bits (in units of log 2): in 32 bits a chunk of strong decays would
 // lose what its neighbouring tokens have in common.  Matrix operands are bf16 pieces of a value, each the upper 8 bits of what
 // the ones before it left: one piece is a bf16 input, two a float16 one, three a float32 one, so products of inputs are exact.
-// Decayed keys go into the state as three pieces (24 bits, as the state is held).  The scores and the state that the outputs
-// read go in as three pieces for float32 outputs and as two (17 bits, the last rounded) for the 16-bit ones, whose own
-// rounding is 2^5 to 2^8 times that.
+// What is held in float32, the state, the scores and the decayed keys, goes in as three pieces for every type: with two the
+// outputs of states and scores that cancel would be off by more than the rounding of a 16-bit output.
 constexpr int kChunk = 64;
 // Padding of rows in LDS, in 16-bit words.  kPad: 16 rows' reads of 16 bytes meet no bank more often than they must; kPadT: so
 // do 16 channels' writes of four tokens, four rows apart, and reads of 8 bytes.
 constexpr int kPad = 8, kPadT = 4;
 
+constexpr int kWhole = 3;  // pieces of a float32
 template <class X>
-struct Pieces;
-template <>
-struct Pieces<bf16> {
-    static constexpr int in = 1, mid = 2;
-};
-template <>
-struct Pieces<f16> {
-    static constexpr int in = 2, mid = 2;
-};
-template <>
-struct Pieces<float> {
-    static constexpr int in = 3, mid = 3;
-};
+constexpr int kPieces = std::is_same<X, float>::value ? kWhole : std::is_same<X, f16>::value ? 2 : 1;  // of an input
+// of a key for the scores, products of inputs alone: 16-bit ones go in as they are
+template <class X>
+constexpr int kKeyPieces = std::is_same<X, float>::value ? kWhole : 1;
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
@@ -220,7 +211,7 @@ struct Four {
     __device__ __forceinline__ float operator[](int i) const { return to_f32((X)__builtin_bit_cast(x4, raw)[i]); }
 };
 
-// a row's four channels as they are in memory, in pieces
+// a row's four channels as they are in memory, in pieces; in one: as they are
 template <class X, int N>
 __device__ __forceinline__ void pieces(const Four<X>& x, u32x2 (&to)[N]) {
     if constexpr (N == 1) to[0] = x.raw;
@@ -239,6 +230,14 @@ __device__ inline f32x4 mma(const bf16x8 (&a)[A], const bf16x8 (&b)[B], f32x4 c)
         for (int i = 0; i < A; i++)
             if (s - i >= 0 && s - i < B) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
     return c;
+}
+
+// the same of 16-bit inputs as they are: their products are exact
+template <class X>
+__device__ inline f32x4 mma_inputs(bf16x8 a, bf16x8 b, f32x4 c) {
+    if constexpr (std::is_same<X, f16>::value)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
 __device__ inline bf16x8 read8(const uint16_t* p) { return *(const bf16x8*)p; }
@@ -261,24 +260,24 @@ struct ChunkArgs {
 // to 1024 78 against 89 us).
 template <class X, int DK, int TV>
 struct KeysApart {
-    uint16_t k[Pieces<X>::in][kChunk][DK + kPad];
-    uint16_t st[Pieces<X>::mid][TV][DK + kPad];
-    uint16_t kt[3][DK][kChunk + kPadT];
+    uint16_t k[kKeyPieces<X>][kChunk][DK + kPad];
+    uint16_t st[kWhole][TV][DK + kPad];
+    uint16_t kt[kWhole][DK][kChunk + kPadT];
 };
 template <class X, int DK, int TV>
 struct KeysInTurn {
     union {
         struct {
-            uint16_t k[Pieces<X>::in][kChunk][DK + kPad];
-            uint16_t st[Pieces<X>::mid][TV][DK + kPad];
+            uint16_t k[kKeyPieces<X>][kChunk][DK + kPad];
+            uint16_t st[kWhole][TV][DK + kPad];
         };
-        uint16_t kt[3][DK][kChunk + kPadT];
+        uint16_t kt[kWhole][DK][kChunk + kPadT];
     };
 };
 constexpr bool in_turn(int DK) { return DK > 64; }
 template <class X, int DK, int TV>
 struct ChunkShared : std::conditional<in_turn(DK), KeysInTurn<X, DK, TV>, KeysApart<X, DK, TV>>::type {
-    uint16_t vt[Pieces<X>::in][TV][kChunk + kPadT];  // values, a channel a row
+    uint16_t vt[kPieces<X>][TV][kChunk + kPadT];  // values, a channel a row
     double sum[kChunk];
     int poisoned;                                    // the last chunk (its first token + 1) with a value not finite
 };
@@ -293,7 +292,7 @@ struct ChunkShared : std::conditional<in_turn(DK), KeysInTurn<X, DK, TV>, KeysAp
 // take 80 us; one of 8,192 tokens 47 us, 14 of them for what segments add, 6.5 to join them and 27 for the outputs.
 template <class X, int DK, int TV, bool kOut>
 __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>) * 2 <= 160 << 10 ? 2 : 1)) void k_chunks(ChunkArgs c) {
-    constexpr int P = Pieces<X>::in, M = Pieces<X>::mid, KK = DK / 32, CT = TV / 16, ST = DK / 16 * CT / 4;
+    constexpr int P = kPieces<X>, PK = kKeyPieces<X>, KK = DK / 32, CT = TV / 16, ST = DK / 16 * CT / 4;
     constexpr int kKeyBlocks = DK * kChunk / 16 / 256 ? DK * kChunk / 16 / 256 : 1;  // 4 x 4 blocks of a thread
     constexpr int kValueBlocks = TV * kChunk / 16 / 256 ? TV * kChunk / 16 / 256 : 1;
     extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
@@ -452,10 +451,10 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
                 if (t < kChunk) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        u32x2 piece[P];
+                        u32x2 piece[PK];
                         pieces(kx[b][i], piece);
 #pragma unroll
-                        for (int p = 0; p < P; p++) *(u32x2*)&s.k[p][t + i][d] = piece[p];
+                        for (int p = 0; p < PK; p++) *(u32x2*)&s.k[p][t + i][d] = piece[p];
                     }
                 }
             }
@@ -472,10 +471,10 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const float f[4] = {kx[b][0][e] * w[0], kx[b][1][e] * w[1], kx[b][2][e] * w[2], kx[b][3][e] * w[3]};
-                        u32x2 piece[3];
+                        u32x2 piece[kWhole];
                         split4(f, piece);
 #pragma unroll
-                        for (int p = 0; p < 3; p++) *(u32x2*)&s.kt[p][d + e][t] = piece[p];
+                        for (int p = 0; p < kWhole; p++) *(u32x2*)&s.kt[p][d + e][t] = piece[p];
                     }
                 }
             }
@@ -514,15 +513,15 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
             }
         }
         if (kOut && odd) s.poisoned = t0 + 1;
-        bf16x8 Q[KK][P];
+        bf16x8 Q[KK][P], q_scores[KK][PK];  // for the state, and for the scores
         if constexpr (kOut) {
 #pragma unroll
             for (int i = 0; i < ST; i++) {
                 const float f[4] = {S[i][0], S[i][1], S[i][2], S[i][3]};
-                u32x2 piece[M];
+                u32x2 piece[kWhole];
                 split4(f, piece);
 #pragma unroll
-                for (int p = 0; p < M; p++) *(u32x2*)&s.st[p][c0(i) + lr][d0(i) + lg * 4] = piece[p];
+                for (int p = 0; p < kWhole; p++) *(u32x2*)&s.st[p][c0(i) + lr][d0(i) + lg * 4] = piece[p];
             }
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
@@ -532,6 +531,11 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
 #pragma unroll
                 for (int p = 0; p < P; p++)
                     Q[kk][p] = __builtin_bit_cast(bf16x8, u32x4{piece[0][p].x, piece[0][p].y, piece[1][p].x, piece[1][p].y});
+                if constexpr (PK == 1)
+                    q_scores[kk][0] = __builtin_bit_cast(bf16x8, u32x4{qx[kk][0].raw.x, qx[kk][0].raw.y, qx[kk][1].raw.x, qx[kk][1].raw.y});
+                else
+#pragma unroll
+                    for (int p = 0; p < PK; p++) q_scores[kk][p] = Q[kk][p];
             }
         }
         __syncthreads();
@@ -551,9 +555,9 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
                 O[ct] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++) {
-                    bf16x8 st[M];
+                    bf16x8 st[kWhole];
 #pragma unroll
-                    for (int p = 0; p < M; p++) st[p] = read8(&s.st[p][ct * 16 + lr][kk * 32 + lg * 8]);
+                    for (int p = 0; p < kWhole; p++) st[p] = read8(&s.st[p][ct * 16 + lr][kk * 32 + lg * 8]);
                     O[ct] = mma(st, Q[kk], O[ct]);
                 }
                 O[ct] *= before;
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
 #pragma unroll
             for (int pair = 0; pair < 2; pair++) {
                 if (pair * 2 > wave) break;
-                u32x2 piece[2][M];
+                u32x2 piece[2][kWhole];
                 float p4[2][4];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
@@ -574,10 +578,11 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
                         f32x4 score = {0, 0, 0, 0};
 #pragma unroll
                         for (int kk = 0; kk < KK; kk++) {
-                            bf16x8 kr[P];
+                            bf16x8 kr[PK];
 #pragma unroll
-                            for (int p = 0; p < P; p++) kr[p] = read8(&s.k[p][jt * 16 + lr][kk * 32 + lg * 8]);
-                            score = mma(kr, Q[kk], score);
+                            for (int p = 0; p < PK; p++) kr[p] = read8(&s.k[p][jt * 16 + lr][kk * 32 + lg * 8]);
+                            if constexpr (PK == 1) score = mma_inputs<X>(kr[0], q_scores[kk][0], score);
+                            else score = mma(kr, q_scores[kk], score);
                         }
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
@@ -589,9 +594,9 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
                     split4(p4[u], piece[u]);
                 }
                 if (!poisoned) {
-                    bf16x8 pr[M];
+                    bf16x8 pr[kWhole];
 #pragma unroll
-                    for (int p = 0; p < M; p++)
+                    for (int p = 0; p < kWhole; p++)
                         pr[p] = __builtin_bit_cast(bf16x8, u32x4{piece[0][p].x, piece[0][p].y, piece[1][p].x, piece[1][p].y});
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++) {
@@ -663,9 +668,9 @@ __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>)
             S[i] *= all;
 #pragma unroll
             for (int kk = 0; kk < kChunk / 32; kk++) {
-                bf16x8 kt[3], vt[P];
+                bf16x8 kt[kWhole], vt[P];
 #pragma unroll
-                for (int p = 0; p < 3; p++) kt[p] = read44(&s.kt[p][d0(i) + lr][kk * 32 + lg * 8], &s.kt[p][d0(i) + lr][kk * 32 + lg * 8 + 4]);
+                for (int p = 0; p < kWhole; p++) kt[p] = read44(&s.kt[p][d0(i) + lr][kk * 32 + lg * 8], &s.kt[p][d0(i) + lr][kk * 32 + lg * 8 + 4]);
 #pragma unroll
                 for (int p = 0; p < P; p++) vt[p] = read44(&s.vt[p][c0(i) + lr][kk * 32 + lg * 8], &s.vt[p][c0(i) + lr][kk * 32 + lg * 8 + 4]);
                 S[i] = mma(kt, vt, S[i]);

@@ -1,0 +1,63 @@
+"""GPU tests of what the operators in the clear keep of their inputs: results that live in the low bits of large operands, as
+they do where a sum cancels, and draws near 0 from entries that hardly weigh.  Bounds are derived at each test, from sums that
+are cut off rather than rounded at worst (2^-23 of what is summed each)."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_clear_ops import TYPES, ROUNDING, run_prompt
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ linear attention
+@pytest.mark.parametrize("T, dv", [(5, 16), (63, 64), (130, 64), (300, 96)])
+@pytest.mark.parametrize("kind", TYPES)
+def test_prompt_outputs_read_the_whole_state(T, dv, kind):
+    """Two rows of the state near 1000 that differ by up to 1/4, read with q = (1, -1): their difference.  Products with 1 are
+    exact; two rows of three pieces at most are six terms, each sum off by at most 2^-23 of 2,000."""
+    kind, B, H = TYPES[kind], 3, 4
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    low = 900 + 100 * torch.rand((B, H, 1, dv), generator=gen, device="cuda")
+    state = torch.cat((low, low + torch.rand((B, H, 1, dv), generator=gen, device="cuda") / 4), 2)
+    q = torch.tensor([1.0, -1.0], device="cuda").to(kind).expand(B, T, H, 2).contiguous()
+    k, v = torch.zeros((B, T, H, 2), device="cuda").to(kind), torch.zeros((B, T, H, dv), device="cuda").to(kind)
+    out, into = run_prompt(q, k, v, torch.zeros((B, T, H), device="cuda"), state)
+    want = (state[:, :, 0].double() - state[:, :, 1].double())[:, None].expand(B, T, H, dv)
+    assert ((out.double() - want).abs() <= 6 * 2.0**-23 * 2000 + ROUNDING[kind] * want.abs()).all()
+    assert torch.equal(into, state)
+
+
+@pytest.mark.parametrize("T", [5, 64, 200])
+@pytest.mark.parametrize("kind", TYPES)
+def test_prompt_outputs_read_whole_scores(T, kind):
+    """Scores 1000 + x_j against values 1 and -1 in turn: after two tokens x_0 - x_1, after four the sum of two differences.  A
+    score is one sum of two exact products (its pieces: six terms at most, the largest 1,000), and is read as three pieces."""
+    kind, B, H, dv = TYPES[kind], 8, 8, 32
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.rand((B, T, H), generator=gen, device="cuda").to(kind)
+    k = torch.stack((torch.full_like(x, 1000.0), x), -1)  # 1000 and the x are numbers of the type
+    q = torch.ones((B, T, H, 2), device="cuda").to(kind)
+    sign = (1.0 - 2.0 * (torch.arange(T, device="cuda") % 2))[None, :, None]
+    v = sign[..., None].expand(B, T, H, dv).contiguous().to(kind)
+    out, _ = run_prompt(q, k, v, torch.zeros((B, T, H), device="cuda"), None)
+    want = ((1000 + x.double()) * sign.double()).cumsum(1)
+    for t in (1, 3):
+        allowed = (6 + 3) * (t + 1) * 2.0**-23 * 1001 + ROUNDING[kind] * want[:, t, :, None].abs()
+        assert ((out[:, t].double() - want[:, t, :, None]).abs() <= allowed).all(), t
+
+
+@pytest.mark.parametrize("T", [5, 100])
+def test_prompt_takes_float16_inputs_below_the_normal_ones(T):
+    """queries of 2^-20 and 3 2^-24 with keys of 2^10, and the other way round: exact products, one a token"""
+    small = torch.tensor([2.0**-20, 3 * 2.0**-24], device="cuda").half().reshape(1, 1, 2, 1).expand(1, T, 2, 1).contiguous()
+    large = torch.full((1, T, 2, 1), 1024.0, device="cuda").half()
+    v = torch.ones((1, T, 2, 16), device="cuda").half()
+    g = torch.full((1, T, 2), -math.inf, device="cuda")
+    want = (small.float() * large.float()).expand(v.shape)
+    for q, k in ((small, large), (large, small)):
+        out, into = run_prompt(q, k, v, g, None)
+        assert torch.equal(out.float(), want)
+        assert torch.equal(into, k[:, -1].float()[..., None].expand(into.shape))
