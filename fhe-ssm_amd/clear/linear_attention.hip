@@ -142,7 +142,7 @@ void launch_recurrent(const Args& a, uint32_t grid, hipStream_t st) {
 //     o_i = exp(G_i) q_i S + sum_{j <= i} exp(G_i - G_j) (q_i . k_j) v_j,   S' = exp(G_63) S + sum_j exp(G_63 - G_j) k_j v_j^T
 // The sums of decays and their differences are taken in 64 bits (in units of log 2): in 32 bits a chunk of strong decays would
 // lose what its neighbouring tokens have in common.  Matrix operands are bf16 pieces of a value, each the upper 8 bits of what
-// the ones before it left: one piece is a bf16 input, two a float16 one, three a float32 one, so products of inputs are exact.
+// the ones before it left: one piece is a bf16 input, two a float16 one, three a float32 one.
 // What is held in float32, the state, the scores and the decayed keys, goes in as three pieces for every type: with two the
 // outputs of states and scores that cancel would be off by more than the rounding of a 16-bit output.
 constexpr int kChunk = 64;
@@ -221,11 +221,12 @@ __device__ __forceinline__ void pieces(const Four<X>& x, u32x2 (&to)[N]) {
     }
 }
 
-// c += a b over the pieces of both, the smallest first; what is left out is below 2^-24 of the product
+// c += a b over the pieces of both, the smallest first.  Pieces are cut off, so the second is below 2^-7 and the third below
+// 2^-15 of the value; what is left out, the product of two third ones, is below 2^-30 of a product.
 template <int A, int B>
 __device__ inline f32x4 mma(const bf16x8 (&a)[A], const bf16x8 (&b)[B], f32x4 c) {
 #pragma unroll
-    for (int s = A + B - 2 < 2 ? A + B - 2 : 2; s >= 0; s--)
+    for (int s = A + B - 2 < 3 ? A + B - 2 : 3; s >= 0; s--)
 #pragma unroll
         for (int i = 0; i < A; i++)
             if (s - i >= 0 && s - i < B) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);

@@ -61,3 +61,22 @@ def test_prompt_takes_float16_inputs_below_the_normal_ones(T):
         out, into = run_prompt(q, k, v, g, None)
         assert torch.equal(out.float(), want)
         assert torch.equal(into, k[:, -1].float()[..., None].expand(into.shape))
+
+
+@pytest.mark.parametrize("T", [5, 64, 300])
+def test_prompt_keeps_the_products_of_low_pieces(T):
+    """x = 1 + 2^-7 - 2^-23, whose three pieces of 8 bits are 1, 2^-7 - 2^-15 and 2^-15 - 2^-23: the products of its second and
+    third are 2^-21 of x x.  As a score, as what goes into the state, as what the state gives: a product is a sum of its
+    pieces' products, of which those left out are below 2^-30, off by at most 2^-23 of itself, twice for outputs by scores."""
+    x = 1 + 2.0**-7 - 2.0**-23
+    B, H, zero = 2, 3, torch.zeros((2, T, 3), device="cuda")
+    one = torch.zeros((B, T, H, 1), device="cuda")
+    one[:, 0] = 1
+    q, v = torch.full((B, T, H, 1), x, device="cuda"), torch.ones((B, T, H, 8), device="cuda")
+    out, _ = run_prompt(q, one * x, v, zero, None)  # a key at the first token only
+    assert ((out.double() - x * x).abs() <= 2.5 * 2.0**-23 * x * x).all()
+    _, into = run_prompt(q, one * x, x * v, zero, None)
+    assert ((into.double() - x * x).abs() <= 1.5 * 2.0**-23 * x * x).all()
+    out, into = run_prompt(q, 0 * one, v, zero, torch.full((B, H, 1, 8), x, device="cuda"))
+    assert ((out.double() - x * x).abs() <= 1.5 * 2.0**-23 * x * x).all()
+    assert (into == x).all()
