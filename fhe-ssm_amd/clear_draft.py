@@ -37,9 +37,8 @@ def answer(hidden, head: clear_ops.Q4Matrix, draws, logprobs=None, **filters):
     x = x.to("cuda", torch.float32) if not x.is_cuda else x
     logits = torch.empty((x.shape[0], head.out_features), dtype=x.dtype, device="cuda")
     tokens = torch.empty(x.shape[0], dtype=torch.int64, device="cuda")
-    stream = torch.cuda.current_stream().cuda_stream
-    head.product(x, logits, stream=stream)
-    clear_ops.sample(logits, draws, tokens, logprobs, stream=stream, **filters)
+    head.product(x, logits)
+    clear_ops.sample(logits, draws, tokens, logprobs, **filters)
     return tokens
 
 
@@ -63,7 +62,7 @@ class Draft:
     def _product(self, m, x):
         rows = x.reshape(-1, x.shape[-1])
         out = torch.empty((rows.shape[0], m.out_features), dtype=self.dtype, device="cuda")
-        m.product(rows, out, stream=torch.cuda.current_stream().cuda_stream)
+        m.product(rows, out)
         return out.view(*x.shape[:-1], m.out_features)
 
     def _norm(self, x):
@@ -72,18 +71,17 @@ class Draft:
 
     def _run(self, tokens, lengths):
         """tokens [lanes, n] or, for one step, [lanes]: hidden rows of the same shape, the states carried on"""
-        stream = torch.cuda.current_stream().cuda_stream
         x = self.embedding[tokens].float()
         for w_in, w_out, state in zip(self.w_in, self.w_out, self.states):
             q, k, v, gate = self._product(w_in, self._norm(x)).unflatten(-1, (4, self.heads, self.hs)).unbind(-3)
             o = torch.empty(v.shape, dtype=self.dtype, device="cuda")
             if tokens.dim() == 1:
-                clear_ops.linear_attention_step(q, k, v, self.log_decay, state, state, o, scale=self.hs**-0.5, stream=stream)
+                clear_ops.linear_attention_step(q, k, v, self.log_decay, state, state, o, scale=self.hs**-0.5)
             else:
                 need = clear_ops.linear_attention_workspace(q, k, v)
                 work = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
                 clear_ops.linear_attention_prompt(q, k, v, self.log_decay, state, state, o, scale=self.hs**-0.5,
-                                                  lengths=lengths, workspace=work, stream=stream)
+                                                  lengths=lengths, workspace=work)
             o = self._norm(o) * torch.nn.functional.silu(gate.float())
             x = x + self._product(w_out, o.flatten(-2).to(self.dtype)).float()
         return self._norm(x)

@@ -2,14 +2,16 @@
 clear -- linear attention with a decay for each head, products with 4-bit weights, the draw of a token.
 
 Arguments are device tensors (torch's, or anything with data_ptr, dtype, shape and stride); outputs are tensors that the
-caller brings.  Calls go to `stream` (a hipStream_t as an int, for torch `stream.cuda_stream`; None is the null stream) and
-return without waiting, so the tensors must stay until that stream has passed them.  Shapes, types and strides are checked
-here and ClearError raised; there is no fallback: if the library is missing, loading raises.
+caller brings.  Calls go to `stream` (a hipStream_t as an int, for torch `stream.cuda_stream`; 0 is the null stream; None is
+torch's current stream, and the null stream for tensors that are not torch's) and return without waiting, so the tensors must
+stay until that stream has passed them.  Shapes, types and strides are checked here and ClearError raised; there is no
+fallback: if the library is missing, loading raises.
 """
 from __future__ import annotations
 
 import ctypes
 import os
+import sys
 
 import numpy as np
 
@@ -117,6 +119,16 @@ def _on_device(*tensors) -> None:
             raise ClearError("tensors must be on the GPU")
 
 
+def _queue(stream, t):
+    """the stream of a call on tensor t"""
+    if stream is not None:
+        return stream
+    torch = sys.modules.get("torch")
+    if torch is None or not isinstance(t, torch.Tensor):
+        return None
+    return torch._C._cuda_getCurrentRawStream(t.get_device())  # current_stream() makes an object a call
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -202,7 +214,8 @@ def linear_attention_prompt(q, k, v, log_decay, state_in, state_out, out, scale:
     a = _described(q, k, v, log_decay, state_in, state_out, out, scale, True)
     check(load().fhe_ssm_linear_attention_prompt(
         a[1], q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(lengths), _ptr(state_in), _ptr(state_out),
-        out.data_ptr(), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), stream))
+        out.data_ptr(), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+        _queue(stream, v)))
 
 
 def linear_attention_step(q, k, v, log_decay, state_in, state_out, out, scale: float = 1.0, stream=None) -> None:
@@ -210,7 +223,7 @@ def linear_attention_step(q, k, v, log_decay, state_in, state_out, out, scale: f
     _on_device(q, k, v, log_decay, state_in, state_out, out)
     a = _described(q, k, v, log_decay, state_in, state_out, out, scale, False)
     check(load().fhe_ssm_linear_attention_step(a[1], q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
-                                               _ptr(state_in), _ptr(state_out), out.data_ptr(), stream))
+                                               _ptr(state_in), _ptr(state_out), out.data_ptr(), _queue(stream, v)))
 
 
 # ------------------------------------------------------------------------------------------------ 4-bit products
@@ -262,7 +275,7 @@ class Q4Matrix:
         self._at = -(-self.weights.data_ptr() // 256) * 256
         self.out_features, self.in_features, self._m = out, n_in, ctypes.addressof(m)
         check(load().fhe_ssm_q4_arrange(self._m, codes.data_ptr(), codes.stride()[0], scales.data_ptr(), _ptr(zeros),
-                                        self._at, stream))
+                                        self._at, _queue(stream, codes)))
 
     def product(self, x, out, stream=None) -> None:
         """out[r] = matrix times x[r] for rows x [rows, in_features], out [rows, out_features] of one type"""
@@ -273,7 +286,8 @@ class Q4Matrix:
         _need(kind == _type(out) and n_in == self.in_features and tuple(out.shape) == (rows, self.out_features),
               f"x must be [rows, {self.in_features}] and out [rows, {self.out_features}], of one type")
         _need((x1 == 1 or n_in == 1) and (y1 == 1 or self.out_features == 1), "rows must be contiguous")
-        check(load().fhe_ssm_q4_product(self._m, self._at, kind, rows, x.data_ptr(), xs, out.data_ptr(), ys, stream))
+        check(load().fhe_ssm_q4_product(self._m, self._at, kind, rows, x.data_ptr(), xs, out.data_ptr(), ys,
+                                          _queue(stream, x)))
 
 
 # ------------------------------------------------------------------------------------------------ sampling
@@ -295,4 +309,5 @@ def sample(logits, draws, tokens, logprobs=None, temperature=None, top_k=None, t
             raise ClearError(f"{name} must be contiguous {dtype[6:]} [{rows}]")
     p = SampleParams(_ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p))
     check(load().fhe_ssm_sample(_type(logits), logits.data_ptr(), rows, vocab, stride[0], draws.data_ptr(),
-                                ctypes.addressof(p), tokens.data_ptr(), _ptr(logprobs), stream))
+                                ctypes.addressof(p), tokens.data_ptr(), _ptr(logprobs),
+                                _queue(stream, logits)))
