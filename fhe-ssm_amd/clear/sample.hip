@@ -193,7 +193,8 @@ struct Prefix {
 
 // The first index up to which the weights w(logit, index) >= 0 sum to more than target(their whole sum); mine: the sum over
 // the thread's own entries, which s.extra adds to by waves.  Where rounding leaves none, the last one that weighs.  At least
-// one weight is above 0.  First the wave whose part it lies in, then all threads on that part, a vector each.
+// one weight is above 0.  First the wave whose part it lies in, then all threads on that part, a vector each, and on what
+// follows it where the part's entries do not reach the target: sums are rounded, and `mine` may count weights that w does not.
 template <class R, class W, class T>
 __device__ __forceinline__ uint32_t locate(const R& row, Shared& s, double mine, double& whole, W&& w, T&& target_of) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64;
@@ -221,8 +222,9 @@ __device__ __forceinline__ uint32_t locate(const R& row, Shared& s, double mine,
     const int from = max(reaching(part, target, before, reached, all), 0);
     reached = false;
     double* split = (double*)s.part[1];
-    for (int v0 = 0; v0 < row.vectors * 64 && !reached; v0 += kThreads) {
-        const bool in = v0 + (int)threadIdx.x < row.vectors * 64;
+    const int vectors = (kWaves - from) * row.vectors * 64;  // to the row's end
+    for (int v0 = 0; v0 < vectors && !reached; v0 += kThreads) {
+        const bool in = v0 + (int)threadIdx.x < vectors;
         const int i = from * row.vectors * R::kStep + (v0 + (int)threadIdx.x) * R::kVec;
         typename R::vec v;
         if (in && i >= row.skip && i + R::kVec <= row.end) v = *(const typename R::vec*)(row.x + i);

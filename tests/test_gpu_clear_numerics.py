@@ -6,7 +6,7 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_clear_ops import TYPES, ROUNDING, run_prompt
+from test_gpu_clear_ops import TYPES, ROUNDING, run_prompt, run_sample
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -80,3 +80,29 @@ def test_prompt_keeps_the_products_of_low_pieces(T):
     out, into = run_prompt(q, 0 * one, v, zero, torch.full((B, H, 1, 8), x, device="cuda"))
     assert ((out.double() - x * x).abs() <= 1.5 * 2.0**-23 * x * x).all()
     assert (into == x).all()
+
+
+# ------------------------------------------------------------------------------------------------ sampling
+def drawn(x, draws, **params):
+    rows = torch.from_numpy(np.asarray(x, dtype=np.float32)).cuda()[None].expand(len(draws), len(x))
+    return run_sample(rows, draws, **params)[0].tolist()
+
+
+FORMS = [{}, dict(min_p=1e-30), dict(top_p=0.99999), dict(top_k=60000), dict(top_k=50), dict(top_p=0.5), dict(temperature=0.9)]
+
+
+@pytest.mark.parametrize("params", FORMS, ids=str)
+@pytest.mark.parametrize("front", [1, 700, 8192, 65000])
+def test_sample_draws_near_0_pass_over_entries_that_weigh_nothing(front, params):
+    """entries 55 and more powers of two below the largest stand before all others: no draw, 0 itself included, takes them"""
+    x = np.full(65536, -40.0)
+    x[front:] = -np.arange(65536 - front) / 65536  # the largest first
+    assert drawn(x, [0.0, 1e-30, 1e-12], **params) == [front] * 3
+
+
+def test_sample_draws_near_0_between_entries_that_weigh_nothing():
+    """one light entry far along, none else beside the largest at the end"""
+    x = np.full(50277, -np.inf)
+    x[::3] = -45.0
+    x[30000], x[50000] = -10.0, 0.0
+    assert drawn(x, [0.0, 1e-20, 1e-3, 0.5]) == [30000, 30000, 50000, 50000]
