@@ -1,7 +1,7 @@
 // sample.hip -- the draw of a token under temperature, top-k, top-p and min-p.
 //
 // With the largest logit m, an entry lies d = log2(e) (m - l) / temperature below it and weighs e = 2^-d.  Entries with
-// d >= 46.5 weigh nothing: all 2^18 of them together would be below 2^-28 of the largest, and no draw of 24 bits tells them.
+// d >= 44 weigh nothing, on every path: all 2^18 of them together would be below 2^-26 of the largest.
 // Weights that are summed in no fixed order (by LDS atomics, over lists) are whole numbers of 2^-44, sums over all entries
 // 64-bit floats in a fixed order: a row gives the same token every time.  Entries are ordered by a key, the logit's bits
 // turned so that unsigned comparison orders them, and equal keys by index.
@@ -25,8 +25,8 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kList = 1024, kBins = 1024;
-constexpr float kSpan = 46.5f, kBinsEach = 22.f;  // d below kSpan; bins of d, the last below kBins
-constexpr int kUnit = 44;                         // whole weights are in units of 2^-44
+constexpr float kSpan = 44.f, kBinsEach = 22.f;  // d below kSpan; bins of d, the last below kBins
+constexpr int kUnit = 44;                         // whole weights are in units of 2^-44: one at least below kSpan
 constexpr uint32_t kMostVocab = 1u << 18;         // their sums fit 64 bits
 constexpr uint32_t kNever = 0xffffffffu;
 constexpr uint32_t kCus = 256;

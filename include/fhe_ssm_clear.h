@@ -97,7 +97,8 @@ int fhe_ssm_q4_product(const fhe_ssm_q4_matrix* m, const void* weights, uint32_t
  * up to which the kept mass is above draw times the whole kept mass; its log-probability is among the kept entries.
  * temperature <= 0 takes the largest logit (the lowest index of equal ones).  k <= 0, top_p >= 1 and min_p <= 0 turn a
  * filter off; top_p <= 0 leaves the first entry, min_p >= 1 those that equal it.  draw is held to [0, 1).  A NaN logit or -inf is never
- * drawn, entries of +inf share the whole mass; a row of nothing else gives token -1 and log-probability -inf.  A
+ * drawn, entries of +inf share the whole mass; a row of nothing else gives token -1 and log-probability -inf.  An entry
+ * of 2^-44 of the largest mass or less counts for nothing, also where a filter keeps it.  A
  * parameter that is NaN turns its filter off (temperature: 0, draw: 0).
  * Each parameter array holds one value per row, or a null pointer turns it off (temperature null: 1).  float32, k int32.
  */

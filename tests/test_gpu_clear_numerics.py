@@ -106,3 +106,19 @@ def test_sample_draws_near_0_between_entries_that_weigh_nothing():
     x[::3] = -45.0
     x[30000], x[50000] = -10.0, 0.0
     assert drawn(x, [0.0, 1e-20, 1e-3, 0.5]) == [30000, 30000, 50000, 50000]
+
+
+@pytest.mark.parametrize("params", [{}, dict(min_p=1e-25), dict(top_k=5), dict(top_k=5, min_p=1e-25)], ids=str)
+def test_sample_what_weighs_does_not_hang_on_the_filters(params):
+    """44 powers of two below the largest is where weights end, whatever filter keeps the entry: of 30.4 (43.86 powers of two)
+    and 30.6 (44.15) below it, before it, draw 0 takes the first and not the second"""
+    assert drawn([-30.4, 0.0, -1.0, -2.0, -3.0, -50.0], [0.0], **params) == [0]
+    assert drawn([-30.6, 0.0, -1.0, -2.0, -3.0, -50.0], [0.0], **params) == [1]
+
+
+def test_sample_what_weighs_among_thousands_of_equal_entries():
+    for light, token in ((-30.4, 0), (-30.6, 1)):
+        x = np.zeros(3005)
+        x[0], x[3001:] = light, -np.inf
+        for params in ({}, dict(min_p=1e-25), dict(top_k=3004), dict(top_k=3003, min_p=1e-25)):
+            assert drawn(x, [0.0], **params) == [token], (light, params)
