@@ -87,10 +87,13 @@ class Draft:
         return self._norm(x)
 
     def prompt(self, tokens, lengths=None):
-        """tokens [lanes, n], of lane b the first lengths[b] (int32): the hidden rows after each lane's last token"""
+        """tokens [lanes, n], of lane b the first lengths[b] (int32, held to [0, n]): the hidden rows after each lane's last
+        token"""
         h = self._run(tokens, lengths)
-        last = (lengths.long() if lengths is not None else torch.full((len(h),), h.shape[1], device="cuda")) - 1
-        return h[torch.arange(len(h), device="cuda"), last.clamp_min(0)]
+        if lengths is None:
+            return h[:, -1]
+        last = lengths.long().clamp(0, h.shape[1]) - 1
+        return h[torch.arange(len(h), device=h.device), last.clamp_min(0)]
 
     def step(self, tokens):
         """one token [lanes] for every lane: the hidden rows after it"""

@@ -1,0 +1,31 @@
+"""CPU-side checks of the drafting model's own code (clear_draft.py), over hidden rows that stand in for what its kernels give."""
+import pytest
+
+from engine_loader import load_module
+
+torch = pytest.importorskip("torch")
+
+
+def model_of(hidden):
+    """a model whose run gives these hidden rows"""
+    draft = load_module("clear_draft").Draft
+    model = draft.__new__(draft)
+    model._run = lambda tokens, lengths: hidden
+    return model
+
+
+HIDDEN = torch.arange(4 * 5 * 3, dtype=torch.float32).reshape(4, 5, 3)
+
+
+def test_prompt_gives_the_row_of_each_lanes_last_token():
+    lengths = torch.tensor([1, 5, 3, 4], dtype=torch.int32)
+    got = model_of(HIDDEN).prompt(torch.zeros(4, 5, dtype=torch.int64), lengths)
+    assert torch.equal(got, torch.stack([HIDDEN[b, n - 1] for b, n in enumerate(lengths.tolist())]))
+    assert torch.equal(model_of(HIDDEN).prompt(torch.zeros(4, 5, dtype=torch.int64)), HIDDEN[:, -1])
+
+
+def test_prompt_holds_lengths_to_the_tokens_there_are():
+    """as the kernels do: past the last row lies nothing that may be read"""
+    lengths = torch.tensor([6, 5, 2**31 - 1, 2], dtype=torch.int32)
+    got = model_of(HIDDEN).prompt(torch.zeros(4, 5, dtype=torch.int64), lengths)
+    assert torch.equal(got, torch.stack([HIDDEN[0, 4], HIDDEN[1, 4], HIDDEN[2, 4], HIDDEN[3, 1]]))
