@@ -88,12 +88,15 @@ class Draft:
 
     def prompt(self, tokens, lengths=None):
         """tokens [lanes, n], of lane b the first lengths[b] (int32, held to [0, n]): the hidden rows after each lane's last
-        token"""
+        token, zeros for a lane that has none"""
         h = self._run(tokens, lengths)
+        if h.shape[1] == 0:
+            return h.new_zeros((len(h), h.shape[2]))
         if lengths is None:
             return h[:, -1]
         last = lengths.long().clamp(0, h.shape[1]) - 1
-        return h[torch.arange(len(h), device=h.device), last.clamp_min(0)]
+        rows = h[torch.arange(len(h), device=h.device), last.clamp_min(0)]
+        return torch.where((last >= 0)[:, None], rows, 0.0)
 
     def step(self, tokens):
         """one token [lanes] for every lane: the hidden rows after it"""

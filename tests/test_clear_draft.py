@@ -29,3 +29,13 @@ def test_prompt_holds_lengths_to_the_tokens_there_are():
     lengths = torch.tensor([6, 5, 2**31 - 1, 2], dtype=torch.int32)
     got = model_of(HIDDEN).prompt(torch.zeros(4, 5, dtype=torch.int64), lengths)
     assert torch.equal(got, torch.stack([HIDDEN[0, 4], HIDDEN[1, 4], HIDDEN[2, 4], HIDDEN[3, 1]]))
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_prompt_gives_zeros_where_there_is_no_last_token(kind):
+    hidden = (HIDDEN + 1).to(kind)
+    got = model_of(hidden).prompt(torch.zeros(4, 5, dtype=torch.int64), torch.tensor([0, 2, -3, 5], dtype=torch.int32))
+    assert got.dtype == kind and torch.equal(got[[1, 3]], torch.stack([hidden[1, 1], hidden[3, 4]])) and (got[[0, 2]] == 0).all()
+    for lengths in (None, torch.zeros(4, dtype=torch.int32)):
+        none = model_of(hidden[:, :0]).prompt(torch.zeros(4, 0, dtype=torch.int64), lengths)
+        assert none.shape == (4, 3) and none.dtype == kind and (none == 0).all()
