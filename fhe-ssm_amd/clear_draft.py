@@ -43,7 +43,7 @@ def answer(hidden, head: clear_ops.Q4Matrix, draws, logprobs=None, **filters):
 
 
 class Draft:
-    """the model and, between calls, the lanes' states"""
+    """the model and, between calls, the lanes' states (reset makes them)"""
 
     def __init__(self, layers: int = 2, d: int = M.D, heads: int = M.HEADS, vocab: int = M.VOCAB, seed: int = 7,
                  dtype=torch.bfloat16):
@@ -71,6 +71,7 @@ class Draft:
 
     def _run(self, tokens, lengths):
         """tokens [lanes, n] or, for one step, [lanes]: hidden rows of the same shape, the states carried on"""
+        clear_ops._need(len(self.states) == len(self.w_in), "reset(lanes) makes the states that prompt and step carry on")
         x = self.embedding[tokens].float()
         for w_in, w_out, state in zip(self.w_in, self.w_out, self.states):
             q, k, v, gate = self._product(w_in, self._norm(x)).unflatten(-1, (4, self.heads, self.hs)).unbind(-3)

@@ -39,3 +39,14 @@ def test_prompt_gives_zeros_where_there_is_no_last_token(kind):
     for lengths in (None, torch.zeros(4, dtype=torch.int32)):
         none = model_of(hidden[:, :0]).prompt(torch.zeros(4, 0, dtype=torch.int64), lengths)
         assert none.shape == (4, 3) and none.dtype == kind and (none == 0).all()
+
+
+@pytest.mark.parametrize("call", ["prompt", "step"])
+def test_a_model_without_states_refuses(call):
+    """before the first reset; without the check no layer would run, and the embeddings come out as hidden rows"""
+    draft = load_module("clear_draft")
+    model = draft.Draft.__new__(draft.Draft)
+    model.w_in, model.w_out, model.states, model.dtype = [None, None], [None, None], [], torch.float32
+    model.embedding = torch.ones(7, 8)
+    with pytest.raises(draft.clear_ops.ClearError, match="reset"):
+        getattr(model, call)(torch.zeros((2, 3) if call == "prompt" else 2, dtype=torch.int64))
