@@ -111,7 +111,7 @@ class Draft:
             out.append(answer(hidden, self.head, draws[i], **filters))
             if i + 1 < count:
                 hidden = self.step(out[-1])
-        return torch.stack(out, 1)
+        return torch.stack(out, 1) if out else tokens.new_empty((len(tokens), 0))
 
 
 def main() -> None:

@@ -50,3 +50,10 @@ def test_a_model_without_states_refuses(call):
     model.embedding = torch.ones(7, 8)
     with pytest.raises(draft.clear_ops.ClearError, match="reset"):
         getattr(model, call)(torch.zeros((2, 3) if call == "prompt" else 2, dtype=torch.int64))
+
+
+def test_generate_of_no_tokens_gives_none():
+    model = model_of(HIDDEN)
+    model.reset = lambda lanes: None
+    out = model.generate(torch.zeros(4, 5, dtype=torch.int64), 0, torch.zeros(0, 4))
+    assert out.shape == (4, 0) and out.dtype == torch.int64
