@@ -34,7 +34,8 @@ def answer(hidden, head: clear_ops.Q4Matrix, draws, logprobs=None, **filters):
     """The client's answer to a step: rows of hidden states [lanes, channels] as ckks_decrypt_decode gives them (float64 on the
     host, or a device tensor) to tokens [lanes].  draws and filters are clear_ops.sample's."""
     x = torch.as_tensor(hidden)
-    x = x.to("cuda", torch.float32) if not x.is_cuda else x
+    if not x.is_cuda or x.dtype == torch.float64:
+        x = x.to("cuda", torch.float32)
     logits = torch.empty((x.shape[0], head.out_features), dtype=x.dtype, device="cuda")
     tokens = torch.empty(x.shape[0], dtype=torch.int64, device="cuda")
     head.product(x, logits)

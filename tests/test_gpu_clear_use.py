@@ -49,3 +49,19 @@ def test_calls_are_recorded_with_the_current_stream():
         assert torch.equal(tokens, want)
         c.sample(logits, draws, tokens)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+@pytest.mark.parametrize("kind", [torch.float64, torch.float32, torch.bfloat16])
+def test_answer_takes_rows_of_every_kind(where, kind):
+    """rows of decrypted values as they come, on the host or on the GPU: the tokens of the same values in float32"""
+    d = load_module("clear_draft")
+    head = d.matrix(d.np.random.default_rng(3), VOCAB, D, scale=3.0)
+    rows = torch.randn((9, D), generator=torch.Generator().manual_seed(4), dtype=torch.float64).to(torch.bfloat16)
+    draws = torch.rand(9, generator=torch.Generator().manual_seed(5)).cuda()
+    want = d.answer(rows.float().cuda(), head, torch.zeros(9, device="cuda"), temperature=torch.zeros(9, device="cuda"))
+    got = d.answer(rows.to(kind).to(where), head, draws, temperature=torch.zeros(9, device="cuda"))
+    if kind == torch.bfloat16 and where == "cuda":  # logits of that type
+        assert ((got >= 0) & (got < VOCAB)).all()
+    else:
+        assert torch.equal(got, want)
