@@ -280,6 +280,7 @@ class Q4Matrix:
     def product(self, x, out, stream=None) -> None:
         """out[r] = matrix times x[r] for rows x [rows, in_features], out [rows, out_features] of one type"""
         _on_device(x, out)
+        _need(len(x.shape) == len(out.shape) == 2, "x and out are [rows, columns]")
         kind = _type(x)
         rows, n_in = x.shape
         (xs, x1), (ys, y1) = x.stride(), out.stride()
@@ -298,6 +299,7 @@ def sample(logits, draws, tokens, logprobs=None, temperature=None, top_k=None, t
     top_p, min_p: float32 [rows]; top_k: int32 [rows]; None turns a filter off (temperature: 1).  What they keep, and which
     token a number draws, is defined in include/fhe_ssm_clear.h."""
     _on_device(logits, draws, tokens, logprobs, temperature, top_k, top_p, min_p)
+    _need(len(logits.shape) == 2, "logits are [rows, vocab]")
     rows, vocab = logits.shape
     stride = logits.stride()
     _need(vocab == 1 or stride[1] == 1, "rows of logits must be contiguous")

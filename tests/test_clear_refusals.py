@@ -1,0 +1,17 @@
+"""CPU-side checks of what the operators in the clear refuse, and of what they must not, from Python and through the C ABI."""
+import pytest
+
+from engine_loader import load_module
+from test_clear_streams import on_gpu, ops as library
+
+torch = pytest.importorskip("torch")
+
+
+def test_rows_that_are_no_matrix_are_refused(library):
+    m = library.Q4Matrix(on_gpu(torch.zeros(8, 32, dtype=torch.uint8)), on_gpu(torch.zeros(8, 1)), group=64)
+    for x, out in (((64,), (8,)), ((64,), (1, 8)), ((1, 64), (8,)), ((1, 1, 64), (1, 1, 8))):
+        with pytest.raises(library.ClearError, match=r"\[rows, columns\]"):
+            m.product(on_gpu(torch.zeros(x)), on_gpu(torch.zeros(out)))
+    for shape in ((9,), (1, 1, 9), ()):
+        with pytest.raises(library.ClearError, match=r"\[rows, vocab\]"):
+            library.sample(on_gpu(torch.zeros(shape)), on_gpu(torch.zeros(1)), on_gpu(torch.zeros(1, dtype=torch.int64)))
