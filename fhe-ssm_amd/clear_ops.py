@@ -211,6 +211,7 @@ def linear_attention_prompt(q, k, v, log_decay, state_in, state_out, out, scale:
     if lengths is not None:
         _need(_is(lengths, "torch.int32") and tuple(lengths.shape) == (v.shape[0],) and lengths.is_contiguous(),
               "lengths must be contiguous int32 [lanes]")
+    _need(workspace is None or workspace.is_contiguous(), "workspace must be contiguous")
     a = _described(q, k, v, log_decay, state_in, state_out, out, scale, True)
     check(load().fhe_ssm_linear_attention_prompt(
         a[1], q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(lengths), _ptr(state_in), _ptr(state_out),

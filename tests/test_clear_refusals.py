@@ -15,3 +15,11 @@ def test_rows_that_are_no_matrix_are_refused(library):
     for shape in ((9,), (1, 1, 9), ()):
         with pytest.raises(library.ClearError, match=r"\[rows, vocab\]"):
             library.sample(on_gpu(torch.zeros(shape)), on_gpu(torch.zeros(1)), on_gpu(torch.zeros(1, dtype=torch.int64)))
+
+
+def test_a_workspace_that_is_smaller_than_its_shape_is_refused(library):
+    """an expanded tensor has many elements and little memory"""
+    x, g = on_gpu(torch.zeros(1, 2, 3, 4)), on_gpu(torch.zeros(3))
+    few = on_gpu(torch.zeros(1, dtype=torch.uint8)).expand(4096)
+    with pytest.raises(library.ClearError, match="workspace must be contiguous"):
+        library.linear_attention_prompt(x, x, x, g, None, None, x, workspace=few)
