@@ -119,7 +119,8 @@ int fhe_ssm_q4_arrange(const fhe_ssm_q4_matrix* m, const uint8_t* codes, int64_t
     if (int rc = check(m)) return rc;
     if (!codes || !scales || !weights || !zeros != !m->has_zeros)
         return fail(CKKS_EINVAL, "4-bit product: null argument, or zero points where none are announced");
-    if (code_stride < (int64_t)((m->in + 1) / 2)) return fail(CKKS_EINVAL, "4-bit product: rows of codes overlap");
+    if (code_stride < 0 || (m->out > 1 && code_stride < (int64_t)((m->in + 1) / 2)))
+        return fail(CKKS_EINVAL, "4-bit product: rows of codes overlap");
     if (!aligned(weights, 256)) return fail(CKKS_EINVAL, "4-bit product: the arranged weights must lie on 256 bytes");
     const Layout y = layout(*m);
     const hipStream_t st = (hipStream_t)stream;

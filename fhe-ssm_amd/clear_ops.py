@@ -260,7 +260,8 @@ class Q4Matrix:
 
     def __init__(self, codes, scales, zeros=None, in_features: int | None = None, group: int = 64, stream=None):
         _on_device(codes, scales, zeros)
-        _need(_is(codes, "torch.uint8") and len(codes.shape) == 2 and codes.stride()[1] == 1, "codes must be uint8 rows")
+        _need(_is(codes, "torch.uint8") and len(codes.shape) == 2 and (codes.stride()[1] == 1 or codes.shape[1] == 1),
+              "codes must be uint8 rows")
         out, row = codes.shape
         n_in = 2 * row if in_features is None else in_features
         _need((n_in + 1) // 2 == row, f"rows of {row} bytes do not hold {n_in} codes")

@@ -23,3 +23,8 @@ def test_a_workspace_that_is_smaller_than_its_shape_is_refused(library):
     few = on_gpu(torch.zeros(1, dtype=torch.uint8)).expand(4096)
     with pytest.raises(library.ClearError, match="workspace must be contiguous"):
         library.linear_attention_prompt(x, x, x, g, None, None, x, workspace=few)
+
+
+def test_rows_of_one_byte_have_any_stride_inside(library):
+    library.Q4Matrix(on_gpu(torch.zeros(8, 40, dtype=torch.uint8))[:, 7:8], on_gpu(torch.zeros(8, 1)), group=32, in_features=2)
+    library.Q4Matrix(on_gpu(torch.zeros(1, 8, dtype=torch.uint8).t()), on_gpu(torch.zeros(8, 1)), group=32, in_features=1)

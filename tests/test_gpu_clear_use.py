@@ -65,3 +65,23 @@ def test_answer_takes_rows_of_every_kind(where, kind):
         assert ((got >= 0) & (got < VOCAB)).all()
     else:
         assert torch.equal(got, want)
+
+
+def test_matrices_of_one_row_and_of_one_byte_a_row():
+    """strides of axes that have one entry say nothing, and must not be refused"""
+    c = load_module("clear_ops")
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    column = torch.randint(0, 256, (32, 1), generator=gen, device="cuda", dtype=torch.uint8)
+    codes = torch.stack((column & 15, column >> 4), -1).double() - 8  # [32, 1, 2]
+    one_row = column.t()  # [1, 32], one byte from row to row
+    assert one_row.stride() == (1, 1)
+    x, y = torch.randn((3, 64), generator=gen, device="cuda"), torch.empty((3, 1), device="cuda")
+    c.Q4Matrix(one_row, torch.ones((1, 2), device="cuda"), group=32).product(x, y)
+    want = x.double() @ codes.reshape(64, 1)
+    assert ((y.double() - want).abs() <= 2 * (32 + 2 + 16) * 2.0**-24 * 32 * x.double().abs().sum(1, keepdim=True)).all()
+    wide = torch.zeros((32, 40), dtype=torch.uint8, device="cuda")
+    wide[:, 7:8] = column
+    x, y = torch.randn((3, 2), generator=gen, device="cuda"), torch.empty((3, 32), device="cuda")
+    c.Q4Matrix(wide[:, 7:8], torch.ones((32, 1), device="cuda"), group=32).product(x, y)
+    want = x.double() @ codes.reshape(32, 2).t().contiguous()
+    assert ((y.double() - want).abs() <= 2 * (2 + 1 + 16) * 2.0**-24 * 32 * x.double().abs().sum(1, keepdim=True)).all()
