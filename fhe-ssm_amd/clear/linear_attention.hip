@@ -816,11 +816,22 @@ int launch_chunks(const ChunkArgs& c, uint32_t items, hipStream_t st) {
     return go(k_chunks<X, DK, TV, true>, c);
 }
 
+// Rows of out that certainly meet: neighbours along an axis, closer than a row is long.
+bool rows_meet(const fhe_ssm_linear_attention* a) {
+    const uint32_t count[3] = {a->lanes, a->tokens, a->heads};
+    for (int i = 0; i < 3; i++) {
+        const int64_t s = a->out_stride[i];
+        if (count[i] > 1 && s < (int64_t)a->dv && s > -(int64_t)a->dv) return true;
+    }
+    return false;
+}
+
 int run(const fhe_ssm_linear_attention* a, const void* q, const void* k, const void* v, const float* g,
         const int32_t* lengths, const float* state_in, float* state_out, void* out, void* workspace,
         size_t workspace_bytes, void* stream) {
     if (a->lanes == 0) return CKKS_OK;
     if (a->tokens && (!q || !k || !v || !g || !out)) return fail(CKKS_EINVAL, "linear attention: null argument");
+    if (a->tokens && rows_meet(a)) return fail(CKKS_EINVAL, "linear attention: rows of out overlap");
     Args r = arguments(a, q, k, v, g, lengths, state_in, state_out, out);
     const hipStream_t st = (hipStream_t)stream;
     const Plan p = plan(a);
