@@ -72,7 +72,9 @@ int fhe_ssm_linear_attention_step(const fhe_ssm_linear_attention* a, const void*
  * Codes 0..15, two in a byte (the lower index in the low four bits), rows of (in + 1) / 2 bytes; zero points 0..15 per
  * group, or 8 throughout; the last group may be cut short.  group is 32, 64 or a multiple of 128.
  * The matrix is laid out once (fhe_ssm_q4_arrange) in the order the kernel reads it; bf16 scales are widened to float32
- * there, float16 ones stay.  Codes and zero points are used exactly; float32 rows are used to their full 24 bits. */
+ * there, float16 ones stay.  Codes and zero points are used exactly; float32 rows are used to their full 24 bits.
+ * Sums go through codes held as 16 + c: a row of x with an infinity or a NaN gives NaN in all its outputs and leaves other
+ * rows alone, and a row's magnitudes have to sum to less than 2^122 in every group, or its outputs may be NaN. */
 typedef struct {
     uint32_t out, in, group;
     uint32_t scale_type; /* of the scales given to fhe_ssm_q4_arrange */

@@ -1,12 +1,13 @@
 """GPU tests of what the operators in the clear keep of their inputs: results that live in the low bits of large operands, as
-they do where a sum cancels, and draws near 0 from entries that hardly weigh.  Bounds are derived at each test, from sums that
-are cut off rather than rounded at worst (2^-23 of what is summed each)."""
+they do where a sum cancels, operands at the ends of their range, draws near 0 from entries that hardly weigh.  Bounds are
+derived at each test, from sums that are cut off rather than rounded at worst (2^-23 of what is summed each)."""
 import math
 
 import numpy as np
 import pytest
 
-from test_gpu_clear_ops import TYPES, ROUNDING, run_prompt, run_sample
+from engine_loader import load_module
+from test_gpu_clear_ops import TYPES, ROUNDING, check_product, product_case, run_prompt, run_sample
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -122,3 +123,32 @@ def test_sample_what_weighs_among_thousands_of_equal_entries():
         x[0], x[3001:] = light, -np.inf
         for params in ({}, dict(min_p=1e-25), dict(top_k=3004), dict(top_k=3003, min_p=1e-25)):
             assert drawn(x, [0.0], **params) == [token], (light, params)
+
+
+# ------------------------------------------------------------------------------------------------ 4-bit products
+@pytest.mark.parametrize("rows", [1, 3, 20, 70])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_product_of_very_large_rows(rows, kind):
+    """magnitudes that sum to just below 2^122 in every group, scales that bring the results back: sums of 62 times as much at
+    most stay below 2^128"""
+    for group, zeros in ((32, True), (128, False)):
+        x, codes, scales, z = product_case(rows, 50, 384, group, TYPES[kind], torch.float16, zeros, rows)
+        signs = torch.where(x > 0, 1.0, -1.0)
+        x = (signs * (2.0**122 / group) * (0.5 + x.abs().clamp(max=2) / 4.1)).to(TYPES[kind])
+        x[:, ::7] = x[:, ::7].abs()
+        assert (x.double().abs().reshape(rows, -1, group).sum(-1) < 2.0**122).all()
+        check_product(x, codes, (scales / 1024).float(), z, group)
+
+
+@pytest.mark.parametrize("rows", [3, 20, 70])
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_product_of_a_row_that_is_not_finite(rows, kind, value):
+    x, codes, scales, z = product_case(rows, 50, 300, 64, TYPES[kind], torch.float16, True, rows)
+    want = check_product(x, codes, scales, z, 64)
+    x[1, 217] = value
+    y = torch.empty_like(want)
+    load_module("clear_ops").Q4Matrix(codes, scales, z, in_features=300, group=64).product(x, y)
+    assert torch.isnan(y[1]).all()
+    keep = torch.arange(rows) != 1
+    assert torch.equal(y[keep], want[keep])
