@@ -85,3 +85,38 @@ def test_matrices_of_one_row_and_of_one_byte_a_row():
     c.Q4Matrix(wide[:, 7:8], torch.ones((32, 1), device="cuda"), group=32).product(x, y)
     want = x.double() @ codes.reshape(32, 2).t().contiguous()
     assert ((y.double() - want).abs() <= 2 * (2 + 1 + 16) * 2.0**-24 * 32 * x.double().abs().sum(1, keepdim=True)).all()
+
+
+def test_logits_of_prompt_and_steps_are_float32s():
+    """What CLOSE of test_gpu_clear_draft.py derives, 1e-4 for each of three products in a row where roundings fall as they may
+    and the norms between them, without a factor on it"""
+    from test_gpu_clear_draft import CLOSE, plain_logits
+    model, gen = make(), torch.Generator(device="cuda").manual_seed(8)
+    tokens = torch.randint(0, VOCAB, (3, 75), generator=gen, device="cuda")
+    lengths = torch.tensor([70, 1, 33], dtype=torch.int32, device="cuda")
+    model.reset(3)
+    hidden = [model.prompt(tokens[:, :70], lengths)] + [model.step(tokens[:, 70 + t]) for t in range(5)]
+    logits = torch.stack([torch.stack([h[lane] for h in hidden]) for lane in range(3)])  # lane, step, channel
+    out = torch.empty((18, VOCAB), device="cuda")
+    model.head.product(logits.flatten(0, 1), out)
+    for lane, n in enumerate(lengths.tolist()):
+        rows = torch.cat((tokens[lane, :n], tokens[lane, 70:])).tolist()
+        want = torch.from_numpy(plain_logits(rows)[n - 1:])
+        off = (out.view(3, 6, VOCAB)[lane].double().cpu() - want).abs().amax(1)
+        assert (off <= CLOSE * want.square().mean(1).sqrt()).all(), (lane, off)
+
+
+def test_lanes_without_tokens_draft_like_any_other():
+    """a lane of length 0 begins from zeros; the others are not touched by it"""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    tokens, draws = torch.randint(0, VOCAB, (3, 20), generator=gen, device="cuda"), torch.rand((4, 3), generator=gen, device="cuda")
+    lengths = torch.tensor([20, 0, 7], dtype=torch.int32, device="cuda")
+    model = make()
+    out = model.generate(tokens, 4, draws, lengths=lengths)
+    assert ((out >= 0) & (out < VOCAB)).all()
+    keep = torch.tensor([0, 2], device="cuda")
+    assert torch.equal(model.generate(tokens[keep], 4, draws[:, keep], lengths=lengths[keep]), out[keep])
+    assert model.generate(tokens[:, :0], 2, draws[:2]).shape == (3, 2)
+    model.reset(2)
+    with pytest.raises(load_module("clear_ops").ClearError):
+        model.step(tokens[:, 0])  # three lanes for two states
