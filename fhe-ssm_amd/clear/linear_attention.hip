@@ -257,8 +257,9 @@ struct ChunkArgs {
 
 // What the outputs read, keys (a token a row) and the state before the chunk (a column a row), and what the state's update
 // reads, decayed keys (a channel a row).  Of more than 64 channels the second takes the place of the first, at two barriers
-// more, so that two workgroups fit a CU (4 prompts of 2,048, heads of 128: 140 against 97 us; of 64 it costs: 32 prompts of 512
-// to 1024 78 against 89 us).
+// more, so that two workgroups fit a CU (4 prompts of 2,048, heads of 128: 141 against 102 us; of 64 it costs: 32 prompts of 512
+// to 1024 85 against 89 us, in float16 101 against 108).  256 registers are then all that a lane has: the kernels that make
+// outputs of heads above 64 spill 44 (bf16), 8 and 40 of them (32 columns, bf16 and float16).
 template <class X, int DK, int TV>
 struct KeysApart {
     uint16_t k[kKeyPieces<X>][kChunk][DK + kPad];
@@ -288,9 +289,9 @@ struct ChunkShared : std::conditional<in_turn(DK), KeysInTurn<X, DK, TV>, KeysAp
 // 16 x 16 tiles.  The scores of a token, as they come out of one product (a lane: one query, four neighbouring keys), go into
 // the next one without leaving their registers: the values are read in the order of keys that this makes.
 // kOut: outputs from the state before the segment; otherwise what the segment adds to the state, and its log decay.
-// It is bound by the latency of a chunk's chain (decays, LDS, scores, outputs, state; about 9,400 cycles, in which the vector
-// units are busy for a third and the matrix units for a tenth): 32 prompts of 512 to 1,024 tokens, 12 heads of 64, 120 MB,
-// take 80 us; one of 8,192 tokens 47 us, 14 of them for what segments add, 6.5 to join them and 27 for the outputs.
+// It is bound by the latency of a chunk's chain (decays, LDS, scores, outputs, state; about 11,500 cycles of a wave, for 31 % of
+// which it issues vector and for 10 % matrix instructions): 32 prompts of 512 to 1,024 tokens, 12 heads of 64, 120 MB, take 82
+// to 87 us; one of 8,192 tokens 47 to 49 us, 14 of them for what segments add, 6.5 to join them and 28 for the outputs.
 template <class X, int DK, int TV, bool kOut>
 __global__ __launch_bounds__(256, (in_turn(DK) && sizeof(ChunkShared<X, DK, TV>) * 2 <= 160 << 10 ? 2 : 1)) void k_chunks(ChunkArgs c) {
     constexpr int P = kPieces<X>, PK = kKeyPieces<X>, KK = DK / 32, CT = TV / 16, ST = DK / 16 * CT / 4;
@@ -764,7 +765,7 @@ auto by_type(uint32_t type, F&& f) {
 }
 
 // how a prompt is cut: by token (segments 0), or by chunks in so many segments
-// By token 12 heads of 64 take 4.2 us for one token, 9.8 for 8 and 0.9 for each more, by chunks 7.0 us for up to 64.
+// By token 12 heads of 64 take 4.2 us for one token, 9.8 for 8 and 0.9 for each more, by chunks 7.2 us for up to 64.
 struct Plan {
     uint32_t tile, segments, segment;
     size_t sums_at, bytes;
@@ -775,15 +776,15 @@ Plan plan(const fhe_ssm_linear_attention* a) {
     if (a->tokens <= (uint32_t)kByToken || !a->lanes) return p;
     const uint32_t items = a->lanes * a->heads, chunks = (a->tokens + kChunk - 1) / kChunk;
     // 64 columns of the state to a workgroup, or 32 where that leaves the GPU empty, though their keys and scores are worked
-    // out twice (12 heads of one prompt: 64 tokens 8.3 against 7.0 us, 2,048 29.1 against 27.1; 8,192 50 against 58).  The
-    // three pieces of float32 leave LDS for two workgroups of 32 columns on a CU (4 prompts of 2,048: 79.7 against 70.4 us).
+    // out twice (12 heads of one prompt: 64 tokens 8.8 against 7.7 us, 2,048 27.4 against 26.5; 8,192 49 against 58).  The
+    // three pieces of float32 leave LDS for two workgroups of 32 columns on a CU (4 prompts of 2,048: 82 against 73 us).
     const uint64_t wide = (uint64_t)items * ((a->dv + 63) / 64);
     p.tile = a->type == FHE_SSM_F32 || (wide <= 192 && wide * chunks <= 384) ? 32 : 64;
     const uint32_t groups = items * ((a->dv + p.tile - 1) / p.tile);
     p.segments = 1;
     // the chunks of a prompt one after the other, or in segments on 512 workgroups, with two launches more (12 heads of one
-    // prompt: 256 tokens 15.8 against 13.8 us, 8,192 450 against 47, on 1,024 workgroups 51.6; 32 ragged prompts, which are
-    // 384 workgroups in themselves, 80 against 126)
+    // prompt: 256 tokens 16.1 against 14.7 us, 8,192 485 against 49, on 1,024 workgroups 52; 32 ragged prompts, which are 384
+    // workgroups in themselves, 86 against 111)
     if (groups < 256 && chunks >= 4) p.segments = std::min(chunks, 512 / groups);
     const uint32_t each = (chunks + p.segments - 1) / p.segments;
     p.segment = each * kChunk;

@@ -436,8 +436,8 @@ __device__ __forceinline__ Prefix shortest(const R& row, const Scale& scale, Sha
     return p;
 }
 
-// kWavesEach: waves that a SIMD has to hold.  4, one row on a CU, leaves enough registers; 8 costs some spills and lets two
-// rows share a CU: 300 rows of 50,277 by top-k 30.5 against 23.7 us, 256 rows of 65,536 27.9 against 28.8 us.
+// kWavesEach: waves that a SIMD has to hold.  4, one row on a CU, leaves enough registers; 8 spills 40 and lets two rows
+// share a CU: 300 rows of 50,277 by top-k 30.5 against 23.7 us, 256 rows of 65,536 27.9 against 28.8 us.
 template <class X, int kWavesEach>
 __global__ __launch_bounds__(kThreads, kWavesEach) void k_sample(const X* __restrict__ logits, uint32_t vocab, int64_t stride,
                                                         const float* __restrict__ draws, fhe_ssm_sample_params p,

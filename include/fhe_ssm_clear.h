@@ -38,8 +38,8 @@ const char* fhe_ssm_clear_last_error(void);
 /* ---- linear attention with a decay for each head ------------------------------------------------------------------
  * Per lane and head, with the state S in R^{dk x dv} (float32) and the log decay g_t <= 0:
  *     S_t = exp(g_t) S_{t-1} + k_t v_t^T        o_t = scale * q_t S_t
- * lanes and tokens may be 0.  Shared heads: head h reads query head h / (heads / q_heads) and key head
- * h / (heads / k_heads); values, decays, outputs and states are per head.  dk <= 128.
+ * lanes and tokens may be 0.  dk <= 128, tokens <= 2^24, lanes * heads * ceil(dv / 32) < 2^24.  Shared heads: head h reads
+ * query head h / (heads / q_heads) and key head h / (heads / k_heads); values, decays, outputs and states are per head.
  * Strides are in elements, in the order lane, token, head, and may be any (0 shares one row among many), except that
  * different output rows must not overlap; channels are contiguous.  State: [lanes][heads][dk][dv], contiguous;
  * state_in null means zero, state_out null drops the new state, and the two may be the same buffer.  out must overlap
@@ -70,7 +70,8 @@ int fhe_ssm_linear_attention_step(const fhe_ssm_linear_attention* a, const void*
 /* ---- products with 4-bit weights and group scales -----------------------------------------------------------------
  *     y[r][o] = sum_j scale[o][j / group] (code[o][j] - zero[o][j / group]) x[r][j]
  * Codes 0..15, two in a byte (the lower index in the low four bits), rows of (in + 1) / 2 bytes; zero points 0..15 per
- * group, or 8 throughout; the last group may be cut short.  group is 32, 64 or a multiple of 128.
+ * group, or 8 throughout; the last group may be cut short.  group is 32, 64 or a multiple of 128, rows <= 2^20,
+ * ceil(out / 16) * ceil(in / 128) < 2^24.
  * The matrix is laid out once (fhe_ssm_q4_arrange) in the order the kernel reads it; bf16 scales are widened to float32
  * there, float16 ones stay.  Codes and zero points are used exactly; float32 rows are used to their full 24 bits.
  * Sums go through codes held as 16 + c: a row of x with an infinity or a NaN gives NaN in all its outputs and leaves other
@@ -101,7 +102,7 @@ int fhe_ssm_q4_product(const fhe_ssm_q4_matrix* m, const void* weights, uint32_t
  * filter off; top_p <= 0 leaves the first entry, min_p >= 1 those that equal it.  draw is held to [0, 1).  A NaN logit or -inf is never
  * drawn, entries of +inf share the whole mass; a row of nothing else gives token -1 and log-probability -inf.  An entry
  * of 2^-44 of the largest mass or less counts for nothing, also where a filter keeps it.  A
- * parameter that is NaN turns its filter off (temperature: 0, draw: 0).
+ * parameter that is NaN turns its filter off (temperature: 0, draw: 0).  vocab <= 2^18, rows < 2^22.
  * Each parameter array holds one value per row, or a null pointer turns it off (temperature null: 1).  float32, k int32.
  */
 typedef struct {
