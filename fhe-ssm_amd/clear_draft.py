@@ -72,7 +72,8 @@ class Draft:
 
     def _run(self, tokens, lengths):
         """tokens [lanes, n] or, for one step, [lanes]: hidden rows of the same shape, the states carried on"""
-        clear_ops._need(len(self.states) == len(self.w_in), "reset(lanes) makes the states that prompt and step carry on")
+        if len(self.states) != len(self.w_in):
+            raise clear_ops.ClearError("reset(lanes) makes the states that prompt and step carry on")
         x = self.embedding[tokens].float()
         for w_in, w_out, state in zip(self.w_in, self.w_out, self.states):
             q, k, v, gate = self._product(w_in, self._norm(x)).unflatten(-1, (4, self.heads, self.hs)).unbind(-3)
