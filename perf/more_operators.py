@@ -52,9 +52,11 @@ def listed():
         {"name": "embedding few", "op": "embedding", "tokens": 701, "vocab": 50277, "channels": 1101, "pad": False,
          "add": True, "type": "f32"},
         # the draft's view of the answered tokens of all lanes, with the alternatives that a client shows
-        {"name": "score lanes", "op": "score", "rows": 32, "vocab": 65536, "top": 20, "train": False, "type": "f32"},
-        # the loss of a part of the training batch, and its gradient
-        {"name": "score train", "op": "score", "rows": 4096, "vocab": 65536, "top": 0, "train": True, "type": "bf16"},
+        {"name": "score lanes", "op": "score", "rows": 32, "vocab": 65536, "top": 20, "train": False, "later": False,
+         "type": "f32"},
+        # the loss of a part of the training batch, and its gradient with weights that are known before
+        {"name": "score train", "op": "score", "rows": 4096, "vocab": 65536, "top": 0, "train": True, "later": False,
+         "type": "bf16"},
         # the step of a small model's tensors, among them many short ones, in float32
         {"name": "adamw 32", "op": "adamw", "bits": 32, "count": 40, "most": 2359296, "type": "f32"},
         # the step of a large model's, its states in 8 bits
@@ -89,7 +91,8 @@ def draw(rng):
     if op == "score":
         vocab = _log(rng, 100, 131072)
         return {**case, "vocab": vocab, "rows": _log(rng, 1, min(16384, (1 << 27) // vocab)),
-                "top": min(rng.choice([0, 1, 5, 20, 32]), vocab // 97), "train": rng.random() < 0.5}
+                "top": min(rng.choice([0, 1, 5, 20, 32]), vocab // 97), "train": rng.random() < 0.5,
+                "later": rng.random() < 0.3}
     most = _log(rng, 300, 1 << 24)
     return {**case, "bits": rng.choice([8, 32]), "most": most, "count": _log(rng, 1, 60 if most < (1 << 21) else 6)}
 
@@ -306,12 +309,16 @@ def _own(st):
         return {"out": st.out, "grad": st.grad}
     if op == "score":
         logits, tokens, weight, weight_entropy = st.inputs
-        ops.token_logprobs(logits, tokens, st.logprobs, st.entropy, st.lse, st.top, st.top_logprobs, workspace=st.workspace)
+        known = {} if not case["train"] or case["later"] else \
+            {"weights": weight, "entropy_weights": weight_entropy, "gradient": st.grad}
+        ops.token_logprobs(logits, tokens, st.logprobs, st.entropy, st.lse, st.top, st.top_logprobs, workspace=st.workspace,
+                           **known)
         out = {"logprobs": st.logprobs, "entropy": st.entropy}
         if case["top"]:
             out.update(top=st.top, top_logprobs=st.top_logprobs)
         if case["train"]:
-            ops.token_logprobs_gradient(logits, tokens, st.lse, weight, st.grad, weight_entropy, st.entropy)
+            if case["later"]:  # weights that hang on the log-probabilities
+                ops.token_logprobs_gradient(logits, tokens, st.lse, weight, st.grad, weight_entropy, st.entropy)
             out["grad"] = st.grad
         return out
     p, _, states = st.inputs
@@ -441,11 +448,11 @@ def _of_8_bits(codes, exponent):
 
 
 def _draws(case, device):
-    """two times 16 bits for every entry, by its tensor's place and its own"""
+    """two times 16 bits for every entry, by the step, its tensor's place and its own"""
     starts, length = _starts(case)
     begin = torch.tensor(starts, device=device)
     whole = torch.diff(begin, append=begin.new_tensor([length]))
-    key = _mixed(ADAMW["seed"] + 0x9E3779B1 * torch.arange(len(starts), device=device) & 0xffffffff)
+    key = _mixed(ADAMW["seed"] + 0xB7E15163 * ADAMW["step"] + 0x9E3779B1 * torch.arange(len(starts), device=device) & 0xffffffff)
     local = torch.arange(length, device=device) - begin.repeat_interleave(whole)
     h = _mixed(key.repeat_interleave(whole) + local & 0xffffffff)
     return h & 0xffff, h >> 16
