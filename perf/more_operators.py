@@ -248,7 +248,7 @@ def prepare(case, seed):
     elif op == "score":
         logits = st.inputs[0]
         rows = len(logits)
-        st.logprobs, st.entropy, st.lse = (torch.empty(rows, device="cuda") for _ in range(3))
+        st.logprobs, st.entropy, st.stats = (torch.empty(n, device="cuda") for n in (rows, rows, (rows, 2)))
         st.top = torch.empty((rows, case["top"]), dtype=torch.int64, device="cuda") if case["top"] else None
         st.top_logprobs = torch.empty((rows, case["top"]), device="cuda") if case["top"] else None
         st.workspace = _bytes(ops.token_logprobs_workspace(logits, case["top"]))
@@ -311,14 +311,14 @@ def _own(st):
         logits, tokens, weight, weight_entropy = st.inputs
         known = {} if not case["train"] or case["later"] else \
             {"weights": weight, "entropy_weights": weight_entropy, "gradient": st.grad}
-        ops.token_logprobs(logits, tokens, st.logprobs, st.entropy, st.lse, st.top, st.top_logprobs, workspace=st.workspace,
+        ops.token_logprobs(logits, tokens, st.logprobs, st.entropy, st.stats, st.top, st.top_logprobs, workspace=st.workspace,
                            **known)
         out = {"logprobs": st.logprobs, "entropy": st.entropy}
         if case["top"]:
             out.update(top=st.top, top_logprobs=st.top_logprobs)
         if case["train"]:
             if case["later"]:  # weights that hang on the log-probabilities
-                ops.token_logprobs_gradient(logits, tokens, st.lse, weight, st.grad, weight_entropy, st.entropy)
+                ops.token_logprobs_gradient(logits, tokens, st.stats, weight, st.grad, weight_entropy, st.entropy)
             out["grad"] = st.grad
         return out
     p, _, states = st.inputs
