@@ -1,0 +1,371 @@
+// gated_recurrence.hip -- the gated linear recurrence over a prompt, its gradient, and its step of one token.
+//
+//   a_t = sigmoid(z_t),   h_t = a_t h_{t-1} + (1 - a_t) x_t                          (per channel; h in float32)
+//   d_t = dy_t + c_t,   c_{t-1} = a_t d_t,   dx_t = (1 - a_t) d_t,   dz_t = a_t (1 - a_t) d_t (h_{t-1} - x_t)
+//
+// c after the last token is the gradient of the state that is handed on, c before the first that of the state it began with.
+// A run of tokens maps h to A h + H and, backwards, c to A c + G, with the same A, the product of its a.
+//
+// A workgroup has 64 channels of a lane and goes over its tokens tile by tile: each of its eight waves loads 16 tokens, folds
+// them to A and H (and G), and finds the state before its own tokens from those of the waves before it, through LDS with one
+// barrier a tile.  So every input is read once, in rows of 64 channels, and no token waits for more than its own wave's.  The
+// backward pass needs h again, which it forms from z and x as it reads them anyway, from the states at the tiles' beginnings
+// that the forward pass kept (one float a channel for 128 tokens); so it reads no outputs, and h is float32 whatever their type.
+// Few lanes with many tokens are cut into segments of tiles: a first pass folds every segment to one A and H (or G), and a
+// segment's workgroup begins with those of the segments before it.  Then the inputs are read twice.
+// Bound by bytes: about 12 (backward 25) vector instructions an element.
+#include <algorithm>
+
+#include "rows.hpp"
+
+namespace clear {
+namespace {
+
+constexpr int kWaves = 8, kRun = 16;      // waves of a workgroup; tokens of a wave
+constexpr int kTile = kWaves * kRun;      // tokens between kept states
+constexpr uint32_t kEnough = 512;         // workgroups: two for each CU
+
+struct Args {
+    const void *z, *x, *dy;
+    void *out, *dz, *dx;
+    const int32_t* lengths;
+    const float* in;     // forward the state before, backward the gradient of the state after; null: 0
+    float* last;         // forward the state after, backward the gradient of the state before
+    float* saved;        // [lane][tile][channel]: states before tiles
+    float* folded;       // of segments: [lane][segment][2][channel], then copies of `in` [lane][channel]
+    uint32_t lanes, tokens, channels, strips, tiles, segments, each;  // each: tiles of a segment
+    int64_t zs[2], xs[2], dys[2], outs[2], dzs[2], dxs[2];
+};
+
+// sigmoid(z) and sigmoid(-z), both to their last bits: the smaller is e / (1 + e) with e = exp(-|z|), the larger 1 less that, so
+// that gates near 1, of which many are multiplied, are rounded and no more (a reciprocal is off to one side)
+__device__ inline void gates(float z, float& a, float& rest) {
+    const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(z));
+    const float small = e * __builtin_amdgcn_rcpf(1.f + e), large = 1.f - small;
+    a = z < 0.f ? small : large;
+    rest = z < 0.f ? large : small;
+}
+
+__device__ inline uint32_t length_of(const Args& a, uint32_t lane) {
+    return a.lengths ? (uint32_t)min(max(a.lengths[lane], 0), (int)a.tokens) : a.tokens;
+}
+
+// the state (or gradient) that a segment begins with: what came in, through the segments before it (after it)
+template <bool kBack>
+__device__ inline float begin(const Args& a, uint32_t lane, uint32_t segment, uint32_t c) {
+    if (a.segments == 1) return a.in ? a.in[(size_t)lane * a.channels + c] : 0.f;
+    float s = a.folded[((size_t)a.lanes * a.segments * 2 + lane) * a.channels + c];
+    const float* f = a.folded + (size_t)lane * a.segments * 2 * a.channels + c;
+    const uint32_t n = kBack ? a.segments - 1 - segment : segment;
+#pragma unroll 8
+    for (uint32_t i = 0; i < n; i++) {
+        const float* at = f + (size_t)(kBack ? a.segments - 1 - i : i) * 2 * a.channels;
+        s = at[0] * s + at[a.channels];
+    }
+    return s;
+}
+
+// The forward pass; !kOut: only the segments' A and H.
+template <class T, bool kOut>
+__global__ __launch_bounds__(kWaves * 64) void k_forward(Args a) {
+    __shared__ float s_a[2][kWaves][64], s_h[2][kWaves][64];
+    const uint32_t strip = blockIdx.x % a.strips, segment = blockIdx.x / a.strips % a.segments, lane = blockIdx.x / a.strips / a.segments;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64, c = strip * 64 + l;
+    const bool in = c < a.channels;
+    const uint32_t length = length_of(a, lane);
+    const uint32_t tile1 = min(a.tiles, (segment + 1) * a.each);
+    const T *z = (const T*)a.z + lane * a.zs[0], *x = (const T*)a.x + lane * a.xs[0];
+    T* out = kOut ? (T*)a.out + lane * a.outs[0] : nullptr;
+    const size_t at = (size_t)lane * a.channels + c;
+    float state = 0.f, product = 1.f;
+    if (kOut && in) state = begin<false>(a, lane, segment, c);
+    for (uint32_t tile = segment * a.each; tile < tile1; tile++) {
+        const uint32_t t0 = tile * kTile + wave * kRun;
+        float g[kRun], b[kRun], A = 1.f, H = 0.f;
+        if (kOut && a.saved && wave == 0 && in) a.saved[((size_t)lane * a.tiles + tile) * a.channels + c] = state;
+        if (t0 + kRun <= length) {
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                g[i] = in ? to_f32(z[(int64_t)(t0 + i) * a.zs[1] + c]) : 0.f;
+                b[i] = in ? to_f32(x[(int64_t)(t0 + i) * a.xs[1] + c]) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                float rest;
+                gates(g[i], g[i], rest);
+                b[i] *= rest;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                g[i] = 1.f, b[i] = 0.f;  // a token that is not there keeps the state
+                if (t0 + i < length && in) {
+                    float rest;
+                    gates(to_f32(z[(int64_t)(t0 + i) * a.zs[1] + c]), g[i], rest);
+                    b[i] = rest * to_f32(x[(int64_t)(t0 + i) * a.xs[1] + c]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kRun; i++) {
+            H = g[i] * H + b[i];
+            A *= g[i];
+        }
+        const int turn = tile & 1;
+        s_a[turn][wave][l] = A;
+        s_h[turn][wave][l] = H;
+        __syncthreads();
+        float mine = state;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) {
+            if (w == wave) mine = state;
+            state = s_a[turn][w][l] * state + s_h[turn][w][l];
+            if (!kOut) product *= s_a[turn][w][l];
+        }
+        if (kOut && in) {
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                mine = g[i] * mine + b[i];
+                if (t0 + i < a.tokens) out[(int64_t)(t0 + i) * a.outs[1] + c] = from_f32<T>(t0 + i < length ? mine : 0.f);
+            }
+        }
+    }
+    if (wave != 0 || !in) return;
+    if (kOut) {
+        if (a.last && segment == a.segments - 1) a.last[at] = state;
+    } else {
+        float* f = a.folded + ((size_t)lane * a.segments + segment) * 2 * a.channels + c;
+        f[0] = product;
+        f[a.channels] = state;
+        // `in` and `last` may be one buffer, and workgroups of the second pass read the one while one of them writes the other
+        if (segment == 0) a.folded[((size_t)a.lanes * a.segments * 2) * a.channels + at] = a.in ? a.in[at] : 0.f;
+    }
+}
+
+// The backward pass, from the last tile to the first; !kOut: only the segments' A and G.
+template <class T, bool kOut>
+__global__ __launch_bounds__(kWaves * 64) void k_backward(Args a) {
+    __shared__ float s_a[2][kWaves][64], s_h[2][kWaves][64], s_g[2][kWaves][64];
+    const uint32_t strip = blockIdx.x % a.strips, segment = blockIdx.x / a.strips % a.segments, lane = blockIdx.x / a.strips / a.segments;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64, c = strip * 64 + l;
+    const bool in = c < a.channels;
+    const uint32_t length = length_of(a, lane);
+    const uint32_t tile0 = segment * a.each, tile1 = min(a.tiles, tile0 + a.each);
+    const T *z = (const T*)a.z + lane * a.zs[0], *x = (const T*)a.x + lane * a.xs[0];
+    const T* dy = a.dy ? (const T*)a.dy + lane * a.dys[0] : nullptr;
+    T *dz = (T*)a.dz + lane * a.dzs[0], *dx = (T*)a.dx + lane * a.dxs[0];
+    const size_t at = (size_t)lane * a.channels + c;
+    float carry = 0.f, product = 1.f;
+    if (kOut && in) carry = begin<true>(a, lane, segment, c);
+    for (uint32_t tile = tile1; tile-- > tile0;) {
+        const uint32_t t0 = tile * kTile + wave * kRun;
+        float g[kRun], r[kRun], b[kRun], d[kRun];
+        float h = kOut && in ? a.saved[((size_t)lane * a.tiles + tile) * a.channels + c] : 0.f;
+        if (t0 + kRun <= length) {
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                g[i] = in ? to_f32(z[(int64_t)(t0 + i) * a.zs[1] + c]) : 0.f;
+                b[i] = kOut && in ? to_f32(x[(int64_t)(t0 + i) * a.xs[1] + c]) : 0.f;
+                d[i] = dy && in ? to_f32(dy[(int64_t)(t0 + i) * a.dys[1] + c]) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kRun; i++) gates(g[i], g[i], r[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                g[i] = 1.f, r[i] = b[i] = d[i] = 0.f;
+                if (t0 + i < length && in) {
+                    gates(to_f32(z[(int64_t)(t0 + i) * a.zs[1] + c]), g[i], r[i]);
+                    if (kOut) b[i] = to_f32(x[(int64_t)(t0 + i) * a.xs[1] + c]);
+                    if (dy) d[i] = to_f32(dy[(int64_t)(t0 + i) * a.dys[1] + c]);
+                }
+            }
+        }
+        float A = 1.f, H = 0.f, G = 0.f;
+#pragma unroll
+        for (int i = 0; i < kRun; i++) {
+            A *= g[i];
+            H = g[i] * H + r[i] * b[i];
+        }
+#pragma unroll
+        for (int i = kRun; i-- > 0;) G = g[i] * (G + d[i]);
+        const int turn = tile & 1;
+        s_a[turn][wave][l] = A;
+        if (kOut) s_h[turn][wave][l] = H;
+        s_g[turn][wave][l] = G;
+        __syncthreads();
+        float mine = carry;
+#pragma unroll
+        for (int w = kWaves; w-- > 0;) {
+            if ((uint32_t)w == wave) mine = carry;
+            carry = s_a[turn][w][l] * carry + s_g[turn][w][l];
+            if (!kOut) product *= s_a[turn][w][l];
+        }
+        if (kOut) {
+#pragma unroll
+            for (uint32_t w = 0; w < kWaves - 1; w++)
+                if (w < wave) h = s_a[turn][w][l] * h + s_h[turn][w][l];
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {  // b: what dz takes besides d
+                const float next = g[i] * h + r[i] * b[i];
+                b[i] = g[i] * r[i] * (h - b[i]);
+                h = next;
+            }
+            if (in) {
+#pragma unroll
+                for (int i = kRun; i-- > 0;) {
+                    const float now = d[i] + mine;
+                    mine = g[i] * now;
+                    if (t0 + i < a.tokens) {
+                        const bool there = t0 + i < length;
+                        dz[(int64_t)(t0 + i) * a.dzs[1] + c] = from_f32<T>(there ? now * b[i] : 0.f);
+                        dx[(int64_t)(t0 + i) * a.dxs[1] + c] = from_f32<T>(there ? now * r[i] : 0.f);
+                    }
+                }
+            }
+        }
+    }
+    if (wave != 0 || !in) return;
+    if (kOut) {
+        if (a.last && segment == 0) a.last[at] = carry;
+    } else {
+        float* f = a.folded + ((size_t)lane * a.segments + segment) * 2 * a.channels + c;
+        f[0] = product;
+        f[a.channels] = carry;
+        if (segment == 0) a.folded[((size_t)a.lanes * a.segments * 2) * a.channels + at] = a.in ? a.in[at] : 0.f;
+    }
+}
+
+// One token for every lane: an element a thread.  Bound by its launch.
+template <class T>
+__global__ __launch_bounds__(256) void k_step(Args a) {
+    const uint32_t at = blockIdx.x * 256 + threadIdx.x;
+    if (at >= a.lanes * a.channels) return;
+    const uint32_t lane = at / a.channels, c = at - lane * a.channels;
+    float gate, rest;
+    gates(to_f32(((const T*)a.z)[lane * a.zs[0] + c]), gate, rest);
+    const float h = gate * (a.in ? a.in[at] : 0.f) + rest * to_f32(((const T*)a.x)[lane * a.xs[0] + c]);
+    ((T*)a.out)[lane * a.outs[0] + c] = from_f32<T>(h);
+    if (a.last) a.last[at] = h;
+}
+
+int check(const fhe_ssm_gated_recurrence* a) {
+    if (!a) return fail(CKKS_EINVAL, "gated recurrence: null description");
+    if (a->type > FHE_SSM_F16) return fail(CKKS_EINVAL, "gated recurrence: unknown type %u", a->type);
+    if (a->channels < 1) return fail(CKKS_EINVAL, "gated recurrence: no channels");
+    // a launch has less than 2^32 threads
+    if (a->tokens > 1u << 24 || a->channels > 1u << 24 || (uint64_t)a->lanes * ((a->channels + 63) / 64) >= 1ull << 23)
+        return fail(CKKS_EINVAL, "gated recurrence: too many tokens, lanes or channels");
+    return CKKS_OK;
+}
+
+// rows of an output must not meet, whether they follow lane by lane or token by token
+bool apart(const int64_t* s, const fhe_ssm_gated_recurrence& a) {
+    const int64_t c = a.channels, n = a.tokens, m = a.lanes;
+    if (n <= 1) return m <= 1 || s[0] >= c;
+    if (m <= 1) return s[1] >= c;
+    return (s[1] >= c && s[0] >= (n - 1) * s[1] + c) || (s[0] >= c && s[1] >= (m - 1) * s[0] + c);
+}
+
+void lay_out(Args& k, const fhe_ssm_gated_recurrence& a) {
+    k.lanes = a.lanes, k.tokens = a.tokens, k.channels = a.channels;
+    k.strips = (a.channels + 63) / 64;
+    k.tiles = (a.tokens + kTile - 1) / kTile;
+    // segments where lanes and strips leave CUs without work; each of two tiles at least
+    const uint64_t have = (uint64_t)std::max(1u, a.lanes) * k.strips;
+    uint32_t want = have >= kEnough / 2 ? 1 : (uint32_t)(kEnough / have);
+    want = std::max(1u, std::min(want, k.tiles / 2));
+    k.each = std::max(1u, (k.tiles + want - 1) / want);
+    k.segments = std::max(1u, (k.tiles + k.each - 1) / k.each);
+    for (int i = 0; i < 2; i++) k.zs[i] = a.z_stride[i], k.xs[i] = a.x_stride[i], k.outs[i] = a.out_stride[i];
+}
+
+size_t folded_bytes(const Args& k) {
+    return k.segments > 1 ? (size_t)k.lanes * k.channels * (2 * k.segments + 1) * sizeof(float) : 0;
+}
+
+int workspace_of(Args& k, void* workspace, size_t bytes) {
+    const size_t need = folded_bytes(k);
+    if (need && (!workspace || !aligned(workspace, 16) || bytes < need))
+        return fail(CKKS_EINVAL, "gated recurrence: the workspace must have %zu bytes and lie on 16", need);
+    k.folded = (float*)workspace;
+    return CKKS_OK;
+}
+
+}  // namespace
+}  // namespace clear
+
+extern "C" {
+
+int fhe_ssm_gated_recurrence_workspace(const fhe_ssm_gated_recurrence* a, size_t* workspace_bytes, size_t* saved_bytes) {
+    using namespace clear;
+    if (int rc = check(a)) return rc;
+    Args k{};
+    lay_out(k, *a);
+    if (workspace_bytes) *workspace_bytes = folded_bytes(k);
+    if (saved_bytes) *saved_bytes = (size_t)k.lanes * k.tiles * k.channels * sizeof(float);
+    return CKKS_OK;
+}
+
+int fhe_ssm_gated_recurrence_prompt(const fhe_ssm_gated_recurrence* a, const void* z, const void* x, const int32_t* lengths,
+                                    const float* state_in, float* state_out, void* out, void* saved, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+    using namespace clear;
+    if (int rc = check(a)) return rc;
+    if (a->lanes == 0) return CKKS_OK;
+    if (a->tokens && (!z || !x || !out)) return fail(CKKS_EINVAL, "gated recurrence: null argument");
+    if (!apart(a->out_stride, *a)) return fail(CKKS_EINVAL, "gated recurrence: output rows overlap");
+    Args k{};
+    lay_out(k, *a);
+    if (int rc = workspace_of(k, workspace, workspace_bytes)) return rc;
+    k.z = z, k.x = x, k.out = out, k.lengths = lengths, k.in = state_in, k.last = state_out, k.saved = (float*)saved;
+    return by_type(a->type, [&](auto t) {
+        typedef decltype(t) T;
+        const dim3 grid(k.lanes * k.segments * k.strips), block(kWaves * 64);
+        if (k.segments > 1) hipLaunchKernelGGL((k_forward<T, false>), grid, block, 0, (hipStream_t)stream, k);
+        hipLaunchKernelGGL((k_forward<T, true>), grid, block, 0, (hipStream_t)stream, k);
+        return launched("gated recurrence");
+    });
+}
+
+int fhe_ssm_gated_recurrence_backward(const fhe_ssm_gated_recurrence* a, const void* z, const void* x, const int32_t* lengths,
+                                      const void* saved, const void* dout, const float* dstate_out, void* dz, void* dx,
+                                      float* dstate_in, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace clear;
+    if (int rc = check(a)) return rc;
+    if (a->lanes == 0) return CKKS_OK;
+    if (a->tokens && (!z || !x || !saved || !dz || !dx)) return fail(CKKS_EINVAL, "gated recurrence: null argument");
+    if (!apart(a->dz_stride, *a) || !apart(a->dx_stride, *a)) return fail(CKKS_EINVAL, "gated recurrence: output rows overlap");
+    Args k{};
+    lay_out(k, *a);
+    if (int rc = workspace_of(k, workspace, workspace_bytes)) return rc;
+    k.z = z, k.x = x, k.dy = dout, k.dz = dz, k.dx = dx, k.lengths = lengths, k.in = dstate_out, k.last = dstate_in, k.saved = (float*)saved;
+    for (int i = 0; i < 2; i++) k.dys[i] = a->dout_stride[i], k.dzs[i] = a->dz_stride[i], k.dxs[i] = a->dx_stride[i];
+    return by_type(a->type, [&](auto t) {
+        typedef decltype(t) T;
+        const dim3 grid(k.lanes * k.segments * k.strips), block(kWaves * 64);
+        if (k.segments > 1) hipLaunchKernelGGL((k_backward<T, false>), grid, block, 0, (hipStream_t)stream, k);
+        hipLaunchKernelGGL((k_backward<T, true>), grid, block, 0, (hipStream_t)stream, k);
+        return launched("gated recurrence: gradient");
+    });
+}
+
+int fhe_ssm_gated_recurrence_step(const fhe_ssm_gated_recurrence* a, const void* z, const void* x, const float* state_in,
+                                  float* state_out, void* out, void* stream) {
+    using namespace clear;
+    if (int rc = check(a)) return rc;
+    if (a->tokens != 1) return fail(CKKS_EINVAL, "gated recurrence: a step has one token, not %u", a->tokens);
+    if (a->lanes == 0) return CKKS_OK;
+    if (!z || !x || !out) return fail(CKKS_EINVAL, "gated recurrence: null argument");
+    if (!apart(a->out_stride, *a)) return fail(CKKS_EINVAL, "gated recurrence: output rows overlap");
+    Args k{};
+    lay_out(k, *a);
+    k.z = z, k.x = x, k.out = out, k.in = state_in, k.last = state_out;
+    const dim3 grid((uint32_t)(((uint64_t)k.lanes * k.channels + 255) / 256));
+    return by_type(a->type, [&](auto t) {
+        hipLaunchKernelGGL(k_step<decltype(t)>, grid, dim3(256), 0, (hipStream_t)stream, k);
+        return launched("gated recurrence: step");
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,325 @@
+// layer_norm.hip -- layer norm over the channels of rows, and its gradient.
+//
+//   h = (x - mean) rstd,  y = h w + b;      with t = dy w:  dx = rstd (t - mean(t) - h mean(t h)),  dw = sum dy h,  db = sum dy
+//
+// Both are bound by the bytes of x, y and dy, dx: a row is read once and stays in registers, where its mean and then the sum of
+// its squared distances from that mean are taken (a difference of two large sums would lose a row that lies far from 0).  L
+// lanes share a row: 16, a wave, or a workgroup, whichever holds its channels at 4 to 32 a lane.  They walk on to other rows with
+// the weights still in registers, and in the backward pass with their channels' sums of dw and db, which a workgroup joins in
+// LDS and writes as one part; a second kernel adds the parts.  No order depends on timing.
+#include <algorithm>
+
+#include "rows.hpp"
+
+namespace clear {
+namespace {
+
+constexpr uint32_t kMostChannels = 16384;
+
+struct Args {
+    const void *x, *dy, *w, *b;
+    void* y;  // the output, backward dx
+    float *mean, *rstd, *dw, *db, *parts;
+    uint32_t rows, d;
+    bool wide;  // weights are float32
+    int64_t xs, dys, ys;
+    float eps, n, each;  // d as a float, and its reciprocal
+};
+
+template <class T>
+__device__ inline float weight(const void* w, bool wide, uint32_t i, float none) {
+    return !w ? none : wide ? ((const float*)w)[i] : to_f32(((const T*)w)[i]);
+}
+
+// the row's elements of this lane, zeros past its end: group j of V lies at (j L + lane) V
+template <int L, int V, int E, class T>
+__device__ inline void load_row(const T* p, uint32_t lane, uint32_t d, float (&f)[E]) {
+#pragma unroll
+    for (int j = 0; j < E / V; j++) {
+        const uint32_t i = (j * L + lane) * V;
+        if (i < d) load<V>(p + i, f + j * V);
+        else
+#pragma unroll
+            for (int c = 0; c < V; c++) f[j * V + c] = 0.f;
+    }
+}
+template <int L, int V, int E, class T>
+__device__ inline void store_row(T* p, uint32_t lane, uint32_t d, const float (&f)[E]) {
+#pragma unroll
+    for (int j = 0; j < E / V; j++) {
+        const uint32_t i = (j * L + lane) * V;
+        if (i < d) store<V>(p + i, f + j * V);
+    }
+}
+
+constexpr int threads(int L, int most) { return L > 64 ? L : most; }  // of a workgroup
+
+template <class T, int L, int V, int E>
+__global__ __launch_bounds__(threads(L, 256)) void k_forward(Args a) {
+    constexpr int kSlots = threads(L, 256) / L;
+    __shared__ Sums<L, 1> s;
+    const uint32_t lane = threadIdx.x % L;
+    float w[E], b[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const uint32_t i = (e / V * L + lane) * V + e % V;
+        w[e] = i < a.d ? weight<T>(a.w, a.wide, i, 1.f) : 0.f;
+        b[e] = i < a.d ? weight<T>(a.b, a.wide, i, 0.f) : 0.f;
+    }
+    for (uint32_t row = blockIdx.x * kSlots + threadIdx.x / L; row < a.rows; row += gridDim.x * kSlots) {
+        float f[E];
+        load_row<L, V>((const T*)a.x + row * a.xs, lane, a.d, f);
+        float sum[1] = {0.f};
+#pragma unroll
+        for (int e = 0; e < E; e++) sum[0] += f[e];
+        sum_over<L>(sum, s, 0);
+        const float mean = sum[0] / a.n;  // divided, so that a row of equal channels is at 0 from it
+        sum[0] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            f[e] = (e / V * L + lane) * V + e % V < a.d ? f[e] - mean : 0.f;
+            sum[0] += f[e] * f[e];
+        }
+        sum_over<L>(sum, s, 1);
+        const float rstd = 1.f / __builtin_sqrtf(sum[0] * a.each + a.eps);
+#pragma unroll
+        for (int e = 0; e < E; e++) f[e] = f[e] * rstd * w[e] + b[e];
+        store_row<L, V>((T*)a.y + row * a.ys, lane, a.d, f);
+        if (lane == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+    }
+}
+
+// kParam: dw and db are asked for
+template <class T, int L, int V, int E, bool kParam>
+__global__ __launch_bounds__(threads(L, 512)) void k_backward(Args a) {
+    constexpr int kSlots = threads(L, 512) / L;
+    __shared__ Sums<L, 2> s;
+    const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L;
+    float w[E], dw[E], db[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const uint32_t i = (e / V * L + lane) * V + e % V;
+        w[e] = i < a.d ? weight<T>(a.w, a.wide, i, 1.f) : 0.f;
+        dw[e] = db[e] = 0.f;
+    }
+    int turn = 0;
+    for (uint32_t row = blockIdx.x * kSlots + slot; row < a.rows; row += gridDim.x * kSlots) {
+        float h[E], t[E];
+        load_row<L, V>((const T*)a.x + row * a.xs, lane, a.d, h);
+        load_row<L, V>((const T*)a.dy + row * a.dys, lane, a.d, t);
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            h[e] = (e / V * L + lane) * V + e % V < a.d ? (h[e] - mean) * rstd : 0.f;
+            if constexpr (kParam) {
+                dw[e] += t[e] * h[e];
+                db[e] += t[e];
+            }
+            t[e] *= w[e];
+            sum[0] += t[e];
+            sum[1] += t[e] * h[e];
+        }
+        sum_over<L>(sum, s, turn);
+        turn ^= 1;
+        const float flat = sum[0] * a.each, along = sum[1] * a.each;
+#pragma unroll
+        for (int e = 0; e < E; e++) h[e] = rstd * (t[e] - flat - h[e] * along);
+        store_row<L, V>((T*)a.y + row * a.ys, lane, a.d, h);
+    }
+    if constexpr (kParam) {
+        // the slots' sums, the upper half's to the lower half's
+        if constexpr (kSlots > 1) {
+            __shared__ float half[kSlots / 2][2][E * L];
+#pragma unroll
+            for (int n = kSlots / 2; n > 0; n /= 2) {
+                __syncthreads();
+                if (slot >= n && slot < 2 * n)
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        half[slot - n][0][e * L + lane] = dw[e];
+                        half[slot - n][1][e * L + lane] = db[e];
+                    }
+                __syncthreads();
+                if (slot < n)
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        dw[e] += half[slot][0][e * L + lane];
+                        db[e] += half[slot][1][e * L + lane];
+                    }
+            }
+        }
+        if (slot == 0) {
+            float* part = a.parts ? a.parts + (size_t)blockIdx.x * 2 * a.d : nullptr;  // none: the one workgroup's are all
+            float *to_w = part ? part : a.dw, *to_b = part ? part + a.d : a.db;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const uint32_t i = (e / V * L + lane) * V + e % V;
+                if (i < a.d && to_w) to_w[i] = dw[e];
+                if (i < a.d && to_b) to_b[i] = db[e];
+            }
+        }
+    }
+}
+
+// The parts' sums: 64 columns of dw and db a workgroup, whose waves take every sixteenth part.
+__global__ __launch_bounds__(1024) void k_columns(const float* __restrict__ parts, uint32_t n, uint32_t d, float* dw, float* db) {
+    __shared__ float s[16][64];
+    const uint32_t col = blockIdx.x * 64 + threadIdx.x % 64, wave = threadIdx.x / 64;
+    float sum = 0.f;
+    if (col < 2 * d)
+#pragma unroll 8
+        for (uint32_t p = wave; p < n; p += 16) sum += parts[(size_t)p * 2 * d + col];
+    s[wave][threadIdx.x % 64] = sum;
+    __syncthreads();
+    if (wave == 0 && col < 2 * d) {
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) sum += s[i][threadIdx.x];
+        float* to = col < d ? dw : db;
+        if (to) to[col < d ? col : col - d] = sum;
+    }
+}
+
+// Which lanes share a row: the fewest that hold its channels, with vectors of 16 bytes where every row lies on them.
+template <class T, class F>
+int choose(bool vectors, uint32_t d, F&& f) {
+    constexpr int V = 16 / sizeof(T);
+#define CLEAR_FITS(L, E, W) \
+    if (d <= (L) * (E)) return f(std::integral_constant<int, L>{}, std::integral_constant<int, E>{}, std::integral_constant<int, W>{})
+    if (vectors) {
+        CLEAR_FITS(16, 8, V);
+        CLEAR_FITS(64, 8, V);
+        CLEAR_FITS(64, 16, V);
+        CLEAR_FITS(64, 32, V);
+        CLEAR_FITS(256, 16, V);
+        CLEAR_FITS(256, 32, V);
+        CLEAR_FITS(1024, 16, V);
+    }
+    CLEAR_FITS(16, 4, 1);
+    CLEAR_FITS(64, 4, 1);
+    CLEAR_FITS(64, 16, 1);
+    CLEAR_FITS(256, 16, 1);
+    CLEAR_FITS(1024, 16, 1);
+#undef CLEAR_FITS
+    return fail(CKKS_EINVAL, "layer norm: %u channels", d);
+}
+
+// the backward pass' workgroups, as many as its parts: 16 waves a CU
+template <class T>
+uint32_t parts_of(bool vectors, uint32_t rows, uint32_t d) {
+    return choose<T>(vectors, d, [&](auto l, auto, auto) {
+        constexpr int L = decltype(l)::value, kSlots = threads(L, 512) / L;
+        return (int)std::min<uint64_t>(((uint64_t)rows + kSlots - 1) / kSlots, 256 * 1024 / threads(L, 512));
+    });
+}
+uint32_t most_parts(const fhe_ssm_layer_norm& a) {
+    const auto of = [&](auto t) {
+        typedef decltype(t) T;
+        return std::max(parts_of<T>(true, a.rows, a.channels), parts_of<T>(false, a.rows, a.channels));
+    };
+    return by_type(a.type, of);
+}
+
+int check(const fhe_ssm_layer_norm* a) {
+    if (!a) return fail(CKKS_EINVAL, "layer norm: null description");
+    if (a->type > FHE_SSM_F16) return fail(CKKS_EINVAL, "layer norm: unknown type %u", a->type);
+    if (a->weight_type != FHE_SSM_F32 && a->weight_type != a->type)
+        return fail(CKKS_EINVAL, "layer norm: weights of type %u are neither float32 nor like the rows", a->weight_type);
+    if (a->channels < 1 || a->channels > kMostChannels) return fail(CKKS_EINVAL, "layer norm: %u channels", a->channels);
+    if (a->rows > 0x7fffffffu) return fail(CKKS_EINVAL, "layer norm: too many rows");
+    if (a->rows > 1 && (a->x_stride < 0 || a->dy_stride < 0 || a->out_stride < (int64_t)a->channels))
+        return fail(CKKS_EINVAL, "layer norm: output rows overlap, or a negative stride");
+    if (!(a->eps >= 0.f)) return fail(CKKS_EINVAL, "layer norm: eps below 0");
+    return CKKS_OK;
+}
+
+Args args(const fhe_ssm_layer_norm& a, const void* x, const void* weight, void* y) {
+    Args k{};
+    k.x = x, k.w = weight, k.y = y;
+    k.rows = a.rows, k.d = a.channels, k.wide = a.weight_type == FHE_SSM_F32;
+    k.xs = a.x_stride, k.dys = a.dy_stride, k.ys = a.out_stride;
+    k.eps = a.eps, k.n = (float)a.channels, k.each = 1.f / k.n;
+    return k;
+}
+
+bool on_vectors(const void* p, int64_t stride, size_t size) { return aligned(p, 16) && stride * size % 16 == 0; }
+
+}  // namespace
+}  // namespace clear
+
+extern "C" {
+
+int fhe_ssm_layer_norm_workspace(const fhe_ssm_layer_norm* a, size_t* bytes) {
+    using namespace clear;
+    if (int rc = check(a)) return rc;
+    if (!bytes) return fail(CKKS_EINVAL, "layer norm: null argument");
+    const uint32_t n = most_parts(*a);
+    *bytes = n > 1 ? (size_t)n * 2 * a->channels * sizeof(float) : 0;
+    return CKKS_OK;
+}
+
+int fhe_ssm_layer_norm_forward(const fhe_ssm_layer_norm* a, const void* x, const void* weight, const void* bias, void* out,
+                               float* mean, float* rstd, void* stream) {
+    using namespace clear;
+    if (int rc = check(a)) return rc;
+    if (a->rows == 0) return CKKS_OK;
+    if (!x || !out) return fail(CKKS_EINVAL, "layer norm: null argument");
+    Args k = args(*a, x, weight, out);
+    k.b = bias, k.mean = mean, k.rstd = rstd;
+    const auto run = [&](auto t) {
+        typedef decltype(t) T;
+        const size_t size = sizeof(T);
+        const bool vectors = k.d * size % 16 == 0 && on_vectors(x, k.rows > 1 ? k.xs : 0, size) && on_vectors(out, k.rows > 1 ? k.ys : 0, size);
+        return choose<T>(vectors, k.d, [&](auto l, auto e, auto v) {
+            constexpr int L = decltype(l)::value, E = decltype(e)::value, V = decltype(v)::value;
+            constexpr int kThreads = threads(L, 256), kSlots = kThreads / L;
+            const uint32_t blocks = std::min<uint32_t>((k.rows + kSlots - 1) / kSlots, 256 * 2048 / kThreads);
+            hipLaunchKernelGGL((k_forward<T, L, V, E>), dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream, k);
+            return launched("layer norm");
+        });
+    };
+    return by_type(a->type, run);
+}
+
+int fhe_ssm_layer_norm_backward(const fhe_ssm_layer_norm* a, const void* dy, const void* x, const void* weight,
+                                const float* mean, const float* rstd, void* dx, float* dweight, float* dbias, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+    using namespace clear;
+    if (int rc = check(a)) return rc;
+    if (a->rows > 0 && (!dy || !x || !mean || !rstd || !dx)) return fail(CKKS_EINVAL, "layer norm: null argument");
+    Args k = args(*a, x, weight, dx);
+    k.dy = dy, k.mean = (float*)mean, k.rstd = (float*)rstd, k.dw = dweight, k.db = dbias;
+    const bool param = dweight || dbias;
+    size_t need;
+    if (int rc = fhe_ssm_layer_norm_workspace(a, &need)) return rc;
+    if (param && need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
+        return fail(CKKS_EINVAL, "layer norm: the workspace must have %zu bytes and lie on 16", need);
+    const hipStream_t st = (hipStream_t)stream;
+    const auto run = [&](auto t) {
+        typedef decltype(t) T;
+        const size_t size = sizeof(T);
+        const auto on = [&](const void* p, int64_t stride) { return on_vectors(p, k.rows > 1 ? stride : 0, size); };
+        const bool vectors = k.d * size % 16 == 0 && on(x, k.xs) && on(dy, k.dys) && on(dx, k.ys);
+        const uint32_t blocks = parts_of<T>(vectors, k.rows, k.d);
+        k.parts = blocks > 1 ? (float*)workspace : nullptr;
+        if (blocks)
+            if (int rc = choose<T>(vectors, k.d, [&](auto l, auto e, auto v) {
+                    constexpr int L = decltype(l)::value, E = decltype(e)::value, V = decltype(v)::value;
+                    const dim3 grid(blocks), block(threads(L, 512));
+                    if (param) hipLaunchKernelGGL((k_backward<T, L, V, E, true>), grid, block, 0, st, k);
+                    else hipLaunchKernelGGL((k_backward<T, L, V, E, false>), grid, block, 0, st, k);
+                    return launched("layer norm: gradient");
+                }))
+                return rc;
+        if (!param || blocks == 1) return (int)CKKS_OK;
+        hipLaunchKernelGGL(k_columns, dim3((2 * k.d + 63) / 64), dim3(1024), 0, st, k.parts, blocks, k.d, dweight, dbias);
+        return launched("layer norm: the weight's gradient");
+    };
+    return by_type(a->type, run);
+}
+
+}  // extern "C"

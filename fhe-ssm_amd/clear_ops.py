@@ -1,5 +1,7 @@
 """ctypes front end of libfhe_ssm_clear.so (include/fhe_ssm_clear.h): what a client of the encrypted step computes in the
-clear -- linear attention with a decay for each head, products with 4-bit weights, the draw of a token.
+clear -- linear attention with a decay for each head, products with 4-bit weights, the draw of a token; and what scores and
+trains its drafting model: layer norm, a gated linear recurrence, the embedding, log-probabilities of given tokens, each with
+its gradient, and the AdamW step.
 
 Arguments are device tensors (torch's, or anything with data_ptr, dtype, shape and stride); outputs are tensors that the
 caller brings.  Calls go to `stream` (a hipStream_t as an int, for torch `stream.cuda_stream`; 0 is the null stream; None is
@@ -44,6 +46,44 @@ class SampleParams(ctypes.Structure):
     _fields_ = [("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp)]
 
 
+class LayerNormSizes(ctypes.Structure):
+    """fhe_ssm_layer_norm"""
+    _fields_ = [("type", _u32), ("weight_type", _u32), ("rows", _u32), ("channels", _u32), ("eps", ctypes.c_float),
+                ("x_stride", _i64), ("out_stride", _i64), ("dy_stride", _i64)]
+
+
+class GatedRecurrenceSizes(ctypes.Structure):
+    """fhe_ssm_gated_recurrence"""
+    _fields_ = [("type", _u32), ("lanes", _u32), ("tokens", _u32), ("channels", _u32), ("z_stride", _i64 * 2),
+                ("x_stride", _i64 * 2), ("out_stride", _i64 * 2), ("dout_stride", _i64 * 2), ("dz_stride", _i64 * 2),
+                ("dx_stride", _i64 * 2)]
+
+
+class EmbeddingSizes(ctypes.Structure):
+    """fhe_ssm_embedding"""
+    _fields_ = [("table_type", _u32), ("row_type", _u32), ("tokens", _u32), ("vocab", _u32), ("channels", _u32),
+                ("scale", ctypes.c_float), ("table_stride", _i64), ("row_stride", _i64)]
+
+
+class TokenLogprobsSizes(ctypes.Structure):
+    """fhe_ssm_token_logprobs"""
+    _fields_ = [("type", _u32), ("rows", _u32), ("vocab", _u32), ("top", _u32), ("row_stride", _i64),
+                ("gradient_stride", _i64)]
+
+
+class AdamWSizes(ctypes.Structure):
+    """fhe_ssm_adamw"""
+    _fields_ = [("gradient_type", _u32), ("copy_type", _u32), ("state_bits", _u32), ("step", _u32), ("seed", _u32),
+                ("lr", ctypes.c_float), ("eps", ctypes.c_float), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("lr_at", _vp), ("scale_at", _vp), ("step_at", _vp)]
+
+
+class AdamWTensor(ctypes.Structure):
+    """fhe_ssm_adamw_tensor"""
+    _fields_ = [("param", _vp), ("gradient", _vp), ("first", _vp), ("second", _vp), ("powers", _vp), ("copy", _vp),
+                ("n", ctypes.c_uint64), ("weight_decay", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); the exported C ABI (kept in step with include/fhe_ssm_clear.h)
 SIGNATURES = {
     "fhe_ssm_clear_last_error": (ctypes.c_char_p, []),
@@ -54,6 +94,20 @@ SIGNATURES = {
     "fhe_ssm_q4_arrange": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "fhe_ssm_q4_product": (_int, [_vp, _vp, _u32, _u32, _vp, _i64, _vp, _i64, _vp]),
     "fhe_ssm_sample": (_int, [_u32, _vp, _u32, _u32, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "fhe_ssm_layer_norm_workspace": (_int, [_vp, ctypes.POINTER(_size)]),
+    "fhe_ssm_layer_norm_forward": (_int, [_vp] * 8),
+    "fhe_ssm_layer_norm_backward": (_int, [_vp] * 10 + [_size, _vp]),
+    "fhe_ssm_gated_recurrence_workspace": (_int, [_vp, ctypes.POINTER(_size), ctypes.POINTER(_size)]),
+    "fhe_ssm_gated_recurrence_prompt": (_int, [_vp] * 9 + [_size, _vp]),
+    "fhe_ssm_gated_recurrence_backward": (_int, [_vp] * 11 + [_size, _vp]),
+    "fhe_ssm_gated_recurrence_step": (_int, [_vp] * 7),
+    "fhe_ssm_embedding_lookup": (_int, [_vp] * 5),
+    "fhe_ssm_embedding_workspace": (_int, [_vp, ctypes.POINTER(_size)]),
+    "fhe_ssm_embedding_gradient": (_int, [_vp, _vp, _vp, _vp, _int, _vp, _size, _vp]),
+    "fhe_ssm_token_logprobs_workspace": (_int, [_vp, ctypes.POINTER(_size)]),
+    "fhe_ssm_token_logprobs_forward": (_int, [_vp] * 12 + [_size, _vp]),
+    "fhe_ssm_token_logprobs_gradient": (_int, [_vp] * 9),
+    "fhe_ssm_adamw_step": (_int, [_vp, _u32, _vp, _vp]),
 }
 
 
@@ -315,3 +369,359 @@ def sample(logits, draws, tokens, logprobs=None, temperature=None, top_k=None, t
     check(load().fhe_ssm_sample(_type(logits), logits.data_ptr(), rows, vocab, stride[0], draws.data_ptr(),
                                 ctypes.addressof(p), tokens.data_ptr(), _ptr(logprobs),
                                 _queue(stream, logits)))
+
+
+# ------------------------------------------------------------------------------------------------ what the operators below share
+def _bytes_of(workspace) -> int:
+    """the size of a workspace, which is checked here too"""
+    if workspace is None:
+        return 0
+    _need(workspace.is_contiguous(), "workspace must be contiguous")
+    return workspace.numel() * workspace.element_size()
+
+
+def _floats(shape, **tensors) -> None:
+    """each is None or contiguous float32 of the shape"""
+    for name, t in tensors.items():
+        if t is not None and not (t.shape == shape and _is(t, "torch.float32") and t.is_contiguous()):
+            raise ClearError(f"{name} must be contiguous float32 {list(shape)}")
+
+
+def _matrix(t, name: str):
+    """the stride of the rows of a [rows, columns] tensor with contiguous rows"""
+    _need(len(t.shape) == 2, f"{name} must be [rows, columns]")
+    s = t.stride()
+    _need(s[1] == 1 or t.shape[1] <= 1, f"rows of {name} must be contiguous")
+    return s[0]
+
+
+def _token_ids(tokens, rows=None):
+    _need(_is(tokens, "torch.int64") and len(tokens.shape) == 1 and tokens.is_contiguous()
+          and (rows is None or tokens.shape[0] == rows), "tokens must be contiguous int64, one for each row")
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+def _norm_sizes(x, out, weight, bias, eps=0.0, dy=None):
+    rows, channels = x.shape if len(x.shape) == 2 else (0, 0)
+    a = LayerNormSizes(_type(x), F32, rows, channels, eps, _matrix(x, "x"), 0, 0)
+    if out is not None:
+        _need(out.shape == x.shape and out.dtype == x.dtype, "the output must be like x")
+        a.out_stride = _matrix(out, "the output")
+    if dy is not None:
+        _need(dy.shape == x.shape and dy.dtype == x.dtype, "dy must be like x")
+        a.dy_stride = _matrix(dy, "dy")
+    kinds = {_type(t) for t in (weight, bias) if t is not None}
+    _need(len(kinds) < 2, "weight and bias differ in type")
+    a.weight_type = kinds.pop() if kinds else F32
+    for name, t in (("weight", weight), ("bias", bias)):
+        _need(t is None or (tuple(t.shape) == (channels,) and t.is_contiguous()), f"{name} must be contiguous [{channels}]")
+    return a
+
+
+def layer_norm_workspace(x) -> int:
+    """device bytes that layer_norm_backward needs for the weight's gradient of rows x (0 for few)"""
+    a, n = _norm_sizes(x, None, None, None), _size()
+    a.out_stride = a.channels
+    check(load().fhe_ssm_layer_norm_workspace(ctypes.addressof(a), ctypes.byref(n)))
+    return n.value
+
+
+def layer_norm(x, weight, bias, out, mean=None, rstd=None, eps: float = 1e-5, stream=None) -> None:
+    """out = (x - mean) rstd weight + bias over the channels of x [rows, channels], rstd = 1 / sqrt(variance + eps).
+
+    out like x, or x itself; weight and bias [channels], float32 or of x's type, None: 1 and 0; mean and rstd float32 [rows] or
+    None: what layer_norm_backward takes."""
+    _on_device(x, weight, bias, out, mean, rstd)
+    a = _norm_sizes(x, out, weight, bias, eps)
+    _floats((a.rows,), mean=mean, rstd=rstd)
+    check(load().fhe_ssm_layer_norm_forward(ctypes.addressof(a), x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(),
+                                            _ptr(mean), _ptr(rstd), _queue(stream, x)))
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, workspace=None, stream=None) -> None:
+    """The gradients of layer_norm from that of its output: dx like x (it may be dy), dweight and dbias float32 [channels] where
+    they are given.  workspace: a uint8 tensor of layer_norm_workspace(x) bytes, needed for dweight and dbias."""
+    _on_device(dy, x, weight, mean, rstd, dx, dweight, dbias, workspace)
+    a = _norm_sizes(x, dx, weight, None, dy=dy)
+    _floats((a.rows,), mean=mean, rstd=rstd)
+    _floats((a.channels,), dweight=dweight, dbias=dbias)
+    check(load().fhe_ssm_layer_norm_backward(
+        ctypes.addressof(a), dy.data_ptr(), x.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
+        _ptr(dweight), _ptr(dbias), _ptr(workspace), _bytes_of(workspace), _queue(stream, x)))
+
+
+# ------------------------------------------------------------------------------------------------ gated recurrence
+def _recurrence_sizes(z, tokens_axis, **others):
+    """others: names of the description's strides -> tensors like z, or None"""
+    n = 3 if tokens_axis else 2
+    shape = z.shape
+    _need(len(shape) == n, "z is [lanes, tokens, channels], of one token [lanes, channels]")
+    a = GatedRecurrenceSizes(_type(z), shape[0], shape[1] if tokens_axis else 1, shape[-1])
+    for name, t in (("z", z), *others.items()):
+        if t is None:
+            continue
+        _need(t.shape == shape and t.dtype == z.dtype, f"{name} must be like z")
+        s = t.stride()
+        _need(s[-1] == 1 or shape[-1] <= 1, f"{name}: channels must be contiguous")
+        setattr(a, name + "_stride", (s[0], s[1]) if tokens_axis else (s[0], 0))
+    return a
+
+
+def _lengths(lengths, lanes) -> None:
+    _need(lengths is None or (_is(lengths, "torch.int32") and tuple(lengths.shape) == (lanes,) and lengths.is_contiguous()),
+          "lengths must be contiguous int32 [lanes]")
+
+
+def _recurrence_bytes(z):
+    work, saved = _size(), _size()
+    a = _recurrence_sizes(z, True)
+    check(load().fhe_ssm_gated_recurrence_workspace(ctypes.addressof(a), ctypes.byref(work), ctypes.byref(saved)))
+    return work.value, saved.value
+
+
+def gated_recurrence_workspace(z) -> int:
+    """device bytes that gated_recurrence and its backward pass need for gates of this shape (0 for many)"""
+    return _recurrence_bytes(z)[0]
+
+
+def gated_recurrence_saved(z) -> int:
+    """device bytes that gated_recurrence saves for its backward pass"""
+    return _recurrence_bytes(z)[1]
+
+
+def _saved(saved, a) -> None:
+    need = _size()
+    check(load().fhe_ssm_gated_recurrence_workspace(ctypes.addressof(a), None, ctypes.byref(need)))
+    _need(saved.is_contiguous() and saved.numel() * saved.element_size() >= need.value and saved.data_ptr() % 16 == 0,
+          f"saved must have {need.value} bytes, contiguous, on 16")
+
+
+def gated_recurrence(z, x, state_in, state_out, out, lengths=None, saved=None, workspace=None, stream=None) -> None:
+    """h_t = sigmoid(z_t) h_{t-1} + sigmoid(-z_t) x_t over a prompt, per lane and channel; out_t = h_t.
+
+    z, x and out [lanes, tokens, channels]; states float32 [lanes, channels] (state_in None: zero; state_out None: not kept; both
+    may be one tensor); lengths int32 [lanes]: tokens past a lane's length change nothing and give zeros; saved: None, or a uint8
+    tensor of gated_recurrence_saved(z) bytes for the backward pass; workspace: one of gated_recurrence_workspace(z) bytes, None
+    where that is 0."""
+    _on_device(z, x, state_in, state_out, out, lengths, saved, workspace)
+    a = _recurrence_sizes(z, True, x=x, out=out)
+    _floats((a.lanes, a.channels), state_in=state_in, state_out=state_out)
+    _lengths(lengths, a.lanes)
+    if saved is not None:
+        _saved(saved, a)
+    check(load().fhe_ssm_gated_recurrence_prompt(
+        ctypes.addressof(a), z.data_ptr(), x.data_ptr(), _ptr(lengths), _ptr(state_in), _ptr(state_out), out.data_ptr(),
+        _ptr(saved), _ptr(workspace), _bytes_of(workspace), _queue(stream, z)))
+
+
+def gated_recurrence_backward(z, x, saved, dout, dstate_out, dz, dx, dstate_in=None, lengths=None, workspace=None,
+                              stream=None) -> None:
+    """The gradients of gated_recurrence: dz and dx like z, dstate_in float32 [lanes, channels] where it is given, from those of
+    out and of state_out (None: zeros).  z, x, lengths and saved are the prompt's; dstate_in may be dstate_out."""
+    _on_device(z, x, saved, dout, dstate_out, dz, dx, dstate_in, lengths, workspace)
+    a = _recurrence_sizes(z, True, x=x, dout=dout, dz=dz, dx=dx)
+    _floats((a.lanes, a.channels), dstate_in=dstate_in, dstate_out=dstate_out)
+    _lengths(lengths, a.lanes)
+    _saved(saved, a)
+    check(load().fhe_ssm_gated_recurrence_backward(
+        ctypes.addressof(a), z.data_ptr(), x.data_ptr(), _ptr(lengths), saved.data_ptr(), _ptr(dout), _ptr(dstate_out),
+        dz.data_ptr(), dx.data_ptr(), _ptr(dstate_in), _ptr(workspace), _bytes_of(workspace), _queue(stream, z)))
+
+
+def gated_recurrence_step(z, x, state_in, state_out, out, stream=None) -> None:
+    """gated_recurrence for one token of every lane: the same tensors without the token axis"""
+    _on_device(z, x, state_in, state_out, out)
+    a = _recurrence_sizes(z, False, x=x, out=out)
+    _floats((a.lanes, a.channels), state_in=state_in, state_out=state_out)
+    check(load().fhe_ssm_gated_recurrence_step(ctypes.addressof(a), z.data_ptr(), x.data_ptr(), _ptr(state_in),
+                                               _ptr(state_out), out.data_ptr(), _queue(stream, z)))
+
+
+# ------------------------------------------------------------------------------------------------ embedding
+def embedding(tokens, table, out, scale: float = 1.0, stream=None) -> None:
+    """out[t] = scale table[tokens[t]]; zeros for a token outside the table.  tokens int64 [n], table [vocab, channels], out
+    [n, channels], each of any of the three types."""
+    _on_device(tokens, table, out)
+    _token_ids(tokens)
+    n = tokens.shape[0]
+    strides = _matrix(table, "table"), _matrix(out, "out")
+    vocab, channels = table.shape
+    _need(tuple(out.shape) == (n, channels), f"out must be [{n}, {channels}]")
+    a = EmbeddingSizes(_type(table), _type(out), n, vocab, channels, scale, *strides)
+    if vocab == 1:
+        a.table_stride = max(channels, strides[0])
+    check(load().fhe_ssm_embedding_lookup(ctypes.addressof(a), tokens.data_ptr(), table.data_ptr(), out.data_ptr(),
+                                          _queue(stream, table)))
+
+
+def _embedding_gradient_sizes(tokens, dtable, scale=1.0):
+    _token_ids(tokens)
+    _need(len(dtable.shape) == 2 and dtable.is_contiguous(), "dtable must be contiguous [vocab, channels]")
+    vocab, channels = dtable.shape
+    return EmbeddingSizes(_type(dtable), F32, tokens.shape[0], vocab, channels, scale, channels, channels)
+
+
+def embedding_gradient_workspace(tokens, dtable) -> int:
+    """device bytes that embedding_gradient needs"""
+    n = _size()
+    a = _embedding_gradient_sizes(tokens, dtable)
+    check(load().fhe_ssm_embedding_workspace(ctypes.addressof(a), ctypes.byref(n)))
+    return n.value
+
+
+def embedding_gradient(tokens, dout, dtable, scale: float = 1.0, accumulate: bool = False, workspace=None, stream=None) -> None:
+    """dtable[v] = scale times the sum of dout[t] over the t with tokens[t] = v, in their order; with `accumulate` added to what
+    is there.  dout [n, channels]; dtable contiguous [vocab, channels], float32 or of dout's type; workspace: a uint8 tensor of
+    embedding_gradient_workspace(tokens, dtable) bytes."""
+    _on_device(tokens, dout, dtable, workspace)
+    a = _embedding_gradient_sizes(tokens, dtable, scale)
+    a.row_type, a.row_stride = _type(dout), _matrix(dout, "dout")
+    _need(tuple(dout.shape) == (a.tokens, a.channels), f"dout must be [{a.tokens}, {a.channels}]")
+    check(load().fhe_ssm_embedding_gradient(ctypes.addressof(a), tokens.data_ptr(), dout.data_ptr(), dtable.data_ptr(),
+                                            bool(accumulate), _ptr(workspace), _bytes_of(workspace), _queue(stream, dout)))
+
+
+# ------------------------------------------------------------------------------------------------ log-probabilities
+def _logprobs_sizes(logits, top=0, gradient=None):
+    stride = _matrix(logits, "logits")
+    rows, vocab = logits.shape
+    a = TokenLogprobsSizes(_type(logits), rows, vocab, top, stride, 0)
+    if gradient is not None:
+        _need(gradient.shape == logits.shape and gradient.dtype == logits.dtype, "the gradient must be like logits")
+        a.gradient_stride = _matrix(gradient, "the gradient")
+    return a
+
+
+def token_logprobs_workspace(logits, top: int = 0) -> int:
+    """device bytes that token_logprobs needs for logits of this shape and so many alternatives (0 for many)"""
+    a, n = _logprobs_sizes(logits, top), _size()
+    check(load().fhe_ssm_token_logprobs_workspace(ctypes.addressof(a), ctypes.byref(n)))
+    return n.value
+
+
+def token_logprobs(logits, tokens, logprobs, entropy=None, statistics=None, top_tokens=None, top_logprobs=None, workspace=None,
+                   weights=None, entropy_weights=None, gradient=None, stream=None) -> None:
+    """Log-probabilities of given tokens under softmax of logits [rows, vocab], with the rows' entropy and the alternatives.
+
+    tokens int64 [rows], one outside the vocabulary is a padded position; logprobs and entropy float32 [rows], statistics float32
+    [rows, 2]: what token_logprobs_gradient takes; top_tokens int64 and top_logprobs float32 [rows, k], k <= 32, in the order of
+    falling logits, equal ones by rising index.  gradient (like logits, or logits itself) receives that of
+    sum(weights logprobs + entropy_weights entropy) in the same call, with weights float32 [rows].  All but logits may be None.
+    workspace: a uint8 tensor of token_logprobs_workspace(logits, k) bytes, None where that is 0."""
+    _on_device(logits, tokens, logprobs, entropy, statistics, top_tokens, top_logprobs, workspace, weights, entropy_weights, gradient)
+    top = 0
+    if top_tokens is not None or top_logprobs is not None:
+        _need(top_tokens is not None and top_logprobs is not None, "top_tokens and top_logprobs come together")
+        _need(_is(top_tokens, "torch.int64") and len(top_tokens.shape) == 2 and top_tokens.is_contiguous()
+              and top_tokens.shape[0] == logits.shape[0], "top_tokens must be contiguous int64 [rows, k]")
+        top = top_tokens.shape[1]
+    a = _logprobs_sizes(logits, top, gradient)
+    if tokens is not None:
+        _token_ids(tokens, a.rows)
+    _floats((a.rows,), logprobs=logprobs, entropy=entropy, weights=weights, entropy_weights=entropy_weights)
+    _floats((a.rows, 2), statistics=statistics)
+    _floats((a.rows, top), top_logprobs=top_logprobs)
+    check(load().fhe_ssm_token_logprobs_forward(
+        ctypes.addressof(a), logits.data_ptr(), _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(statistics),
+        _ptr(top_tokens), _ptr(top_logprobs), _ptr(weights), _ptr(entropy_weights), _ptr(gradient), _ptr(workspace),
+        _bytes_of(workspace), _queue(stream, logits)))
+
+
+def token_logprobs_gradient(logits, tokens, statistics, weights, gradient, entropy_weights=None, entropy=None,
+                            stream=None) -> None:
+    """The gradient that token_logprobs writes, where its weights were not known then: from the statistics, and the entropy if it
+    has weights."""
+    _on_device(logits, tokens, statistics, weights, gradient, entropy_weights, entropy)
+    a = _logprobs_sizes(logits, 0, gradient)
+    if tokens is not None:
+        _token_ids(tokens, a.rows)
+    _floats((a.rows,), weights=weights, entropy_weights=entropy_weights, entropy=entropy)
+    _floats((a.rows, 2), statistics=statistics)
+    check(load().fhe_ssm_token_logprobs_gradient(
+        ctypes.addressof(a), logits.data_ptr(), _ptr(tokens), statistics.data_ptr(), _ptr(entropy), _ptr(weights),
+        _ptr(entropy_weights), gradient.data_ptr(), _queue(stream, logits)))
+
+
+# ------------------------------------------------------------------------------------------------ AdamW
+class AdamW:
+    """The AdamW step over a model's tensors, and its states.
+
+    params: contiguous float32 tensors, updated in place.  weight_decay: one for all, or one for each.  copies: bfloat16 or
+    float16 tensors (one type) that receive the parameters after every step, or None.  bits: 32 for states in float32, 8 for
+    states in 8-bit floats with a power of two for each 256 entries: m and the root of v as float8_e4m3fn, and the powers.
+    states: (m, v) or (m, root, powers), lists of tensors like params (powers uint8 [blocks, 2]); None begins with zeros."""
+
+    BLOCK = 256
+
+    def __init__(self, params, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, bits: int = 32, copies=None, states=None):
+        self.params, n = list(params), len(params)
+        _need(n > 0, "no parameters")
+        _on_device(*self.params)
+        for p in self.params:
+            _need(_is(p, "torch.float32") and p.is_contiguous(), "parameters must be contiguous float32")
+            _need(p.device == self.params[0].device, "parameters lie on different devices")
+        _need(bits in (8, 32), f"states have 8 or 32 bits, not {bits}")
+        self.bits, self.copies = bits, None if copies is None else list(copies)
+        decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        _need(len(decay) == n, "one weight_decay for all, or one for each parameter")
+        if states is None:
+            states = self._zeros()
+        _need(len(states) == (2 if bits == 32 else 3) and all(len(s) == n for s in states), "states are lists as long as params")
+        self.states = tuple(list(s) for s in states)
+        kind = "torch.float32" if bits == 32 else "torch.float8_e4m3fn"
+        for name, s in zip(("the first state", "the second state"), self.states):
+            for p, t in zip(self.params, s):
+                _need(t.is_cuda and t.shape == p.shape and _is(t, kind) and t.is_contiguous(), f"{name} must be contiguous {kind[6:]} like its parameter")
+        if bits == 8:
+            for p, t in zip(self.params, self.states[2]):
+                _need(t.is_cuda and tuple(t.shape) == (-(-p.numel() // self.BLOCK), 2) and _is(t, "torch.uint8") and t.is_contiguous(),
+                      "powers must be contiguous uint8 [blocks, 2]")
+        copy_type = BF16
+        if self.copies is not None:
+            _need(len(self.copies) == n, "one copy for each parameter")
+            copy_type = _type(self.copies[0])
+            for p, t in zip(self.params, self.copies):
+                _need(t.is_cuda and t.shape == p.shape and t.dtype == self.copies[0].dtype and copy_type != F32 and t.is_contiguous(),
+                      "copies must be contiguous bfloat16 or float16 like their parameters")
+        self._sizes = AdamWSizes(F32, copy_type, bits, 0, 0, 0.0, eps, *betas)
+        self._tensors = (AdamWTensor * n)()
+        for i, (t, p) in enumerate(zip(self._tensors, self.params)):
+            t.param, t.first, t.second, t.n = p.data_ptr(), self.states[0][i].data_ptr(), self.states[1][i].data_ptr(), p.numel()
+            t.weight_decay = decay[i]
+            if bits == 8:
+                t.powers = self.states[2][i].data_ptr()
+            if self.copies is not None:
+                t.copy = self.copies[i].data_ptr()
+        self._gradients = np.frombuffer(self._tensors, np.uint64).reshape(n, -1)[:, 1]
+
+    def _zeros(self):
+        if self.bits == 32:
+            return [p.new_zeros(p.shape) for p in self.params], [p.new_zeros(p.shape) for p in self.params]
+        import torch
+        codes = [[p.new_zeros(p.shape, dtype=torch.uint8).view(torch.float8_e4m3fn) for p in self.params] for _ in range(2)]
+        return *codes, [p.new_zeros((-(-p.numel() // self.BLOCK), 2), dtype=torch.uint8) for p in self.params]
+
+    def step(self, gradients, lr, step, seed: int = 0, scale=None, stream=None) -> None:
+        """One step with the gradients, contiguous tensors of one type like the parameters.  lr: a number or a float32 tensor of
+        one; step, from 1: a number or an int32 tensor of one; scale: a float32 tensor of one that the gradients are multiplied
+        by, or None.  Tensors are read when the step runs, so that a recorded one follows them.  seed goes, with the step, into
+        how 8-bit states are rounded."""
+        _need(len(gradients) == len(self.params), f"{len(self.params)} gradients are needed")
+        kind = gradients[0].dtype
+        for g, p in zip(gradients, self.params):
+            if not (g.is_cuda and g.dtype == kind and g.shape == p.shape and g.is_contiguous()):
+                raise ClearError("gradients must be contiguous tensors of one type, like their parameters, on the GPU")
+        a = self._sizes
+        a.gradient_type, a.seed = _type(gradients[0]), seed & 0xffffffff
+        a.lr, a.lr_at = (lr, None) if isinstance(lr, (int, float)) else (0.0, self._one(lr, "lr", "torch.float32"))
+        a.step, a.step_at = (step, None) if isinstance(step, int) else (0, self._one(step, "step", "torch.int32"))
+        a.scale_at = None if scale is None else self._one(scale, "scale", "torch.float32")
+        self._gradients[:] = [g.data_ptr() for g in gradients]
+        check(load().fhe_ssm_adamw_step(ctypes.addressof(a), len(self.params), ctypes.addressof(self._tensors),
+                                        _queue(stream, self.params[0])))
+
+    @staticmethod
+    def _one(t, name: str, dtype: str):
+        _need(hasattr(t, "data_ptr") and t.is_cuda and _is(t, dtype) and t.numel() == 1,
+              f"{name} must be a number or a {dtype[6:]} tensor of one on the GPU")
+        return t.data_ptr()

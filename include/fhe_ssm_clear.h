@@ -9,6 +9,15 @@
  *   4-bit products     rows times a matrix of 4-bit codes with group scales: the head, and the draft's projections
  *   sampling           the draw of a token under temperature, top-k, top-p and min-p, from given random numbers
  *
+ * The draft is worth as much as it foresees what the encrypted model answers, so the client scores answered tokens with it
+ * and trains it on them (the reference trains its models in ml-eval/train_fhe_native_ssm.py).  For that, each with its gradient:
+ *
+ *   layer norm         over the channels of rows
+ *   gated recurrence   h <- sigmoid(z) h + sigmoid(-z) x per channel: over a prompt, backwards, and over one token
+ *   embedding          rows of a table by token
+ *   log-probabilities  of given tokens, with entropy and the most likely alternatives
+ *   AdamW              the step over all tensors of a model, with states in 32 or 8 bits
+ *
  * Device pointers may come from any HIP allocator and belong to the current device.  Every call that computes takes a
  * hipStream_t (as void*, NULL is the null stream), issues its work there and returns without waiting; no call allocates
  * or copies to the host, and calls may be recorded into a graph.  Sums, states and statistics are held in 32 bits or
@@ -117,6 +126,153 @@ typedef struct {
 int fhe_ssm_sample(uint32_t type, const void* logits, uint32_t rows, uint32_t vocab, int64_t row_stride,
                    const float* draws, const fhe_ssm_sample_params* params, int64_t* tokens, float* logprobs,
                    void* stream);
+
+/* ---- layer norm ---------------------------------------------------------------------------------------------------
+ *     y = (x - mean) rstd weight + bias,  rstd = 1 / sqrt(mean of (x - mean)^2 + eps)      over the channels of a row
+ * channels <= 16384, rows < 2^31.  Rows are `type`, their strides in elements; weight and bias have `channels` elements of
+ * weight_type, float32 or `type`, and null stands for 1 and 0.  mean and rstd (float32[rows], either may be null) are what the
+ * backward pass takes.  out may be x; other overlaps are not allowed.  A row that holds a NaN or an infinity comes out NaN and
+ * leaves the others alone. */
+typedef struct {
+    uint32_t type, weight_type; /* of x, out, dy and dx; of weight and bias */
+    uint32_t rows, channels;
+    float eps;
+    int64_t x_stride, out_stride; /* out, backward dx */
+    int64_t dy_stride;            /* backward only */
+} fhe_ssm_layer_norm;
+
+/* Device memory that a backward pass of these sizes needs for the weight's gradient (0: workspace may be null). */
+int fhe_ssm_layer_norm_workspace(const fhe_ssm_layer_norm* a, size_t* bytes);
+
+int fhe_ssm_layer_norm_forward(const fhe_ssm_layer_norm* a, const void* x, const void* weight, const void* bias, void* out,
+                               float* mean, float* rstd, void* stream);
+
+/* dx; dweight and dbias (float32[channels]) where they are not null, without rows zeros.  dx may be dy. */
+int fhe_ssm_layer_norm_backward(const fhe_ssm_layer_norm* a, const void* dy, const void* x, const void* weight,
+                                const float* mean, const float* rstd, void* dx, float* dweight, float* dbias,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- gated linear recurrence --------------------------------------------------------------------------------------
+ * Per lane and channel, with the state h in float32:
+ *     a_t = sigmoid(z_t),   h_t = a_t h_{t-1} + (1 - a_t) x_t,   out_t = h_t
+ * lanes and tokens may be 0; tokens <= 2^24, channels <= 2^24, lanes * ceil(channels / 64) < 2^23.  Strides are in elements, in
+ * the order lane, token, and may be any, except that rows of an output must not overlap; channels are contiguous.  States are
+ * float32 [lanes][channels]: state_in null means zero, state_out null drops the new one, and the two may be the same buffer.
+ * Outputs must overlap no input.  lengths as for linear attention: behind them nothing is read, outputs and gradients are zero.
+ * What is not finite reaches its own channel of its own lane, from its token on, in the gradients back from it too. */
+typedef struct {
+    uint32_t type; /* of z, x, out and their gradients */
+    uint32_t lanes, tokens, channels;
+    int64_t z_stride[2], x_stride[2], out_stride[2];
+    int64_t dout_stride[2], dz_stride[2], dx_stride[2]; /* backward only */
+} fhe_ssm_gated_recurrence;
+
+/* Device memory that a prompt or its backward pass of these sizes needs (0: workspace may be null), and that of what a prompt
+ * saves for its backward pass. */
+int fhe_ssm_gated_recurrence_workspace(const fhe_ssm_gated_recurrence* a, size_t* workspace_bytes, size_t* saved_bytes);
+
+/* A prompt.  saved: null, or what the backward pass is given. */
+int fhe_ssm_gated_recurrence_prompt(const fhe_ssm_gated_recurrence* a, const void* z, const void* x, const int32_t* lengths,
+                                    const float* state_in, float* state_out, void* out, void* saved, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* From the gradients dout (null: zeros) and dstate_out (null: zeros) those of z, x and, where it is not null, state_in; z, x,
+ * lengths, sizes and saved are the prompt's.  dstate_in may be dstate_out. */
+int fhe_ssm_gated_recurrence_backward(const fhe_ssm_gated_recurrence* a, const void* z, const void* x, const int32_t* lengths,
+                                      const void* saved, const void* dout, const float* dstate_out, void* dz, void* dx,
+                                      float* dstate_in, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token for every lane: the same with tokens = 1 and no lengths. */
+int fhe_ssm_gated_recurrence_step(const fhe_ssm_gated_recurrence* a, const void* z, const void* x, const float* state_in,
+                                  float* state_out, void* out, void* stream);
+
+/* ---- embedding ----------------------------------------------------------------------------------------------------
+ *     out_t = scale table[token_t]        dtable[v] = scale sum of dout_t over the t with token_t = v, in their order
+ * tokens: int64 on the device; one outside [0, vocab) gives a row of zeros and adds to no gradient.  vocab <= 2^18, tokens <=
+ * 2^26, channels <= 2^20.  The lookup takes any of the types for either side. */
+typedef struct {
+    uint32_t table_type, row_type; /* of the table and its gradient; of out and dout */
+    uint32_t tokens, vocab, channels;
+    float scale;
+    int64_t table_stride, row_stride; /* elements from row to row; the table's gradient is contiguous */
+} fhe_ssm_embedding;
+
+int fhe_ssm_embedding_lookup(const fhe_ssm_embedding* a, const int64_t* tokens, const void* table, void* out, void* stream);
+
+/* Device memory that the gradient needs. */
+int fhe_ssm_embedding_workspace(const fhe_ssm_embedding* a, size_t* bytes);
+
+/* All of dtable (float32, or row_type) is written, or with `accumulate` the sums are added to what is there.  Sums are taken in
+ * float32 in the tokens' order and rounded once. */
+int fhe_ssm_embedding_gradient(const fhe_ssm_embedding* a, const int64_t* tokens, const void* dout, void* dtable,
+                               int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- log-probabilities of given tokens ----------------------------------------------------------------------------
+ * Per row of logits l, with p = softmax(l):
+ *     logprob = log p[token],  entropy = - sum p log p,  the `top` largest logits' tokens and log-probabilities
+ * Alternatives are in the order of falling logits, equal ones by rising index.  A token outside [0, vocab) has log-probability
+ * 0 and its weight counts for nothing: a padded position.  A logit of -inf has probability 0; a row of nothing else has
+ * entropy 0 and log-probability -inf.  A NaN or +inf makes its row's numbers NaN (and a gradient whose weights are not 0); it
+ * leaves other rows alone.  NaN and -inf are no alternatives: where there are fewer than `top`, the rest is token -1 with
+ * log-probability -inf.  vocab <= 2^18, rows < 2^22, top <= 32. */
+typedef struct {
+    uint32_t type;
+    uint32_t rows, vocab, top;
+    int64_t row_stride, gradient_stride; /* in elements */
+} fhe_ssm_token_logprobs;
+
+/* Device memory that the log-probabilities of these sizes need (0: workspace may be null). */
+int fhe_ssm_token_logprobs_workspace(const fhe_ssm_token_logprobs* a, size_t* bytes);
+
+/* tokens: int64[rows], null where no token is given.  logprobs, entropy: float32[rows], statistics: float32[rows][2], a row's
+ * largest logit and the log of sum exp(l - largest); each may be null.  top_tokens int64[rows][top], top_logprobs
+ * float32[rows][top], unless top is 0.  gradient, where it is not null: that of
+ *     sum over rows of weights logprob + entropy_weights entropy          (float32[rows], null: 0)
+ * with respect to the logits, in their type; it may be the logits' own buffer, with their stride. */
+int fhe_ssm_token_logprobs_forward(const fhe_ssm_token_logprobs* a, const void* logits, const int64_t* tokens,
+                                   float* logprobs, float* entropy, float* statistics, int64_t* top_tokens,
+                                   float* top_logprobs, const float* weights, const float* entropy_weights, void* gradient,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same gradient where its weights were not known before: from the statistics, and the entropy if it has weights. */
+int fhe_ssm_token_logprobs_gradient(const fhe_ssm_token_logprobs* a, const void* logits, const int64_t* tokens,
+                                    const float* statistics, const float* entropy, const float* weights,
+                                    const float* entropy_weights, void* gradient, void* stream);
+
+/* ---- AdamW --------------------------------------------------------------------------------------------------------
+ * For every entry of every tensor, with g the gradient times *scale_at:
+ *     m <- beta1 m + (1 - beta1) g,  v <- beta2 v + (1 - beta2) g^2,
+ *     p <- p - lr (weight_decay p + m / (1 - beta1^step) / (sqrt(v / (1 - beta2^step)) + eps))
+ * Parameters are float32; copy, where it is not null, receives them rounded to copy_type, for the products of the next pass.
+ * With state_bits 32, first and second are m and v in float32.  With 8 they are m and sqrt(v) as 8-bit floats (a sign, 4 bits
+ * of exponent with bias 7, 3 of mantissa), in blocks of 256 entries from the tensor's beginning; powers[block] has the powers of
+ * two behind the codes of m and of the root, as their exponent plus 134, 255 for NaN.  Zeros are the beginning of all.  8-bit
+ * states are rounded at random, by (seed, step, the tensor's place, the entry): equal calls give equal results.
+ * lr_at, step_at and scale_at, where they are not null, are read on the device in place of lr, step and 1, so that a recorded
+ * step follows them.  Tensors of no entries are passed over; one has less than 2^32.  eps >= 1e-30. */
+typedef struct {
+    uint32_t gradient_type, copy_type; /* copies are bf16 or f16 */
+    uint32_t state_bits;               /* 32 or 8 */
+    uint32_t step, seed;               /* steps count from 1 */
+    float lr, eps;
+    double beta1, beta2;
+    const float* lr_at;
+    const float* scale_at;
+    const int32_t* step_at;
+} fhe_ssm_adamw;
+
+typedef struct {
+    float* param;
+    const void* gradient;
+    void *first, *second;
+    uint8_t* powers; /* [ceil(n / 256)][2], only with 8 bits */
+    void* copy;
+    uint64_t n;
+    float weight_decay;
+} fhe_ssm_adamw_tensor;
+
+/* tensors: an array on the host, read before the call returns. */
+int fhe_ssm_adamw_step(const fhe_ssm_adamw* a, uint32_t count, const fhe_ssm_adamw_tensor* tensors, void* stream);
 
 #ifdef __cplusplus
 }
