@@ -15,13 +15,14 @@
 // segment's workgroup begins with those of the segments before it.  Then the inputs are read twice.
 // Bound by bytes: about 12 (backward 25) vector instructions an element.
 #include <algorithm>
+#include <type_traits>
 
 #include "rows.hpp"
 
 namespace clear {
 namespace {
 
-constexpr int kWaves = 8, kRun = 16;      // waves of a workgroup; tokens of a wave
+constexpr int kWaves = 8, kRun = 12;      // waves of a workgroup; tokens of a wave
 constexpr int kTile = kWaves * kRun;      // tokens between kept states
 constexpr uint32_t kEnough = 512;         // workgroups: two for each CU
 
@@ -37,17 +38,49 @@ struct Args {
     int64_t zs[2], xs[2], dys[2], outs[2], dzs[2], dxs[2];
 };
 
-// sigmoid(z) and sigmoid(-z), both to their last bits: the smaller is e / (1 + e) with e = exp(-|z|), the larger 1 less that, so
-// that gates near 1, of which many are multiplied, are rounded and no more (a reciprocal is off to one side)
+// sigmoid(z) and sigmoid(-z), both to their last bits.  A gate near 1 is 1 less the other, so that of the many that are
+// multiplied each is rounded and no more (a reciprocal is off to one side).
 __device__ inline void gates(float z, float& a, float& rest) {
-    const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(z));
-    const float small = e * __builtin_amdgcn_rcpf(1.f + e), large = 1.f - small;
-    a = z < 0.f ? small : large;
-    rest = z < 0.f ? large : small;
+    const float e = __builtin_amdgcn_exp2f(1.44269504f * z);
+    rest = __builtin_amdgcn_rcpf(1.f + e);
+    a = z < 0.f ? e * rest : 1.f - rest;
 }
 
 __device__ inline uint32_t length_of(const Args& a, uint32_t lane) {
     return a.lengths ? (uint32_t)min(max(a.lengths[lane], 0), (int)a.tokens) : a.tokens;
+}
+
+// An element of a row that all lanes share, by its place in bytes.  (The row's address is kept from being taken apart into a sum
+// for each lane and each row, which costs a vector instruction every time.)
+template <class T>
+__device__ inline __attribute__((address_space(1))) T& in_row(T* row, uint32_t bytes) {
+    uint64_t at = (uint64_t)row;
+    asm("" : "+s"(at));
+    return *(__attribute__((address_space(1))) T*)(at + bytes);
+}
+// A wave's rows from t0 on as their bits, each in a register of its own (two 16-bit ones in one would be waited for to be put
+// there); past `end` the last row again (kAll: none is).  `at` is the channel, or for lanes past the last that one.
+template <bool kAll, class T>
+__device__ inline void fetch(const T* rows, int64_t stride, uint32_t t0, uint32_t end, uint32_t at, uint32_t (&to)[kRun]) {
+    typedef std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t> bits;
+    const T* row = rows + (int64_t)(kAll ? t0 : min(t0, end - 1)) * stride;
+#pragma unroll
+    for (int i = 0; i < kRun; i++) {
+        to[i] = in_row((const bits*)row, at * (uint32_t)sizeof(T));
+        row += kAll || t0 + i + 1 < end ? stride : 0;
+    }
+}
+template <bool kAll, class T>
+__device__ inline void put(T* rows, int64_t stride, uint32_t t0, uint32_t end, uint32_t at, const float (&from)[kRun]) {
+    T* row = rows + (int64_t)t0 * stride;
+#pragma unroll
+    for (int i = 0; i < kRun; i++, row += stride)
+        if (kAll || t0 + i < end) in_row(row, at * (uint32_t)sizeof(T)) = from_f32<T>(from[i]);
+}
+template <class T>
+__device__ inline float of_bits(uint32_t x) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(x);
+    else return to_f32(__builtin_bit_cast(T, (uint16_t)x));
 }
 
 // the state (or gradient) that a segment begins with: what came in, through the segments before it (after it)
@@ -65,80 +98,98 @@ __device__ inline float begin(const Args& a, uint32_t lane, uint32_t segment, ui
     return s;
 }
 
-// The forward pass; !kOut: only the segments' A and H.
+// What the two passes' workgroups have in common: which lane, segment and channels are theirs.
+struct Place {
+    uint32_t lane, segment, c, from, wave, l, length, tile0, tile1, whole;  // whole: the end of the tiles that have all tokens
+    bool in;
+    size_t at;
+    __device__ Place(const Args& a) {
+        // workgroups go to the eight XCDs in turn; here each XCD gets neighbours, which read the same rows of memory
+        const uint32_t most = gridDim.x / 8 * 8, id = blockIdx.x < most ? blockIdx.x % 8 * (most / 8) + blockIdx.x / 8 : blockIdx.x;
+        const uint32_t strip = id % a.strips;
+        segment = id / a.strips % a.segments, lane = id / a.strips / a.segments;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64, c = strip * 64 + l;
+        in = c < a.channels;
+        from = min(c, a.channels - 1);
+        length = length_of(a, lane);
+        tile0 = segment * a.each, tile1 = min(a.tiles, tile0 + a.each);
+        whole = max(tile0, min(tile1, length / kTile));
+        at = (size_t)lane * a.channels + from;
+    }
+};
+
+// The forward pass; !kOut: only the segments' A and H.  Tiles that have all their tokens come first, the rows of each on their
+// way while the one before is worked on; then one that has some, and those behind the lane's length, which are zeros.
 template <class T, bool kOut>
 __global__ __launch_bounds__(kWaves * 64) void k_forward(Args a) {
     __shared__ float s_a[2][kWaves][64], s_h[2][kWaves][64];
-    const uint32_t strip = blockIdx.x % a.strips, segment = blockIdx.x / a.strips % a.segments, lane = blockIdx.x / a.strips / a.segments;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64, c = strip * 64 + l;
-    const bool in = c < a.channels;
-    const uint32_t length = length_of(a, lane);
-    const uint32_t tile1 = min(a.tiles, (segment + 1) * a.each);
-    const T *z = (const T*)a.z + lane * a.zs[0], *x = (const T*)a.x + lane * a.xs[0];
-    T* out = kOut ? (T*)a.out + lane * a.outs[0] : nullptr;
-    const size_t at = (size_t)lane * a.channels + c;
-    float state = 0.f, product = 1.f;
-    if (kOut && in) state = begin<false>(a, lane, segment, c);
-    for (uint32_t tile = segment * a.each; tile < tile1; tile++) {
-        const uint32_t t0 = tile * kTile + wave * kRun;
+    const Place p(a);
+    const T *z = (const T*)a.z + p.lane * a.zs[0], *x = (const T*)a.x + p.lane * a.xs[0];
+    T* out = kOut ? (T*)a.out + p.lane * a.outs[0] : nullptr;
+    uint32_t zr[kRun], xr[kRun];
+    const auto next = [&](auto all, uint32_t tile) {
+        fetch<all.value>(z, a.zs[1], tile * kTile + p.wave * kRun, p.length, p.from, zr);
+        fetch<all.value>(x, a.xs[1], tile * kTile + p.wave * kRun, p.length, p.from, xr);
+    };
+    if (p.tile0 < p.whole) next(std::true_type{}, p.tile0);
+    float state = kOut ? begin<false>(a, p.lane, p.segment, p.from) : 0.f, product = 1.f;
+    const auto work = [&](auto all, uint32_t tile) {
+        constexpr bool kAll = all.value;
+        const uint32_t t0 = tile * kTile + p.wave * kRun;
+        if (kOut && a.saved && p.wave == 0 && p.in) a.saved[((size_t)p.lane * a.tiles + tile) * a.channels + p.c] = state;
         float g[kRun], b[kRun], A = 1.f, H = 0.f;
-        if (kOut && a.saved && wave == 0 && in) a.saved[((size_t)lane * a.tiles + tile) * a.channels + c] = state;
-        if (t0 + kRun <= length) {
 #pragma unroll
-            for (int i = 0; i < kRun; i++) {
-                g[i] = in ? to_f32(z[(int64_t)(t0 + i) * a.zs[1] + c]) : 0.f;
-                b[i] = in ? to_f32(x[(int64_t)(t0 + i) * a.xs[1] + c]) : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < kRun; i++) {
-                float rest;
-                gates(g[i], g[i], rest);
-                b[i] *= rest;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kRun; i++) {
-                g[i] = 1.f, b[i] = 0.f;  // a token that is not there keeps the state
-                if (t0 + i < length && in) {
-                    float rest;
-                    gates(to_f32(z[(int64_t)(t0 + i) * a.zs[1] + c]), g[i], rest);
-                    b[i] = rest * to_f32(x[(int64_t)(t0 + i) * a.xs[1] + c]);
-                }
-            }
+        for (int i = 0; i < kRun; i++) {
+            float rest;
+            gates(of_bits<T>(zr[i]), g[i], rest);
+            b[i] = rest * of_bits<T>(xr[i]);
+            if (!kAll && t0 + i >= p.length) g[i] = 1.f, b[i] = 0.f;  // a token that is not there keeps the state
         }
+        if (kAll && tile + 1 < p.whole) next(all, tile + 1);
 #pragma unroll
         for (int i = 0; i < kRun; i++) {
             H = g[i] * H + b[i];
             A *= g[i];
         }
         const int turn = tile & 1;
-        s_a[turn][wave][l] = A;
-        s_h[turn][wave][l] = H;
+        s_a[turn][p.wave][p.l] = A;
+        s_h[turn][p.wave][p.l] = H;
         __syncthreads();
         float mine = state;
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; w++) {
-            if (w == wave) mine = state;
-            state = s_a[turn][w][l] * state + s_h[turn][w][l];
-            if (!kOut) product *= s_a[turn][w][l];
+            if (w == p.wave) mine = state;
+            state = s_a[turn][w][p.l] * state + s_h[turn][w][p.l];
+            if (!kOut) product *= s_a[turn][w][p.l];
         }
-        if (kOut && in) {
+        if (kOut) {
 #pragma unroll
             for (int i = 0; i < kRun; i++) {
-                mine = g[i] * mine + b[i];
-                if (t0 + i < a.tokens) out[(int64_t)(t0 + i) * a.outs[1] + c] = from_f32<T>(t0 + i < length ? mine : 0.f);
+                b[i] = mine = g[i] * mine + b[i];
+                if (!kAll && t0 + i >= p.length) b[i] = 0.f;
             }
+            if (p.in) put<kAll>(out, a.outs[1], t0, a.tokens, p.c, b);
+        }
+    };
+    for (uint32_t tile = p.tile0; tile < p.whole; tile++) work(std::true_type{}, tile);
+    for (uint32_t tile = p.whole; tile < p.tile1; tile++) {
+        if (tile * kTile < p.length) {
+            next(std::false_type{}, tile);
+            work(std::false_type{}, tile);
+        } else if (kOut && p.in) {
+            const float none[kRun] = {};
+            put<false>(out, a.outs[1], tile * kTile + p.wave * kRun, a.tokens, p.c, none);
         }
     }
-    if (wave != 0 || !in) return;
+    if (p.wave != 0 || !p.in) return;
     if (kOut) {
-        if (a.last && segment == a.segments - 1) a.last[at] = state;
+        if (a.last && p.segment == a.segments - 1) a.last[p.at] = state;
     } else {
-        float* f = a.folded + ((size_t)lane * a.segments + segment) * 2 * a.channels + c;
+        float* f = a.folded + ((size_t)p.lane * a.segments + p.segment) * 2 * a.channels + p.c;
         f[0] = product;
         f[a.channels] = state;
         // `in` and `last` may be one buffer, and workgroups of the second pass read the one while one of them writes the other
-        if (segment == 0) a.folded[((size_t)a.lanes * a.segments * 2) * a.channels + at] = a.in ? a.in[at] : 0.f;
+        if (p.segment == 0) a.folded[((size_t)a.lanes * a.segments * 2) * a.channels + p.at] = a.in ? a.in[p.at] : 0.f;
     }
 }
 
@@ -146,41 +197,35 @@ __global__ __launch_bounds__(kWaves * 64) void k_forward(Args a) {
 template <class T, bool kOut>
 __global__ __launch_bounds__(kWaves * 64) void k_backward(Args a) {
     __shared__ float s_a[2][kWaves][64], s_h[2][kWaves][64], s_g[2][kWaves][64];
-    const uint32_t strip = blockIdx.x % a.strips, segment = blockIdx.x / a.strips % a.segments, lane = blockIdx.x / a.strips / a.segments;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64, c = strip * 64 + l;
-    const bool in = c < a.channels;
-    const uint32_t length = length_of(a, lane);
-    const uint32_t tile0 = segment * a.each, tile1 = min(a.tiles, tile0 + a.each);
-    const T *z = (const T*)a.z + lane * a.zs[0], *x = (const T*)a.x + lane * a.xs[0];
-    const T* dy = a.dy ? (const T*)a.dy + lane * a.dys[0] : nullptr;
-    T *dz = (T*)a.dz + lane * a.dzs[0], *dx = (T*)a.dx + lane * a.dxs[0];
-    const size_t at = (size_t)lane * a.channels + c;
-    float carry = 0.f, product = 1.f;
-    if (kOut && in) carry = begin<true>(a, lane, segment, c);
-    for (uint32_t tile = tile1; tile-- > tile0;) {
-        const uint32_t t0 = tile * kTile + wave * kRun;
-        float g[kRun], r[kRun], b[kRun], d[kRun];
-        float h = kOut && in ? a.saved[((size_t)lane * a.tiles + tile) * a.channels + c] : 0.f;
-        if (t0 + kRun <= length) {
+    const Place p(a);
+    const T *z = (const T*)a.z + p.lane * a.zs[0], *x = (const T*)a.x + p.lane * a.xs[0];
+    const T* dy = a.dy ? (const T*)a.dy + p.lane * a.dys[0] : nullptr;
+    T *dz = (T*)a.dz + p.lane * a.dzs[0], *dx = (T*)a.dx + p.lane * a.dxs[0];
+    uint32_t zr[kRun], xr[kRun], dr[kRun];
+    float h_next = 0.f;
+    const auto next = [&](auto all, uint32_t tile) {
+        const uint32_t t0 = tile * kTile + p.wave * kRun;
+        fetch<all.value>(z, a.zs[1], t0, p.length, p.from, zr);
+        if (kOut) fetch<all.value>(x, a.xs[1], t0, p.length, p.from, xr);
+        if (dy) fetch<all.value>(dy, a.dys[1], t0, p.length, p.from, dr);
+        else
 #pragma unroll
-            for (int i = 0; i < kRun; i++) {
-                g[i] = in ? to_f32(z[(int64_t)(t0 + i) * a.zs[1] + c]) : 0.f;
-                b[i] = kOut && in ? to_f32(x[(int64_t)(t0 + i) * a.xs[1] + c]) : 0.f;
-                d[i] = dy && in ? to_f32(dy[(int64_t)(t0 + i) * a.dys[1] + c]) : 0.f;
-            }
+            for (int i = 0; i < kRun; i++) dr[i] = 0;
+        if (kOut) h_next = a.saved[((size_t)p.lane * a.tiles + tile) * a.channels + p.from];
+    };
+    float carry = kOut ? begin<true>(a, p.lane, p.segment, p.from) : 0.f, product = 1.f;
+    const auto work = [&](auto all, uint32_t tile) {
+        constexpr bool kAll = all.value;
+        const uint32_t t0 = tile * kTile + p.wave * kRun;
+        float g[kRun], r[kRun], b[kRun], d[kRun], h = h_next;
 #pragma unroll
-            for (int i = 0; i < kRun; i++) gates(g[i], g[i], r[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kRun; i++) {
-                g[i] = 1.f, r[i] = b[i] = d[i] = 0.f;
-                if (t0 + i < length && in) {
-                    gates(to_f32(z[(int64_t)(t0 + i) * a.zs[1] + c]), g[i], r[i]);
-                    if (kOut) b[i] = to_f32(x[(int64_t)(t0 + i) * a.xs[1] + c]);
-                    if (dy) d[i] = to_f32(dy[(int64_t)(t0 + i) * a.dys[1] + c]);
-                }
-            }
+        for (int i = 0; i < kRun; i++) {
+            gates(of_bits<T>(zr[i]), g[i], r[i]);
+            b[i] = kOut ? of_bits<T>(xr[i]) : 0.f;
+            d[i] = of_bits<T>(dr[i]);
+            if (!kAll && t0 + i >= p.length) g[i] = 1.f, r[i] = b[i] = d[i] = 0.f;
         }
+        if (kAll && tile > p.tile0) next(all, tile - 1);
         float A = 1.f, H = 0.f, G = 0.f;
 #pragma unroll
         for (int i = 0; i < kRun; i++) {
@@ -190,49 +235,61 @@ __global__ __launch_bounds__(kWaves * 64) void k_backward(Args a) {
 #pragma unroll
         for (int i = kRun; i-- > 0;) G = g[i] * (G + d[i]);
         const int turn = tile & 1;
-        s_a[turn][wave][l] = A;
-        if (kOut) s_h[turn][wave][l] = H;
-        s_g[turn][wave][l] = G;
+        s_a[turn][p.wave][p.l] = A;
+        if (kOut) s_h[turn][p.wave][p.l] = H;
+        s_g[turn][p.wave][p.l] = G;
         __syncthreads();
         float mine = carry;
 #pragma unroll
         for (int w = kWaves; w-- > 0;) {
-            if ((uint32_t)w == wave) mine = carry;
-            carry = s_a[turn][w][l] * carry + s_g[turn][w][l];
-            if (!kOut) product *= s_a[turn][w][l];
+            if ((uint32_t)w == p.wave) mine = carry;
+            carry = s_a[turn][w][p.l] * carry + s_g[turn][w][p.l];
+            if (!kOut) product *= s_a[turn][w][p.l];
         }
         if (kOut) {
 #pragma unroll
             for (uint32_t w = 0; w < kWaves - 1; w++)
-                if (w < wave) h = s_a[turn][w][l] * h + s_h[turn][w][l];
+                if (w < p.wave) h = s_a[turn][w][p.l] * h + s_h[turn][w][p.l];
 #pragma unroll
             for (int i = 0; i < kRun; i++) {  // b: what dz takes besides d
-                const float next = g[i] * h + r[i] * b[i];
+                const float after = g[i] * h + r[i] * b[i];
                 b[i] = g[i] * r[i] * (h - b[i]);
-                h = next;
+                h = after;
             }
-            if (in) {
 #pragma unroll
-                for (int i = kRun; i-- > 0;) {
-                    const float now = d[i] + mine;
-                    mine = g[i] * now;
-                    if (t0 + i < a.tokens) {
-                        const bool there = t0 + i < length;
-                        dz[(int64_t)(t0 + i) * a.dzs[1] + c] = from_f32<T>(there ? now * b[i] : 0.f);
-                        dx[(int64_t)(t0 + i) * a.dxs[1] + c] = from_f32<T>(there ? now * r[i] : 0.f);
-                    }
-                }
+            for (int i = kRun; i-- > 0;) {
+                const float now = d[i] + mine;
+                mine = g[i] * now;
+                b[i] *= now;
+                r[i] *= now;
+                if (!kAll && t0 + i >= p.length) b[i] = r[i] = 0.f;
+            }
+            if (p.in) {
+                put<kAll>(dz, a.dzs[1], t0, a.tokens, p.c, b);
+                put<kAll>(dx, a.dxs[1], t0, a.tokens, p.c, r);
             }
         }
+    };
+    for (uint32_t tile = p.tile1; tile-- > p.whole;) {
+        if (tile * kTile < p.length) {
+            next(std::false_type{}, tile);
+            work(std::false_type{}, tile);
+        } else if (kOut && p.in) {
+            const float none[kRun] = {};
+            put<false>(dz, a.dzs[1], tile * kTile + p.wave * kRun, a.tokens, p.c, none);
+            put<false>(dx, a.dxs[1], tile * kTile + p.wave * kRun, a.tokens, p.c, none);
+        }
     }
-    if (wave != 0 || !in) return;
+    if (p.tile0 < p.whole) next(std::true_type{}, p.whole - 1);
+    for (uint32_t tile = p.whole; tile-- > p.tile0;) work(std::true_type{}, tile);
+    if (p.wave != 0 || !p.in) return;
     if (kOut) {
-        if (a.last && segment == 0) a.last[at] = carry;
+        if (a.last && p.segment == 0) a.last[p.at] = carry;
     } else {
-        float* f = a.folded + ((size_t)lane * a.segments + segment) * 2 * a.channels + c;
+        float* f = a.folded + ((size_t)p.lane * a.segments + p.segment) * 2 * a.channels + p.c;
         f[0] = product;
         f[a.channels] = carry;
-        if (segment == 0) a.folded[((size_t)a.lanes * a.segments * 2) * a.channels + at] = a.in ? a.in[at] : 0.f;
+        if (p.segment == 0) a.folded[((size_t)a.lanes * a.segments * 2) * a.channels + p.at] = a.in ? a.in[p.at] : 0.f;
     }
 }
 
