@@ -18,8 +18,8 @@
 namespace clear {
 namespace {
 
-constexpr uint32_t kPiece = 32, kSmall = 8192;
-constexpr uint32_t kTile = 4096, kMostParts = 256, kDigits = 1024;  // sorted at a time by a workgroup; workgroups; values of a digit
+constexpr uint32_t kPiece = 32, kFew = 1024, kSmall = 8192;
+constexpr uint32_t kTile = 2048, kMostParts = 256, kDigits = 1024;  // sorted at a time by a workgroup; workgroups; values of a digit
 constexpr uint32_t kMostVocab = 1u << 18, kMostTokens = 1u << 26;
 
 struct Args {
@@ -50,28 +50,30 @@ __device__ inline uint32_t id_of(const Args& a, uint32_t i) {
 }
 
 // ---------------------------------------------------------------- lookup
-// A row for each L lanes, in vectors of V.
-template <class F, class T, int V, int L>
+// A vector of V a thread, kEach times, over all rows.
+template <class F, class T, int V>
 __global__ __launch_bounds__(256) void k_lookup(Args a) {
-    const uint32_t lane = threadIdx.x % L;
-    const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    if (i >= a.n) return;
-    const int64_t token = a.tokens[i];
-    const bool in = token >= 0 && token < (int64_t)a.vocab;
-    const F* from = (const F*)a.from + (in ? token : 0) * a.from_stride;
-    T* to = (T*)a.to + i * a.to_stride;
-#pragma unroll 4
-    for (uint32_t c = lane * V; c < a.d; c += L * V) {
-        float f[V];
+    constexpr int kEach = 4;
+    const uint32_t vectors = (a.d + V - 1) / V;
+    const uint64_t all = (uint64_t)a.n * vectors, at = (uint64_t)blockIdx.x * 256 * kEach + threadIdx.x;
+    float f[kEach][V];
+    T* to[kEach];
 #pragma unroll
-        for (int e = 0; e < V; e++) f[e] = 0.f;
-        if (in) {
-            load<V>(from + c, f);
+    for (int k = 0; k < kEach; k++) {
+        const uint64_t i = min(at + k * 256, all - 1);
+        uint32_t row, c;
+        if (all <= 0xffffffffull) row = (uint32_t)i / vectors, c = ((uint32_t)i - row * vectors) * V;
+        else row = (uint32_t)(i / vectors), c = (uint32_t)(i - (uint64_t)row * vectors) * V;
+        const int64_t token = a.tokens[row];
+        const bool in = token >= 0 && token < (int64_t)a.vocab;
+        load<V>((const F*)a.from + (in ? token : 0) * a.from_stride + c, f[k]);
+        to[k] = (T*)a.to + row * a.to_stride + c;
 #pragma unroll
-            for (int e = 0; e < V; e++) f[e] *= a.scale;
-        }
-        store<V>(to + c, f);
+        for (int e = 0; e < V; e++) f[k][e] = in ? f[k][e] * a.scale : 0.f;
     }
+#pragma unroll
+    for (int k = 0; k < kEach; k++)
+        if (at + k * 256 < all) store<V>(to[k], f[k]);
 }
 
 // ---------------------------------------------------------------- the sort
@@ -146,12 +148,14 @@ __device__ inline void zero(const Args& a, uint32_t block) {
             if (threadIdx.x < a.edges[e]) a.edge[e][threadIdx.x] = 0;
 }
 
-// Up to kSmall positions in one workgroup; the others set to 0.
+__global__ __launch_bounds__(1024) void k_zero(Args a) { zero(a, blockIdx.x); }
+
+// Up to 1,024 kRounds positions in one workgroup; the others set to 0.
+template <int kRounds>
 __global__ __launch_bounds__(1024) void k_sort_small(Args a) {
     __shared__ Sort s;
     __shared__ uint32_t keys[kSmall];
     if (blockIdx.x > 0) return zero(a, blockIdx.x - 1);
-    constexpr int kRounds = kSmall / 1024;
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const uint32_t each = (a.n + 1023) / 1024 * 64;  // of a wave
     uint32_t key[kRounds], digit[kRounds], rank[kRounds];
@@ -258,10 +262,24 @@ __global__ __launch_bounds__(1024) void k_move(Args a) {
 // Channels of a wave: groups of V, kGroups of them a lane, then the next 64 V kGroups.
 constexpr int kGroups = 2;
 
-// Adds n rows to f, in order; row(j) is where row j begins.  kFlight rows are on their way at once; a lane past the row's end
+// Adds n rows to f, in order; row(j) is where row j begins.  Up to kFlight rows are on their way at once, at the end the last
+// of them again for those that are not there: a row that is waited for alone takes as long as all.  A lane past the row's end
 // reads its beginning.
-constexpr int kFlight = 4;
-template <int V, class F>
+template <int kRows, int V, class F>
+__device__ inline void add_batch(uint32_t j, uint32_t n, const uint32_t (&c)[kGroups], float (&f)[kGroups * V], F&& row) {
+    float x[kRows][kGroups * V];
+#pragma unroll
+    for (int i = 0; i < kRows; i++) {
+        const auto* at = row(min(j + i, n - 1));
+#pragma unroll
+        for (int g = 0; g < kGroups; g++) load<V>(at + c[g], x[i] + g * V);
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; i++)
+#pragma unroll
+        for (int e = 0; e < kGroups * V; e++) f[e] = j + i < n ? f[e] + x[i][e] : f[e];
+}
+template <int kFlight, int V, class F>
 __device__ inline void add_rows(uint32_t n, uint32_t c0, uint32_t d, float (&f)[kGroups * V], F&& row) {
     uint32_t c[kGroups];
 #pragma unroll
@@ -269,39 +287,32 @@ __device__ inline void add_rows(uint32_t n, uint32_t c0, uint32_t d, float (&f)[
         c[g] = c0 + (g * 64 + threadIdx.x % 64) * V;
         c[g] = c[g] < d ? c[g] : 0;
     }
-    uint32_t j = 0;
-    for (; j + kFlight <= n; j += kFlight) {
-        float x[kFlight][kGroups * V];
-#pragma unroll
-        for (int i = 0; i < kFlight; i++) {
-            const auto* at = row(j + i);
-#pragma unroll
-            for (int g = 0; g < kGroups; g++) load<V>(at + c[g], x[i] + g * V);
-        }
-#pragma unroll
-        for (int i = 0; i < kFlight; i++)
-#pragma unroll
-            for (int e = 0; e < kGroups * V; e++) f[e] += x[i][e];
-    }
-    for (; j < n; j++) {
-        const auto* at = row(j);
-        float x[kGroups * V];
-#pragma unroll
-        for (int g = 0; g < kGroups; g++) load<V>(at + c[g], x + g * V);
-#pragma unroll
-        for (int e = 0; e < kGroups * V; e++) f[e] += x[e];
+    for (uint32_t j = 0; j < n; j += kFlight) {
+        if (n - j <= 2) add_batch<2, V>(j, n, c, f, row);
+        else add_batch<kFlight, V>(j, n, c, f, row);
     }
 }
-// rows from .. to - 1 of the sorted positions
-template <class T, int V>
-__device__ inline void add_sorted(const Args& a, uint32_t from, uint32_t to, uint32_t c0, float (&f)[kGroups * V]) {
-    const uint32_t lane = threadIdx.x % 64;
-    for (uint32_t i = from; i < to; i += 64) {
-        const uint32_t n = min(64u, to - i);
-        const int mine = (int)(lane < n ? a.at[0][i + lane] : 0);
-        add_rows<V>(n, c0, a.d, f, [&](uint32_t j) {
-            return (const T*)a.from + (int64_t)(uint32_t)__builtin_amdgcn_readlane(mine, (int)j) * a.from_stride;
-        });
+// rows at .. at + n - 1 of 64 sorted positions, of which each lane holds one
+template <class T, int kFlight, int V>
+__device__ inline void add_held(const Args& a, uint32_t held, uint32_t at, uint32_t n, uint32_t c0, float (&f)[kGroups * V]) {
+    add_rows<kFlight, V>(n, c0, a.d, f, [&](uint32_t j) {
+        return (const T*)a.from + (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)held, (int)(at + j)) * a.from_stride;
+    });
+}
+
+// scales a row's sum and writes it, or adds it to what is there
+template <class G, int V>
+__device__ inline void write_row(const Args& a, uint32_t id, uint32_t c0, float (&f)[kGroups * V]) {
+    G* to = (G*)a.to + (size_t)id * a.d;
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+        const uint32_t c = c0 + (g * 64 + threadIdx.x % 64) * V;
+        if (c >= a.d) continue;
+        float x[V], *y = f + g * V;
+        if (a.add) load<V>(to + c, x);
+#pragma unroll
+        for (int e = 0; e < V; e++) y[e] = y[e] * a.scale + (a.add ? x[e] : 0.f);
+        store<V>(to + c, y);
     }
 }
 
@@ -311,11 +322,11 @@ __global__ __launch_bounds__(256) void k_pieces(Args a) {
     const uint32_t piece = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / 64), lane = threadIdx.x % 64;
     const uint64_t from = (uint64_t)piece * kPiece;
     if (from + kPiece > a.n) return;
-    const uint32_t id = a.ids[0][from];
-    if (id >= a.vocab || a.ids[0][from + kPiece - 1] != id) return;
+    const uint32_t id = a.ids[0][from], id_last = a.ids[0][from + kPiece - 1], held = a.at[0][from + lane % kPiece];
+    if (id >= a.vocab || id_last != id) return;
     for (uint32_t c0 = 0; c0 < a.d; c0 += 64 * V * kGroups) {
         float f[kGroups * V] = {};
-        add_sorted<T, V>(a, (uint32_t)from, (uint32_t)from + kPiece, c0, f);
+        add_held<T, 8, V>(a, held, 0, kPiece, c0, f);
 #pragma unroll
         for (int g = 0; g < kGroups; g++) {
             const uint32_t c = c0 + (g * 64 + lane) * V;
@@ -324,39 +335,130 @@ __global__ __launch_bounds__(256) void k_pieces(Args a) {
     }
 }
 
-// A wave for every sorted position; the first of its token's run adds the run.
+// A wave for every sorted position; the first of its token's run adds the run.  A run of 64 and more is added by all waves of
+// the workgroup, each a share of its rows and pieces, once they are done with their own.  (Their positions follow each other, so
+// no second long run begins among them.)
 template <class T, class G, int V>
 __global__ __launch_bounds__(256) void k_runs(Args a) {
-    const uint64_t at = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const uint32_t lane = threadIdx.x % 64;
-    if (at >= a.n) return;
-    const uint32_t i = __builtin_amdgcn_readfirstlane((uint32_t)at);
-    const uint32_t id = a.ids[0][i];
-    if (id >= a.vocab || (i > 0 && a.ids[0][i - 1] == id)) return;
-    uint32_t end = i;
-    for (;; end += 64) {
-        const uint64_t more = __ballot(end + lane < a.n && a.ids[0][min(end + lane, a.n - 1)] == id);
-        if (more == ~0ull) continue;
-        end += __popcll(more);
-        break;
-    }
-    const uint32_t first = min((i + kPiece - 1) / kPiece * kPiece, end), last = max(first, end / kPiece * kPiece);
-    for (uint32_t c0 = 0; c0 < a.d; c0 += 64 * V * kGroups) {
-        float f[kGroups * V] = {};
-        add_sorted<T, V>(a, i, first, c0, f);
-        add_rows<V>((last - first) / kPiece, c0, a.d, f, [&](uint32_t j) { return a.sums + (size_t)(first / kPiece + j) * a.d; });
-        add_sorted<T, V>(a, last, end, c0, f);
-        G* to = (G*)a.to + (size_t)id * a.d;
-#pragma unroll
-        for (int g = 0; g < kGroups; g++) {
-            const uint32_t c = c0 + (g * 64 + lane) * V;
-            if (c >= a.d) continue;
-            float x[V], *y = f + g * V;
-            if (a.add) load<V>(to + c, x);
-#pragma unroll
-            for (int e = 0; e < V; e++) y[e] = y[e] * a.scale + (a.add ? x[e] : 0.f);
-            store<V>(to + c, y);
+    constexpr int kCols = 64 * V * kGroups;
+    __shared__ float s_sum[3][kCols];
+    __shared__ uint32_t s_begin;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const uint32_t i = min(blockIdx.x * 4 + wave, a.n - 1), here = min(i + lane, a.n - 1);
+    if (threadIdx.x == 0) s_begin = a.n;
+    __syncthreads();
+    // one wait for all that a short run needs to know
+    const uint32_t ahead = a.ids[0][here], held = a.at[0][here], previous = a.ids[0][max(i, 1u) - 1];
+    const uint32_t id = __builtin_amdgcn_readfirstlane(ahead);
+    if (blockIdx.x * 4 + wave < a.n && id < a.vocab && (i == 0 || previous != id)) {
+        const uint32_t n = __popcll(__ballot(i + lane < a.n && ahead == id));
+        if (n == 64) {
+            if (lane == 0) s_begin = i;
+        } else {
+            const uint32_t end = i + n, first = min((i + kPiece - 1) / kPiece * kPiece, end), last = max(first, end / kPiece * kPiece);
+            for (uint32_t c0 = 0; c0 < a.d; c0 += kCols) {
+                float f[kGroups * V] = {};
+                add_held<T, 4, V>(a, held, 0, first - i, c0, f);
+                if (last > first) add_rows<1, V>((last - first) / kPiece, c0, a.d, f, [&](uint32_t j) { return a.sums + (size_t)(first / kPiece + j) * a.d; });
+                add_held<T, 4, V>(a, held, last - i, end - last, c0, f);
+                write_row<G, V>(a, id, c0, f);
+            }
         }
+    }
+    __syncthreads();
+    const uint32_t begin = __builtin_amdgcn_readfirstlane(s_begin);
+    if (begin == a.n) return;
+    // the run's end, by 64 looks at a time ever further ahead, and then ever nearer
+    const uint32_t run = a.ids[0][begin];
+    uint64_t last_of = begin + 63;
+    const auto equal_ahead = [&](uint64_t stride) {
+        const uint64_t j = last_of + (lane + 1) * stride;
+        return (uint32_t)__popcll(__ballot(j < a.n && a.ids[0][j < a.n ? j : begin] == run));
+    };
+    uint64_t stride = 64;
+    for (;; stride *= 64) {
+        const uint32_t more = equal_ahead(stride);
+        last_of += more * stride;
+        if (more < 64) break;
+    }
+    while (stride > 1) {
+        stride /= 64;
+        last_of += equal_ahead(stride) * stride;
+    }
+    const uint32_t end = (uint32_t)last_of + 1, first = (begin + kPiece - 1) / kPiece * kPiece, last = end / kPiece * kPiece;
+    const uint32_t before = first - begin, pieces = (last - first) / kPiece, behind = end - last;
+    const uint32_t held0 = a.at[0][min(begin + lane, a.n - 1)], held1 = a.at[0][min(last + lane, a.n - 1)];
+    const auto share = [&](uint32_t n, uint32_t w) { return (uint32_t)((uint64_t)n * w / 4); };
+    for (uint32_t c0 = 0; c0 < a.d; c0 += kCols) {
+        float f[kGroups * V] = {};
+        uint32_t from = share(before, wave);
+        add_held<T, 4, V>(a, held0, from, share(before, wave + 1) - from, c0, f);
+        from = first / kPiece + share(pieces, wave);
+        add_rows<4, V>(share(pieces, wave + 1) - share(pieces, wave), c0, a.d, f, [&](uint32_t j) { return a.sums + (size_t)(from + j) * a.d; });
+        const uint32_t rest = share(behind, wave);
+        add_held<T, 4, V>(a, held1, rest, share(behind, wave + 1) - rest, c0, f);
+        if (wave)
+#pragma unroll
+            for (int e = 0; e < kGroups * V; e++) s_sum[wave - 1][e * 64 + lane] = f[e];
+        __syncthreads();
+        if (!wave) {
+#pragma unroll
+            for (int w = 0; w < 3; w++)
+#pragma unroll
+                for (int e = 0; e < kGroups * V; e++) f[e] += s_sum[w][e * 64 + lane];
+            write_row<G, V>(a, run, c0, f);
+        }
+        __syncthreads();
+    }
+}
+
+// Few tokens without a sort: a workgroup for every position looks for its token in all of them, ends if it stands at an earlier
+// one, and adds the rows of those where it stands: each of its waves 64 V kGroups channels, or where there are many, each a
+// part of the rows.
+template <class T, class G, int V>
+__global__ __launch_bounds__(256) void k_few(Args a) {
+    constexpr int kRounds = kFew / 64, kCols = 64 * V * kGroups;
+    __shared__ uint32_t s_at[kFew];
+    __shared__ float s_sum[3][kCols];
+    const uint32_t i = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const uint32_t id = id_of(a, i);
+    if (id >= a.vocab) return;
+    uint32_t n = 0;
+    bool earlier = false;
+#pragma unroll
+    for (int r = 0; r < kRounds; r++) {
+        const uint32_t j = r * 64 + lane;
+        if (r * 64u < a.n) {
+            const bool same = j < a.n && id_of(a, min(j, a.n - 1)) == id;
+            const uint64_t all = __ballot(same);
+            earlier |= __ballot(same && j < i) != 0;
+            if (same && wave == 0) s_at[n + __popcll(all & ((1ull << lane) - 1))] = j;
+            n += __popcll(all);
+        }
+    }
+    if (earlier) return;  // in all waves alike
+    __syncthreads();
+    const auto row = [&](uint32_t j) { return (const T*)a.from + (int64_t)__builtin_amdgcn_readfirstlane(s_at[j]) * a.from_stride; };
+    const uint32_t c_from = blockIdx.y * 4 * kCols, c_to = min(a.d, c_from + 4 * kCols);
+    const bool split = n > 16;
+    const uint32_t j0 = split ? n * wave / 4 : 0, j1 = split ? n * (wave + 1) / 4 : n;
+    for (uint32_t c0 = c_from + (split ? 0 : wave * kCols); c0 < c_to; c0 += split ? kCols : 4 * kCols) {
+        float f[kGroups * V] = {};
+        add_rows<8, V>(j1 - j0, c0, a.d, f, [&](uint32_t j) { return row(j0 + j); });
+        if (split) {
+            if (wave)
+#pragma unroll
+                for (int e = 0; e < kGroups * V; e++) s_sum[wave - 1][e * 64 + lane] = f[e];
+            __syncthreads();
+            if (!wave)
+#pragma unroll
+                for (int w = 0; w < 3; w++)
+#pragma unroll
+                    for (int e = 0; e < kGroups * V; e++) f[e] += s_sum[w][e * 64 + lane];
+            __syncthreads();
+            if (wave) continue;
+        }
+        write_row<G, V>(a, id, c0, f);
     }
 }
 
@@ -387,6 +489,7 @@ Layout layout(const fhe_ssm_embedding& a) {
         y.bytes += (n + 255) / 256 * 256;
         return at;
     };
+    if (a.tokens <= kFew) return y;
     const size_t list = a.tokens * sizeof(uint32_t);
     y.ids[0] = put(list), y.at[0] = put(list);
     y.ids[1] = put(small ? 0 : list), y.at[1] = put(small ? 0 : list);
@@ -418,17 +521,13 @@ int fhe_ssm_embedding_lookup(const fhe_ssm_embedding* a, const int64_t* tokens, 
             typedef decltype(t) T;
             constexpr int V = 16 / (sizeof(F) > sizeof(T) ? sizeof(F) : sizeof(T));
             const bool vectors = k.d % V == 0 && on_vectors(table, k.from_stride, sizeof(F), V) && on_vectors(out, k.to_stride, sizeof(T), V);
-            const auto run = [&](auto v, auto l) {
-                constexpr int kV = decltype(v)::value, L = decltype(l)::value;
-                hipLaunchKernelGGL((k_lookup<F, T, kV, L>), dim3((uint32_t)(((uint64_t)k.n * L + 255) / 256)), dim3(256), 0, (hipStream_t)stream, k);
+            const auto run = [&](auto v) {
+                constexpr int kV = decltype(v)::value;
+                const uint64_t all = (uint64_t)k.n * ((k.d + kV - 1) / kV);
+                hipLaunchKernelGGL((k_lookup<F, T, kV>), dim3((uint32_t)((all + 1023) / 1024)), dim3(256), 0, (hipStream_t)stream, k);
                 return launched("embedding");
             };
-            const std::integral_constant<int, V> wide;
-            const std::integral_constant<int, 1> one;
-            const std::integral_constant<int, 16> few;
-            const std::integral_constant<int, 64> many;
-            const bool narrow = k.d <= 16u * (vectors ? V : 1);
-            return vectors ? narrow ? run(wide, few) : run(wide, many) : narrow ? run(one, few) : run(one, many);
+            return vectors ? run(std::integral_constant<int, V>{}) : run(std::integral_constant<int, 1>{});
         });
     });
 }
@@ -437,7 +536,7 @@ int fhe_ssm_embedding_workspace(const fhe_ssm_embedding* a, size_t* bytes) {
     using namespace clear;
     if (int rc = check(a)) return rc;
     if (!bytes) return fail(CKKS_EINVAL, "embedding: null argument");
-    *bytes = a->tokens ? layout(*a).bytes : 0;
+    *bytes = layout(*a).bytes;
     return CKKS_OK;
 }
 
@@ -451,7 +550,7 @@ int fhe_ssm_embedding_gradient(const fhe_ssm_embedding* a, const int64_t* tokens
     if (!aligned(dtable, type_bytes(a->table_type))) return fail(CKKS_EINVAL, "embedding: the table's gradient lies between elements");
     if (a->tokens > 1 && a->row_stride < 0) return fail(CKKS_EINVAL, "embedding: a negative stride");
     const Layout y = layout(*a);
-    if (a->tokens && (!workspace || !aligned(workspace, 16) || workspace_bytes < y.bytes))
+    if (y.bytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < y.bytes))
         return fail(CKKS_EINVAL, "embedding: the workspace must have %zu bytes and lie on 16", y.bytes);
     Args k{};
     k.tokens = tokens, k.from = dout, k.to = dtable, k.n = a->tokens, k.vocab = a->vocab, k.d = a->channels;
@@ -474,7 +573,12 @@ int fhe_ssm_embedding_gradient(const fhe_ssm_embedding* a, const int64_t* tokens
         k.zero_from = words * i / of, k.zero_to = words * (i + 1) / of;
         hipLaunchKernelGGL(kernel, dim3(parts + k.zero_blocks), dim3(1024), 0, st, k);
     };
-    if (small) sort(k_sort_small, 0, 1, 1);
+    const bool few = k.n <= kFew;
+    if (few) {
+        if (!k.add) sort(k_zero, 0, 1, 0);
+    } else if (k.n <= 2048) sort(k_sort_small<2>, 0, 1, 1);
+    else if (k.n <= 4096) sort(k_sort_small<4>, 0, 1, 1);
+    else if (small) sort(k_sort_small<8>, 0, 1, 1);
     else {
         sort(k_count<0>, 0, 4, k.parts);
         sort(k_move<0>, 1, 4, k.parts);
@@ -488,6 +592,10 @@ int fhe_ssm_embedding_gradient(const fhe_ssm_embedding* a, const int64_t* tokens
         const auto add = [&](auto g, auto v) {
             typedef decltype(g) G;
             constexpr int V = decltype(v)::value;
+            if (few) {
+                hipLaunchKernelGGL((k_few<T, G, V>), dim3(k.n, (k.d + 256 * V * kGroups - 1) / (256 * V * kGroups)), dim3(256), 0, st, k);
+                return launched("embedding: gradient");
+            }
             if (k.n >= kPiece) hipLaunchKernelGGL((k_pieces<T, V>), dim3((k.n / kPiece + 3) / 4), dim3(256), 0, st, k);
             hipLaunchKernelGGL((k_runs<T, G, V>), dim3((k.n + 3) / 4), dim3(256), 0, st, k);
             return launched("embedding: gradient");

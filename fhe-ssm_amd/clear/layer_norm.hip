@@ -26,29 +26,45 @@ struct Args {
     float eps, n, each;  // d as a float, and its reciprocal
 };
 
-template <class T>
-__device__ inline float weight(const void* w, bool wide, uint32_t i, float none) {
-    return !w ? none : wide ? ((const float*)w)[i] : to_f32(((const T*)w)[i]);
-}
-
-// the row's elements of this lane, zeros past its end: group j of V lies at (j L + lane) V
-template <int L, int V, int E, class T>
-__device__ inline void load_row(const T* p, uint32_t lane, uint32_t d, float (&f)[E]) {
+// A row's elements of this lane as they lie in memory: group j of V lies at (j L + lane) V; none of a group past the row's end.
+template <class T, int L, int V, int E>
+struct Raw {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec v[E / V];
+    __device__ void read(const T* p, uint32_t lane, uint32_t d) {
 #pragma unroll
-    for (int j = 0; j < E / V; j++) {
-        const uint32_t i = (j * L + lane) * V;
-        if (i < d) load<V>(p + i, f + j * V);
-        else
-#pragma unroll
-            for (int c = 0; c < V; c++) f[j * V + c] = 0.f;
+        for (int j = 0; j < E / V; j++) {
+            const uint32_t i = (j * L + lane) * V;
+            if (i < d) v[j] = *(const vec*)(p + i);
+        }
     }
-}
+    // with zeros past the row's end
+    __device__ void to(float (&f)[E], uint32_t lane, uint32_t d) const {
+#pragma unroll
+        for (int e = 0; e < E; e++) f[e] = (e / V * L + lane) * V < d ? to_f32((T)v[e / V][e % V]) : 0.f;
+    }
+};
 template <int L, int V, int E, class T>
 __device__ inline void store_row(T* p, uint32_t lane, uint32_t d, const float (&f)[E]) {
 #pragma unroll
     for (int j = 0; j < E / V; j++) {
         const uint32_t i = (j * L + lane) * V;
         if (i < d) store<V>(p + i, f + j * V);
+    }
+}
+// the lane's weights, zeros past the row's end
+template <class T, int L, int V, int E>
+__device__ inline void weights(const void* w, bool wide, uint32_t lane, uint32_t d, float none, float (&f)[E]) {
+#pragma unroll
+    for (int j = 0; j < E / V; j++) {
+        const uint32_t i = (j * L + lane) * V;
+#pragma unroll
+        for (int c = 0; c < V; c++) f[j * V + c] = i + c < d ? none : 0.f;
+        if (!w || i >= d) continue;
+        if (!wide) load<V>((const T*)w + i, f + j * V);
+        else
+#pragma unroll
+            for (int c = 0; c < V; c += 4) load<V < 4 ? V : 4>((const float*)w + i + c, f + j * V + c);
     }
 }
 
@@ -59,16 +75,17 @@ __global__ __launch_bounds__(threads(L, 256)) void k_forward(Args a) {
     constexpr int kSlots = threads(L, 256) / L;
     __shared__ Sums<L, 1> s;
     const uint32_t lane = threadIdx.x % L;
+    const uint32_t step = gridDim.x * kSlots;
+    uint32_t row = blockIdx.x * kSlots + threadIdx.x / L;
+    Raw<T, L, V, E> next;
+    if (row < a.rows) next.read((const T*)a.x + row * a.xs, lane, a.d);
     float w[E], b[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const uint32_t i = (e / V * L + lane) * V + e % V;
-        w[e] = i < a.d ? weight<T>(a.w, a.wide, i, 1.f) : 0.f;
-        b[e] = i < a.d ? weight<T>(a.b, a.wide, i, 0.f) : 0.f;
-    }
-    for (uint32_t row = blockIdx.x * kSlots + threadIdx.x / L; row < a.rows; row += gridDim.x * kSlots) {
+    weights<T, L, V>(a.w, a.wide, lane, a.d, 1.f, w);
+    weights<T, L, V>(a.b, a.wide, lane, a.d, 0.f, b);
+    for (; row < a.rows; row += step) {
         float f[E];
-        load_row<L, V>((const T*)a.x + row * a.xs, lane, a.d, f);
+        next.to(f, lane, a.d);
+        if (row + step < a.rows) next.read((const T*)a.x + (row + step) * a.xs, lane, a.d);
         float sum[1] = {0.f};
 #pragma unroll
         for (int e = 0; e < E; e++) sum[0] += f[e];
@@ -98,18 +115,26 @@ __global__ __launch_bounds__(threads(L, 512)) void k_backward(Args a) {
     constexpr int kSlots = threads(L, 512) / L;
     __shared__ Sums<L, 2> s;
     const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L;
-    float w[E], dw[E], db[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const uint32_t i = (e / V * L + lane) * V + e % V;
-        w[e] = i < a.d ? weight<T>(a.w, a.wide, i, 1.f) : 0.f;
-        dw[e] = db[e] = 0.f;
+    const uint32_t step = gridDim.x * kSlots;
+    uint32_t row = blockIdx.x * kSlots + slot;
+    Raw<T, L, V, E> next, next_dy;
+    if (row < a.rows) {
+        next.read((const T*)a.x + row * a.xs, lane, a.d);
+        next_dy.read((const T*)a.dy + row * a.dys, lane, a.d);
     }
+    float w[E], dw[E], db[E];
+    weights<T, L, V>(a.w, a.wide, lane, a.d, 1.f, w);
+#pragma unroll
+    for (int e = 0; e < E; e++) dw[e] = db[e] = 0.f;
     int turn = 0;
-    for (uint32_t row = blockIdx.x * kSlots + slot; row < a.rows; row += gridDim.x * kSlots) {
+    for (; row < a.rows; row += step) {
         float h[E], t[E];
-        load_row<L, V>((const T*)a.x + row * a.xs, lane, a.d, h);
-        load_row<L, V>((const T*)a.dy + row * a.dys, lane, a.d, t);
+        next.to(h, lane, a.d);
+        next_dy.to(t, lane, a.d);
+        if (row + step < a.rows) {
+            next.read((const T*)a.x + (row + step) * a.xs, lane, a.d);
+            next_dy.read((const T*)a.dy + (row + step) * a.dys, lane, a.d);
+        }
         const float mean = a.mean[row], rstd = a.rstd[row];
         float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -202,6 +227,7 @@ int choose(bool vectors, uint32_t d, F&& f) {
     CLEAR_FITS(16, 4, 1);
     CLEAR_FITS(64, 4, 1);
     CLEAR_FITS(64, 16, 1);
+    CLEAR_FITS(256, 8, 1);
     CLEAR_FITS(256, 16, 1);
     CLEAR_FITS(1024, 16, 1);
 #undef CLEAR_FITS
@@ -273,7 +299,7 @@ int fhe_ssm_layer_norm_forward(const fhe_ssm_layer_norm* a, const void* x, const
     const auto run = [&](auto t) {
         typedef decltype(t) T;
         const size_t size = sizeof(T);
-        const bool vectors = k.d * size % 16 == 0 && on_vectors(x, k.rows > 1 ? k.xs : 0, size) && on_vectors(out, k.rows > 1 ? k.ys : 0, size);
+        const bool vectors = k.d * size % 16 == 0 && aligned(weight, 16) && aligned(bias, 16) && on_vectors(x, k.rows > 1 ? k.xs : 0, size) && on_vectors(out, k.rows > 1 ? k.ys : 0, size);
         return choose<T>(vectors, k.d, [&](auto l, auto e, auto v) {
             constexpr int L = decltype(l)::value, E = decltype(e)::value, V = decltype(v)::value;
             constexpr int kThreads = threads(L, 256), kSlots = kThreads / L;
@@ -303,7 +329,7 @@ int fhe_ssm_layer_norm_backward(const fhe_ssm_layer_norm* a, const void* dy, con
         typedef decltype(t) T;
         const size_t size = sizeof(T);
         const auto on = [&](const void* p, int64_t stride) { return on_vectors(p, k.rows > 1 ? stride : 0, size); };
-        const bool vectors = k.d * size % 16 == 0 && on(x, k.xs) && on(dy, k.dys) && on(dx, k.ys);
+        const bool vectors = k.d * size % 16 == 0 && aligned(weight, 16) && on(x, k.xs) && on(dy, k.dys) && on(dx, k.ys);
         const uint32_t blocks = parts_of<T>(vectors, k.rows, k.d);
         k.parts = blocks > 1 ? (float*)workspace : nullptr;
         if (blocks)

@@ -562,7 +562,7 @@ def _embedding_gradient_sizes(tokens, dtable, scale=1.0):
 
 
 def embedding_gradient_workspace(tokens, dtable) -> int:
-    """device bytes that embedding_gradient needs"""
+    """device bytes that embedding_gradient needs (0 for few tokens)"""
     n = _size()
     a = _embedding_gradient_sizes(tokens, dtable)
     check(load().fhe_ssm_embedding_workspace(ctypes.addressof(a), ctypes.byref(n)))
@@ -572,7 +572,7 @@ def embedding_gradient_workspace(tokens, dtable) -> int:
 def embedding_gradient(tokens, dout, dtable, scale: float = 1.0, accumulate: bool = False, workspace=None, stream=None) -> None:
     """dtable[v] = scale times the sum of dout[t] over the t with tokens[t] = v, in their order; with `accumulate` added to what
     is there.  dout [n, channels]; dtable contiguous [vocab, channels], float32 or of dout's type; workspace: a uint8 tensor of
-    embedding_gradient_workspace(tokens, dtable) bytes."""
+    embedding_gradient_workspace(tokens, dtable) bytes, None where that is 0."""
     _on_device(tokens, dout, dtable, workspace)
     a = _embedding_gradient_sizes(tokens, dtable, scale)
     a.row_type, a.row_stride = _type(dout), _matrix(dout, "dout")

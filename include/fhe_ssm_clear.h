@@ -199,7 +199,7 @@ typedef struct {
 
 int fhe_ssm_embedding_lookup(const fhe_ssm_embedding* a, const int64_t* tokens, const void* table, void* out, void* stream);
 
-/* Device memory that the gradient needs. */
+/* Device memory that the gradient needs (0 for few tokens: workspace may be null). */
 int fhe_ssm_embedding_workspace(const fhe_ssm_embedding* a, size_t* bytes);
 
 /* All of dtable (float32, or row_type) is written, or with `accumulate` the sums are added to what is there.  Sums are taken in
