@@ -4,14 +4,17 @@
 //   entropy = log S - sum_j p_j (l_j - m);    d(w logprob + u entropy) / d l_j = w ([j = tok] - p_j) - u p_j (log p_j + entropy)
 //
 // Differences from the largest, nowhere of large numbers.  A workgroup takes a row and reads it once: a thread holds a
-// reference that is at most kSlack below its largest logit so far, sum e and sum d e with d = l - reference, e = exp d; when
-// a vector passes the reference by more, the sums follow it.  The threads' join in a fixed order.
+// reference that is at most kSlack below its largest logit so far, sum e and sum d e with d = (l - reference) log2(e), e = 2^d;
+// when a vector passes the reference by more, the sums follow it.  Of d only the reference's part is rounded besides d itself,
+// which all its summands share.  The threads' sums join in a fixed order.
 //
-// The alternatives: 256 strips of the row (a thread's vectors, or four neighbours') each know their largest logit and the vector
-// where it came first.  The k-th of these in the order of falling logits, then rising index, bounds the k largest from below,
-// and they all lie in the k strips that are not behind it: only those are read again, what is not below the bound goes to a
-// list, and the list is ranked entry against entry.  Where the list would overflow (strips whose logits lie high together) the
-// row is passed over k times for the next largest instead.
+// The alternatives: each of 256 threads knows the largest logit of its vectors and the vector where it came first.  The k-th of
+// these in the order of falling logits, then rising index, bounds the k largest from below, and they all lie in the vectors of
+// the k threads that are not behind it: only those are read again, what is not below the bound goes to a list, and the list is
+// ranked entry against entry.  Where the list would overflow (large logits that lie together) the row is passed over k times
+// for the next largest instead.
+//
+// Few rows are cut into parts, a workgroup each; a second kernel joins the parts' sums and ranks their alternatives.
 //
 // Where the weights of the gradient are known the row is read again at once, from the caches, and the gradient written.
 // Bound by bytes for many rows; of one row by the vector instructions of its one CU, about 11 a logit.
@@ -22,9 +25,10 @@
 namespace clear {
 namespace {
 
-constexpr uint32_t kMostTop = 32, kStrips = 256, kList = 1024;
+constexpr uint32_t kMostTop = 32, kMostParts = 16, kList = 1024, kWide = 8192;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
-constexpr float kLowest = -3.40282347e38f, kSlack = 5.5f;
+constexpr float kSlack = 8.f;    // powers of two
+constexpr float kHuge = 0x1p100f;  // two different floats of this size or more weigh 1 and 0 beside each other
 constexpr int kFlight = 4;  // vectors of a thread on their way
 
 struct Args {
@@ -37,6 +41,11 @@ struct Args {
     void* grad;
     uint32_t rows, vocab, k;
     int64_t stride, grad_stride;
+    // rows in parts of `each` logits
+    uint32_t parts, each;
+    float* sums;     // [row][part][4]: the part's largest, sum 2^-d, sum d 2^-d
+    uint64_t* best;  // [row][part][k]: its largest entries
+    float* result;   // [row][4]: the row's largest, log2 S and entropy
 };
 
 // 0 for NaN and -inf; otherwise rising with the logit; 0 and -0 are one
@@ -68,36 +77,41 @@ struct Row {
 #pragma unroll
             for (int c = 0; c < V; c++) f[c] = at + c >= skip && at + c < end ? to_f32(x[at + c]) : -INFINITY;
     }
+    // the thread's vectors first .. first + n - 1; one question for all threads where all are inside the row
+    template <int n>
+    __device__ void read(int first, float (&f)[n][V]) const {
+        const int at = first * kThreads * V;
+        if (at >= skip && at + n * kThreads * V <= end)
+#pragma unroll
+            for (int i = 0; i < n; i++) load<V>(x + at + (i * kThreads + (int)threadIdx.x) * V, f[i]);
+        else
+#pragma unroll
+            for (int i = 0; i < n; i++) read((first + i) * kThreads + (int)threadIdx.x, f[i]);
+    }
 };
 
-// what is known of a part of a row: its largest, and with e = exp(l - m): sum e, sum (m - l) e
+// what is known of a part of a row: its largest, and with d = (m - l) log2(e): sum 2^-d, sum d 2^-d
 struct Part {
     float m, s, t;
 };
-__device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 __device__ inline Part joined(Part a, Part b) {
     const float m = a.m > b.m ? a.m : b.m;
-    const float da = a.m == m ? 0.f : m - a.m, db = b.m == m ? 0.f : m - b.m;  // none where both are -inf
-    const float ea = exp_of(-da), sa = a.s * ea, eb = exp_of(-db), sb = b.s * eb;
+    const float da = a.m == m ? 0.f : (m - a.m) * kLog2e, db = b.m == m ? 0.f : (m - b.m) * kLog2e;  // 0 where both are -inf
+    const float ea = __builtin_amdgcn_exp2f(-da), sa = a.s * ea, eb = __builtin_amdgcn_exp2f(-db), sb = b.s * eb;
     return {m, sa + sb, (a.t * ea + (sa > 0.f ? da * sa : 0.f)) + (b.t * eb + (sb > 0.f ? db * sb : 0.f))};
 }
 
 template <int kThreads>
 struct Shared {
     Part part[kThreads / 64];
-    uint64_t best[kStrips], list[kList];
-    uint32_t chosen[kMostTop];
-    uint64_t bound;
-    uint32_t listed, strips;
-    uint64_t wave[kThreads / 64];
+};
+struct Alternatives {
+    uint64_t best[256], list[kList + 16], bound, wave[4];
+    uint32_t chosen[kMostTop], listed, chosen_count;
 };
 
-template <int kControl>
-__device__ inline uint64_t swapped64(uint64_t x) {
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, kControl, 0xf, 0xf, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), kControl, 0xf, 0xf, false);
-    return (uint64_t)hi << 32 | lo;
-}
+__device__ inline float log2_p(float x, float m, float log2s) { return __builtin_fmaf(x - m, kLog2e, -log2s); }
+__device__ inline float log_p(float x, float m, float log2s) { return (x - m) - kLn2 * log2s; }
 
 // An entry's place in the order: its logit's key, then the flipped index; 0 for what is no alternative.
 __device__ inline uint64_t entry(float x, uint32_t index) {
@@ -105,19 +119,25 @@ __device__ inline uint64_t entry(float x, uint32_t index) {
     return k ? (uint64_t)k << 32 | (uint32_t)~index : 0;
 }
 
-// The k largest entries below `under` are found one by one where the list does not hold them.
-template <class T, int kThreads>
-__device__ void one_by_one(const Row<T, kThreads>& row, uint32_t k, Shared<kThreads>& s) {
+// Sets the 16 entries behind the list's end to 0, before the barrier that ends its making.
+__device__ inline void close_list(Alternatives& s, uint32_t n) {
+    if (threadIdx.x < 16) s.list[n + threadIdx.x] = 0;
+}
+
+// The k largest entries one by one, to the list.
+template <class T>
+__device__ void one_by_one(const Row<T, 256>& row, uint32_t from, uint32_t k, Alternatives& s) {
+    constexpr int V = Row<T, 256>::V;
     uint64_t under = ~0ull;
     for (uint32_t i = 0; i < k; i++) {
         uint64_t best = 0;
         for (int j = 0; j < row.vectors; j++) {
-            float f[Row<T, kThreads>::V];
-            const int v = j * kThreads + threadIdx.x;
+            float f[V];
+            const int v = j * 256 + threadIdx.x;
             row.read(v, f);
 #pragma unroll
-            for (int c = 0; c < Row<T, kThreads>::V; c++) {
-                const uint64_t e = entry(f[c], v * Row<T, kThreads>::V + c - row.skip);
+            for (int c = 0; c < V; c++) {
+                const uint64_t e = entry(f[c], from + v * V + c - row.skip);
                 if (e < under && e > best) best = e;
             }
         }
@@ -127,123 +147,138 @@ __device__ void one_by_one(const Row<T, kThreads>& row, uint32_t k, Shared<kThre
         }
         if (threadIdx.x % 64 == 0) s.wave[threadIdx.x / 64] = best;
         __syncthreads();
-        for (int w = 0; w < kThreads / 64; w++) best = s.wave[w] > best ? s.wave[w] : best;
+        for (int w = 0; w < 4; w++) best = s.wave[w] > best ? s.wave[w] : best;
         __syncthreads();
         if (threadIdx.x == 0) s.list[i] = best;
         under = best;
     }
     if (threadIdx.x == 0) s.listed = k;
+    close_list(s, k);
     __syncthreads();
 }
 
-// The row's k largest to a.top, from each thread's largest `m` and the vector `first` where it came first.
-template <class T, int kThreads>
-__device__ void alternatives(const Args& a, const Row<T, kThreads>& row, uint32_t r, float mine, int first, float m, float logs,
-                             Shared<kThreads>& s) {
-    constexpr int V = Row<T, kThreads>::V, kEach = kThreads / kStrips;  // threads of a strip
-    // ordered by a vector's first index; the bound takes its last, as the logit itself may lie anywhere in it
-    uint64_t best = entry(mine, (uint32_t)(first * kThreads + (int)threadIdx.x) * V);
-    if constexpr (kEach == 4) {
-        uint64_t other = swapped64<0xb1>(best);
-        best = other > best ? other : best;
-        other = swapped64<0x4e>(best);
-        best = other > best ? other : best;
+// put(i, entry) for the i-th largest of the list's entries, i < k, and put(i, 0) for what is missing
+template <class F>
+__device__ void ranked(uint32_t k, const Alternatives& s, F&& put) {
+    const uint32_t n = s.listed;
+    uint32_t have = n;
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        const uint64_t x = s.list[i];
+        uint32_t before = 0;
+        for (uint32_t j = 0; j < n; j += 16) {  // behind the list's end lie 16 zeros
+            uint64_t y[16];
+#pragma unroll
+            for (int q = 0; q < 16; q++) y[q] = s.list[j + q];
+#pragma unroll
+            for (int q = 0; q < 16; q++) before += y[q] > x;
+        }
+        if (x && before < k) put(before, x);
     }
-    const uint32_t strip = threadIdx.x / kEach;
-    if (threadIdx.x % kEach == 0) s.best[strip] = best;
-    if (threadIdx.x == 0) s.listed = s.strips = 0, s.bound = 0;
+    if (n <= k || s.list[n - 1] == 0) {  // fewer logits than k may be numbers above -inf
+        have = 0;
+        for (uint32_t j = 0; j < n; j++) have += s.list[j] != 0;
+    }
+    for (uint32_t i = have + threadIdx.x; i < k; i += 256) put(i, 0);
+}
+
+// A row's (or its part's, which begins at `from`) k largest to the list, and more; from each thread's largest and the vector
+// `first` where it came first.
+template <class T>
+__device__ void find_alternatives(const Row<T, 256>& row, uint32_t from, uint32_t k, float largest, int first, Alternatives& s) {
+    constexpr int V = Row<T, 256>::V;
+    // ordered by a vector's first place; the bound takes its last, as the logit itself may lie anywhere in it
+    const uint64_t mine = entry(largest, (uint32_t)(first * 256 + (int)threadIdx.x) * V);
+    s.best[threadIdx.x] = mine;
+    if (threadIdx.x == 0) s.listed = s.chosen_count = 0, s.bound = 0;
     __syncthreads();
     uint32_t rank = 0;
-    {
-        constexpr int kPart = kStrips / kEach;  // each of a strip's threads compares it with a part of the others
-        const uint32_t from = threadIdx.x % kEach * kPart;
-#pragma unroll 8
-        for (int i = 0; i < kPart; i++) rank += s.best[from + i] > best;
-        if constexpr (kEach == 4) {
-            rank += __builtin_amdgcn_update_dpp(0, (int)rank, 0xb1, 0xf, 0xf, false);
-            rank += __builtin_amdgcn_update_dpp(0, (int)rank, 0x4e, 0xf, 0xf, false);
-        }
-    }
-    if (best && rank < a.k && threadIdx.x % kEach == 0) {
-        s.chosen[atomicAdd(&s.strips, 1u)] = strip;  // their order says nothing
-        if (rank == a.k - 1) s.bound = best - (V - 1);
+#pragma unroll 16
+    for (int i = 0; i < 256; i++) rank += s.best[i] > mine;
+    if (mine && rank < k) {
+        s.chosen[atomicAdd(&s.chosen_count, 1u)] = threadIdx.x;  // their order says nothing
+        if (rank == k - 1) s.bound = mine - (V - 1);
     }
     __syncthreads();
     const uint64_t bound = s.bound;
-    const uint32_t per = (uint32_t)row.vectors * kEach, items = s.strips * per;
-    for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
-        const uint32_t q = i / per, j = i - q * per;
-        const int v = (int)(j / kEach) * kThreads + (int)(s.chosen[q] * kEach + j % kEach);
+    const uint32_t per = (uint32_t)row.vectors, items = s.chosen_count * per;
+    for (uint32_t i = threadIdx.x; i < items; i += 256) {
+        const uint32_t q = i / per;
+        const int v = (int)((i - q * per) * 256 + s.chosen[q]);
         float f[V];
         row.read(v, f);
 #pragma unroll
         for (int c = 0; c < V; c++) {
-            const int at = v * V + c;  // bounds and entries by places that count from the vectors' beginning
-            const uint64_t e = entry(f[c], at);
+            const uint64_t e = entry(f[c], v * V + c);
             if (e && e >= bound) {
                 const uint32_t to = atomicAdd(&s.listed, 1u);
-                if (to < kList) s.list[to] = e + row.skip;  // the flipped index of at - skip
+                if (to < kList) s.list[to] = e + row.skip - from;  // the flipped index of the row's place
             }
         }
     }
     __syncthreads();
-    if (s.listed > kList) one_by_one(row, a.k, s);
-    const uint32_t n = s.listed;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        const uint64_t x = s.list[i];
-        uint32_t before = 0;
-        for (uint32_t j = 0; j < n; j++) before += s.list[j] > x;
-        if (before < a.k && x) {
-            a.top[(size_t)r * a.k + before] = (uint32_t)~(uint32_t)x;
-            a.top_logprobs[(size_t)r * a.k + before] = (of_key((uint32_t)(x >> 32)) - m) - logs;
-        }
-    }
-    // fewer than k logits are numbers above -inf
-    __syncthreads();
-    uint32_t have = n;
-    if (n && n <= a.k) {
-        have = 0;
-        for (uint32_t j = 0; j < n; j++) have += s.list[j] != 0;
-    }
-    for (uint32_t i = have + threadIdx.x; i < a.k; i += kThreads) {
-        a.top[(size_t)r * a.k + i] = -1;
-        a.top_logprobs[(size_t)r * a.k + i] = -INFINITY;
-    }
+    if (s.listed > kList) return one_by_one(row, from, k, s);
+    close_list(s, s.listed);
     __syncthreads();
 }
 
+// the token and log-probability of the i-th alternative
+__device__ inline void put_alternative(const Args& a, uint32_t r, uint32_t i, uint64_t e, float m, float log2s) {
+    a.top[(size_t)r * a.k + i] = e ? (int64_t)(uint32_t)~(uint32_t)e : -1;
+    a.top_logprobs[(size_t)r * a.k + i] = e ? log_p(of_key((uint32_t)(e >> 32)), m, log2s) : -INFINITY;
+}
+
+// With q = log2 p the gradient is p (-u ln 2 q - (w + u entropy)), and w more at the token.
+// The gradient of group `from` of kFlight vectors a thread, of every `step`-th after it.
 template <class T, int kThreads>
-__device__ void write_gradient(const Args& a, uint32_t r, int64_t token, float m, float logs, float entropy) {
+__device__ void write_gradient(const Args& a, uint32_t r, int64_t token, float m, float log2s, float entropy, int from_group = 0,
+                               int step = 1) {
     const T* from = (const T*)a.logits + r * a.stride;
     T* to = (T*)a.grad + r * a.grad_stride;
     const Row<T, kThreads> row(from, a.vocab);
     constexpr int V = Row<T, kThreads>::V;
     const float w = token >= 0 && a.weights ? a.weights[r] : 0.f, u = a.entropy_weights ? a.entropy_weights[r] : 0.f;
-    const bool nothing = (w == 0.f && u == 0.f) || (m == -INFINITY && logs == 0.f);  // whatever the logits are
+    const bool nothing = (w == 0.f && u == 0.f) || (m == -INFINITY && log2s == 0.f);  // whatever the logits are
     const bool same = ((uintptr_t)from ^ (uintptr_t)to) % 16 == 0;
     const int at_token = nothing || token < 0 ? -1 : (int)token + row.skip;
+    const float slope = -kLn2 * u, level = -(w + u * entropy);
     to -= row.skip;
-    for (int j = 0; j < row.vectors; j++) {
-        const int v = j * kThreads + threadIdx.x, at = v * V;
-        float f[V];
-        if (at >= row.end) break;
+    for (int j = from_group * kFlight; j < row.vectors; j += step * kFlight) {
+        float f[kFlight][V];
         if (nothing) {
 #pragma unroll
-            for (int c = 0; c < V; c++) f[c] = 0.f;
-        } else {
-            row.read(v, f);
+            for (int i = 0; i < kFlight; i++)
 #pragma unroll
-            for (int c = 0; c < V; c++) {
-                const float log = (f[c] - m) - logs, p = exp_of(log);
-                f[c] = p == 0.f ? 0.f : -p * (w + u * (log + entropy));  // a log of -inf times 0 is 0; a NaN stays
-                if (at + c == at_token) f[c] += w;
+                for (int c = 0; c < V; c++) f[i][c] = 0.f;
+        } else {
+            row.read(j, f);
+#pragma unroll
+            for (int i = 0; i < kFlight; i++) {
+#pragma unroll
+                for (int c = 0; c < V; c++) {
+                    const float q = log2_p(f[i][c], m, log2s), p = __builtin_amdgcn_exp2f(q);
+                    f[i][c] = p * __builtin_fmaf(__builtin_fmaxf(q, -1e30f), slope, level);  // p of 0 times a q of -inf is 0
+                }
+                const int at = ((j + i) * kThreads + (int)threadIdx.x) * V;
+                if (at_token >= at && at_token < at + V)
+#pragma unroll
+                    for (int c = 0; c < V; c++) f[i][c] = at + c == at_token ? f[i][c] + w : f[i][c];
             }
         }
-        if (same && at >= row.skip && at + V <= row.end) store<V>(to + at, f);
-        else
+        const int begin = j * kThreads * V;
+        if (same && begin >= row.skip && begin + kFlight * kThreads * V <= row.end) {
 #pragma unroll
-            for (int c = 0; c < V; c++)
-                if (at + c >= row.skip && at + c < row.end) to[at + c] = from_f32<T>(f[c]);
+            for (int i = 0; i < kFlight; i++) store<V>(to + begin + (i * kThreads + (int)threadIdx.x) * V, f[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kFlight; i++) {
+                const int at = begin + (i * kThreads + (int)threadIdx.x) * V;
+                if (same && at >= row.skip && at + V <= row.end) store<V>(to + at, f[i]);
+                else
+#pragma unroll
+                    for (int c = 0; c < V; c++)
+                        if (at + c >= row.skip && at + c < row.end) to[at + c] = from_f32<T>(f[i][c]);
+            }
+        }
     }
 }
 
@@ -253,43 +288,76 @@ __device__ inline int64_t token_of(const Args& a, uint32_t r) {
     return token < (int64_t)a.vocab ? token : -1;
 }
 
-// kTop: alternatives are asked for; kGrad: the gradient too
-template <class T, int kThreads, bool kTop, bool kGrad>
+// a row's numbers from all its logits' sums
+struct Numbers {
+    float m, log2s, entropy;
+    bool none;  // nothing above -inf
+    __device__ Numbers(Part p) : m(p.m), none(p.m == -INFINITY && p.s == 0.f) {
+        log2s = none ? 0.f : __builtin_amdgcn_logf(p.s);
+        entropy = none ? 0.f : kLn2 * (log2s + p.t / p.s);
+    }
+};
+__device__ inline void put_numbers(const Args& a, uint32_t r, int64_t token, float logit, const Numbers& n) {
+    if (a.logprobs) a.logprobs[r] = token < 0 ? 0.f : n.none ? -INFINITY : log_p(logit, n.m, n.log2s);
+    if (a.entropy) a.entropy[r] = n.entropy;
+    if (a.stats) {
+        a.stats[2 * (size_t)r] = n.m;
+        a.stats[2 * (size_t)r + 1] = n.log2s * kLn2;
+    }
+}
+
+// kTop: alternatives are asked for; kGrad: the gradient too, at once; kPart: a row's part, for k_join
+template <class T, int kThreads, bool kTop, bool kGrad, bool kPart>
 __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
+    static_assert(!kTop || kThreads == 256);
     __shared__ Shared<kThreads> s;
     constexpr int V = 16 / sizeof(T);
-    const uint32_t r = blockIdx.x;
+    const uint32_t r = kPart ? blockIdx.x / a.parts : blockIdx.x, from = kPart ? blockIdx.x % a.parts * a.each : 0;
     const T* logits = (const T*)a.logits + r * a.stride;
-    const Row<T, kThreads> row(logits, a.vocab);
-    float reference = kLowest, largest = -INFINITY, sum = 0.f, along = 0.f;
+    const Row<T, kThreads> row(logits + from, kPart ? min(a.each, a.vocab - from) : a.vocab);
+    const int64_t token = kPart ? -1 : token_of(a, r);
+    const float given = token < 0 ? 0.f : to_f32(logits[token]);  // asked for before it is needed
+    float reference = -INFINITY, largest = -INFINITY, sum = 0.f, along = 0.f;  // the reference times log2(e)
     int first = 0;
     for (int j = 0; j < row.vectors; j += kFlight) {
         float f[kFlight][V];
-#pragma unroll
-        for (int i = 0; i < kFlight; i++) row.read((j + i) * kThreads + threadIdx.x, f[i]);
+        row.read(j, f);
 #pragma unroll
         for (int i = 0; i < kFlight; i++) {
             float m = f[i][0];
 #pragma unroll
             for (int c = 1; c < V; c++) m = __builtin_fmaxf(m, f[i][c]);
-            if (m > largest) largest = m, first = j + i;
-            if (m - reference > kSlack) {
-                const float d = __builtin_fminf(m - reference, 1e6f), e = exp_of(-d);
+            if (!(__builtin_fabsf(m) < kHuge)) {  // masked, or out of all proportion: only what equals the largest counts
+                bool bad = false;
+#pragma unroll
+                for (int c = 0; c < V; c++) bad |= f[i][c] != f[i][c] || f[i][c] == INFINITY;
+                if (m > largest) largest = m, first = j + i, reference = m * kLog2e, sum = along = 0.f;
+                if (m == largest && m > -INFINITY)
+#pragma unroll
+                    for (int c = 0; c < V; c++) sum += f[i][c] == m ? 1.f : 0.f;
+                if (bad) sum = __builtin_nanf("");
+                continue;
+            }
+            if (kTop) first = m > largest ? j + i : first;
+            largest = __builtin_fmaxf(largest, m);
+            const float above = __builtin_fmaf(m, kLog2e, -reference);
+            if (above > kSlack) {
+                const float d = __builtin_fminf(above, 1e6f), e = __builtin_amdgcn_exp2f(-d);
                 along = (along - d * sum) * e;
                 sum *= e;
-                reference = m;
+                reference = m * kLog2e;
             }
 #pragma unroll
             for (int c = 0; c < V; c++) {
-                const float d = f[i][c] - reference, e = exp_of(d);
+                const float d = __builtin_fmaf(f[i][c], kLog2e, -reference), e = __builtin_amdgcn_exp2f(d);
                 sum += e;
-                along += e * __builtin_fmaxf(d, kLowest);  // -inf weighs nothing
+                along += e * __builtin_fmaxf(d, -1e30f);  // -inf weighs nothing
             }
         }
     }
     Part p{largest, sum, -along};
-    if (largest > -INFINITY) {
-        const float d = largest - reference, e = exp_of(-d);
+    if (__builtin_fabsf(largest) < kHuge) {
+        const float d = __builtin_fmaf(largest, kLog2e, -reference), e = __builtin_amdgcn_exp2f(-d);
         p.t = (d * sum - along) * e;
         p.s = sum * e;
     }
@@ -300,32 +368,88 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
     }
     if (threadIdx.x % 64 == 0) s.part[threadIdx.x / 64] = p;
     __syncthreads();
-    p = s.part[0];
+    constexpr int kWaves = kThreads / 64;
+    p = s.part[threadIdx.x % kWaves];
 #pragma unroll
-    for (int w = 1; w < kThreads / 64; w++) p = joined(p, s.part[w]);
-    const bool none = p.m == -INFINITY && p.s == 0.f;  // nothing above -inf
-    const float logs = none ? 0.f : __builtin_amdgcn_logf(p.s) * kLn2, entropy = none ? 0.f : logs + p.t / p.s;
-    const int64_t token = token_of(a, r);
-    if (threadIdx.x == 0) {
-        if (a.logprobs) a.logprobs[r] = token < 0 ? 0.f : none ? -INFINITY : (to_f32(logits[token]) - p.m) - logs;
-        if (a.entropy) a.entropy[r] = entropy;
-        if (a.stats) {
-            a.stats[2 * (size_t)r] = p.m;
-            a.stats[2 * (size_t)r + 1] = logs;
-        }
+    for (int o = 1; o < kWaves; o *= 2) {
+        const Part q{__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o)};
+        p = threadIdx.x & o ? joined(q, p) : joined(p, q);
     }
-    if constexpr (kTop) alternatives(a, row, r, largest, first, p.m, logs, s);
-    if constexpr (kGrad) {
-        __syncthreads();  // the gradient may take the logits' place, and their readers are done
-        write_gradient<T, kThreads>(a, r, token, p.m, logs, entropy);
+    if constexpr (kPart) {
+        if (threadIdx.x == 0) {
+            float* to = a.sums + (size_t)blockIdx.x * 4;
+            to[0] = p.m, to[1] = p.s, to[2] = p.t;
+        }
+        if constexpr (kTop) {
+            __shared__ Alternatives found;
+            find_alternatives(row, from, a.k, largest, first, found);
+            ranked(a.k, found, [&](uint32_t i, uint64_t e) { a.best[(size_t)blockIdx.x * a.k + i] = e; });
+        }
+    } else {
+        const Numbers n(p);
+        if (threadIdx.x == 0) put_numbers(a, r, token, given, n);
+        if constexpr (kTop) {
+            __shared__ Alternatives found;
+            find_alternatives(row, 0, a.k, largest, first, found);
+            ranked(a.k, found, [&](uint32_t i, uint64_t e) { put_alternative(a, r, i, e, n.m, n.log2s); });
+        }
+        if constexpr (kGrad) {
+            __syncthreads();  // the gradient may take the logits' place, and their readers are done
+            write_gradient<T, kThreads>(a, r, token, n.m, n.log2s, n.entropy);
+        }
     }
 }
 
+// A row from its parts.
+template <class T>
+__global__ __launch_bounds__(256) void k_join(Args a) {
+    __shared__ Alternatives s;
+    // all that is read is asked for at once: a part's sums and last entry by a lane each
+    static_assert(kMostParts == 16 && kMostParts * kMostTop <= 512 && 512 <= kList);
+    const uint32_t r = blockIdx.x, all = a.parts * a.k, part = threadIdx.x % 16;
+    const uint64_t* best = a.best + (size_t)r * all;
+    const float* sums = a.sums + ((size_t)r * a.parts + part) * 4;
+    const int64_t token = token_of(a, r);
+    const float given = token < 0 ? 0.f : to_f32(((const T*)a.logits)[r * a.stride + token]);
+    Part p{-INFINITY, 0.f, 0.f};
+    if (part < a.parts) p = {sums[0], sums[1], sums[2]};
+    uint64_t bound = a.k && part < a.parts ? best[part * a.k + a.k - 1] : 0;
+    const uint64_t e0 = threadIdx.x < all ? best[threadIdx.x] : 0, e1 = threadIdx.x + 256 < all ? best[threadIdx.x + 256] : 0;
+    if (threadIdx.x == 0) s.listed = 0;
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) {
+        const Part q{__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o)};
+        p = threadIdx.x & o ? joined(q, p) : joined(p, q);
+        const uint64_t other = __shfl_xor((unsigned long long)bound, o);
+        bound = max(bound, other);
+    }
+    if (a.k) {  // no entry below some part's last is among the row's
+        __syncthreads();
+        if (e0 && e0 >= bound) s.list[atomicAdd(&s.listed, 1u)] = e0;
+        if (e1 && e1 >= bound) s.list[atomicAdd(&s.listed, 1u)] = e1;
+        __syncthreads();
+        close_list(s, s.listed);
+        __syncthreads();
+    }
+    const Numbers n(p);
+    if (threadIdx.x == 0) {
+        put_numbers(a, r, token, given, n);
+        if (a.grad) {
+            float* to = a.result + (size_t)r * 4;
+            to[0] = n.m, to[1] = n.log2s, to[2] = n.entropy;
+        }
+    }
+    if (a.k) ranked(a.k, s, [&](uint32_t i, uint64_t e) { put_alternative(a, r, i, e, n.m, n.log2s); });
+}
+
+// a row's gradient by itself, `parts` workgroups a row; from the joined parts or from what the caller kept
 template <class T, int kThreads>
 __global__ __launch_bounds__(kThreads) void k_gradient(Args a) {
-    const uint32_t r = blockIdx.x;
-    write_gradient<T, kThreads>(a, r, token_of(a, r), a.stats[2 * (size_t)r], a.stats[2 * (size_t)r + 1],
-                                a.entropy ? a.entropy[r] : 0.f);
+    const uint32_t r = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const float m = a.result ? a.result[4 * (size_t)r] : a.stats[2 * (size_t)r];
+    const float log2s = a.result ? a.result[4 * (size_t)r + 1] : a.stats[2 * (size_t)r + 1] * kLog2e;
+    const float entropy = a.result ? a.result[4 * (size_t)r + 2] : a.entropy ? a.entropy[r] : 0.f;
+    write_gradient<T, kThreads>(a, r, token_of(a, r), m, log2s, entropy, (int)part, (int)a.parts);
 }
 
 int check(const fhe_ssm_token_logprobs* a) {
@@ -350,8 +474,22 @@ Args args(const fhe_ssm_token_logprobs& a, const void* logits, const int64_t* to
     k.stride = a.row_stride, k.grad_stride = a.gradient_stride;
     return k;
 }
-// few rows: every thread that a CU has for a row; many: more workgroups, whose ends overlap
-bool wide(const fhe_ssm_token_logprobs& a) { return a.rows <= 256 && a.vocab > 4096; }
+// Parts of a row: where rows leave CUs without work, of 4,096 logits at least.  (32 rows of 65,536 with 20 alternatives take
+// 21 us whole.)
+void cut(Args& k) {
+    k.parts = k.rows < 256 ? std::min({(255 + k.rows) / k.rows, (k.vocab + 4095) / 4096, kMostParts}) : 1;
+    k.each = (k.vocab + k.parts - 1) / k.parts;
+    k.parts = (k.vocab + k.each - 1) / k.each;
+}
+size_t workspace_bytes_of(const Args& k) {
+    return k.parts > 1 ? (size_t)k.rows * (k.parts * (4 * sizeof(float) + k.k * sizeof(uint64_t)) + 4 * sizeof(float)) : 0;
+}
+
+template <class T, int kThreads>
+int run_gradient(const Args& k, hipStream_t st) {
+    hipLaunchKernelGGL((k_gradient<T, kThreads>), dim3(k.rows * k.parts), dim3(kThreads), 0, st, k);
+    return launched("token log-probabilities: gradient");
+}
 
 }  // namespace
 }  // namespace clear
@@ -362,7 +500,10 @@ int fhe_ssm_token_logprobs_workspace(const fhe_ssm_token_logprobs* a, size_t* by
     using namespace clear;
     if (int rc = check(a)) return rc;
     if (!bytes) return fail(CKKS_EINVAL, "token log-probabilities: null argument");
-    *bytes = 0;
+    Args k{};
+    k.rows = a->rows, k.vocab = a->vocab, k.k = a->top;
+    if (k.rows) cut(k);
+    *bytes = workspace_bytes_of(k);
     return CKKS_OK;
 }
 
@@ -371,7 +512,6 @@ int fhe_ssm_token_logprobs_forward(const fhe_ssm_token_logprobs* a, const void* 
                                    const float* weights, const float* entropy_weights, void* gradient, void* workspace,
                                    size_t workspace_bytes, void* stream) {
     using namespace clear;
-    (void)workspace, (void)workspace_bytes;
     if (int rc = check(a)) return rc;
     if (a->rows == 0) return CKKS_OK;
     if (!logits || (logprobs && !tokens) || (a->top && (!top || !top_logprobs)) || (weights && !tokens))
@@ -381,20 +521,38 @@ int fhe_ssm_token_logprobs_forward(const fhe_ssm_token_logprobs* a, const void* 
     Args k = args(*a, logits, tokens);
     k.logprobs = logprobs, k.entropy = entropy, k.stats = statistics, k.top = top, k.top_logprobs = top_logprobs;
     k.weights = weights, k.entropy_weights = entropy_weights, k.grad = gradient;
+    cut(k);
+    if (const size_t need = workspace_bytes_of(k)) {
+        if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+            return fail(CKKS_EINVAL, "token log-probabilities: the workspace must have %zu bytes and lie on 16", need);
+        k.result = (float*)workspace;
+        k.sums = k.result + 4 * (size_t)k.rows;
+        k.best = (uint64_t*)(k.sums + 4 * (size_t)k.rows * k.parts);
+    }
+    const hipStream_t st = (hipStream_t)stream;
     return by_type(a->type, [&](auto t) {
         typedef decltype(t) T;
-        const auto run = [&](auto n, auto with_top, auto with_grad) {
+        const auto run = [&](auto n, auto top, auto grad, auto part) {
             constexpr int kThreads = decltype(n)::value;
-            hipLaunchKernelGGL((k_logprobs<T, kThreads, decltype(with_top)::value, decltype(with_grad)::value>), dim3(k.rows),
-                               dim3(kThreads), 0, (hipStream_t)stream, k);
+            hipLaunchKernelGGL((k_logprobs<T, kThreads, decltype(top)::value, decltype(grad)::value, decltype(part)::value>),
+                               dim3(k.rows * k.parts), dim3(kThreads), 0, st, k);
             return launched("token log-probabilities");
         };
-        const auto of = [&](auto n) {
-            const std::true_type yes;
-            const std::false_type no;
-            return k.k ? k.grad ? run(n, yes, yes) : run(n, yes, no) : k.grad ? run(n, no, yes) : run(n, no, no);
-        };
-        return wide(*a) ? of(std::integral_constant<int, 1024>{}) : of(std::integral_constant<int, 256>{});
+        const std::true_type yes;
+        const std::false_type no;
+        const std::integral_constant<int, 256> few;
+        const std::integral_constant<int, 1024> many;
+        if (k.parts > 1) {
+            if (int rc = k.k ? run(few, yes, no, yes) : run(few, no, no, yes)) return rc;
+            hipLaunchKernelGGL(k_join<T>, dim3(k.rows), dim3(256), 0, st, k);
+            if (int rc = launched("token log-probabilities: join")) return rc;
+            return k.grad ? run_gradient<T, 256>(k, st) : (int)CKKS_OK;
+        }
+        if (k.k) return k.grad ? run(few, yes, yes, no) : run(few, yes, no, no);
+        // A long row has a whole CU's threads, so that what lies between its two readings stays in the caches: 4,096 rows of
+        // 65,536 in bf16 take 266 us with their gradient, with 256 threads a row 300.
+        if (k.vocab > kWide) return k.grad ? run(many, no, yes, no) : run(many, no, no, no);
+        return k.grad ? run(few, no, yes, no) : run(few, no, no, no);
     });
 }
 
@@ -409,12 +567,8 @@ int fhe_ssm_token_logprobs_gradient(const fhe_ssm_token_logprobs* a, const void*
     if (int rc = check_gradient(a, logits, gradient)) return rc;
     Args k = args(*a, logits, tokens);
     k.stats = (float*)statistics, k.entropy = (float*)entropy, k.weights = weights, k.entropy_weights = entropy_weights, k.grad = gradient;
-    return by_type(a->type, [&](auto t) {
-        typedef decltype(t) T;
-        if (wide(*a)) hipLaunchKernelGGL((k_gradient<T, 1024>), dim3(k.rows), dim3(1024), 0, (hipStream_t)stream, k);
-        else hipLaunchKernelGGL((k_gradient<T, 256>), dim3(k.rows), dim3(256), 0, (hipStream_t)stream, k);
-        return launched("token log-probabilities: gradient");
-    });
+    cut(k);
+    return by_type(a->type, [&](auto t) { return run_gradient<decltype(t), 256>(k, (hipStream_t)stream); });
 }
 
 }  // extern "C"
