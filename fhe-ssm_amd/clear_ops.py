@@ -372,12 +372,39 @@ def sample(logits, draws, tokens, logprobs=None, temperature=None, top_k=None, t
 
 
 # ------------------------------------------------------------------------------------------------ what the operators below share
-def _bytes_of(workspace) -> int:
-    """the size of a workspace, which is checked here too"""
+_calls: dict = {}  # an operator's name, and sizes, types, strides and devices of a call's tensors -> its checked description
+
+
+def _like(t):
+    """all that is checked of a tensor"""
+    return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
+
+
+def _kept(key, a):
+    """keeps a call's checked description: the structure, which the caller holds while it is used, and its address"""
+    _need(len({k[3] for k in key if type(k) is tuple}) <= 1, "tensors lie on different devices")
+    if len(_calls) >= 512:
+        _calls.clear()
+    a = _calls[key] = a, ctypes.addressof(a)
+    return a
+
+
+def _bytes_of(workspace, t) -> int:
+    """the size of the workspace of a call on tensor t, which is checked here too"""
     if workspace is None:
         return 0
-    _need(workspace.is_contiguous(), "workspace must be contiguous")
+    _need(workspace.is_contiguous() and workspace.get_device() == t.get_device(), "workspace must be contiguous, on the tensors' device")
     return workspace.numel() * workspace.element_size()
+
+
+def _here(stream, t):
+    """the stream of a call on tensor t, which has to lie on the current device: kernels are launched there"""
+    torch = sys.modules.get("torch")
+    if torch is not None and isinstance(t, torch.Tensor):
+        device = t.get_device()
+        if device >= 0 and device != torch._C._cuda_getDevice():
+            raise ClearError(f"tensors lie on device {device}, which is not the current one")
+    return _queue(stream, t)
 
 
 def _floats(shape, **tensors) -> None:
@@ -432,22 +459,30 @@ def layer_norm(x, weight, bias, out, mean=None, rstd=None, eps: float = 1e-5, st
     out like x, or x itself; weight and bias [channels], float32 or of x's type, None: 1 and 0; mean and rstd float32 [rows] or
     None: what layer_norm_backward takes."""
     _on_device(x, weight, bias, out, mean, rstd)
-    a = _norm_sizes(x, out, weight, bias, eps)
-    _floats((a.rows,), mean=mean, rstd=rstd)
-    check(load().fhe_ssm_layer_norm_forward(ctypes.addressof(a), x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(),
-                                            _ptr(mean), _ptr(rstd), _queue(stream, x)))
+    key = ("norm", eps, _like(x), _like(weight), _like(bias), _like(out), _like(mean), _like(rstd))
+    a = _calls.get(key)
+    if a is None:
+        sizes = _norm_sizes(x, out, weight, bias, eps)
+        _floats((sizes.rows,), mean=mean, rstd=rstd)
+        a = _kept(key, sizes)
+    check(load().fhe_ssm_layer_norm_forward(a[1], x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), _ptr(mean),
+                                            _ptr(rstd), _here(stream, x)))
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, workspace=None, stream=None) -> None:
     """The gradients of layer_norm from that of its output: dx like x (it may be dy), dweight and dbias float32 [channels] where
     they are given.  workspace: a uint8 tensor of layer_norm_workspace(x) bytes, needed for dweight and dbias."""
     _on_device(dy, x, weight, mean, rstd, dx, dweight, dbias, workspace)
-    a = _norm_sizes(x, dx, weight, None, dy=dy)
-    _floats((a.rows,), mean=mean, rstd=rstd)
-    _floats((a.channels,), dweight=dweight, dbias=dbias)
+    key = ("norm back", _like(x), _like(weight), _like(dx), _like(dy), _like(mean), _like(rstd), _like(dweight), _like(dbias))
+    a = _calls.get(key)
+    if a is None:
+        sizes = _norm_sizes(x, dx, weight, None, dy=dy)
+        _floats((sizes.rows,), mean=mean, rstd=rstd)
+        _floats((sizes.channels,), dweight=dweight, dbias=dbias)
+        a = _kept(key, sizes)
     check(load().fhe_ssm_layer_norm_backward(
-        ctypes.addressof(a), dy.data_ptr(), x.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
-        _ptr(dweight), _ptr(dbias), _ptr(workspace), _bytes_of(workspace), _queue(stream, x)))
+        a[1], dy.data_ptr(), x.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
+        _ptr(dweight), _ptr(dbias), _ptr(workspace), _bytes_of(workspace, x), _here(stream, x)))
 
 
 # ------------------------------------------------------------------------------------------------ gated recurrence
@@ -490,10 +525,11 @@ def gated_recurrence_saved(z) -> int:
 
 
 def _saved(saved, a) -> None:
-    need = _size()
-    check(load().fhe_ssm_gated_recurrence_workspace(ctypes.addressof(a), None, ctypes.byref(need)))
-    _need(saved.is_contiguous() and saved.numel() * saved.element_size() >= need.value and saved.data_ptr() % 16 == 0,
-          f"saved must have {need.value} bytes, contiguous, on 16")
+    if saved is not None:
+        need = _size()
+        check(load().fhe_ssm_gated_recurrence_workspace(ctypes.addressof(a), None, ctypes.byref(need)))
+        _need(saved.is_contiguous() and saved.numel() * saved.element_size() >= need.value,
+              f"saved must have {need.value} bytes, contiguous")
 
 
 def gated_recurrence(z, x, state_in, state_out, out, lengths=None, saved=None, workspace=None, stream=None) -> None:
@@ -504,14 +540,17 @@ def gated_recurrence(z, x, state_in, state_out, out, lengths=None, saved=None, w
     tensor of gated_recurrence_saved(z) bytes for the backward pass; workspace: one of gated_recurrence_workspace(z) bytes, None
     where that is 0."""
     _on_device(z, x, state_in, state_out, out, lengths, saved, workspace)
-    a = _recurrence_sizes(z, True, x=x, out=out)
-    _floats((a.lanes, a.channels), state_in=state_in, state_out=state_out)
-    _lengths(lengths, a.lanes)
-    if saved is not None:
-        _saved(saved, a)
+    key = ("recurrence", _like(z), _like(x), _like(state_in), _like(state_out), _like(out), _like(lengths), _like(saved))
+    a = _calls.get(key)
+    if a is None:
+        sizes = _recurrence_sizes(z, True, x=x, out=out)
+        _floats((sizes.lanes, sizes.channels), state_in=state_in, state_out=state_out)
+        _lengths(lengths, sizes.lanes)
+        _saved(saved, sizes)
+        a = _kept(key, sizes)
     check(load().fhe_ssm_gated_recurrence_prompt(
-        ctypes.addressof(a), z.data_ptr(), x.data_ptr(), _ptr(lengths), _ptr(state_in), _ptr(state_out), out.data_ptr(),
-        _ptr(saved), _ptr(workspace), _bytes_of(workspace), _queue(stream, z)))
+        a[1], z.data_ptr(), x.data_ptr(), _ptr(lengths), _ptr(state_in), _ptr(state_out), out.data_ptr(),
+        _ptr(saved), _ptr(workspace), _bytes_of(workspace, z), _here(stream, z)))
 
 
 def gated_recurrence_backward(z, x, saved, dout, dstate_out, dz, dx, dstate_in=None, lengths=None, workspace=None,
@@ -519,22 +558,32 @@ def gated_recurrence_backward(z, x, saved, dout, dstate_out, dz, dx, dstate_in=N
     """The gradients of gated_recurrence: dz and dx like z, dstate_in float32 [lanes, channels] where it is given, from those of
     out and of state_out (None: zeros).  z, x, lengths and saved are the prompt's; dstate_in may be dstate_out."""
     _on_device(z, x, saved, dout, dstate_out, dz, dx, dstate_in, lengths, workspace)
-    a = _recurrence_sizes(z, True, x=x, dout=dout, dz=dz, dx=dx)
-    _floats((a.lanes, a.channels), dstate_in=dstate_in, dstate_out=dstate_out)
-    _lengths(lengths, a.lanes)
-    _saved(saved, a)
+    key = ("recurrence back", _like(z), _like(x), _like(saved), _like(dout), _like(dstate_out), _like(dz), _like(dx),
+           _like(dstate_in), _like(lengths))
+    a = _calls.get(key)
+    if a is None:
+        sizes = _recurrence_sizes(z, True, x=x, dout=dout, dz=dz, dx=dx)
+        _floats((sizes.lanes, sizes.channels), dstate_in=dstate_in, dstate_out=dstate_out)
+        _lengths(lengths, sizes.lanes)
+        _need(saved is not None, "the backward pass needs what the prompt saved")
+        _saved(saved, sizes)
+        a = _kept(key, sizes)
     check(load().fhe_ssm_gated_recurrence_backward(
-        ctypes.addressof(a), z.data_ptr(), x.data_ptr(), _ptr(lengths), saved.data_ptr(), _ptr(dout), _ptr(dstate_out),
-        dz.data_ptr(), dx.data_ptr(), _ptr(dstate_in), _ptr(workspace), _bytes_of(workspace), _queue(stream, z)))
+        a[1], z.data_ptr(), x.data_ptr(), _ptr(lengths), saved.data_ptr(), _ptr(dout), _ptr(dstate_out),
+        dz.data_ptr(), dx.data_ptr(), _ptr(dstate_in), _ptr(workspace), _bytes_of(workspace, z), _here(stream, z)))
 
 
 def gated_recurrence_step(z, x, state_in, state_out, out, stream=None) -> None:
     """gated_recurrence for one token of every lane: the same tensors without the token axis"""
     _on_device(z, x, state_in, state_out, out)
-    a = _recurrence_sizes(z, False, x=x, out=out)
-    _floats((a.lanes, a.channels), state_in=state_in, state_out=state_out)
-    check(load().fhe_ssm_gated_recurrence_step(ctypes.addressof(a), z.data_ptr(), x.data_ptr(), _ptr(state_in),
-                                               _ptr(state_out), out.data_ptr(), _queue(stream, z)))
+    key = ("recurrence step", _like(z), _like(x), _like(state_in), _like(state_out), _like(out))
+    a = _calls.get(key)
+    if a is None:
+        sizes = _recurrence_sizes(z, False, x=x, out=out)
+        _floats((sizes.lanes, sizes.channels), state_in=state_in, state_out=state_out)
+        a = _kept(key, sizes)
+    check(load().fhe_ssm_gated_recurrence_step(a[1], z.data_ptr(), x.data_ptr(), _ptr(state_in), _ptr(state_out),
+                                               out.data_ptr(), _here(stream, z)))
 
 
 # ------------------------------------------------------------------------------------------------ embedding
@@ -542,16 +591,20 @@ def embedding(tokens, table, out, scale: float = 1.0, stream=None) -> None:
     """out[t] = scale table[tokens[t]]; zeros for a token outside the table.  tokens int64 [n], table [vocab, channels], out
     [n, channels], each of any of the three types."""
     _on_device(tokens, table, out)
-    _token_ids(tokens)
-    n = tokens.shape[0]
-    strides = _matrix(table, "table"), _matrix(out, "out")
-    vocab, channels = table.shape
-    _need(tuple(out.shape) == (n, channels), f"out must be [{n}, {channels}]")
-    a = EmbeddingSizes(_type(table), _type(out), n, vocab, channels, scale, *strides)
-    if vocab == 1:
-        a.table_stride = max(channels, strides[0])
-    check(load().fhe_ssm_embedding_lookup(ctypes.addressof(a), tokens.data_ptr(), table.data_ptr(), out.data_ptr(),
-                                          _queue(stream, table)))
+    key = ("embedding", scale, _like(tokens), _like(table), _like(out))
+    a = _calls.get(key)
+    if a is None:
+        _token_ids(tokens)
+        n = tokens.shape[0]
+        strides = _matrix(table, "table"), _matrix(out, "out")
+        vocab, channels = table.shape
+        _need(tuple(out.shape) == (n, channels), f"out must be [{n}, {channels}]")
+        a = EmbeddingSizes(_type(table), _type(out), n, vocab, channels, scale, *strides)
+        if vocab == 1:  # the stride of the one row says nothing
+            a.table_stride = channels
+        a = _kept(key, a)
+    check(load().fhe_ssm_embedding_lookup(a[1], tokens.data_ptr(), table.data_ptr(), out.data_ptr(),
+                                          _here(stream, table)))
 
 
 def _embedding_gradient_sizes(tokens, dtable, scale=1.0):
@@ -574,11 +627,15 @@ def embedding_gradient(tokens, dout, dtable, scale: float = 1.0, accumulate: boo
     is there.  dout [n, channels]; dtable contiguous [vocab, channels], float32 or of dout's type; workspace: a uint8 tensor of
     embedding_gradient_workspace(tokens, dtable) bytes, None where that is 0."""
     _on_device(tokens, dout, dtable, workspace)
-    a = _embedding_gradient_sizes(tokens, dtable, scale)
-    a.row_type, a.row_stride = _type(dout), _matrix(dout, "dout")
-    _need(tuple(dout.shape) == (a.tokens, a.channels), f"dout must be [{a.tokens}, {a.channels}]")
-    check(load().fhe_ssm_embedding_gradient(ctypes.addressof(a), tokens.data_ptr(), dout.data_ptr(), dtable.data_ptr(),
-                                            bool(accumulate), _ptr(workspace), _bytes_of(workspace), _queue(stream, dout)))
+    key = ("embedding back", scale, _like(tokens), _like(dout), _like(dtable))
+    a = _calls.get(key)
+    if a is None:
+        a = _embedding_gradient_sizes(tokens, dtable, scale)
+        a.row_type, a.row_stride = _type(dout), _matrix(dout, "dout")
+        _need(tuple(dout.shape) == (a.tokens, a.channels), f"dout must be [{a.tokens}, {a.channels}]")
+        a = _kept(key, a)
+    check(load().fhe_ssm_embedding_gradient(a[1], tokens.data_ptr(), dout.data_ptr(), dtable.data_ptr(),
+                                            bool(accumulate), _ptr(workspace), _bytes_of(workspace, dout), _here(stream, dout)))
 
 
 # ------------------------------------------------------------------------------------------------ log-probabilities
@@ -609,22 +666,27 @@ def token_logprobs(logits, tokens, logprobs, entropy=None, statistics=None, top_
     sum(weights logprobs + entropy_weights entropy) in the same call, with weights float32 [rows].  All but logits may be None.
     workspace: a uint8 tensor of token_logprobs_workspace(logits, k) bytes, None where that is 0."""
     _on_device(logits, tokens, logprobs, entropy, statistics, top_tokens, top_logprobs, workspace, weights, entropy_weights, gradient)
-    top = 0
-    if top_tokens is not None or top_logprobs is not None:
-        _need(top_tokens is not None and top_logprobs is not None, "top_tokens and top_logprobs come together")
-        _need(_is(top_tokens, "torch.int64") and len(top_tokens.shape) == 2 and top_tokens.is_contiguous()
-              and top_tokens.shape[0] == logits.shape[0], "top_tokens must be contiguous int64 [rows, k]")
-        top = top_tokens.shape[1]
-    a = _logprobs_sizes(logits, top, gradient)
-    if tokens is not None:
-        _token_ids(tokens, a.rows)
-    _floats((a.rows,), logprobs=logprobs, entropy=entropy, weights=weights, entropy_weights=entropy_weights)
-    _floats((a.rows, 2), statistics=statistics)
-    _floats((a.rows, top), top_logprobs=top_logprobs)
+    key = ("logprobs", _like(logits), _like(tokens), _like(logprobs), _like(entropy), _like(statistics), _like(top_tokens),
+           _like(top_logprobs), _like(weights), _like(entropy_weights), _like(gradient))
+    a = _calls.get(key)
+    if a is None:
+        top = 0
+        if top_tokens is not None or top_logprobs is not None:
+            _need(top_tokens is not None and top_logprobs is not None, "top_tokens and top_logprobs come together")
+            _need(_is(top_tokens, "torch.int64") and len(top_tokens.shape) == 2 and top_tokens.is_contiguous()
+                  and top_tokens.shape[0] == logits.shape[0], "top_tokens must be contiguous int64 [rows, k]")
+            top = top_tokens.shape[1]
+        a = _logprobs_sizes(logits, top, gradient)
+        if tokens is not None:
+            _token_ids(tokens, a.rows)
+        _floats((a.rows,), logprobs=logprobs, entropy=entropy, weights=weights, entropy_weights=entropy_weights)
+        _floats((a.rows, 2), statistics=statistics)
+        _floats((a.rows, top), top_logprobs=top_logprobs)
+        a = _kept(key, a)
     check(load().fhe_ssm_token_logprobs_forward(
-        ctypes.addressof(a), logits.data_ptr(), _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(statistics),
+        a[1], logits.data_ptr(), _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(statistics),
         _ptr(top_tokens), _ptr(top_logprobs), _ptr(weights), _ptr(entropy_weights), _ptr(gradient), _ptr(workspace),
-        _bytes_of(workspace), _queue(stream, logits)))
+        _bytes_of(workspace, logits), _here(stream, logits)))
 
 
 def token_logprobs_gradient(logits, tokens, statistics, weights, gradient, entropy_weights=None, entropy=None,
@@ -632,14 +694,19 @@ def token_logprobs_gradient(logits, tokens, statistics, weights, gradient, entro
     """The gradient that token_logprobs writes, where its weights were not known then: from the statistics, and the entropy if it
     has weights."""
     _on_device(logits, tokens, statistics, weights, gradient, entropy_weights, entropy)
-    a = _logprobs_sizes(logits, 0, gradient)
-    if tokens is not None:
-        _token_ids(tokens, a.rows)
-    _floats((a.rows,), weights=weights, entropy_weights=entropy_weights, entropy=entropy)
-    _floats((a.rows, 2), statistics=statistics)
+    key = ("logprobs back", _like(logits), _like(tokens), _like(statistics), _like(weights), _like(gradient),
+           _like(entropy_weights), _like(entropy))
+    a = _calls.get(key)
+    if a is None:
+        a = _logprobs_sizes(logits, 0, gradient)
+        if tokens is not None:
+            _token_ids(tokens, a.rows)
+        _floats((a.rows,), weights=weights, entropy_weights=entropy_weights, entropy=entropy)
+        _floats((a.rows, 2), statistics=statistics)
+        a = _kept(key, a)
     check(load().fhe_ssm_token_logprobs_gradient(
-        ctypes.addressof(a), logits.data_ptr(), _ptr(tokens), statistics.data_ptr(), _ptr(entropy), _ptr(weights),
-        _ptr(entropy_weights), gradient.data_ptr(), _queue(stream, logits)))
+        a[1], logits.data_ptr(), _ptr(tokens), statistics.data_ptr(), _ptr(entropy), _ptr(weights),
+        _ptr(entropy_weights), gradient.data_ptr(), _here(stream, logits)))
 
 
 # ------------------------------------------------------------------------------------------------ AdamW
@@ -671,17 +738,17 @@ class AdamW:
         kind = "torch.float32" if bits == 32 else "torch.float8_e4m3fn"
         for name, s in zip(("the first state", "the second state"), self.states):
             for p, t in zip(self.params, s):
-                _need(t.is_cuda and t.shape == p.shape and _is(t, kind) and t.is_contiguous(), f"{name} must be contiguous {kind[6:]} like its parameter")
+                _need(t.device == p.device and t.shape == p.shape and _is(t, kind) and t.is_contiguous(), f"{name} must be contiguous {kind[6:]} like its parameter")
         if bits == 8:
             for p, t in zip(self.params, self.states[2]):
-                _need(t.is_cuda and tuple(t.shape) == (-(-p.numel() // self.BLOCK), 2) and _is(t, "torch.uint8") and t.is_contiguous(),
+                _need(t.device == p.device and tuple(t.shape) == (-(-p.numel() // self.BLOCK), 2) and _is(t, "torch.uint8") and t.is_contiguous(),
                       "powers must be contiguous uint8 [blocks, 2]")
         copy_type = BF16
         if self.copies is not None:
             _need(len(self.copies) == n, "one copy for each parameter")
             copy_type = _type(self.copies[0])
             for p, t in zip(self.params, self.copies):
-                _need(t.is_cuda and t.shape == p.shape and t.dtype == self.copies[0].dtype and copy_type != F32 and t.is_contiguous(),
+                _need(t.device == p.device and t.shape == p.shape and t.dtype == self.copies[0].dtype and copy_type != F32 and t.is_contiguous(),
                       "copies must be contiguous bfloat16 or float16 like their parameters")
         self._sizes = AdamWSizes(F32, copy_type, bits, 0, 0, 0.0, eps, *betas)
         self._tensors = (AdamWTensor * n)()
@@ -707,9 +774,9 @@ class AdamW:
         by, or None.  Tensors are read when the step runs, so that a recorded one follows them.  seed goes, with the step, into
         how 8-bit states are rounded."""
         _need(len(gradients) == len(self.params), f"{len(self.params)} gradients are needed")
-        kind = gradients[0].dtype
+        kind, at = gradients[0].dtype, self.params[0].get_device()
         for g, p in zip(gradients, self.params):
-            if not (g.is_cuda and g.dtype == kind and g.shape == p.shape and g.is_contiguous()):
+            if not (g.is_cuda and g.get_device() == at and g.dtype == kind and g.shape == p.shape and g.is_contiguous()):
                 raise ClearError("gradients must be contiguous tensors of one type, like their parameters, on the GPU")
         a = self._sizes
         a.gradient_type, a.seed = _type(gradients[0]), seed & 0xffffffff
@@ -718,7 +785,7 @@ class AdamW:
         a.scale_at = None if scale is None else self._one(scale, "scale", "torch.float32")
         self._gradients[:] = [g.data_ptr() for g in gradients]
         check(load().fhe_ssm_adamw_step(ctypes.addressof(a), len(self.params), ctypes.addressof(self._tensors),
-                                        _queue(stream, self.params[0])))
+                                        _here(stream, self.params[0])))
 
     @staticmethod
     def _one(t, name: str, dtype: str):
