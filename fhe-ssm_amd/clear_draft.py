@@ -105,6 +105,29 @@ class Draft:
         """one token [lanes] for every lane: the hidden rows after it"""
         return self._run(tokens, None)
 
+    def score(self, tokens, lengths=None, top: int = 0):
+        """What the model makes of texts tokens [lanes, n], of lane b the first lengths[b]: the log-probability of every token after
+        those before it and the entropy there, [lanes, n - 1] (log-probabilities past a length are 0), with `top` the likeliest
+        tokens and their log-probabilities [lanes, n - 1, top] too.  Lanes' states are what they were."""
+        states, (lanes, n) = self.states, (len(tokens), max(1, tokens.shape[1]))
+        self.reset(lanes)
+        hidden = self._run(tokens[:, :-1], None if lengths is None else (lengths - 1).clamp(min=0))
+        self.states = states
+        rows, next_tokens = hidden.flatten(0, 1), tokens[:, 1:]
+        if lengths is not None:
+            next_tokens = torch.where(torch.arange(1, n, device=tokens.device)[None] < lengths[:, None], next_tokens, -1)
+        next_tokens = next_tokens.reshape(-1)
+        out = [torch.empty(len(rows), device="cuda") for _ in range(2)]
+        if top:
+            out += [torch.empty((len(rows), top), dtype=torch.int64, device="cuda"), torch.empty((len(rows), top), device="cuda")]
+        for i in range(0, len(rows), 8192):  # so many rows' logits are held at once
+            logits = self._product(self.head, rows[i:i + 8192])
+            need = clear_ops.token_logprobs_workspace(logits, top)
+            logprobs, entropy, *likeliest = (t[i:i + 8192] for t in out)
+            clear_ops.token_logprobs(logits, next_tokens[i:i + 8192], logprobs, entropy, None, *likeliest,
+                                     workspace=torch.empty(need, dtype=torch.uint8, device="cuda") if need else None)
+        return tuple(t.view(lanes, n - 1, *t.shape[1:]) for t in out)
+
     def generate(self, tokens, count: int, draws, lengths=None, **filters):
         """`count` tokens after each lane's prompt: [lanes, count], drawn with draws [count, lanes]"""
         self.reset(len(tokens))
