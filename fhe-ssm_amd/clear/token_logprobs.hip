@@ -8,9 +8,9 @@
 // when a vector passes the reference by more, the sums follow it.  Of d only the reference's part is rounded besides d itself,
 // which all its summands share.  The threads' sums join in a fixed order.
 //
-// The alternatives: each of 256 threads knows the largest logit of its vectors and the vector where it came first.  The k-th of
-// these in the order of falling logits, then rising index, bounds the k largest from below, and they all lie in the vectors of
-// the k threads that are not behind it: only those are read again, what is not below the bound goes to a list, and the list is
+// The alternatives: each strip of a row (the vectors of two neighbouring threads) knows its largest logit and the vector where it
+// came first.  The k-th of these in the order of falling logits, then rising index, bounds the k largest from below, and they all
+// lie in the k strips that are not behind it: only those are read again, what is not below the bound goes to a list, and the list is
 // ranked entry against entry.  Where the list would overflow (large logits that lie together) the row is passed over k times
 // for the next largest instead.
 //
@@ -26,6 +26,7 @@ namespace clear {
 namespace {
 
 constexpr uint32_t kMostTop = 32, kMostParts = 16, kList = 1024, kWide = 8192;
+constexpr uint32_t kEach = 2, kStrips = 256 / kEach;  // threads of a strip
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
 constexpr float kSlack = 8.f;    // powers of two
 constexpr float kHuge = 0x1p100f;  // two different floats of this size or more weigh 1 and 0 beside each other
@@ -105,8 +106,14 @@ template <int kThreads>
 struct Shared {
     Part part[kThreads / 64];
 };
+template <int kControl>
+__device__ inline uint64_t swapped64(uint64_t x) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), kControl, 0xf, 0xf, false) << 32 |
+           (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kControl, 0xf, 0xf, false);
+}
+
 struct Alternatives {
-    uint64_t best[256], list[kList + 16], bound, wave[4];
+    uint64_t best[kStrips], list[kList + 16], bound, wave[4];
     uint32_t chosen[kMostTop], listed, chosen_count;
 };
 
@@ -187,23 +194,29 @@ template <class T>
 __device__ void find_alternatives(const Row<T, 256>& row, uint32_t from, uint32_t k, float largest, int first, Alternatives& s) {
     constexpr int V = Row<T, 256>::V;
     // ordered by a vector's first place; the bound takes its last, as the logit itself may lie anywhere in it
-    const uint64_t mine = entry(largest, (uint32_t)(first * 256 + (int)threadIdx.x) * V);
-    s.best[threadIdx.x] = mine;
+    uint64_t mine = entry(largest, (uint32_t)(first * 256 + (int)threadIdx.x) * V);
+    if constexpr (kEach >= 2) mine = max(mine, swapped64<0xb1>(mine));
+    if constexpr (kEach == 4) mine = max(mine, swapped64<0x4e>(mine));
+    const uint32_t strip = threadIdx.x / kEach, within = threadIdx.x % kEach;
+    if (within == 0) s.best[strip] = mine;
     if (threadIdx.x == 0) s.listed = s.chosen_count = 0, s.bound = 0;
     __syncthreads();
+    // each of a strip's threads compares it with a share of the others
     uint32_t rank = 0;
-#pragma unroll 16
-    for (int i = 0; i < 256; i++) rank += s.best[i] > mine;
-    if (mine && rank < k) {
-        s.chosen[atomicAdd(&s.chosen_count, 1u)] = threadIdx.x;  // their order says nothing
+#pragma unroll
+    for (uint32_t i = 0; i < kStrips / kEach; i++) rank += s.best[i * kEach + within] > mine;
+    if constexpr (kEach >= 2) rank += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)rank, 0xb1, 0xf, 0xf, false);
+    if constexpr (kEach == 4) rank += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)rank, 0x4e, 0xf, 0xf, false);
+    if (mine && rank < k && within == 0) {
+        s.chosen[atomicAdd(&s.chosen_count, 1u)] = strip;  // their order says nothing
         if (rank == k - 1) s.bound = mine - (V - 1);
     }
     __syncthreads();
     const uint64_t bound = s.bound;
-    const uint32_t per = (uint32_t)row.vectors, items = s.chosen_count * per;
+    const uint32_t per = (uint32_t)row.vectors * kEach, items = s.chosen_count * per;
     for (uint32_t i = threadIdx.x; i < items; i += 256) {
-        const uint32_t q = i / per;
-        const int v = (int)((i - q * per) * 256 + s.chosen[q]);
+        const uint32_t q = i / per, j = i - q * per;
+        const int v = (int)(j / kEach * 256 + s.chosen[q] * kEach + j % kEach);
         float f[V];
         row.read(v, f);
 #pragma unroll
@@ -474,10 +487,10 @@ Args args(const fhe_ssm_token_logprobs& a, const void* logits, const int64_t* to
     k.stride = a.row_stride, k.grad_stride = a.gradient_stride;
     return k;
 }
-// Parts of a row: where rows leave CUs without work, of 4,096 logits at least.  (32 rows of 65,536 with 20 alternatives take
-// 21 us whole.)
+// Parts of a row: where rows leave CUs without work, of 4,096 logits at least, two workgroups a CU.  (32 float32 rows of 65,536
+// with 20 alternatives take 21 us whole and 14 in parts, 300 bf16 rows of 131,072 with 32 of them 45 and 36.)
 void cut(Args& k) {
-    k.parts = k.rows < 256 ? std::min({(255 + k.rows) / k.rows, (k.vocab + 4095) / 4096, kMostParts}) : 1;
+    k.parts = k.rows < 512 ? std::min({(511 + k.rows) / k.rows, (k.vocab + 4095) / 4096, kMostParts}) : 1;
     k.each = (k.vocab + k.parts - 1) / k.parts;
     k.parts = (k.vocab + k.each - 1) / k.each;
 }
