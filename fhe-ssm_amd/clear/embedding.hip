@@ -20,7 +20,7 @@ namespace {
 
 constexpr uint32_t kPiece = 32, kFew = 1024, kSmall = 8192;
 constexpr uint32_t kTile = 2048, kMostParts = 256, kDigits = 1024;  // sorted at a time by a workgroup; workgroups; values of a digit
-constexpr uint32_t kMostVocab = 1u << 18, kMostTokens = 1u << 26;
+constexpr uint32_t kMostVocab = 1u << 18, kMostTokens = 1u << 25;
 
 struct Args {
     const int64_t* tokens;
@@ -50,30 +50,32 @@ __device__ inline uint32_t id_of(const Args& a, uint32_t i) {
 }
 
 // ---------------------------------------------------------------- lookup
-// A vector of V a thread, kEach times, over all rows.
+// A vector of V a thread, kEach times, over all rows; where that is more than a launch has threads for, again.
 template <class F, class T, int V>
 __global__ __launch_bounds__(256) void k_lookup(Args a) {
     constexpr int kEach = 4;
     const uint32_t vectors = (a.d + V - 1) / V;
-    const uint64_t all = (uint64_t)a.n * vectors, at = (uint64_t)blockIdx.x * 256 * kEach + threadIdx.x;
-    float f[kEach][V];
-    T* to[kEach];
+    const uint64_t all = (uint64_t)a.n * vectors;
+    for (uint64_t at = (uint64_t)blockIdx.x * 256 * kEach + threadIdx.x; at < all; at += (uint64_t)gridDim.x * 256 * kEach) {
+        float f[kEach][V];
+        T* to[kEach];
 #pragma unroll
-    for (int k = 0; k < kEach; k++) {
-        const uint64_t i = min(at + k * 256, all - 1);
-        uint32_t row, c;
-        if (all <= 0xffffffffull) row = (uint32_t)i / vectors, c = ((uint32_t)i - row * vectors) * V;
-        else row = (uint32_t)(i / vectors), c = (uint32_t)(i - (uint64_t)row * vectors) * V;
-        const int64_t token = a.tokens[row];
-        const bool in = token >= 0 && token < (int64_t)a.vocab;
-        load<V>((const F*)a.from + (in ? token : 0) * a.from_stride + c, f[k]);
-        to[k] = (T*)a.to + row * a.to_stride + c;
+        for (int k = 0; k < kEach; k++) {
+            const uint64_t i = min(at + k * 256, all - 1);
+            uint32_t row, c;
+            if (all <= 0xffffffffull) row = (uint32_t)i / vectors, c = ((uint32_t)i - row * vectors) * V;
+            else row = (uint32_t)(i / vectors), c = (uint32_t)(i - (uint64_t)row * vectors) * V;
+            const int64_t token = a.tokens[row];
+            const bool in = token >= 0 && token < (int64_t)a.vocab;
+            load<V>((const F*)a.from + (in ? token : 0) * a.from_stride + c, f[k]);
+            to[k] = (T*)a.to + row * a.to_stride + c;
 #pragma unroll
-        for (int e = 0; e < V; e++) f[k][e] = in ? f[k][e] * a.scale : 0.f;
+            for (int e = 0; e < V; e++) f[k][e] = in ? f[k][e] * a.scale : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kEach; k++)
+            if (at + k * 256 < all) store<V>(to[k], f[k]);
     }
-#pragma unroll
-    for (int k = 0; k < kEach; k++)
-        if (at + k * 256 < all) store<V>(to[k], f[k]);
 }
 
 // ---------------------------------------------------------------- the sort
@@ -524,7 +526,7 @@ int fhe_ssm_embedding_lookup(const fhe_ssm_embedding* a, const int64_t* tokens, 
             const auto run = [&](auto v) {
                 constexpr int kV = decltype(v)::value;
                 const uint64_t all = (uint64_t)k.n * ((k.d + kV - 1) / kV);
-                hipLaunchKernelGGL((k_lookup<F, T, kV>), dim3((uint32_t)((all + 1023) / 1024)), dim3(256), 0, (hipStream_t)stream, k);
+                hipLaunchKernelGGL((k_lookup<F, T, kV>), dim3((uint32_t)std::min<uint64_t>((all + 1023) / 1024, 1u << 22)), dim3(256), 0, (hipStream_t)stream, k);
                 return launched("embedding");
             };
             return vectors ? run(std::integral_constant<int, V>{}) : run(std::integral_constant<int, 1>{});

@@ -375,6 +375,7 @@ int fhe_ssm_gated_recurrence_prompt(const fhe_ssm_gated_recurrence* a, const voi
     Args k{};
     lay_out(k, *a);
     if (int rc = workspace_of(k, workspace, workspace_bytes)) return rc;
+    if (!aligned(saved, 4)) return fail(CKKS_EINVAL, "gated recurrence: what is saved must lie on 4 bytes");
     k.z = z, k.x = x, k.out = out, k.lengths = lengths, k.in = state_in, k.last = state_out, k.saved = (float*)saved;
     return by_type(a->type, [&](auto t) {
         typedef decltype(t) T;
@@ -396,6 +397,7 @@ int fhe_ssm_gated_recurrence_backward(const fhe_ssm_gated_recurrence* a, const v
     Args k{};
     lay_out(k, *a);
     if (int rc = workspace_of(k, workspace, workspace_bytes)) return rc;
+    if (!aligned(saved, 4)) return fail(CKKS_EINVAL, "gated recurrence: what is saved must lie on 4 bytes");
     k.z = z, k.x = x, k.dy = dout, k.dz = dz, k.dx = dx, k.lengths = lengths, k.in = dstate_out, k.last = dstate_in, k.saved = (float*)saved;
     for (int i = 0; i < 2; i++) k.dys[i] = a->dout_stride[i], k.dzs[i] = a->dz_stride[i], k.dxs[i] = a->dx_stride[i];
     return by_type(a->type, [&](auto t) {

@@ -344,7 +344,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
                 bool bad = false;
 #pragma unroll
                 for (int c = 0; c < V; c++) bad |= f[i][c] != f[i][c] || f[i][c] == INFINITY;
-                if (m > largest) largest = m, first = j + i, reference = m * kLog2e, sum = along = 0.f;
+                if (m > largest) largest = m, first = j + i, reference = m * kLog2e, sum *= 0.f, along *= 0.f;  // a NaN stays
                 if (m == largest && m > -INFINITY)
 #pragma unroll
                     for (int c = 0; c < V; c++) sum += f[i][c] == m ? 1.f : 0.f;

@@ -90,11 +90,12 @@ class Learner:
         return self._norm(x, *self.vectors[:2], kept)
 
     def _targets(self, tokens, lengths):
-        """the next token of every position, -1 where there is none"""
+        """the next token of every position, -1 where there is none of the vocabulary"""
         n = tokens.shape[1]
         ends = n if lengths is None else lengths.clamp(0, n)[:, None]
         after = torch.cat((tokens[:, 1:], tokens[:, :1]), 1)
-        return torch.where(torch.arange(1, n + 1, device="cuda")[None] < ends, after, -1)
+        there = (torch.arange(1, n + 1, device="cuda")[None] < ends) & (after >= 0) & (after < self.vocab)
+        return torch.where(there, after, -1)
 
     # -------------------------------------------------------------------------------------------- scoring
     def score(self, tokens, lengths=None, top: int = 0):

@@ -7,7 +7,8 @@ Arguments are device tensors (torch's, or anything with data_ptr, dtype, shape a
 caller brings.  Calls go to `stream` (a hipStream_t as an int, for torch `stream.cuda_stream`; 0 is the null stream; None is
 torch's current stream, and the null stream for tensors that are not torch's) and return without waiting, so the tensors must
 stay until that stream has passed them.  Shapes, types and strides are checked here and ClearError raised; there is no
-fallback: if the library is missing, loading raises.
+fallback: if the library is missing, loading raises.  What scores and trains is asked for get_device() of its tensors too: they
+lie on one device, the current one.
 """
 from __future__ import annotations
 
@@ -524,10 +525,12 @@ def gated_recurrence_saved(z) -> int:
     return _recurrence_bytes(z)[1]
 
 
-def _saved(saved, a) -> None:
-    if saved is not None:
-        need = _size()
-        check(load().fhe_ssm_gated_recurrence_workspace(ctypes.addressof(a), None, ctypes.byref(need)))
+def _saved(saved, a, needed: bool = False) -> None:
+    need = _size()
+    check(load().fhe_ssm_gated_recurrence_workspace(ctypes.addressof(a), None, ctypes.byref(need)))
+    if saved is None:
+        _need(not needed or need.value == 0, "the backward pass needs what the prompt saved")
+    else:
         _need(saved.is_contiguous() and saved.numel() * saved.element_size() >= need.value,
               f"saved must have {need.value} bytes, contiguous")
 
@@ -565,11 +568,10 @@ def gated_recurrence_backward(z, x, saved, dout, dstate_out, dz, dx, dstate_in=N
         sizes = _recurrence_sizes(z, True, x=x, dout=dout, dz=dz, dx=dx)
         _floats((sizes.lanes, sizes.channels), dstate_in=dstate_in, dstate_out=dstate_out)
         _lengths(lengths, sizes.lanes)
-        _need(saved is not None, "the backward pass needs what the prompt saved")
-        _saved(saved, sizes)
+        _saved(saved, sizes, needed=True)
         a = _kept(key, sizes)
     check(load().fhe_ssm_gated_recurrence_backward(
-        a[1], z.data_ptr(), x.data_ptr(), _ptr(lengths), saved.data_ptr(), _ptr(dout), _ptr(dstate_out),
+        a[1], z.data_ptr(), x.data_ptr(), _ptr(lengths), _ptr(saved), _ptr(dout), _ptr(dstate_out),
         dz.data_ptr(), dx.data_ptr(), _ptr(dstate_in), _ptr(workspace), _bytes_of(workspace, z), _here(stream, z)))
 
 

@@ -132,7 +132,7 @@ int fhe_ssm_sample(uint32_t type, const void* logits, uint32_t rows, uint32_t vo
  * channels <= 16384, rows < 2^31.  Rows are `type`, their strides in elements; weight and bias have `channels` elements of
  * weight_type, float32 or `type`, and null stands for 1 and 0.  mean and rstd (float32[rows], either may be null) are what the
  * backward pass takes.  out may be x; other overlaps are not allowed.  A row that holds a NaN or an infinity comes out NaN and
- * leaves the others alone. */
+ * leaves the others alone; squares of distances from the mean have to sum to less than 2^128. */
 typedef struct {
     uint32_t type, weight_type; /* of x, out, dy and dx; of weight and bias */
     uint32_t rows, channels;
@@ -189,7 +189,7 @@ int fhe_ssm_gated_recurrence_step(const fhe_ssm_gated_recurrence* a, const void*
 /* ---- embedding ----------------------------------------------------------------------------------------------------
  *     out_t = scale table[token_t]        dtable[v] = scale sum of dout_t over the t with token_t = v, in their order
  * tokens: int64 on the device; one outside [0, vocab) gives a row of zeros and adds to no gradient.  vocab <= 2^18, tokens <=
- * 2^26, channels <= 2^20.  The lookup takes any of the types for either side. */
+ * 2^25, channels <= 2^20.  The lookup takes any of the types for either side. */
 typedef struct {
     uint32_t table_type, row_type; /* of the table and its gradient; of out and dout */
     uint32_t tokens, vocab, channels;

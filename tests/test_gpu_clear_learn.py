@@ -87,6 +87,19 @@ def test_gradients_in_bf16_and_the_rows_of_several_products():
             assert (got.double() - g).norm() <= CLOSE_16 * g.norm(), (rows, i)
 
 
+def test_texts_of_no_and_of_one_token_and_tokens_outside():
+    model = learner()
+    for n in (0, 1):
+        loss, dmatrices, dvectors = model.gradients(texts(3, n))
+        assert loss.item() == 0 and all((g == 0).all() for g in dmatrices + dvectors)
+        assert model.score(texts(3, n))[0].shape == (3, n)
+    tokens = texts(2, 20)
+    tokens[0, 7] = VOCAB + 5  # as what follows it counts for nothing, as a token it is a row of zeros
+    want = model.score(tokens)[0]
+    assert want[0, 6] == 0 and torch.isfinite(want).all()
+    assert abs(model.gradients(tokens)[0].item() + want.sum().item() / 37) <= CLOSE
+
+
 def test_a_step_moves_the_parameters_as_adamw_says():
     """the first step's moments are the gradient's: every entry moves by lr, against it, where the gradient is not tiny"""
     model, tokens = learner(), texts(3, 40)

@@ -264,6 +264,8 @@ def test_recurrence_of_no_tokens_hands_the_state_on():
     z, x, state, dy, dlast = gates_case(2, 0, 40, torch.bfloat16, 1)
     out, last, _, _, dstate = run_recurrence(z, x, state, dy, dlast)
     assert out.numel() == 0 and torch.equal(last, state) and torch.equal(dstate, dlast)
+    ops().gated_recurrence_backward(z, x, None, dy, dlast, z.clone(), z.clone(), dstate.fill_(7))  # nothing is saved of nothing
+    assert torch.equal(dstate, dlast)
 
 
 @pytest.mark.parametrize("T", [40, 700])
@@ -721,6 +723,19 @@ def test_score_of_a_row_that_is_not_finite(rows, value):
     w[1] = u[1] = 0
     assert (score(logits, tokens, 3, w, u)[5][1] == 0).all()  # a masked position
     assert (score(logits, tokens, 3, w, u, at_once=True)[5][1] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [3, 600])
+def test_score_of_nan_beside_logits_out_of_all_proportion(rows):
+    """a NaN stays one whatever follows it: logits of 2^120, later and larger ones, rows of nothing but them"""
+    x = torch.zeros((rows, 9000), device="cuda")
+    x[:, 5], x[:, 4000:4004], x[:, 8000] = math.nan, 2.0**120, 2.0**121
+    x[1, 5] = 0.0
+    lp, entropy, _, top, _, grad = score(x, torch.full((rows,), 8000, device="cuda"), 2, torch.ones(rows, device="cuda"))
+    keep = torch.arange(rows, device="cuda") != 1
+    assert torch.isnan(lp[keep]).all() and torch.isnan(entropy[keep]).all() and torch.isnan(grad[keep]).all()
+    assert lp[1].item() == 0 and entropy[1].item() == 0 and (grad[1] == 0).all()
+    assert (top == torch.tensor([8000, 4000], device="cuda")).all()
 
 
 def test_score_without_tokens():
