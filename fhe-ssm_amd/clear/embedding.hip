@@ -18,7 +18,7 @@
 namespace clear {
 namespace {
 
-constexpr uint32_t kPiece = 32, kFew = 1024, kSmall = 8192;
+constexpr uint32_t kPiece = 16, kFew = 1024, kSmall = 8192;
 constexpr uint32_t kTile = 2048, kMostParts = 256, kDigits = 1024;  // sorted at a time by a workgroup; workgroups; values of a digit
 constexpr uint32_t kMostVocab = 1u << 18, kMostTokens = 1u << 25;
 

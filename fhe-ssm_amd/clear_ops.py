@@ -377,7 +377,7 @@ _calls: dict = {}  # an operator's name, and sizes, types, strides and devices o
 
 
 def _like(t):
-    """all that is checked of a tensor"""
+    """all that is checked of a tensor; one on the host, whose device is -1, is refused when its description would be made"""
     return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
 
 
@@ -459,10 +459,10 @@ def layer_norm(x, weight, bias, out, mean=None, rstd=None, eps: float = 1e-5, st
 
     out like x, or x itself; weight and bias [channels], float32 or of x's type, None: 1 and 0; mean and rstd float32 [rows] or
     None: what layer_norm_backward takes."""
-    _on_device(x, weight, bias, out, mean, rstd)
     key = ("norm", eps, _like(x), _like(weight), _like(bias), _like(out), _like(mean), _like(rstd))
     a = _calls.get(key)
     if a is None:
+        _on_device(x, weight, bias, out, mean, rstd)
         sizes = _norm_sizes(x, out, weight, bias, eps)
         _floats((sizes.rows,), mean=mean, rstd=rstd)
         a = _kept(key, sizes)
@@ -473,10 +473,10 @@ def layer_norm(x, weight, bias, out, mean=None, rstd=None, eps: float = 1e-5, st
 def layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, workspace=None, stream=None) -> None:
     """The gradients of layer_norm from that of its output: dx like x (it may be dy), dweight and dbias float32 [channels] where
     they are given.  workspace: a uint8 tensor of layer_norm_workspace(x) bytes, needed for dweight and dbias."""
-    _on_device(dy, x, weight, mean, rstd, dx, dweight, dbias, workspace)
     key = ("norm back", _like(x), _like(weight), _like(dx), _like(dy), _like(mean), _like(rstd), _like(dweight), _like(dbias))
     a = _calls.get(key)
     if a is None:
+        _on_device(dy, x, weight, mean, rstd, dx, dweight, dbias)
         sizes = _norm_sizes(x, dx, weight, None, dy=dy)
         _floats((sizes.rows,), mean=mean, rstd=rstd)
         _floats((sizes.channels,), dweight=dweight, dbias=dbias)
@@ -542,10 +542,10 @@ def gated_recurrence(z, x, state_in, state_out, out, lengths=None, saved=None, w
     may be one tensor); lengths int32 [lanes]: tokens past a lane's length change nothing and give zeros; saved: None, or a uint8
     tensor of gated_recurrence_saved(z) bytes for the backward pass; workspace: one of gated_recurrence_workspace(z) bytes, None
     where that is 0."""
-    _on_device(z, x, state_in, state_out, out, lengths, saved, workspace)
     key = ("recurrence", _like(z), _like(x), _like(state_in), _like(state_out), _like(out), _like(lengths), _like(saved))
     a = _calls.get(key)
     if a is None:
+        _on_device(z, x, state_in, state_out, out, lengths, saved)
         sizes = _recurrence_sizes(z, True, x=x, out=out)
         _floats((sizes.lanes, sizes.channels), state_in=state_in, state_out=state_out)
         _lengths(lengths, sizes.lanes)
@@ -560,11 +560,11 @@ def gated_recurrence_backward(z, x, saved, dout, dstate_out, dz, dx, dstate_in=N
                               stream=None) -> None:
     """The gradients of gated_recurrence: dz and dx like z, dstate_in float32 [lanes, channels] where it is given, from those of
     out and of state_out (None: zeros).  z, x, lengths and saved are the prompt's; dstate_in may be dstate_out."""
-    _on_device(z, x, saved, dout, dstate_out, dz, dx, dstate_in, lengths, workspace)
     key = ("recurrence back", _like(z), _like(x), _like(saved), _like(dout), _like(dstate_out), _like(dz), _like(dx),
            _like(dstate_in), _like(lengths))
     a = _calls.get(key)
     if a is None:
+        _on_device(z, x, saved, dout, dstate_out, dz, dx, dstate_in, lengths)
         sizes = _recurrence_sizes(z, True, x=x, dout=dout, dz=dz, dx=dx)
         _floats((sizes.lanes, sizes.channels), dstate_in=dstate_in, dstate_out=dstate_out)
         _lengths(lengths, sizes.lanes)
@@ -577,10 +577,10 @@ def gated_recurrence_backward(z, x, saved, dout, dstate_out, dz, dx, dstate_in=N
 
 def gated_recurrence_step(z, x, state_in, state_out, out, stream=None) -> None:
     """gated_recurrence for one token of every lane: the same tensors without the token axis"""
-    _on_device(z, x, state_in, state_out, out)
     key = ("recurrence step", _like(z), _like(x), _like(state_in), _like(state_out), _like(out))
     a = _calls.get(key)
     if a is None:
+        _on_device(z, x, state_in, state_out, out)
         sizes = _recurrence_sizes(z, False, x=x, out=out)
         _floats((sizes.lanes, sizes.channels), state_in=state_in, state_out=state_out)
         a = _kept(key, sizes)
@@ -592,10 +592,10 @@ def gated_recurrence_step(z, x, state_in, state_out, out, stream=None) -> None:
 def embedding(tokens, table, out, scale: float = 1.0, stream=None) -> None:
     """out[t] = scale table[tokens[t]]; zeros for a token outside the table.  tokens int64 [n], table [vocab, channels], out
     [n, channels], each of any of the three types."""
-    _on_device(tokens, table, out)
     key = ("embedding", scale, _like(tokens), _like(table), _like(out))
     a = _calls.get(key)
     if a is None:
+        _on_device(tokens, table, out)
         _token_ids(tokens)
         n = tokens.shape[0]
         strides = _matrix(table, "table"), _matrix(out, "out")
@@ -628,10 +628,10 @@ def embedding_gradient(tokens, dout, dtable, scale: float = 1.0, accumulate: boo
     """dtable[v] = scale times the sum of dout[t] over the t with tokens[t] = v, in their order; with `accumulate` added to what
     is there.  dout [n, channels]; dtable contiguous [vocab, channels], float32 or of dout's type; workspace: a uint8 tensor of
     embedding_gradient_workspace(tokens, dtable) bytes, None where that is 0."""
-    _on_device(tokens, dout, dtable, workspace)
     key = ("embedding back", scale, _like(tokens), _like(dout), _like(dtable))
     a = _calls.get(key)
     if a is None:
+        _on_device(tokens, dout, dtable)
         a = _embedding_gradient_sizes(tokens, dtable, scale)
         a.row_type, a.row_stride = _type(dout), _matrix(dout, "dout")
         _need(tuple(dout.shape) == (a.tokens, a.channels), f"dout must be [{a.tokens}, {a.channels}]")
@@ -667,11 +667,11 @@ def token_logprobs(logits, tokens, logprobs, entropy=None, statistics=None, top_
     falling logits, equal ones by rising index.  gradient (like logits, or logits itself) receives that of
     sum(weights logprobs + entropy_weights entropy) in the same call, with weights float32 [rows].  All but logits may be None.
     workspace: a uint8 tensor of token_logprobs_workspace(logits, k) bytes, None where that is 0."""
-    _on_device(logits, tokens, logprobs, entropy, statistics, top_tokens, top_logprobs, workspace, weights, entropy_weights, gradient)
     key = ("logprobs", _like(logits), _like(tokens), _like(logprobs), _like(entropy), _like(statistics), _like(top_tokens),
            _like(top_logprobs), _like(weights), _like(entropy_weights), _like(gradient))
     a = _calls.get(key)
     if a is None:
+        _on_device(logits, tokens, logprobs, entropy, statistics, top_tokens, top_logprobs, weights, entropy_weights, gradient)
         top = 0
         if top_tokens is not None or top_logprobs is not None:
             _need(top_tokens is not None and top_logprobs is not None, "top_tokens and top_logprobs come together")
@@ -695,11 +695,11 @@ def token_logprobs_gradient(logits, tokens, statistics, weights, gradient, entro
                             stream=None) -> None:
     """The gradient that token_logprobs writes, where its weights were not known then: from the statistics, and the entropy if it
     has weights."""
-    _on_device(logits, tokens, statistics, weights, gradient, entropy_weights, entropy)
     key = ("logprobs back", _like(logits), _like(tokens), _like(statistics), _like(weights), _like(gradient),
            _like(entropy_weights), _like(entropy))
     a = _calls.get(key)
     if a is None:
+        _on_device(logits, tokens, statistics, weights, gradient, entropy_weights, entropy)
         a = _logprobs_sizes(logits, 0, gradient)
         if tokens is not None:
             _token_ids(tokens, a.rows)
