@@ -283,6 +283,7 @@ __device__ inline void add_batch(uint32_t j, uint32_t n, const uint32_t (&c)[kGr
 }
 template <int kFlight, int V, class F>
 __device__ inline void add_rows(uint32_t n, uint32_t c0, uint32_t d, float (&f)[kGroups * V], F&& row) {
+    static_assert(kFlight >= 2);
     uint32_t c[kGroups];
 #pragma unroll
     for (int g = 0; g < kGroups; g++) {
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(256) void k_runs(Args a) {
             for (uint32_t c0 = 0; c0 < a.d; c0 += kCols) {
                 float f[kGroups * V] = {};
                 add_held<T, 4, V>(a, held, 0, first - i, c0, f);
-                if (last > first) add_rows<1, V>((last - first) / kPiece, c0, a.d, f, [&](uint32_t j) { return a.sums + (size_t)(first / kPiece + j) * a.d; });
+                if (last > first) add_rows<2, V>((last - first) / kPiece, c0, a.d, f, [&](uint32_t j) { return a.sums + (size_t)(first / kPiece + j) * a.d; });
                 add_held<T, 4, V>(a, held, last - i, end - last, c0, f);
                 write_row<G, V>(a, id, c0, f);
             }
