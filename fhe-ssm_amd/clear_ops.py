@@ -740,17 +740,20 @@ class AdamW:
         kind = "torch.float32" if bits == 32 else "torch.float8_e4m3fn"
         for name, s in zip(("the first state", "the second state"), self.states):
             for p, t in zip(self.params, s):
-                _need(t.device == p.device and t.shape == p.shape and _is(t, kind) and t.is_contiguous(), f"{name} must be contiguous {kind[6:]} like its parameter")
+                _need(t.device == p.device and t.shape == p.shape and _is(t, kind) and t.is_contiguous(),
+                      f"{name} must be contiguous {kind[6:]} like its parameter")
         if bits == 8:
             for p, t in zip(self.params, self.states[2]):
-                _need(t.device == p.device and tuple(t.shape) == (-(-p.numel() // self.BLOCK), 2) and _is(t, "torch.uint8") and t.is_contiguous(),
+                blocks = -(-p.numel() // self.BLOCK)
+                _need(t.device == p.device and tuple(t.shape) == (blocks, 2) and _is(t, "torch.uint8") and t.is_contiguous(),
                       "powers must be contiguous uint8 [blocks, 2]")
         copy_type = BF16
         if self.copies is not None:
             _need(len(self.copies) == n, "one copy for each parameter")
             copy_type = _type(self.copies[0])
+            _need(copy_type != F32, "copies are bfloat16 or float16")
             for p, t in zip(self.params, self.copies):
-                _need(t.device == p.device and t.shape == p.shape and t.dtype == self.copies[0].dtype and copy_type != F32 and t.is_contiguous(),
+                _need(t.device == p.device and t.shape == p.shape and t.dtype == self.copies[0].dtype and t.is_contiguous(),
                       "copies must be contiguous bfloat16 or float16 like their parameters")
         self._sizes = AdamWSizes(F32, copy_type, bits, 0, 0, 0.0, eps, *betas)
         self._tensors = (AdamWTensor * n)()
