@@ -54,6 +54,18 @@ __device__ inline float sum64(float x) {
     return (of_lane(x, 0) + of_lane(x, 16)) + (of_lane(x, 32) + of_lane(x, 48));
 }
 
+// the largest of each 16 lanes, of the wave, in all of them; a NaN is none
+__device__ inline float max16(float x) {
+    x = __builtin_fmaxf(x, swapped<0xb1>(x));
+    x = __builtin_fmaxf(x, swapped<0x4e>(x));
+    x = __builtin_fmaxf(x, swapped<0x141>(x));
+    return __builtin_fmaxf(x, swapped<0x140>(x));
+}
+__device__ inline float max64(float x) {
+    x = max16(x);
+    return __builtin_fmaxf(__builtin_fmaxf(of_lane(x, 0), of_lane(x, 16)), __builtin_fmaxf(of_lane(x, 32), of_lane(x, 48)));
+}
+
 // N sums over the L lanes that share a row, in all of them and always in the same order.  L of 256 or 1,024 is the workgroup:
 // the waves' sums go through LDS, two blocks of them in turn, so that one barrier is enough.
 template <int L, int N>

@@ -97,11 +97,13 @@ struct Row {
 struct Part {
     float m, s, t;
 };
-__device__ inline Part joined(Part a, Part b) {
-    const float m = a.m > b.m ? a.m : b.m;
-    const float da = a.m == m ? 0.f : (m - a.m) * kLog2e, db = b.m == m ? 0.f : (m - b.m) * kLog2e;  // 0 where both are -inf
-    const float ea = __builtin_amdgcn_exp2f(-da), sa = a.s * ea, eb = __builtin_amdgcn_exp2f(-db), sb = b.s * eb;
-    return {m, sa + sb, (a.t * ea + (sa > 0.f ? da * sa : 0.f)) + (b.t * eb + (sb > 0.f ? db * sb : 0.f))};
+// The parts that 16 or 64 lanes hold, as one, in all of them: all follow the largest, and then it is two sums in a fixed order.
+template <int L>
+__device__ inline Part joined(Part p) {
+    const float m = L == 16 ? max16(p.m) : max64(p.m);
+    const float d = p.m == m ? 0.f : (m - p.m) * kLog2e, e = __builtin_amdgcn_exp2f(-d);  // 0 where all are -inf
+    const float s = p.s * e, t = p.t * e + (s > 0.f ? d * s : 0.f);
+    return {m, L == 16 ? sum16(s) : sum64(s), L == 16 ? sum16(t) : sum64(t)};
 }
 
 template <int kThreads>
@@ -356,7 +358,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
             if (kTop) first = m > largest ? j + i : first;
             largest = __builtin_fmaxf(largest, m);
             const float above = __builtin_fmaf(m, kLog2e, -reference);
-            if (above > kSlack) {
+            if (__builtin_expect(above > kSlack, 0)) {  // rare after the first vectors, and not to be done beside
                 const float d = __builtin_fminf(above, 1e6f), e = __builtin_amdgcn_exp2f(-d);
                 along = (along - d * sum) * e;
                 sum *= e;
@@ -376,20 +378,12 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
         p.t = (d * sum - along) * e;
         p.s = sum * e;
     }
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const Part q{__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o)};
-        p = threadIdx.x & o ? joined(q, p) : joined(p, q);
-    }
+    p = joined<64>(p);
     if (threadIdx.x % 64 == 0) s.part[threadIdx.x / 64] = p;
     __syncthreads();
     constexpr int kWaves = kThreads / 64;
-    p = s.part[threadIdx.x % kWaves];
-#pragma unroll
-    for (int o = 1; o < kWaves; o *= 2) {
-        const Part q{__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o)};
-        p = threadIdx.x & o ? joined(q, p) : joined(p, q);
-    }
+    p = threadIdx.x % 16 < kWaves ? s.part[threadIdx.x % 16] : Part{-INFINITY, 0.f, 0.f};
+    p = joined<16>(p);
     if constexpr (kPart) {
         if (threadIdx.x == 0) {
             float* to = a.sums + (size_t)blockIdx.x * 4;
@@ -431,10 +425,9 @@ __global__ __launch_bounds__(256) void k_join(Args a) {
     uint64_t bound = a.k && part < a.parts ? best[part * a.k + a.k - 1] : 0;
     const uint64_t e0 = threadIdx.x < all ? best[threadIdx.x] : 0, e1 = threadIdx.x + 256 < all ? best[threadIdx.x + 256] : 0;
     if (threadIdx.x == 0) s.listed = 0;
+    p = joined<16>(p);
 #pragma unroll
     for (int o = 1; o < 16; o *= 2) {
-        const Part q{__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o)};
-        p = threadIdx.x & o ? joined(q, p) : joined(p, q);
         const uint64_t other = __shfl_xor((unsigned long long)bound, o);
         bound = max(bound, other);
     }
