@@ -9,7 +9,7 @@
 // LDS and writes as one part; a second kernel adds the parts.  No order depends on timing.  The next row is on its way while one is
 // worked on.
 //
-// 32,768 rows of 768 in bf16 take 17.7 us forward (5.7 TB/s) and 31.4 backward (4.8 TB/s) with 4.7 for the 512 parts.  (Weights
+// 32,768 rows of 768 in bf16 take 17.2 us forward (5.8 TB/s) and 28.0 backward (5.4 TB/s) with 4.8 for the 256 parts.  (Weights
 // read element by element: 35 forward, as every wave read them for four rows; without the next row on its way 33.4 backward.)
 #include <algorithm>
 
@@ -215,8 +215,8 @@ __global__ __launch_bounds__(1024) void k_columns(const float* __restrict__ part
 }
 
 // Which lanes share a row: the fewest that hold its channels, with vectors of 16 bytes where every row lies on them.  Without
-// vectors a wave takes up to 16 elements a lane: 2,999 float32 rows of 1,101 take 8.6 + 10.9 us by workgroups of 256 with 8 a lane,
-// 11.4 + 64 by waves with 32.
+// vectors a wave takes up to 16 elements a lane: 2,999 float32 rows of 1,101 took 8.6 + 10.9 us by workgroups of 256 with 8 a lane,
+// 11.4 + 64 by waves with 32, each with twice today's parts of dw.
 template <class T, class F>
 int choose(bool vectors, uint32_t d, F&& f) {
     constexpr int V = 16 / sizeof(T);

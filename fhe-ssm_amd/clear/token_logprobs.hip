@@ -17,9 +17,9 @@
 // Few rows are cut into parts, a workgroup each; a second kernel joins the parts' sums and ranks their alternatives.
 //
 // Where the weights of the gradient are known the row is read again at once, from the caches, and the gradient written.
-// Bound by bytes for many rows: 4,096 bf16 rows of 65,536 with their gradient, read twice and written once, take 245 us, 1.07 GB
-// of logits and gradients at 4.4 TB/s (the second reading comes from the caches); about 11 vector instructions a logit, and as many
-// for its gradient.  32 float32 rows with 20 alternatives take 8.6 us and 6.3 for the join, of which the sums alone are 5 and 2.5.
+// Bound by bytes for many rows: 4,096 bf16 rows of 65,536 with their gradient, read twice and written once, take 236 us, 1.07 GB
+// of logits and gradients at 4.5 TB/s (the second reading comes from the caches); about 11 vector instructions a logit, and as many
+// for its gradient.  32 float32 rows with 20 alternatives take 7.1 us and 5.9 for the join.
 #include <algorithm>
 
 #include "rows.hpp"
@@ -483,7 +483,7 @@ Args args(const fhe_ssm_token_logprobs& a, const void* logits, const int64_t* to
     return k;
 }
 // Parts of a row: where rows leave CUs without work, of 4,096 logits at least, two workgroups a CU.  (32 float32 rows of 65,536
-// with 20 alternatives take 21 us whole and 14 in parts, 300 bf16 rows of 131,072 with 32 of them 45 and 36.)
+// with 20 alternatives take 21 us whole and 13 in parts, 300 bf16 rows of 131,072 with 32 of them 42 and 35.)
 void cut(Args& k) {
     k.parts = k.rows < 512 ? std::min({(511 + k.rows) / k.rows, (k.vocab + 4095) / 4096, kMostParts}) : 1;
     k.each = (k.vocab + k.parts - 1) / k.parts;
@@ -558,7 +558,7 @@ int fhe_ssm_token_logprobs_forward(const fhe_ssm_token_logprobs* a, const void* 
         }
         if (k.k) return k.grad ? run(few, yes, yes, no) : run(few, yes, no, no);
         // A long row has a whole CU's threads, so that what lies between its two readings stays in the caches: 4,096 rows of
-        // 65,536 in bf16 take 266 us with their gradient, with 256 threads a row 300.
+        // 65,536 in bf16 take 236 us with their gradient, with 256 threads a row 288.
         if (k.vocab > kWide) return k.grad ? run(many, no, yes, no) : run(many, no, no, no);
         return k.grad ? run(few, no, yes, no) : run(few, no, no, no);
     });
