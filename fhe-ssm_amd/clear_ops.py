@@ -765,6 +765,10 @@ class AdamW:
             if self.copies is not None:
                 t.copy = self.copies[i].data_ptr()
         self._gradients = np.frombuffer(self._tensors, np.uint64).reshape(n, -1)[:, 1]
+        # the memory stays while this does, and whose tensors the caller gave other memory is told at the next step
+        self._memory = [t.detach() for ts in (self.params, *self.states, self.copies or ()) for t in ts]
+        self._theirs = self.params + (self.copies or [])
+        self._at, self._shapes = [t.data_ptr() for t in self._theirs], [p.shape for p in self.params]
 
     def _zeros(self):
         if self.bits == 32:
@@ -780,20 +784,23 @@ class AdamW:
         how 8-bit states are rounded."""
         _need(len(gradients) == len(self.params), f"{len(self.params)} gradients are needed")
         kind, at = gradients[0].dtype, self.params[0].get_device()
-        for g, p in zip(gradients, self.params):
-            if not (g.is_cuda and g.get_device() == at and g.dtype == kind and g.shape == p.shape and g.is_contiguous()):
+        for g, shape in zip(gradients, self._shapes):
+            if not (g.is_cuda and g.get_device() == at and g.dtype == kind and g.shape == shape and g.is_contiguous()):
                 raise ClearError("gradients must be contiguous tensors of one type, like their parameters, on the GPU")
+        if [t.data_ptr() for t in self._theirs] != self._at:
+            raise ClearError("a parameter or copy has other memory than it had; an AdamW of them and of these states goes on")
+        _need(not isinstance(step, int) or 1 <= step < 1 << 32, f"steps count from 1, not {step}")
         a = self._sizes
         a.gradient_type, a.seed = _type(gradients[0]), seed & 0xffffffff
-        a.lr, a.lr_at = (lr, None) if isinstance(lr, (int, float)) else (0.0, self._one(lr, "lr", "torch.float32"))
-        a.step, a.step_at = (step, None) if isinstance(step, int) else (0, self._one(step, "step", "torch.int32"))
-        a.scale_at = None if scale is None else self._one(scale, "scale", "torch.float32")
+        a.lr, a.lr_at = (lr, None) if isinstance(lr, (int, float)) else (0.0, self._one(lr, "lr", "torch.float32", at))
+        a.step, a.step_at = (step, None) if isinstance(step, int) else (0, self._one(step, "step", "torch.int32", at))
+        a.scale_at = None if scale is None else self._one(scale, "scale", "torch.float32", at)
         self._gradients[:] = [g.data_ptr() for g in gradients]
         check(load().fhe_ssm_adamw_step(ctypes.addressof(a), len(self.params), ctypes.addressof(self._tensors),
                                         _here(stream, self.params[0])))
 
     @staticmethod
-    def _one(t, name: str, dtype: str):
-        _need(hasattr(t, "data_ptr") and t.is_cuda and _is(t, dtype) and t.numel() == 1,
-              f"{name} must be a number or a {dtype[6:]} tensor of one on the GPU")
+    def _one(t, name: str, dtype: str, at: int):
+        _need(hasattr(t, "data_ptr") and t.is_cuda and t.get_device() == at and _is(t, dtype) and t.numel() == 1,
+              f"{name} must be a number or a {dtype[6:]} tensor of one, on the parameters' GPU")
         return t.data_ptr()

@@ -254,6 +254,26 @@ def test_python_refuses_shapes_types_and_strides(library):
         a.step([x, v], lr=0.1, step=z(1))
 
 
+def test_adamw_refuses_steps_before_the_first_and_tensors_with_other_memory(library):
+    z = lambda *s, dtype=torch.float32: on_gpu(torch.zeros(s, dtype=dtype))  # noqa: E731
+    for bits in (32, 8):
+        p, c, g = z(4, 8), z(4, 8, dtype=torch.bfloat16), z(4, 8)
+        a = library.AdamW([p], copies=[c], bits=bits)
+        for step in (0, -1, 1 << 32):
+            with pytest.raises(library.ClearError, match="steps count from 1"):
+                a.step([g], lr=0.1, step=step)
+        a.step([g], lr=0.1, step=(1 << 32) - 1)
+        was, p.data = p.data, torch.zeros(4, 8)
+        with pytest.raises(library.ClearError, match="other memory"):
+            a.step([g], lr=0.1, step=1)
+        p.data = was
+        a.step([g], lr=0.1, step=1)
+        c.data = torch.zeros(4, 8, dtype=torch.bfloat16)
+        with pytest.raises(library.ClearError, match="other memory"):
+            a.step([g], lr=0.1, step=1)
+    assert len(library._lib.streams) == 4
+
+
 def test_what_is_refused_once_is_refused_again_and_what_is_not_goes_through(library):
     x = on_gpu(torch.zeros(4, 8))
     for _ in range(2):
