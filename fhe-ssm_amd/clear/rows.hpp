@@ -39,8 +39,10 @@ template <int kControl>
 __device__ inline float swapped(float x) {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), kControl, 0xf, 0xf, false));
 }
-// the sum over each 16 lanes, in all of them: neighbours, pairs, fours, eights
+// the sum over each 16 lanes, the same in all of them: neighbours, pairs, fours, eights.  (A product summed would be rounded
+// for the other lanes and not for its own, if the addition took it in.)
 __device__ inline float sum16(float x) {
+#pragma clang fp contract(off)
     x += swapped<0xb1>(x);
     x += swapped<0x4e>(x);
     x += swapped<0x141>(x);

@@ -122,7 +122,7 @@ struct Alternatives {
 };
 
 __device__ inline float log2_p(float x, float m, float log2s) { return __builtin_fmaf(x - m, kLog2e, -log2s); }
-__device__ inline float log_p(float x, float m, float log2s) { return (x - m) - kLn2 * log2s; }
+__device__ inline float log_p(float x, float m, float log2s) { return __builtin_fmaf(-kLn2, log2s, x - m); }
 
 // An entry's place in the order: its logit's key, then the flipped index; 0 for what is no alternative.
 __device__ inline uint64_t entry(float x, uint32_t index) {

@@ -738,6 +738,17 @@ def test_score_of_nan_beside_logits_out_of_all_proportion(rows):
     assert (top == torch.tensor([8000, 4000], device="cuda")).all()
 
 
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [20, 600])
+def test_score_alternatives_are_scored_like_given_tokens(rows, kind):
+    """bit for bit, whichever threads find them"""
+    logits = (3 * normal(generator(rows), rows, 40000)).to(kind)
+    _, _, _, top, top_logprobs, _ = score(logits, torch.zeros(rows, dtype=torch.int64, device="cuda"), 7)
+    for j in range(7):
+        logprobs, *_ = score(logits, top[:, j].contiguous(), 7)
+        assert torch.equal(logprobs, top_logprobs[:, j])
+
+
 def test_score_without_tokens():
     logits, _, _, u = score_case(7, 900, torch.float32, 1)
     got, want = score(logits, None, 4), score(logits, torch.zeros(7, dtype=torch.int64, device="cuda"), 4)
