@@ -789,7 +789,8 @@ class AdamW:
                 raise ClearError("gradients must be contiguous tensors of one type, like their parameters, on the GPU")
         if [t.data_ptr() for t in self._theirs] != self._at:
             raise ClearError("a parameter or copy has other memory than it had; an AdamW of them and of these states goes on")
-        _need(not isinstance(step, int) or 1 <= step < 1 << 32, f"steps count from 1, not {step}")
+        if isinstance(step, int) and not 1 <= step < 1 << 32:
+            raise ClearError(f"steps count from 1, not {step}")
         a = self._sizes
         a.gradient_type, a.seed = _type(gradients[0]), seed & 0xffffffff
         a.lr, a.lr_at = (lr, None) if isinstance(lr, (int, float)) else (0.0, self._one(lr, "lr", "torch.float32", at))
