@@ -9,7 +9,8 @@
 // are set to 0 by workgroups that run beside the sort's.
 //
 // 32,768 tokens, one in 16 the most frequent, of 768 channels in bf16 into a table of 65,536 rows in float32: 41 us of sorting
-// beside 201 MB that are set to 0 (4.9 TB/s; its four kernels alone take 25), 9 for pieces, 27 for runs of 10,400 tokens.  (Pieces of 32 rows: 11 and 31, of 8: 12 and 28; a wave alone for a long run 39.)  The lookup takes 16 to 20.
+// beside 201 MB that are set to 0 (4.9 TB/s; its four kernels alone take 25), 9 for pieces, 27 for runs of 10,400 tokens.
+// (Pieces of 32 rows: 11 and 31, of 8: 12 and 28; a wave alone for a long run 39.)  The lookup takes 16 to 20.
 //
 // The sort goes by two digits of half the token's bits.  A digit's pass counts its values in every workgroup's part, and then
 // each workgroup adds up what lies before its own and moves its positions; a wave ranks 64 of them by comparing digits bit by

@@ -107,12 +107,16 @@ class Draft:
 
     def score(self, tokens, lengths=None, top: int = 0):
         """What the model makes of texts tokens [lanes, n], of lane b the first lengths[b]: the log-probability of every token after
-        those before it and the entropy there, [lanes, n - 1] (log-probabilities past a length are 0), with `top` the likeliest
-        tokens and their log-probabilities [lanes, n - 1, top] too.  Lanes' states are what they were."""
+        those before it and the entropy there, [lanes, n - 1] (log-probabilities past a length, and of tokens outside the
+        vocabulary, are 0), with `top` the likeliest tokens and their log-probabilities [lanes, n - 1, top] too.  Lanes' states
+        are what they were."""
         states, (lanes, n) = self.states, (len(tokens), max(1, tokens.shape[1]))
         self.reset(lanes)
-        hidden = self._run(tokens[:, :-1], None if lengths is None else (lengths - 1).clamp(min=0))
-        self.states = states
+        try:  # padding may be of any value, and no row outside the table is read for it
+            hidden = self._run(tokens[:, :-1].clamp(0, len(self.embedding) - 1),
+                               None if lengths is None else (lengths - 1).clamp(min=0))
+        finally:
+            self.states = states
         rows, next_tokens = hidden.flatten(0, 1), tokens[:, 1:]
         if lengths is not None:
             next_tokens = torch.where(torch.arange(1, n, device=tokens.device)[None] < lengths[:, None], next_tokens, -1)

@@ -195,3 +195,19 @@ def test_the_drafting_models_scores_against_64_bits():
             assert abs(entropy[lane, t].item() + (want[t].exp() * want[t]).sum().item()) <= 2e-2 * size
         assert (logprobs[lane, max(0, n - 1):] == 0).all()
     assert [t.shape[1] for t in draft.score(tokens[:, :1])] == [0, 0]
+
+
+def test_the_drafting_models_scores_of_padding_outside_the_vocabulary_and_after_an_error():
+    from test_gpu_clear_draft import D as draft_d, HEADS, LAYERS as draft_layers, VOCAB as draft_vocab
+    draft = load_module("clear_draft").Draft(layers=draft_layers, d=draft_d, heads=HEADS, vocab=draft_vocab, seed=3, dtype=torch.float32)
+    draft.reset(2)
+    states = draft.states
+    tokens, lengths = texts(2, 9) % draft_vocab, torch.tensor([9, 4], dtype=torch.int32, device="cuda")
+    want = draft.score(tokens, lengths)
+    for pad in (-1, -100, draft_vocab, 1 << 40):
+        padded = tokens.clone()
+        padded[1, 4:] = pad
+        assert all(torch.equal(a[0], b[0]) and torch.equal(a[1, :3], b[1, :3]) for a, b in zip(draft.score(padded, lengths), want))
+    with pytest.raises(load_module("clear_ops").ClearError):
+        draft.score(tokens, lengths.long())
+    assert draft.states is states and all(not s.any() for s in states)
