@@ -216,7 +216,8 @@ __global__ __launch_bounds__(1024) void k_columns(const float* __restrict__ part
 
 // Which lanes share a row: the fewest that hold its channels, with vectors of 16 bytes where every row lies on them.  Without
 // vectors a wave takes up to 16 elements a lane: 2,999 float32 rows of 1,101 took 8.6 + 10.9 us by workgroups of 256 with 8 a lane,
-// 11.4 + 64 by waves with 32, each with twice today's parts of dw.
+// 11.4 + 64 by waves with 32, each with twice today's parts of dw.  32 float32 elements a lane do not fit the backward pass'
+// registers: 30,000 rows of 2,048 take 80 + 234 us by waves, 82 + 141 by workgroups; in bf16 41 + 71 and 43 + 88.
 template <class T, class F>
 int choose(bool vectors, uint32_t d, F&& f) {
     constexpr int V = 16 / sizeof(T);
@@ -226,7 +227,11 @@ int choose(bool vectors, uint32_t d, F&& f) {
         CLEAR_FITS(16, 8, V);
         CLEAR_FITS(64, 8, V);
         CLEAR_FITS(64, 16, V);
-        CLEAR_FITS(64, 32, V);
+        if constexpr (V == 4) {
+            CLEAR_FITS(256, 8, V);
+        } else {
+            CLEAR_FITS(64, 32, V);
+        }
         CLEAR_FITS(256, 16, V);
         CLEAR_FITS(256, 32, V);
         CLEAR_FITS(1024, 16, V);
