@@ -82,6 +82,33 @@ __global__ __launch_bounds__(256) void k_lookup(Args a) {
     }
 }
 
+// Rows of 256 vectors and more: a workgroup has kEach vectors a thread of one row, which costs no division for each of them.
+// (5,619 bf16 rows of 4,091, single elements: 28 us, by k_lookup 45; of 4,096 both 19.)
+template <class F, class T, int V>
+__global__ __launch_bounds__(256) void k_lookup_long(Args a) {
+    constexpr uint32_t kEach = 4;
+    const uint32_t vectors = (a.d + V - 1) / V, parts = (vectors + 256 * kEach - 1) / (256 * kEach);
+    const uint64_t all = (uint64_t)a.n * parts;
+    for (uint64_t at = blockIdx.x; at < all; at += gridDim.x) {
+        const uint32_t row = all <= 0xffffffffull ? (uint32_t)at / parts : (uint32_t)(at / parts), part = (uint32_t)(at - (uint64_t)row * parts);
+        const int64_t token = a.tokens[row];
+        const bool in = token >= 0 && token < (int64_t)a.vocab;
+        const F* from = (const F*)a.from + (in ? token : 0) * a.from_stride;
+        T* to = (T*)a.to + row * a.to_stride;
+        const uint32_t first = part * 256 * kEach + threadIdx.x;
+        float f[kEach][V];
+#pragma unroll
+        for (uint32_t k = 0; k < kEach; k++) load<V>(from + min(first + k * 256, vectors - 1) * V, f[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < kEach; k++) {
+            if (first + k * 256 >= vectors) continue;
+#pragma unroll
+            for (int e = 0; e < V; e++) f[k][e] = in ? f[k][e] * a.scale : 0.f;
+            store<V>(to + (first + k * 256) * V, f[k]);
+        }
+    }
+}
+
 // ---------------------------------------------------------------- the sort
 struct Sort {
     uint16_t ranks[16][kDigits];  // of each wave: how many of a digit it has; later where its next one goes, from the part's begin
@@ -265,32 +292,35 @@ __global__ __launch_bounds__(1024) void k_move(Args a) {
 }
 
 // ---------------------------------------------------------------- the gradient
-// Channels of a wave: groups of V, kGroups of them a lane, then the next 64 V kGroups.
-constexpr int kGroups = 2;
+// Channels of a wave: groups of V, kGroups of them a lane, then the next 64 V kGroups.  Single elements take more groups, so that
+// as much of a row is on its way: 5,619 bf16 rows of 4,091 take 27 us for pieces and 78 for runs, with two groups 60 and 181.
+template <int V>
+constexpr int groups() { return V == 1 ? 8 : 2; }
+constexpr int kFewGroups = 2;  // of k_few, whose waves share a row
 
 // Adds n rows to f, in order; row(j) is where row j begins.  Up to kFlight rows are on their way at once, at the end the last
 // of them again for those that are not there: a row that is waited for alone takes as long as all.  A lane past the row's end
 // reads its beginning.
-template <int kRows, int V, class F>
-__device__ inline void add_batch(uint32_t j, uint32_t n, const uint32_t (&c)[kGroups], float (&f)[kGroups * V], F&& row) {
-    float x[kRows][kGroups * V];
+template <int kRows, int V, int N, class F>
+__device__ inline void add_batch(uint32_t j, uint32_t n, const uint32_t (&c)[N / V], float (&f)[N], F&& row) {
+    float x[kRows][N];
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
         const auto* at = row(min(j + i, n - 1));
 #pragma unroll
-        for (int g = 0; g < kGroups; g++) load<V>(at + c[g], x[i] + g * V);
+        for (int g = 0; g < N / V; g++) load<V>(at + c[g], x[i] + g * V);
     }
 #pragma unroll
     for (int i = 0; i < kRows; i++)
 #pragma unroll
-        for (int e = 0; e < kGroups * V; e++) f[e] = j + i < n ? f[e] + x[i][e] : f[e];
+        for (int e = 0; e < N; e++) f[e] = j + i < n ? f[e] + x[i][e] : f[e];
 }
-template <int kFlight, int V, class F>
-__device__ inline void add_rows(uint32_t n, uint32_t c0, uint32_t d, float (&f)[kGroups * V], F&& row) {
+template <int kFlight, int V, int N, class F>
+__device__ inline void add_rows(uint32_t n, uint32_t c0, uint32_t d, float (&f)[N], F&& row) {
     static_assert(kFlight >= 2);
-    uint32_t c[kGroups];
+    uint32_t c[N / V];
 #pragma unroll
-    for (int g = 0; g < kGroups; g++) {
+    for (int g = 0; g < N / V; g++) {
         c[g] = c0 + (g * 64 + threadIdx.x % 64) * V;
         c[g] = c[g] < d ? c[g] : 0;
     }
@@ -300,19 +330,19 @@ __device__ inline void add_rows(uint32_t n, uint32_t c0, uint32_t d, float (&f)[
     }
 }
 // rows at .. at + n - 1 of 64 sorted positions, of which each lane holds one
-template <class T, int kFlight, int V>
-__device__ inline void add_held(const Args& a, uint32_t held, uint32_t at, uint32_t n, uint32_t c0, float (&f)[kGroups * V]) {
+template <class T, int kFlight, int V, int N>
+__device__ inline void add_held(const Args& a, uint32_t held, uint32_t at, uint32_t n, uint32_t c0, float (&f)[N]) {
     add_rows<kFlight, V>(n, c0, a.d, f, [&](uint32_t j) {
         return (const T*)a.from + (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)held, (int)(at + j)) * a.from_stride;
     });
 }
 
 // scales a row's sum and writes it, or adds it to what is there
-template <class G, int V>
-__device__ inline void write_row(const Args& a, uint32_t id, uint32_t c0, float (&f)[kGroups * V]) {
+template <class G, int V, int N>
+__device__ inline void write_row(const Args& a, uint32_t id, uint32_t c0, float (&f)[N]) {
     G* to = (G*)a.to + (size_t)id * a.d;
 #pragma unroll
-    for (int g = 0; g < kGroups; g++) {
+    for (int g = 0; g < N / V; g++) {
         const uint32_t c = c0 + (g * 64 + threadIdx.x % 64) * V;
         if (c >= a.d) continue;
         float x[V], *y = f + g * V;
@@ -326,6 +356,7 @@ __device__ inline void write_row(const Args& a, uint32_t id, uint32_t c0, float 
 // The sums of whole pieces of one token.
 template <class T, int V>
 __global__ __launch_bounds__(256) void k_pieces(Args a) {
+    constexpr int kGroups = groups<V>();
     const uint32_t piece = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / 64), lane = threadIdx.x % 64;
     const uint64_t from = (uint64_t)piece * kPiece;
     if (from + kPiece > a.n) return;
@@ -347,7 +378,7 @@ __global__ __launch_bounds__(256) void k_pieces(Args a) {
 // no second long run begins among them.)
 template <class T, class G, int V>
 __global__ __launch_bounds__(256) void k_runs(Args a) {
-    constexpr int kCols = 64 * V * kGroups;
+    constexpr int kGroups = groups<V>(), kCols = 64 * V * kGroups;
     __shared__ float s_sum[3][kCols];
     __shared__ uint32_t s_begin;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -427,7 +458,7 @@ __global__ __launch_bounds__(256) void k_runs(Args a) {
 // part of the rows.  (701 tokens of 1,101 channels: 9 us.  Sorted by one workgroup 15, and 30 for pieces and runs.)
 template <class T, class G, int V>
 __global__ __launch_bounds__(256) void k_few(Args a) {
-    constexpr int kRounds = kFew / 64, kCols = 64 * V * kGroups;
+    constexpr int kRounds = kFew / 64, kGroups = kFewGroups, kCols = 64 * V * kGroups;
     __shared__ uint32_t s_at[kFew];
     __shared__ float s_sum[3][kCols];
     const uint32_t i = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -535,9 +566,11 @@ int fhe_ssm_embedding_lookup(const fhe_ssm_embedding* a, const int64_t* tokens, 
             const bool vectors = k.d % V == 0 && on_vectors(table, k.from_stride, sizeof(F), V) && on_vectors(out, k.to_stride, sizeof(T), V);
             const auto run = [&](auto v) {
                 constexpr int kV = decltype(v)::value;
-                const uint64_t all = (uint64_t)k.n * ((k.d + kV - 1) / kV);
-                const uint32_t blocks = (uint32_t)std::min<uint64_t>((all + 1023) / 1024, 1u << 22);
-                hipLaunchKernelGGL((k_lookup<F, T, kV>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, k);
+                const uint32_t vectors = (k.d + kV - 1) / kV;
+                const uint64_t all = vectors < 256 ? ((uint64_t)k.n * vectors + 1023) / 1024 : (uint64_t)k.n * ((vectors + 1023) / 1024);
+                const dim3 blocks((uint32_t)std::min<uint64_t>(all, 1u << 22));
+                if (vectors < 256) hipLaunchKernelGGL((k_lookup<F, T, kV>), blocks, dim3(256), 0, (hipStream_t)stream, k);
+                else hipLaunchKernelGGL((k_lookup_long<F, T, kV>), blocks, dim3(256), 0, (hipStream_t)stream, k);
                 return launched("embedding");
             };
             return vectors ? run(std::integral_constant<int, V>{}) : run(std::integral_constant<int, 1>{});
@@ -606,7 +639,7 @@ int fhe_ssm_embedding_gradient(const fhe_ssm_embedding* a, const int64_t* tokens
             typedef decltype(g) G;
             constexpr int V = decltype(v)::value;
             if (few) {
-                hipLaunchKernelGGL((k_few<T, G, V>), dim3(k.n, (k.d + 256 * V * kGroups - 1) / (256 * V * kGroups)), dim3(256), 0, st, k);
+                hipLaunchKernelGGL((k_few<T, G, V>), dim3(k.n, (k.d + 256 * V * kFewGroups - 1) / (256 * V * kFewGroups)), dim3(256), 0, st, k);
                 return launched("embedding: gradient");
             }
             if (k.n >= kPiece) hipLaunchKernelGGL((k_pieces<T, V>), dim3((k.n / kPiece + 3) / 4), dim3(256), 0, st, k);
