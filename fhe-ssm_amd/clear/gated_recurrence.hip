@@ -17,6 +17,8 @@
 // Bound by bytes where lanes fill the GPU: 32 float32 prompts of 1,024 tokens of 768 channels take 62 us forward and 101 backward
 // (4.9 TB/s), in bf16, where a row of 64 channels is 128 bytes, 36 and 66; of lengths from 512 on 32 and 58, as the longest lane
 // decides.  One float32 prompt of 16,384 tokens takes 17.8 to fold 35 segments and 26 for the outputs, backward 17.8 and 45.
+// Texts of up to 12 tokens are taken by one wave, of up to 36 by three: 203 float32 lanes of 768 channels take 5.4 and 6.9 us for 12
+// tokens, 11 and 18 for 36, with eight waves 19 and 29.
 // Eight waves of 12 tokens: of 16 tokens 43 and 80 for the ragged prompts at the time, of 8 36 and 59, sixteen waves of 12 39 and
 // 109, of 8 40 and 73.  Two bf16 channels a lane and two runs a wave, with tiles of 64 to 192 tokens, take the same time within
 // 8 %, both ways.  About 20 (backward 32) vector instructions an element, a third of the cycles.
@@ -30,6 +32,7 @@ namespace {
 
 constexpr int kWaves = 8, kRun = 12;      // waves of a workgroup; tokens of a wave
 constexpr int kTile = kWaves * kRun;      // tokens between kept states
+constexpr int kShort = 3;                 // waves for up to three runs
 constexpr uint32_t kEnough = 512;         // workgroups: two for each CU
 
 struct Args {
@@ -105,6 +108,7 @@ __device__ inline float begin(const Args& a, uint32_t lane, uint32_t segment, ui
 }
 
 // What the two passes' workgroups have in common: which lane, segment and channels are theirs.
+template <int W>
 struct Place {
     uint32_t lane, segment, c, from, wave, l, length, tile0, tile1, whole;  // whole: the end of the tiles that have all tokens
     bool in;
@@ -119,17 +123,18 @@ struct Place {
         from = min(c, a.channels - 1);
         length = length_of(a, lane);
         tile0 = segment * a.each, tile1 = min(a.tiles, tile0 + a.each);
-        whole = max(tile0, min(tile1, length / kTile));
+        whole = max(tile0, min(tile1, length / (W * kRun)));
         at = (size_t)lane * a.channels + from;
     }
 };
 
 // The forward pass; !kOut: only the segments' A and H.  Tiles that have all their tokens come first, the rows of each on their
 // way while the one before is worked on; then one that has some, and those behind the lane's length, which are zeros.
-template <class T, bool kOut>
-__global__ __launch_bounds__(kWaves * 64) void k_forward(Args a) {
-    __shared__ float s_a[2][kWaves][64], s_h[2][kWaves][64];
-    const Place p(a);
+template <class T, bool kOut, int W>
+__global__ __launch_bounds__(W * 64) void k_forward(Args a) {
+    constexpr uint32_t kTile = W * kRun;
+    __shared__ float s_a[2][W][64], s_h[2][W][64];
+    const Place<W> p(a);
     const T *z = (const T*)a.z + p.lane * a.zs[0], *x = (const T*)a.x + p.lane * a.xs[0];
     T* out = kOut ? (T*)a.out + p.lane * a.outs[0] : nullptr;
     uint32_t zr[kRun], xr[kRun];
@@ -163,7 +168,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_forward(Args a) {
         __syncthreads();
         float mine = state;
 #pragma unroll
-        for (uint32_t w = 0; w < kWaves; w++) {
+        for (uint32_t w = 0; w < W; w++) {
             if (w == p.wave) mine = state;
             state = s_a[turn][w][p.l] * state + s_h[turn][w][p.l];
             if (!kOut) product *= s_a[turn][w][p.l];
@@ -200,10 +205,11 @@ __global__ __launch_bounds__(kWaves * 64) void k_forward(Args a) {
 }
 
 // The backward pass, from the last tile to the first; !kOut: only the segments' A and G.
-template <class T, bool kOut>
-__global__ __launch_bounds__(kWaves * 64) void k_backward(Args a) {
-    __shared__ float s_a[2][kWaves][64], s_h[2][kWaves][64], s_g[2][kWaves][64];
-    const Place p(a);
+template <class T, bool kOut, int W>
+__global__ __launch_bounds__(W * 64) void k_backward(Args a) {
+    constexpr uint32_t kTile = W * kRun;
+    __shared__ float s_a[2][W][64], s_h[2][W][64], s_g[2][W][64];
+    const Place<W> p(a);
     const T *z = (const T*)a.z + p.lane * a.zs[0], *x = (const T*)a.x + p.lane * a.xs[0];
     const T* dy = a.dy ? (const T*)a.dy + p.lane * a.dys[0] : nullptr;
     T *dz = (T*)a.dz + p.lane * a.dzs[0], *dx = (T*)a.dx + p.lane * a.dxs[0];
@@ -247,14 +253,14 @@ __global__ __launch_bounds__(kWaves * 64) void k_backward(Args a) {
         __syncthreads();
         float mine = carry;
 #pragma unroll
-        for (int w = kWaves; w-- > 0;) {
+        for (int w = W; w-- > 0;) {
             if ((uint32_t)w == p.wave) mine = carry;
             carry = s_a[turn][w][p.l] * carry + s_g[turn][w][p.l];
             if (!kOut) product *= s_a[turn][w][p.l];
         }
         if (kOut) {
 #pragma unroll
-            for (uint32_t w = 0; w < kWaves - 1; w++)
+            for (uint32_t w = 0; w < W - 1; w++)
                 if (w < p.wave) h = s_a[turn][w][p.l] * h + s_h[turn][w][p.l];
 #pragma unroll
             for (int i = 0; i < kRun; i++) {  // b: what dz takes besides d
@@ -386,8 +392,10 @@ int fhe_ssm_gated_recurrence_prompt(const fhe_ssm_gated_recurrence* a, const voi
     return by_type(a->type, [&](auto t) {
         typedef decltype(t) T;
         const dim3 grid(k.lanes * k.segments * k.strips), block(kWaves * 64);
-        if (k.segments > 1) hipLaunchKernelGGL((k_forward<T, false>), grid, block, 0, (hipStream_t)stream, k);
-        hipLaunchKernelGGL((k_forward<T, true>), grid, block, 0, (hipStream_t)stream, k);
+        if (k.segments > 1) hipLaunchKernelGGL((k_forward<T, false, kWaves>), grid, block, 0, (hipStream_t)stream, k);
+        if (k.tokens <= kRun) hipLaunchKernelGGL((k_forward<T, true, 1>), grid, dim3(64), 0, (hipStream_t)stream, k);
+        else if (k.tokens <= kShort * kRun) hipLaunchKernelGGL((k_forward<T, true, kShort>), grid, dim3(kShort * 64), 0, (hipStream_t)stream, k);
+        else hipLaunchKernelGGL((k_forward<T, true, kWaves>), grid, block, 0, (hipStream_t)stream, k);
         return launched("gated recurrence");
     });
 }
@@ -409,8 +417,10 @@ int fhe_ssm_gated_recurrence_backward(const fhe_ssm_gated_recurrence* a, const v
     return by_type(a->type, [&](auto t) {
         typedef decltype(t) T;
         const dim3 grid(k.lanes * k.segments * k.strips), block(kWaves * 64);
-        if (k.segments > 1) hipLaunchKernelGGL((k_backward<T, false>), grid, block, 0, (hipStream_t)stream, k);
-        hipLaunchKernelGGL((k_backward<T, true>), grid, block, 0, (hipStream_t)stream, k);
+        if (k.segments > 1) hipLaunchKernelGGL((k_backward<T, false, kWaves>), grid, block, 0, (hipStream_t)stream, k);
+        if (k.tokens <= kRun) hipLaunchKernelGGL((k_backward<T, true, 1>), grid, dim3(64), 0, (hipStream_t)stream, k);
+        else if (k.tokens <= kShort * kRun) hipLaunchKernelGGL((k_backward<T, true, kShort>), grid, dim3(kShort * 64), 0, (hipStream_t)stream, k);
+        else hipLaunchKernelGGL((k_backward<T, true, kWaves>), grid, block, 0, (hipStream_t)stream, k);
         return launched("gated recurrence: gradient");
     });
 }

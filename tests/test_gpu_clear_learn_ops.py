@@ -248,6 +248,17 @@ def test_recurrence_lanes_few_and_many(lanes, T):
     check_recurrence(*gates_case(lanes, T, 128, torch.float32, lanes, shift=4.0))
 
 
+@pytest.mark.parametrize("T", [11, 12, 13, 24, 35, 36, 37, 95, 96, 97])
+@pytest.mark.parametrize("kind", TYPES)
+def test_recurrence_short_texts(T, kind):
+    """around what one wave, three and eight take, with lengths of their own, and gradients of the state or of the outputs alone"""
+    lengths = torch.tensor([T, 0, T - 1, 1, T // 2], dtype=torch.int32, device="cuda")
+    z, x, state, dy, dlast = gates_case(5, T, 65, TYPES[kind], T)
+    check_recurrence(z, x, state, dy, dlast, lengths)
+    check_recurrence(z, x, None, None, dlast)
+    check_recurrence(z, x, state, dy, None)
+
+
 @pytest.mark.parametrize("T", [7, 130, 900])
 def test_recurrence_ragged_lengths_hide_what_lies_behind(T):
     lengths = torch.tensor([0, 1, T // 2, T - 1, T, T + 5, -3], dtype=torch.int32, device="cuda")
