@@ -27,8 +27,8 @@
 namespace clear {
 namespace {
 
-constexpr uint32_t kMostTop = 32, kMostParts = 16, kList = 1024, kWide = 8192;
-constexpr uint32_t kEach = 2, kStrips = 256 / kEach;  // threads of a strip
+constexpr uint32_t kMostTop = 32, kMostParts = 16, kList = 1024, kWide = 8192, kShortTop = 16;
+constexpr uint32_t kEach = 2;  // threads of a strip
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
 constexpr float kSlack = 8.f;    // powers of two
 constexpr float kHuge = 0x1p100f;  // two different floats of this size or more weigh 1 and 0 beside each other
@@ -116,8 +116,9 @@ __device__ inline uint64_t swapped64(uint64_t x) {
            (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kControl, 0xf, 0xf, false);
 }
 
+template <int kThreads>
 struct Alternatives {
-    uint64_t best[kStrips], list[kList + 16], bound, wave[4];
+    uint64_t best[kThreads / kEach], list[kList + 16], bound, wave[kThreads / 64];
     uint32_t chosen[kMostTop], listed, chosen_count;
 };
 
@@ -131,20 +132,21 @@ __device__ inline uint64_t entry(float x, uint32_t index) {
 }
 
 // Sets the 16 entries behind the list's end to 0, before the barrier that ends its making.
-__device__ inline void close_list(Alternatives& s, uint32_t n) {
+template <int kThreads>
+__device__ inline void close_list(Alternatives<kThreads>& s, uint32_t n) {
     if (threadIdx.x < 16) s.list[n + threadIdx.x] = 0;
 }
 
 // The k largest entries one by one, to the list.
-template <class T>
-__device__ void one_by_one(const Row<T, 256>& row, uint32_t from, uint32_t k, Alternatives& s) {
-    constexpr int V = Row<T, 256>::V;
+template <class T, int kThreads>
+__device__ void one_by_one(const Row<T, kThreads>& row, uint32_t from, uint32_t k, Alternatives<kThreads>& s) {
+    constexpr int V = Row<T, kThreads>::V;
     uint64_t under = ~0ull;
     for (uint32_t i = 0; i < k; i++) {
         uint64_t best = 0;
         for (int j = 0; j < row.vectors; j++) {
             float f[V];
-            const int v = j * 256 + threadIdx.x;
+            const int v = j * kThreads + threadIdx.x;
             row.read(v, f);
 #pragma unroll
             for (int c = 0; c < V; c++) {
@@ -158,7 +160,7 @@ __device__ void one_by_one(const Row<T, 256>& row, uint32_t from, uint32_t k, Al
         }
         if (threadIdx.x % 64 == 0) s.wave[threadIdx.x / 64] = best;
         __syncthreads();
-        for (int w = 0; w < 4; w++) best = s.wave[w] > best ? s.wave[w] : best;
+        for (int w = 0; w < kThreads / 64; w++) best = s.wave[w] > best ? s.wave[w] : best;
         __syncthreads();
         if (threadIdx.x == 0) s.list[i] = best;
         under = best;
@@ -169,11 +171,11 @@ __device__ void one_by_one(const Row<T, 256>& row, uint32_t from, uint32_t k, Al
 }
 
 // put(i, entry) for the i-th largest of the list's entries, i < k, and put(i, 0) for what is missing
-template <class F>
-__device__ void ranked(uint32_t k, const Alternatives& s, F&& put) {
+template <int kThreads, class F>
+__device__ void ranked(uint32_t k, const Alternatives<kThreads>& s, F&& put) {
     const uint32_t n = s.listed;
     uint32_t have = n;
-    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
         const uint64_t x = s.list[i];
         uint32_t before = 0;
         for (uint32_t j = 0; j < n; j += 16) {  // behind the list's end lie 16 zeros
@@ -189,16 +191,18 @@ __device__ void ranked(uint32_t k, const Alternatives& s, F&& put) {
         have = 0;
         for (uint32_t j = 0; j < n; j++) have += s.list[j] != 0;
     }
-    for (uint32_t i = have + threadIdx.x; i < k; i += 256) put(i, 0);
+    for (uint32_t i = have + threadIdx.x; i < k; i += kThreads) put(i, 0);
 }
 
 // A row's (or its part's, which begins at `from`) k largest to the list, and more; from each thread's largest and the vector
 // `first` where it came first.
-template <class T>
-__device__ void find_alternatives(const Row<T, 256>& row, uint32_t from, uint32_t k, float largest, int first, Alternatives& s) {
-    constexpr int V = Row<T, 256>::V;
+template <class T, int kThreads>
+__device__ void find_alternatives(const Row<T, kThreads>& row, uint32_t from, uint32_t k, float largest, int first,
+                                  Alternatives<kThreads>& s) {
+    constexpr int V = Row<T, kThreads>::V;
+    constexpr uint32_t kStrips = kThreads / kEach;
     // ordered by a vector's first place; the bound takes its last, as the logit itself may lie anywhere in it
-    uint64_t mine = entry(largest, (uint32_t)(first * 256 + (int)threadIdx.x) * V);
+    uint64_t mine = entry(largest, (uint32_t)(first * kThreads + (int)threadIdx.x) * V);
     if constexpr (kEach >= 2) mine = max(mine, swapped64<0xb1>(mine));
     if constexpr (kEach == 4) mine = max(mine, swapped64<0x4e>(mine));
     const uint32_t strip = threadIdx.x / kEach, within = threadIdx.x % kEach;
@@ -218,9 +222,9 @@ __device__ void find_alternatives(const Row<T, 256>& row, uint32_t from, uint32_
     __syncthreads();
     const uint64_t bound = s.bound;
     const uint32_t per = (uint32_t)row.vectors * kEach, items = s.chosen_count * per;
-    for (uint32_t i = threadIdx.x; i < items; i += 256) {
+    for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
         const uint32_t q = i / per, j = i - q * per;
-        const int v = (int)(j / kEach * 256 + s.chosen[q] * kEach + j % kEach);
+        const int v = (int)(j / kEach * kThreads + s.chosen[q] * kEach + j % kEach);
         float f[V];
         row.read(v, f);
 #pragma unroll
@@ -326,7 +330,7 @@ __device__ inline void put_numbers(const Args& a, uint32_t r, int64_t token, flo
 // kTop: alternatives are asked for; kGrad: the gradient too, at once; kPart: a row's part, for k_join
 template <class T, int kThreads, bool kTop, bool kGrad, bool kPart>
 __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
-    static_assert(!kTop || kThreads == 256);
+    static_assert(!kTop || kThreads <= 256);
     __shared__ Shared<kThreads> s;
     constexpr int V = 16 / sizeof(T);
     const uint32_t r = kPart ? blockIdx.x / a.parts : blockIdx.x, from = kPart ? blockIdx.x % a.parts * a.each : 0;
@@ -390,7 +394,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
             to[0] = p.m, to[1] = p.s, to[2] = p.t;
         }
         if constexpr (kTop) {
-            __shared__ Alternatives found;
+            __shared__ Alternatives<kThreads> found;
             find_alternatives(row, from, a.k, largest, first, found);
             ranked(a.k, found, [&](uint32_t i, uint64_t e) { a.best[(size_t)blockIdx.x * a.k + i] = e; });
         }
@@ -398,7 +402,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
         const Numbers n(p);
         if (threadIdx.x == 0) put_numbers(a, r, token, given, n);
         if constexpr (kTop) {
-            __shared__ Alternatives found;
+            __shared__ Alternatives<kThreads> found;
             find_alternatives(row, 0, a.k, largest, first, found);
             ranked(a.k, found, [&](uint32_t i, uint64_t e) { put_alternative(a, r, i, e, n.m, n.log2s); });
         }
@@ -412,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
 // A row from its parts.
 template <class T>
 __global__ __launch_bounds__(256) void k_join(Args a) {
-    __shared__ Alternatives s;
+    __shared__ Alternatives<256> s;
     // all that is read is asked for at once: a part's sums and last entry by a lane each
     static_assert(kMostParts == 16 && kMostParts * kMostTop <= 512 && 512 <= kList);
     const uint32_t r = blockIdx.x, all = a.parts * a.k, part = threadIdx.x % 16;
@@ -482,6 +486,13 @@ Args args(const fhe_ssm_token_logprobs& a, const void* logits, const int64_t* to
     k.stride = a.row_stride, k.grad_stride = a.gradient_stride;
     return k;
 }
+// Rows that a wave reads at once, or where there are many at twice, are a wave's.  (10,000 bf16 rows of 288 with their gradient take
+// 21 us, with 256 threads a row 58, of 4,000 40 and 61; of 4,000 with 8 alternatives 31 and 50, but 100 such rows with 16 of them
+// 13 and 11.)
+template <class T>
+bool short_row(const Args& k) {
+    return k.vocab <= (k.rows > 1024 ? 2 : 1) * kFlight * 64 * (16 / sizeof(T));
+}
 // Parts of a row: where rows leave CUs without work, of 4,096 logits at least, two workgroups a CU.  (32 float32 rows of 65,536
 // with 20 alternatives take 21 us whole and 13 in parts, 300 bf16 rows of 131,072 with 32 of them 42 and 35.)
 void cut(Args& k) {
@@ -548,6 +559,7 @@ int fhe_ssm_token_logprobs_forward(const fhe_ssm_token_logprobs* a, const void* 
         };
         const std::true_type yes;
         const std::false_type no;
+        const std::integral_constant<int, 64> wave;
         const std::integral_constant<int, 256> few;
         const std::integral_constant<int, 1024> many;
         if (k.parts > 1) {
@@ -556,7 +568,12 @@ int fhe_ssm_token_logprobs_forward(const fhe_ssm_token_logprobs* a, const void* 
             if (int rc = launched("token log-probabilities: join")) return rc;
             return k.grad ? run_gradient<T, 256>(k, st) : (int)CKKS_OK;
         }
-        if (k.k) return k.grad ? run(few, yes, yes, no) : run(few, yes, no, no);
+        if (k.k) {
+            // a wave has half as many strips as threads: with 32 alternatives all of them would be read again
+            if (short_row<T>(k) && k.k <= kShortTop) return k.grad ? run(wave, yes, yes, no) : run(wave, yes, no, no);
+            return k.grad ? run(few, yes, yes, no) : run(few, yes, no, no);
+        }
+        if (short_row<T>(k)) return k.grad ? run(wave, no, yes, no) : run(wave, no, no, no);
         // A long row has a whole CU's threads, so that what lies between its two readings stays in the caches: 4,096 rows of
         // 65,536 in bf16 take 236 us with their gradient, with 256 threads a row 288.
         if (k.vocab > kWide) return k.grad ? run(many, no, yes, no) : run(many, no, no, no);
@@ -576,7 +593,10 @@ int fhe_ssm_token_logprobs_gradient(const fhe_ssm_token_logprobs* a, const void*
     Args k = args(*a, logits, tokens);
     k.stats = (float*)statistics, k.entropy = (float*)entropy, k.weights = weights, k.entropy_weights = entropy_weights, k.grad = gradient;
     cut(k);
-    return by_type(a->type, [&](auto t) { return run_gradient<decltype(t), 256>(k, (hipStream_t)stream); });
+    return by_type(a->type, [&](auto t) {
+        typedef decltype(t) T;
+        return short_row<T>(k) ? run_gradient<T, 64>(k, (hipStream_t)stream) : run_gradient<T, 256>(k, (hipStream_t)stream);
+    });
 }
 
 }  // extern "C"

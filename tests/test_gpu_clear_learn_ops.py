@@ -760,6 +760,26 @@ def test_score_alternatives_are_scored_like_given_tokens(rows, kind):
         assert torch.equal(logprobs, top_logprobs[:, j])
 
 
+@pytest.mark.parametrize("vocab, rows", [(1024, 30), (1025, 30), (2048, 30), (2049, 30), (2048, 1100), (4096, 1100), (4097, 1025), (97, 1100)])
+@pytest.mark.parametrize("kind", [torch.float32, torch.float16])
+@pytest.mark.parametrize("k", [0, 16, 17])
+def test_score_short_rows(vocab, rows, kind, k):
+    """around what a wave takes by itself"""
+    check_score(*score_case(rows, vocab, kind, vocab), k)
+
+
+@pytest.mark.parametrize("vocab", [300, 2000])
+def test_score_short_rows_of_logits_that_lie_together(vocab):
+    """more entries at the bound than the list holds, and equal ones"""
+    logits = torch.full((1200, vocab), 2.0, dtype=torch.bfloat16, device="cuda")
+    logits[::3, 5::2] = 2.015625
+    logits[1::3, -1] = 3
+    tokens = torch.arange(1200, device="cuda") % vocab
+    top = score(logits, tokens, 4)[3]
+    want = torch.sort(logits.double(), dim=-1, descending=True, stable=True).indices[:, :4]
+    assert torch.equal(top, want)
+
+
 def test_score_without_tokens():
     logits, _, _, u = score_case(7, 900, torch.float32, 1)
     got, want = score(logits, None, 4), score(logits, torch.zeros(7, dtype=torch.int64, device="cuda"), 4)
