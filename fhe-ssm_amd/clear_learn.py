@@ -30,6 +30,9 @@ class Learner:
     """the model, its optimizer, and between steps of one token the lanes' states (reset makes them)"""
 
     ROWS = 8192  # whose logits are held at once
+    # What a position counts on its way back in float16, whose numbers end at 6e-8 and at 65,504: 1 / 65,536 of it, a token's
+    # probability, keeps all its bits, and 4,096 times as much is in range.  The sums over positions are float32.
+    WEIGHT_16 = 16.0
 
     def __init__(self, layers: int = 2, d: int = M.D, vocab: int = M.VOCAB, seed: int = 7, dtype=torch.bfloat16, bits: int = 32,
                  betas=(0.9, 0.99), weight_decay: float = 0.01):
@@ -114,12 +117,17 @@ class Learner:
         return tuple(t.view(lanes, n, *t.shape[1:]) for t in out)
 
     # -------------------------------------------------------------------------------------------- learning
+    def _sum(self, a, b):
+        """a^T b, a matrix' gradient"""
+        return a.t() @ b if self.dtype != torch.float16 else torch.mm(a.t(), b, out_dtype=torch.float32)
+
     def gradients(self, tokens, lengths=None):
-        """The mean negative log-probability of what follows each position, and its gradients: of the matrices in dtype, of the
-        vectors in float32."""
+        """The mean negative log-probability of what follows each position, and its gradients: of the matrices in dtype, for
+        float16 in float32, of the vectors in float32."""
         kept: list = []
         rows, targets = self._run(tokens, lengths, kept=kept).view(-1, self.d), self._targets(tokens, lengths).reshape(-1)
-        weights = (-1.0 / (targets >= 0).sum().clamp_min(1)).float().expand(len(targets)).contiguous()
+        half, each = self.dtype == torch.float16, 1.0 / (targets >= 0).sum().clamp_min(1)
+        weights = torch.full((len(targets),), -self.WEIGHT_16, device="cuda") if half else (-each).float().expand(len(targets)).contiguous()
         logprobs, drows = torch.empty(len(rows), device="cuda"), torch.empty_like(rows)
         dhead = torch.zeros((self.vocab, self.d), device="cuda")
         for i in range(0, len(rows), self.ROWS):
@@ -128,9 +136,9 @@ class Learner:
             clear_ops.token_logprobs(logits, targets[part], logprobs[part], weights=weights[part], gradient=logits,
                                      workspace=_bytes(clear_ops.token_logprobs_workspace(logits)))
             drows[part] = logits @ self.weights[1]
-            dhead += logits.t() @ rows[part]
+            dhead += self._sum(logits, rows[part])
         dmatrices, dvectors = [None] * len(self.matrices), [None] * len(self.vectors)
-        dmatrices[1] = dhead.to(self.dtype)
+        dmatrices[1] = dhead if half else dhead.to(self.dtype)
 
         def through_norm(dy, j):
             x, w, mean, rstd = kept.pop()
@@ -143,7 +151,7 @@ class Learner:
         for i, (w_in, w_out, *_) in reversed(list(enumerate(self._layers()))):
             n, z, v, s, h, u, saved = kept.pop()
             du = (dx @ w_out).float().view(s.shape)
-            dmatrices[2 * i + 3] = dx.t() @ u.view(-1, self.d)
+            dmatrices[2 * i + 3] = self._sum(dx, u.view(-1, self.d))
             gate = torch.sigmoid(s.float())
             dh = (du * s.float() * gate).to(self.dtype)
             dzvs = torch.empty((*z.shape[:-1], 3 * self.d), dtype=self.dtype, device="cuda")
@@ -153,15 +161,18 @@ class Learner:
             ds.copy_(du * h.float() * gate * (1 + s.float() * (1 - gate)))
             dvectors[3 * i + 4] = dz.float().sum((0, 1))
             dzvs = dzvs.view(-1, 3 * self.d)
-            dmatrices[2 * i + 2] = dzvs.t() @ n.view(-1, self.d)
+            dmatrices[2 * i + 2] = self._sum(dzvs, n.view(-1, self.d))
             dx = dx + through_norm(dzvs @ w_in, 3 * i + 2)
         flat = tokens.contiguous().view(-1)
         if lengths is not None:  # what lies past a lane's length is no token
             there = torch.arange(tokens.shape[1], device="cuda")[None] < lengths[:, None]
             flat = torch.where(there, tokens, -1).reshape(-1)
-        dmatrices[0] = torch.empty_like(self.weights[0])
+        dmatrices[0] = torch.empty_like(self.matrices[0] if half else self.weights[0])
         clear_ops.embedding_gradient(flat, dx, dmatrices[0], scale=self.scale,
                                      workspace=_bytes(clear_ops.embedding_gradient_workspace(flat, dmatrices[0])))
+        if half:
+            for g in dmatrices + dvectors:
+                g *= each / self.WEIGHT_16
         return -logprobs.sum() / (targets >= 0).sum().clamp_min(1), dmatrices, dvectors
 
     def learn(self, tokens, lengths=None, lr: float = 1e-3):

@@ -1,0 +1,43 @@
+"""GPU tests of the learning and the drafting model (clear_learn.py, clear_draft.py) and of AdamW where calls come to the edge of
+what they take."""
+import pytest
+
+from engine_loader import load_module
+from test_gpu_clear_learn import CLOSE_16, D, LAYERS, in_64, plain_loss
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+# float16 has three bits more than bfloat16, whose bound is CLOSE_16
+CLOSE_F16 = CLOSE_16 / 8
+
+
+def float16_gradients(tokens, lengths=None):
+    """loss and gradients of a float16 model of all 65,536 tokens and those of the same model in 64 bits"""
+    model = load_module("clear_learn").Learner(layers=LAYERS, d=D, seed=3, dtype=torch.float16)
+    matrices, vectors = in_64(model)
+    full = torch.full((len(tokens),), tokens.shape[1], device="cuda") if lengths is None else lengths
+    want = plain_loss(matrices, vectors, tokens, full)
+    grads = torch.autograd.grad(want, matrices + vectors)
+    loss, dmatrices, dvectors = model.gradients(tokens, lengths)
+    assert abs(loss.item() - want.item()) <= CLOSE_F16 * want.item()
+    return dmatrices + dvectors, grads
+
+
+@pytest.mark.parametrize("lengths", [None, "ragged"])
+def test_gradients_in_float16_of_many_positions(lengths):
+    """a position's weight times a token's probability is 1 / (4,096 65,536) = 4e-9, float16's smallest number 6e-8"""
+    tokens = torch.randint(0, 65536, (64, 65), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    if lengths is not None:
+        lengths = (torch.arange(64, device="cuda") + 2).int()
+    got, want = float16_gradients(tokens, lengths)
+    for i, (g, w) in enumerate(zip(got, want)):
+        assert (g.double() - w).norm() <= CLOSE_F16 * w.norm(), i
+    assert got[1].any(1).all()  # every row of the head learns
+
+
+def test_gradients_in_float16_of_one_token_all_along():
+    """8,192 positions whose gradients add up"""
+    got, want = float16_gradients(torch.full((64, 129), 77, device="cuda"))
+    for i, (g, w) in enumerate(zip(got, want)):
+        assert torch.isfinite(g).all() and (g.double() - w).norm() <= CLOSE_F16 * w.norm() + 1e-12, i
