@@ -102,8 +102,8 @@ class Learner:
 
     # -------------------------------------------------------------------------------------------- scoring
     def score(self, tokens, lengths=None, top: int = 0):
-        """Of tokens [lanes, n] the log-probabilities and entropies [lanes, n] of what follows each position (0 where nothing
-        does), with `top` the likeliest tokens and their log-probabilities [lanes, n, top] too."""
+        """Of tokens [lanes, n] the log-probabilities and entropies [lanes, n] of what follows each position (0 where no token of the
+        vocabulary does), with `top` the likeliest tokens and their log-probabilities [lanes, n, top] too, of every position."""
         lanes, n = tokens.shape
         rows, targets = self._run(tokens, lengths).view(-1, self.d), self._targets(tokens, lengths).reshape(-1)
         out = [torch.empty(len(rows), device="cuda") for _ in range(2)]
@@ -114,6 +114,7 @@ class Learner:
             logprobs, entropy, *likeliest = (t[i:i + self.ROWS] for t in out)
             clear_ops.token_logprobs(logits, targets[i:i + self.ROWS], logprobs, entropy, None, *likeliest,
                                      workspace=_bytes(clear_ops.token_logprobs_workspace(logits, top)))
+        out[1].masked_fill_(targets < 0, 0.0)  # the operator gives every row's
         return tuple(t.view(lanes, n, *t.shape[1:]) for t in out)
 
     # -------------------------------------------------------------------------------------------- learning

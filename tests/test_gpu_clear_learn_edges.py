@@ -3,7 +3,7 @@ what they take."""
 import pytest
 
 from engine_loader import load_module
-from test_gpu_clear_learn import CLOSE_16, D, LAYERS, in_64, plain_loss
+from test_gpu_clear_learn import CLOSE_16, D, LAYERS, in_64, learner, plain_loss, texts
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -41,3 +41,14 @@ def test_gradients_in_float16_of_one_token_all_along():
     got, want = float16_gradients(torch.full((64, 129), 77, device="cuda"))
     for i, (g, w) in enumerate(zip(got, want)):
         assert torch.isfinite(g).all() and (g.double() - w).norm() <= CLOSE_F16 * w.norm() + 1e-12, i
+
+
+def test_scores_where_nothing_follows_are_zeros():
+    model, tokens = learner(), texts(4, 30)
+    tokens[0, 9] = -5  # no token follows position 8, nor the last of a text
+    lengths = torch.tensor([30, 1, 0, 12], dtype=torch.int32, device="cuda")
+    logprobs, entropy = model.score(tokens, lengths)
+    nothing = torch.arange(1, 31, device="cuda")[None] >= lengths[:, None]
+    nothing[0, 8] = True
+    assert (logprobs[nothing] == 0).all() and (entropy[nothing] == 0).all()
+    assert (logprobs[~nothing] < 0).all() and (entropy[~nothing] > 0).all()
