@@ -192,10 +192,13 @@ class Learner:
         return hidden @ self.weights[1].t()
 
     def prompt(self, tokens, lengths=None):
-        """tokens [lanes, n], of lane b the first lengths[b]: the logits after each lane's last token; the states are carried on"""
+        """tokens [lanes, n], of lane b the first lengths[b]: the logits after each lane's last token, zeros for a lane that has none;
+        the states are carried on"""
         if len(self.states) != len(self._layers()):
             raise clear_ops.ClearError("reset(lanes) makes the states that prompt and step carry on")
         hidden, n = self._run(tokens, lengths, states=self.states), tokens.shape[1]
+        if n == 0:
+            return self._logits(hidden.new_zeros((len(hidden), self.d)))
         last = torch.full((len(tokens),), n, device="cuda") if lengths is None else lengths.long().clamp(0, n)
         rows = hidden[torch.arange(len(tokens), device="cuda"), (last - 1).clamp_min(0)]
         return self._logits(torch.where((last > 0)[:, None], rows, 0.0))

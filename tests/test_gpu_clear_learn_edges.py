@@ -52,3 +52,16 @@ def test_scores_where_nothing_follows_are_zeros():
     nothing[0, 8] = True
     assert (logprobs[nothing] == 0).all() and (entropy[nothing] == 0).all()
     assert (logprobs[~nothing] < 0).all() and (entropy[~nothing] > 0).all()
+
+
+@pytest.mark.parametrize("lengths", [None, (0, 3)])
+def test_a_prompt_of_no_tokens_gives_the_logits_of_rows_of_zeros(lengths):
+    """as one whose lengths are 0 does, and leaves the states"""
+    model = learner()
+    model.reset(2)
+    for s in model.states:
+        s.fill_(0.5)
+    lengths = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    logits = model.prompt(texts(2, 0), lengths)
+    assert logits.shape == (2, 700) and not logits.any() and all((s == 0.5).all() for s in model.states)
+    assert model.generate(texts(2, 0), 3, torch.full((3, 2), 0.5, device="cuda")).shape == (2, 3)
