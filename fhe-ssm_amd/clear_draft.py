@@ -57,8 +57,11 @@ class Draft:
         self.log_decay = -torch.exp2(-torch.linspace(3, 8, heads, device="cuda"))  # one for each head, at every token
         self.states: list = []
 
+    def _zeros(self, lanes: int) -> list:
+        return [torch.zeros((lanes, self.heads, self.hs, self.hs), device="cuda") for _ in self.w_in]
+
     def reset(self, lanes: int) -> None:
-        self.states = [torch.zeros((lanes, self.heads, self.hs, self.hs), device="cuda") for _ in self.w_in]
+        self.states = self._zeros(lanes)
 
     def _product(self, m, x):
         rows = x.reshape(-1, x.shape[-1])
@@ -70,12 +73,12 @@ class Draft:
         f = x.float()
         return (f * torch.rsqrt(f.square().mean(-1, keepdim=True) + 1e-5)).to(self.dtype)
 
-    def _run(self, tokens, lengths):
+    def _run(self, tokens, lengths, states):
         """tokens [lanes, n] or, for one step, [lanes]: hidden rows of the same shape, the states carried on"""
-        if len(self.states) != len(self.w_in):
+        if len(states) != len(self.w_in):
             raise clear_ops.ClearError("reset(lanes) makes the states that prompt and step carry on")
         x = self.embedding[tokens].float()
-        for w_in, w_out, state in zip(self.w_in, self.w_out, self.states):
+        for w_in, w_out, state in zip(self.w_in, self.w_out, states):
             q, k, v, gate = self._product(w_in, self._norm(x)).unflatten(-1, (4, self.heads, self.hs)).unbind(-3)
             o = torch.empty(v.shape, dtype=self.dtype, device="cuda")
             if tokens.dim() == 1:
@@ -92,7 +95,7 @@ class Draft:
     def prompt(self, tokens, lengths=None):
         """tokens [lanes, n], of lane b the first lengths[b] (int32, held to [0, n]): the hidden rows after each lane's last
         token, zeros for a lane that has none"""
-        h = self._run(tokens, lengths)
+        h = self._run(tokens, lengths, self.states)
         if h.shape[1] == 0:
             return h.new_zeros((len(h), h.shape[2]))
         if lengths is None:
@@ -103,20 +106,17 @@ class Draft:
 
     def step(self, tokens):
         """one token [lanes] for every lane: the hidden rows after it"""
-        return self._run(tokens, None)
+        return self._run(tokens, None, self.states)
 
     def score(self, tokens, lengths=None, top: int = 0):
         """What the model makes of texts tokens [lanes, n], of lane b the first lengths[b]: the log-probability of every token after
         those before it and the entropy there, [lanes, n - 1] (log-probabilities past a length, and of tokens outside the
         vocabulary, are 0), with `top` the likeliest tokens and their log-probabilities [lanes, n - 1, top] too.  Lanes' states
-        are what they were."""
-        states, (lanes, n) = self.states, (len(tokens), max(1, tokens.shape[1]))
-        self.reset(lanes)
-        try:  # padding may be of any value, and no row outside the table is read for it
-            hidden = self._run(tokens[:, :-1].clamp(0, len(self.embedding) - 1),
-                               None if lengths is None else (lengths - 1).clamp(min=0))
-        finally:
-            self.states = states
+        are left alone: a score may run beside steps."""
+        lanes, n = len(tokens), max(1, tokens.shape[1])
+        # padding may be of any value, and no row outside the table is read for it
+        hidden = self._run(tokens[:, :-1].clamp(0, len(self.embedding) - 1),
+                           None if lengths is None else (lengths - 1).clamp(min=0), self._zeros(lanes))
         rows, next_tokens = hidden.flatten(0, 1), tokens[:, 1:]
         if lengths is not None:
             next_tokens = torch.where(torch.arange(1, n, device=tokens.device)[None] < lengths[:, None], next_tokens, -1)

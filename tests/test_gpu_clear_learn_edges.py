@@ -65,3 +65,24 @@ def test_a_prompt_of_no_tokens_gives_the_logits_of_rows_of_zeros(lengths):
     logits = model.prompt(texts(2, 0), lengths)
     assert logits.shape == (2, 700) and not logits.any() and all((s == 0.5).all() for s in model.states)
     assert model.generate(texts(2, 0), 3, torch.full((3, 2), 0.5, device="cuda")).shape == (2, 3)
+
+
+def draft():
+    from test_gpu_clear_draft import D as d, HEADS, LAYERS as layers, VOCAB as vocab
+    return load_module("clear_draft").Draft(layers=layers, d=d, heads=HEADS, vocab=vocab, seed=3, dtype=torch.float32), vocab
+
+
+def test_a_score_leaves_the_drafting_models_states_alone_while_it_runs(monkeypatch):
+    """another thread's step meets its own lanes"""
+    model, vocab = draft()
+    model.reset(2)
+    states, ops, calls = model.states, load_module("clear_draft").clear_ops, []
+    prompt = ops.linear_attention_prompt
+
+    def during(*args, **more):
+        calls.append(model.states is states)
+        return prompt(*args, **more)
+
+    monkeypatch.setattr(ops, "linear_attention_prompt", during)
+    model.score(texts(3, 9) % vocab)
+    assert len(calls) == len(states) and all(calls)
