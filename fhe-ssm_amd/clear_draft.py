@@ -73,11 +73,12 @@ class Draft:
         f = x.float()
         return (f * torch.rsqrt(f.square().mean(-1, keepdim=True) + 1e-5)).to(self.dtype)
 
-    def _run(self, tokens, lengths, states):
-        """tokens [lanes, n] or, for one step, [lanes]: hidden rows of the same shape, the states carried on"""
+    def _run(self, tokens, lengths, states, x=None):
+        """tokens [lanes, n] or, for one step, [lanes]: hidden rows of the same shape, the states carried on; x: the tokens' rows,
+        where they are known"""
         if len(states) != len(self.w_in):
             raise clear_ops.ClearError("reset(lanes) makes the states that prompt and step carry on")
-        x = self.embedding[tokens].float()
+        x = self.embedding[tokens].float() if x is None else x
         for w_in, w_out, state in zip(self.w_in, self.w_out, states):
             q, k, v, gate = self._product(w_in, self._norm(x)).unflatten(-1, (4, self.heads, self.hs)).unbind(-3)
             o = torch.empty(v.shape, dtype=self.dtype, device="cuda")
@@ -111,12 +112,14 @@ class Draft:
     def score(self, tokens, lengths=None, top: int = 0):
         """What the model makes of texts tokens [lanes, n], of lane b the first lengths[b]: the log-probability of every token after
         those before it and the entropy there, [lanes, n - 1] (log-probabilities past a length, and of tokens outside the
-        vocabulary, are 0), with `top` the likeliest tokens and their log-probabilities [lanes, n - 1, top] too.  Lanes' states
-        are left alone: a score may run beside steps."""
+        vocabulary, are 0; entropies are of every position), with `top` the likeliest tokens and their log-probabilities
+        [lanes, n - 1, top] too.  To what follows it a token outside the vocabulary is a row of zeros.  Lanes' states are left
+        alone: a score may run beside steps."""
         lanes, n = len(tokens), max(1, tokens.shape[1])
-        # padding may be of any value, and no row outside the table is read for it
-        hidden = self._run(tokens[:, :-1].clamp(0, len(self.embedding) - 1),
-                           None if lengths is None else (lengths - 1).clamp(min=0), self._zeros(lanes))
+        before = tokens[:, :-1].contiguous()
+        x = torch.empty((*before.shape, self.d), device="cuda")
+        clear_ops.embedding(before.view(-1), self.embedding, x.view(-1, self.d))
+        hidden = self._run(before, None if lengths is None else (lengths - 1).clamp(min=0), self._zeros(lanes), x)
         rows, next_tokens = hidden.flatten(0, 1), tokens[:, 1:]
         if lengths is not None:
             next_tokens = torch.where(torch.arange(1, n, device=tokens.device)[None] < lengths[:, None], next_tokens, -1)

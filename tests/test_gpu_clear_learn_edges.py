@@ -86,3 +86,19 @@ def test_a_score_leaves_the_drafting_models_states_alone_while_it_runs(monkeypat
     monkeypatch.setattr(ops, "linear_attention_prompt", during)
     model.score(texts(3, 9) % vocab)
     assert len(calls) == len(states) and all(calls)
+
+
+def test_a_token_outside_the_vocabulary_is_a_row_of_zeros_to_the_drafting_models_scores():
+    """whichever it is; it takes no other token's place"""
+    model, vocab = draft()
+    tokens = texts(1, 12) % vocab
+    scores = []
+    for outside in (-1, vocab, 1 << 40, -(1 << 40)):
+        tokens[0, 5] = outside
+        logprobs, entropy = model.score(tokens)
+        assert logprobs[0, 4].item() == 0 and torch.isfinite(logprobs).all()
+        scores.append((logprobs, entropy))
+    assert all(torch.equal(a, b) for s in scores[1:] for a, b in zip(s, scores[0]))
+    model.embedding = torch.cat((model.embedding, torch.zeros_like(model.embedding[:1])))  # the last token's row
+    tokens[0, 5] = vocab
+    assert torch.equal(model.score(tokens)[1], scores[0][1])
