@@ -203,6 +203,7 @@ __global__ __launch_bounds__(256) void k_adamw(Args a) {
     }
     const Tensor& t = a.tensors[low];
     Step s;
+    if (a.step_at && *a.step_at < 1) return;  // 1 - b^0 is 0, and every parameter would be NaN
     const uint32_t step = a.step_at ? (uint32_t)*a.step_at : a.step;
     s.lr = a.lr_at ? *a.lr_at : a.lr;
     s.scale = a.scale_at ? *a.scale_at : 1.f;

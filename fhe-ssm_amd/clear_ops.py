@@ -780,7 +780,8 @@ class AdamW:
     def step(self, gradients, lr, step, seed: int = 0, scale=None, stream=None) -> None:
         """One step with the gradients, contiguous tensors of one type like the parameters.  lr: a number or a float32 tensor of
         one; step, from 1: a number or an int32 tensor of one; scale: a float32 tensor of one that the gradients are multiplied
-        by, or None.  Tensors are read when the step runs, so that a recorded one follows them.  seed goes, with the step, into
+        by, or None.  Tensors are read when the step runs, so that a recorded one follows them; one of a step below 1 leaves all as
+        it is.  seed goes, with the step, into
         how 8-bit states are rounded."""
         _need(len(gradients) == len(self.params), f"{len(self.params)} gradients are needed")
         kind, at = gradients[0].dtype, self.params[0].get_device()

@@ -102,3 +102,21 @@ def test_a_token_outside_the_vocabulary_is_a_row_of_zeros_to_the_drafting_models
     model.embedding = torch.cat((model.embedding, torch.zeros_like(model.embedding[:1])))  # the last token's row
     tokens[0, 5] = vocab
     assert torch.equal(model.score(tokens)[1], scores[0][1])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("before", [0, -1, -(1 << 31)])
+def test_adamw_of_a_step_on_the_device_before_the_first_changes_nothing(bits, before):
+    c = load_module("clear_ops")
+    gen = torch.Generator(device="cuda").manual_seed(bits)
+    p, g = torch.randn(5000, generator=gen, device="cuda"), torch.randn(5000, generator=gen, device="cuda")
+    copy = torch.full((5000,), 7.0, device="cuda").bfloat16()
+    opt = c.AdamW([p], bits=bits, copies=[copy])
+    opt.step([g], lr=0.1, step=1)
+    kept = [t.clone().view(torch.uint8) for t in (p, copy, *(s[0] for s in opt.states))]
+    step = torch.tensor([before], dtype=torch.int32, device="cuda")
+    opt.step([g], lr=0.1, step=step)
+    assert all(torch.equal(t.view(torch.uint8), k) for t, k in zip((p, copy, *(s[0] for s in opt.states)), kept))
+    step.fill_(2)
+    opt.step([g], lr=0.1, step=step)
+    assert torch.isfinite(p).all() and not torch.equal(p.view(torch.uint8), kept[0])
