@@ -718,7 +718,8 @@ class AdamW:
     params: contiguous float32 tensors, updated in place.  weight_decay: one for all, or one for each.  copies: bfloat16 or
     float16 tensors (one type) that receive the parameters after every step, or None.  bits: 32 for states in float32, 8 for
     states in 8-bit floats with a power of two for each 256 entries: m and the root of v as float8_e4m3fn, and the powers.
-    states: (m, v) or (m, root, powers), lists of tensors like params (powers uint8 [blocks, 2]); None begins with zeros."""
+    states: (m, v) or (m, root, powers), lists of tensors like params (powers uint8 [blocks, 2]); None begins with zeros.  No two of
+    all these tensors may share memory."""
 
     BLOCK = 256
 
@@ -755,6 +756,9 @@ class AdamW:
             for p, t in zip(self.params, self.copies):
                 _need(t.device == p.device and t.shape == p.shape and t.dtype == self.copies[0].dtype and t.is_contiguous(),
                       "copies must be contiguous bfloat16 or float16 like their parameters")
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                       for ts in (self.params, *self.states, self.copies or ()) for t in ts if t.numel())
+        _need(all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), "parameters, states or copies share memory")
         self._sizes = AdamWSizes(F32, copy_type, bits, 0, 0, 0.0, eps, *betas)
         self._tensors = (AdamWTensor * n)()
         for i, (t, p) in enumerate(zip(self._tensors, self.params)):

@@ -250,7 +250,7 @@ int fhe_ssm_token_logprobs_gradient(const fhe_ssm_token_logprobs* a, const void*
  * states are rounded at random, by (seed, step, the tensor's place, the entry): equal calls give equal results.
  * lr_at, step_at and scale_at, where they are not null, are read on the device in place of lr, step and 1, so that a recorded
  * step follows them; a step there that is below 1 changes nothing.  Tensors of no entries are passed over; one has less than
- * 2^32.  eps >= 1e-30. */
+ * 2^32.  What is written (parameters, states, powers, copies) must not overlap.  eps >= 1e-30. */
 typedef struct {
     uint32_t gradient_type, copy_type; /* copies are bf16 or f16 */
     uint32_t state_bits;               /* 32 or 8 */

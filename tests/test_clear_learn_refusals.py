@@ -301,3 +301,25 @@ def test_calls_go_to_the_current_stream_or_the_one_they_are_given(library, strea
     library.token_logprobs_gradient(x, ids, z(4, 2), v, x, **stream)
     library.AdamW([x]).step([x], lr=0.1, step=1, **stream)
     assert library._lib.streams == [stream.get("stream", CURRENT)] * 10
+
+
+def test_adamw_refuses_tensors_that_share_memory(library):
+    """a parameter twice, parts of one another, states or copies of two parameters: what one entry's thread writes another reads"""
+    z = lambda *s, dtype=torch.float32: on_gpu(torch.zeros(s, dtype=dtype))  # noqa: E731
+    a, b, half, flat = z(8), z(8), z(8, dtype=torch.bfloat16), torch.zeros(20)
+    bad = [
+        lambda: library.AdamW([a, a]), lambda: library.AdamW([a, b, a], bits=8),
+        lambda: library.AdamW([on_gpu(flat[:8]), on_gpu(flat[7:15])]), lambda: library.AdamW([on_gpu(flat), on_gpu(flat[:1])]),
+        lambda: library.AdamW([a], states=([b], [b])), lambda: library.AdamW([a], states=([a], [b])),
+        lambda: library.AdamW([a, b], states=([z(8)] * 2, [z(8), z(8)])), lambda: library.AdamW([a, b], copies=[half, half]),
+        lambda: library.AdamW([a], copies=[on_gpu(a.view(torch.bfloat16)[:8])]),
+    ]
+    for i, call in enumerate(bad):
+        try:
+            call()
+        except library.ClearError as e:
+            assert "share memory" in str(e), i
+            continue
+        raise AssertionError(f"call {i} is not refused")
+    library.AdamW([on_gpu(flat[:8]), on_gpu(flat[8:15]), on_gpu(flat[3:3])], bits=8, copies=[half, z(7, dtype=torch.bfloat16), half[:0]])
+    library.AdamW([a]).step([a], lr=0.1, step=1)  # a gradient is only read, each entry by the thread that writes it
