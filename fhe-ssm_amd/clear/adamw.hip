@@ -108,6 +108,13 @@ __device__ inline void write_copy(const Tensor& t, uint32_t type, uint32_t at, c
     else store<V>((f16*)t.copy + at, p);
 }
 
+// The root of an average of squares; the instruction takes numbers below the normal ones for 0, and eps may be smaller.
+__device__ inline float root_of(float v) {
+    const bool low = v < 0x1p-126f;
+    const float root = __builtin_amdgcn_sqrtf(low ? v * 0x1p64f : v);
+    return low ? root * 0x1p-32f : root;
+}
+
 // V entries of a thread, in 32 bits
 template <class G, int V>
 __device__ inline void update(const Args& a, const Tensor& t, const Step& s, uint32_t at) {
@@ -120,7 +127,7 @@ __device__ inline void update(const Args& a, const Tensor& t, const Step& s, uin
     for (int c = 0; c < V; c++) {
         const Moments x = moments(a, m[c], v[c], g[c] * s.scale);
         m[c] = x.m, v[c] = x.v;
-        p[c] = moved(a, s, p[c], x.m, __builtin_amdgcn_sqrtf(x.v), t.decay);
+        p[c] = moved(a, s, p[c], x.m, root_of(x.v), t.decay);
     }
     store<V>(t.p + at, p);
     store<V>((float*)t.m + at, m);

@@ -120,3 +120,16 @@ def test_adamw_of_a_step_on_the_device_before_the_first_changes_nothing(bits, be
     step.fill_(2)
     opt.step([g], lr=0.1, step=step)
     assert torch.isfinite(p).all() and not torch.equal(p.view(torch.uint8), kept[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("g", [1e-15, 1e-18, 3e-19, 1e-19, 3e-20])
+def test_adamw_of_gradients_whose_squares_are_below_the_normal_numbers(bits, g):
+    """beside an eps that is smaller still: the first step moves by lr.  The square and v lie on steps of 2^-149 there, which is
+    half of that over v in the root, and the rest is 40 2^-24 as for other gradients"""
+    p = torch.zeros(1029, device="cuda")
+    grad = torch.full((1029,), g, device="cuda")
+    opt = load_module("clear_ops").AdamW([p], betas=(0.9, 0.99), eps=1e-30, weight_decay=0.0, bits=bits)
+    opt.step([grad], lr=1.0, step=1)
+    off = 40 * 2.0**-24 + 0.5 * 1.01 * 2.0**-150 / (0.01 * g * g)
+    assert ((p + 1).abs() <= off).all()
