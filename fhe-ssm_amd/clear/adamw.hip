@@ -13,7 +13,9 @@
 // brings the largest of them into [128, 256).  2^17 below it a magnitude ends.  They are rounded up or down at random, in
 // proportion to what is cut off: with b2 near 1 an average that is rounded to nearest would never move.  The random bits are a
 // mix of (seed, step, tensor, entry): the same call gives the same result.  An r above 0 is kept above 0, so that m / r stays
-// bounded.  A block with a value that is not finite is NaN from then on (its power is 255), as it would be in float32.
+// bounded.  A block with a moment that is not finite is NaN from then on (its power is 255), all 256 entries of it; in float32 only
+// the entry is lost.  A finite gradient above 1.8e19 has such a moment too, as its square overflows: in float32 its v is infinite
+// and the entry does not move any more, in 8 bits, which have no infinity, its block is NaN.
 #include <algorithm>
 #include <cmath>
 

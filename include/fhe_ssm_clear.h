@@ -247,7 +247,9 @@ int fhe_ssm_token_logprobs_gradient(const fhe_ssm_token_logprobs* a, const void*
  * With state_bits 32, first and second are m and v in float32.  With 8 they are m and sqrt(v) as 8-bit floats (a sign, 4 bits
  * of exponent with bias 7, 3 of mantissa), in blocks of 256 entries from the tensor's beginning; powers[block] has the powers of
  * two behind the codes of m and of the root, as their exponent plus 134, 255 for NaN.  Zeros are the beginning of all.  8-bit
- * states are rounded at random, by (seed, step, the tensor's place, the entry): equal calls give equal results.
+ * states are rounded at random, by (seed, step, the tensor's place, the entry): equal calls give equal results.  A moment that
+ * is not finite loses its entry, with 8 bits its block, whose parameters are NaN from the next step on.  A finite gradient whose
+ * square overflows, above 1.8e19, stops its entry (v is infinite), with 8 bits it loses the block.
  * lr_at, step_at and scale_at, where they are not null, are read on the device in place of lr, step and 1, so that a recorded
  * step follows them; a step there that is below 1 changes nothing.  Tensors of no entries are passed over; one has less than
  * 2^32.  What is written (parameters, states, powers, copies) must not overlap.  eps >= 1e-30. */

@@ -133,3 +133,26 @@ def test_adamw_of_gradients_whose_squares_are_below_the_normal_numbers(bits, g):
     opt.step([grad], lr=1.0, step=1)
     off = 40 * 2.0**-24 + 0.5 * 1.01 * 2.0**-150 / (0.01 * g * g)
     assert ((p + 1).abs() <= off).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_a_gradient_whose_square_overflows(bits):
+    """in 32 bits its v is infinite and its entry stays where it is from then on, in 8 its block of 256 is lost"""
+    c = load_module("clear_ops")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    first, second = torch.randn(2000, generator=gen, device="cuda"), torch.randn(2000, generator=gen, device="cuda")
+    large = first.clone()
+    large[700] = 1e20
+    clean, p = torch.zeros(2000, device="cuda"), torch.zeros(2000, device="cuda")
+    for param, gradients in ((clean, (first, second)), (p, (large, second))):
+        opt = c.AdamW([param], bits=bits)
+        for i, g in enumerate(gradients):
+            opt.step([g], lr=0.01, step=i + 1)
+    hit = torch.zeros(2000, dtype=torch.bool, device="cuda")
+    if bits == 32:
+        hit[700] = True
+        assert p[700].item() == 0
+    else:
+        hit[512:768] = True
+        assert torch.isnan(p[hit]).all()
+    assert torch.equal(p[~hit], clean[~hit])
