@@ -2,10 +2,12 @@
 //
 //   out_t = s E[id_t],    dE[v] = s sum over t with id_t = v of dy_t
 //
-// The gradient adds rows in the order of their positions, whatever runs when: the positions are sorted by token (stable, so
-// that equal tokens keep their order), and a wave takes each token's run.  A frequent token's run would keep one wave for long:
-// where kPiece sorted positions that begin at a multiple of kPiece are of one token, a wave of their own has added them before,
-// and the run's wave takes the sums.  Both read whole rows and are bound by their bytes.  Rows of the table that no token names
+// The gradient adds a token's rows in an order that its tokens alone decide, whatever runs when: the positions are sorted by token
+// (stable, so that equal tokens keep their order), and a wave takes each token's run.  A frequent token's run would keep one wave
+// for long: where kPiece sorted positions that begin at a multiple of kPiece are of one token, a wave of their own has added them
+// before, and the run's wave takes the sums; of a run of 64 and more four waves add a quarter each.  So a token's sum is the same
+// in every call with the same tokens, but where its run begins among the sorted ones, which other tokens decide, may change its
+// last bits.  Both read whole rows and are bound by their bytes.  Rows of the table that no token names
 // are set to 0 by workgroups that run beside the sort's.
 //
 // 32,768 tokens, one in 16 the most frequent, of 768 channels in bf16 into a table of 65,536 rows in float32: 41 us of sorting

@@ -47,8 +47,9 @@ struct Args {
     int64_t zs[2], xs[2], dys[2], outs[2], dzs[2], dxs[2];
 };
 
-// sigmoid(z) and sigmoid(-z), both to their last bits.  A gate near 1 is 1 less the other, so that of the many that are
-// multiplied each is rounded and no more (a reciprocal is off to one side).
+// sigmoid(z) and sigmoid(-z).  A gate near 1 is 1 less the other, so that of the many that are multiplied each is rounded and no
+// more (a reciprocal is off to one side).  The small one is off by up to (|z| + 4) 2^-24 of itself, as the exponent z log2(e) is
+// rounded before its power is taken; below 2^-126 it is 0.
 __device__ inline void gates(float z, float& a, float& rest) {
     const float e = __builtin_amdgcn_exp2f(1.44269504f * z);
     rest = __builtin_amdgcn_rcpf(1.f + e);

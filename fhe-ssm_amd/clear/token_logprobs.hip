@@ -19,7 +19,8 @@
 // Where the weights of the gradient are known the row is read again at once, from the caches, and the gradient written.
 // Bound by bytes for many rows: 4,096 bf16 rows of 65,536 with their gradient, read twice and written once, take 236 us, 1.07 GB
 // of logits and gradients at 4.5 TB/s (the second reading comes from the caches); about 11 vector instructions a logit, and as many
-// for its gradient.  32 float32 rows with 20 alternatives take 7.1 us and 5.9 for the join.
+// for its gradient.  The gradient by itself, where the weights come later, takes 210 us, 5.1 TB/s.  8,192 rows with 20 alternatives
+// take 236 us, without 190 (5.7 TB/s); 32 float32 rows with 20 of them 7.1 us and 5.9 for the join.
 #include <algorithm>
 
 #include "rows.hpp"

@@ -625,8 +625,8 @@ def embedding_gradient_workspace(tokens, dtable) -> int:
 
 
 def embedding_gradient(tokens, dout, dtable, scale: float = 1.0, accumulate: bool = False, workspace=None, stream=None) -> None:
-    """dtable[v] = scale times the sum of dout[t] over the t with tokens[t] = v, in their order; with `accumulate` added to what
-    is there.  dout [n, channels]; dtable contiguous [vocab, channels], float32 or of dout's type; workspace: a uint8 tensor of
+    """dtable[v] = scale times the sum of dout[t] over the t with tokens[t] = v, the same in equal calls; with `accumulate` added to
+    what is there.  dout [n, channels]; dtable contiguous [vocab, channels], float32 or of dout's type; workspace: a uint8 tensor of
     embedding_gradient_workspace(tokens, dtable) bytes, None where that is 0."""
     key = ("embedding back", scale, _like(tokens), _like(dout), _like(dtable))
     a = _calls.get(key)
@@ -785,8 +785,7 @@ class AdamW:
         """One step with the gradients, contiguous tensors of one type like the parameters.  lr: a number or a float32 tensor of
         one; step, from 1: a number or an int32 tensor of one; scale: a float32 tensor of one that the gradients are multiplied
         by, or None.  Tensors are read when the step runs, so that a recorded one follows them; one of a step below 1 leaves all as
-        it is.  seed goes, with the step, into
-        how 8-bit states are rounded."""
+        it is.  seed goes, with the step, into how 8-bit states are rounded."""
         _need(len(gradients) == len(self.params), f"{len(self.params)} gradients are needed")
         kind, at = gradients[0].dtype, self.params[0].get_device()
         for g, shape in zip(gradients, self._shapes):

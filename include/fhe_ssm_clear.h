@@ -132,7 +132,8 @@ int fhe_ssm_sample(uint32_t type, const void* logits, uint32_t rows, uint32_t vo
  * channels <= 16384, rows < 2^31.  Rows are `type`, their strides in elements; weight and bias have `channels` elements of
  * weight_type, float32 or `type`, and null stands for 1 and 0.  mean and rstd (float32[rows], either may be null) are what the
  * backward pass takes.  out may be x; other overlaps are not allowed.  A row that holds a NaN or an infinity comes out NaN and
- * leaves the others alone; squares of distances from the mean have to sum to less than 2^128. */
+ * leaves the others alone.  Sums are float32: magnitudes of a row, and squares of its distances from the mean, have to sum to less
+ * than 2^128, and with eps 0 squares below 2^-126 are lost. */
 typedef struct {
     uint32_t type, weight_type; /* of x, out, dy and dx; of weight and bias */
     uint32_t rows, channels;
@@ -187,7 +188,7 @@ int fhe_ssm_gated_recurrence_step(const fhe_ssm_gated_recurrence* a, const void*
                                   float* state_out, void* out, void* stream);
 
 /* ---- embedding ----------------------------------------------------------------------------------------------------
- *     out_t = scale table[token_t]        dtable[v] = scale sum of dout_t over the t with token_t = v, in their order
+ *     out_t = scale table[token_t]        dtable[v] = scale sum of dout_t over the t with token_t = v
  * tokens: int64 on the device; one outside [0, vocab) gives a row of zeros and adds to no gradient.  vocab <= 2^18, tokens <=
  * 2^25, channels <= 2^20.  The lookup takes any of the types for either side. */
 typedef struct {
@@ -203,7 +204,8 @@ int fhe_ssm_embedding_lookup(const fhe_ssm_embedding* a, const int64_t* tokens, 
 int fhe_ssm_embedding_workspace(const fhe_ssm_embedding* a, size_t* bytes);
 
 /* All of dtable (float32, or row_type) is written, or with `accumulate` the sums are added to what is there.  Sums are taken in
- * float32 in the tokens' order and rounded once. */
+ * float32, in an order that the tokens decide, and rounded once: equal calls give equal results.  Other tokens among them may
+ * change the last bits of a token's sum. */
 int fhe_ssm_embedding_gradient(const fhe_ssm_embedding* a, const int64_t* tokens, const void* dout, void* dtable,
                                int accumulate, void* workspace, size_t workspace_bytes, void* stream);
 
