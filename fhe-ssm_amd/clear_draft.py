@@ -73,9 +73,10 @@ class Draft:
         f = x.float()
         return (f * torch.rsqrt(f.square().mean(-1, keepdim=True) + 1e-5)).to(self.dtype)
 
-    def _run(self, tokens, lengths, states, x=None):
-        """tokens [lanes, n] or, for one step, [lanes]: hidden rows of the same shape, the states carried on; x: the tokens' rows,
-        where they are known"""
+    def _run(self, tokens, lengths, states=None, x=None):
+        """tokens [lanes, n] or, for one step, [lanes]: hidden rows of the same shape, the states (the lanes' own, unless others are
+        given) carried on; x: the tokens' rows, where they are known"""
+        states = self.states if states is None else states
         if len(states) != len(self.w_in):
             raise clear_ops.ClearError("reset(lanes) makes the states that prompt and step carry on")
         x = self.embedding[tokens].float() if x is None else x
@@ -96,7 +97,7 @@ class Draft:
     def prompt(self, tokens, lengths=None):
         """tokens [lanes, n], of lane b the first lengths[b] (int32, held to [0, n]): the hidden rows after each lane's last
         token, zeros for a lane that has none"""
-        h = self._run(tokens, lengths, self.states)
+        h = self._run(tokens, lengths)
         if h.shape[1] == 0:
             return h.new_zeros((len(h), h.shape[2]))
         if lengths is None:
@@ -107,7 +108,7 @@ class Draft:
 
     def step(self, tokens):
         """one token [lanes] for every lane: the hidden rows after it"""
-        return self._run(tokens, None, self.states)
+        return self._run(tokens, None)
 
     def score(self, tokens, lengths=None, top: int = 0):
         """What the model makes of texts tokens [lanes, n], of lane b the first lengths[b]: the log-probability of every token after
