@@ -43,6 +43,16 @@ def test_gradients_in_float16_of_one_token_all_along():
         assert torch.isfinite(g).all() and (g.double() - w).norm() <= CLOSE_F16 * w.norm() + 1e-12, i
 
 
+@pytest.mark.parametrize("lanes, n", [(3, 0), (0, 5), (3, 1), (1, 2)])
+def test_gradients_in_float16_of_hardly_any_positions(lanes, n):
+    model, tokens = learner(dtype=torch.float16), texts(lanes, n)
+    used = [torch.full_like(w, 7.0) for w in model.matrices for _ in range(4)]
+    del used  # what is not written is not 0
+    loss, dmatrices, dvectors = model.gradients(tokens)
+    assert all(torch.isfinite(g).all() and g.dtype == torch.float32 for g in dmatrices + dvectors)
+    assert n == 2 or loss.item() == 0 and not any(g.any() for g in dmatrices + dvectors)
+
+
 def test_scores_where_nothing_follows_are_zeros():
     model, tokens = learner(), texts(4, 30)
     tokens[0, 9] = -5  # no token follows position 8, nor the last of a text
