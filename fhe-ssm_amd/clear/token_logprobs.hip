@@ -4,9 +4,10 @@
 //   entropy = log S - sum_j p_j (l_j - m);    d(w logprob + u entropy) / d l_j = w ([j = tok] - p_j) - u p_j (log p_j + entropy)
 //
 // Differences from the largest, nowhere of large numbers.  A workgroup takes a row and reads it once: a thread holds a
-// reference that is at most kSlack below its largest logit so far, sum e and sum d e with d = (l - reference) log2(e), e = 2^d;
-// when a vector passes the reference by more, the sums follow it.  Of d only the reference's part is rounded besides d itself,
-// which all its summands share.  The threads' sums join in a fixed order.
+// reference R that is at most kSlack below its largest logit so far, in powers of two and rounded, sum e and sum d e with
+// d = l log2(e) - R, e = 2^d, rounded once; when a vector passes R by more, the sums follow it by the difference of the rounded
+// ones, and in the end by how far R is from the largest.  That may be 32 powers of two for logits near kHuge; from there on only
+// what equals the largest counts.  The threads' sums join in a fixed order.
 //
 // The alternatives: each strip of a row (the vectors of two neighbouring threads) knows its largest logit and the vector where it
 // came first.  The k-th of these in the order of falling logits, then rising index, bounds the k largest from below, and they all
@@ -32,7 +33,9 @@ constexpr uint32_t kMostTop = 32, kMostParts = 16, kList = 1024, kWide = 8192, k
 constexpr uint32_t kEach = 2;  // threads of a strip
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
 constexpr float kSlack = 8.f;    // powers of two
-constexpr float kHuge = 0x1p100f;  // two different floats of this size or more weigh 1 and 0 beside each other
+// Beside a logit of this size or more every other is 32 or more away and weighs nothing, 2^-46; and below it a rounded reference is
+// within 32 powers of two of what it stands for, so that no weight leaves float32's range.
+constexpr float kHuge = 0x1p29f;
 constexpr int kFlight = 4;  // vectors of a thread on their way
 
 struct Args {
@@ -328,6 +331,12 @@ __device__ inline void put_numbers(const Args& a, uint32_t r, int64_t token, flo
     }
 }
 
+// a logit as the reference of others: rounded, and not taken into what is done with it
+__device__ inline float reference_of(float x) {
+#pragma clang fp contract(off)
+    return x * kLog2e;
+}
+
 // kTop: alternatives are asked for; kGrad: the gradient too, at once; kPart: a row's part, for k_join
 template <class T, int kThreads, bool kTop, bool kGrad, bool kPart>
 __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
@@ -353,7 +362,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
                 bool bad = false;
 #pragma unroll
                 for (int c = 0; c < V; c++) bad |= f[i][c] != f[i][c] || f[i][c] == INFINITY;
-                if (m > largest) largest = m, first = j + i, reference = m * kLog2e, sum *= 0.f, along *= 0.f;  // a NaN stays
+                // a NaN stays in the sums; what is smaller weighs nothing from here on, what is larger takes the reference along
+                if (m > largest) largest = m, first = j + i, reference = __builtin_copysignf(INFINITY, m), sum *= 0.f, along *= 0.f;
                 if (m == largest && m > -INFINITY)
 #pragma unroll
                     for (int c = 0; c < V; c++) sum += f[i][c] == m ? 1.f : 0.f;
@@ -362,12 +372,13 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(Args a) {
             }
             if (kTop) first = m > largest ? j + i : first;
             largest = __builtin_fmaxf(largest, m);
-            const float above = __builtin_fmaf(m, kLog2e, -reference);
+            // from one rounded reference to the other, as the summands go by them
+            const float next = reference_of(m), above = next - reference;
             if (__builtin_expect(above > kSlack, 0)) {  // rare after the first vectors, and not to be done beside
                 const float d = __builtin_fminf(above, 1e6f), e = __builtin_amdgcn_exp2f(-d);
                 along = (along - d * sum) * e;
                 sum *= e;
-                reference = m * kLog2e;
+                reference = next;
             }
 #pragma unroll
             for (int c = 0; c < V; c++) {

@@ -91,6 +91,40 @@ def test_score_of_long_rows_with_nan_beside_logits_out_of_all_proportion():
         assert lp[1].item() == 0 and entropy[1].item() == 0 and (grad[1] == 0).all()
 
 
+# ------------------------------------------------------------------------------------------------ large and masked logits
+# by a wave, by 256 threads, in parts or by 1,024 threads
+SHAPES = [(4, 300), (4, 5000), (4, 20011), (600, 300), (600, 5000), (520, 20011)]
+
+
+@pytest.mark.parametrize("rows, vocab", SHAPES)
+@pytest.mark.parametrize("k", [0, 5])
+def test_score_of_logits_masked_by_large_numbers(rows, vocab, k):
+    """before the others, behind them, among them, all of a row and all but one of it"""
+    w, u = normal(generator(1), rows), normal(generator(2), rows)
+    tokens = torch.randint(0, vocab, (rows,), generator=generator(3), device="cuda")
+    for mask in (-1e4, -1e9, -1e10, -1e20, -1e30, -3e38, 5e8, 1e10, 1e30):
+        for kind in (torch.float32, torch.bfloat16):
+            print(f"{mask}, {kind}", flush=True)
+            x = 2 * normal(generator(vocab), rows, vocab)
+            x[0::4, :vocab // 2], x[1::4, vocab // 3:], x[2::4], x[3::4, ::3] = mask, mask, mask, mask
+            x[1::8, 5::7] = mask
+            x[2::8, vocab - 2] = mask + abs(mask) / 64
+            check_score(x.to(kind), tokens, w, u, k)
+
+
+@pytest.mark.parametrize("rows, vocab", SHAPES)
+def test_score_of_rising_logits_far_from_zero(rows, vocab):
+    """the largest moves up again and again, by more and by less than the logits' own steps at that size"""
+    ramp = torch.arange(vocab, device="cuda") * (60.0 / vocab) + normal(generator(4), rows, vocab)
+    w, u = normal(generator(1), rows), normal(generator(2), rows)
+    tokens = torch.randint(0, vocab, (rows,), generator=generator(3), device="cuda")
+    for offset in (1e3, 1e4, 1e5, -1e5, 3e7, -3e8, 2.0**29, -2.0**29, 2.0**30, 2e12, -1e25):
+        print(offset, flush=True)
+        x = (ramp.double() + offset).float()
+        x[::3] = (offset + 64.0 * ramp[::3].double().round()).float()
+        check_score(x, tokens, w, u)
+
+
 # ------------------------------------------------------------------------------------------------ the gradient of sorted tokens
 @pytest.mark.parametrize("d", [1, 3, 130, 513, 768, 1025, 2056, 4091])
 @pytest.mark.parametrize("kind", TYPES)
